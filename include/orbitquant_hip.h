@@ -458,6 +458,85 @@ int oq_pack_lowbit(const uint8_t *values, int bits, int64_t count, uint8_t *pack
 int oq_dequantize_packed_weight(const uint8_t *packed_weight, int bits, const uint16_t *row_norms, const float *centroids,
                                 int64_t N, int64_t K, void *out, int out_dtype, void *stream);
 
+/*
+ * ---- The 4-bit key/value cache of a serving program and the attention that reads it (no counterpart in the reference) ----
+ *
+ * A token's key or value of one head, x[D], is held as y = H(signs * x), H the unnormalised Walsh-Hadamard transform
+ * (butterfly distance 1, 2, 4, ...), in fp32:
+ *   a    = bf16(max|y| * fp32(1/6)), 0 where that is below 2^-126, NaN where y has an infinity or a NaN
+ *   code = the E2M1 value (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign: bit 3) nearest to y * (1 / a), ties to the even code
+ * and stands for x^ = signs * H(a * code) / D.  The struct is host memory, read during the call.  Pages hold page_size
+ * tokens; a slot is page * page_size + place in the page.
+ */
+typedef struct {
+  uint8_t *k_codes;     /* [pages, kv_heads, page_size, D/2]; byte j: dimension 2j in the low half, 2j+1 in the high half */
+  uint16_t *k_scales;   /* bf16 [pages, kv_heads, page_size]                                                                */
+  uint8_t *v_codes;     /* [pages, kv_heads, D/2, page_size]: the same bytes, a page's tokens side by side                 */
+  uint16_t *v_scales;   /* bf16 [pages, kv_heads, page_size]                                                                */
+  const int8_t *signs;  /* [D], +1/-1, 8-byte aligned; the four above 16-byte aligned                                       */
+  int64_t pages;        /* 1 .. 2^31 - 1                                                                                    */
+  int64_t kv_heads;     /* 1 .. 65535                                                                                       */
+  int64_t page_size;    /* a power of two, 16 .. 1024                                                                       */
+  int64_t head_dim;     /* D: 64, 128 or 256                                                                                */
+} oq_kv_cache;
+
+/*
+ * Pages and slots for the new tokens of a batch.  Request r holds lengths[r] tokens in the first ceil(lengths[r] /
+ * page_size) pages of its row of the block table and gets new_lengths[r] more (negative counts are taken as 0); the
+ * pages this needs are taken from the front of free_pages in request order, behind the *taken that are already given out.
+ *
+ * lengths, new_lengths  int32 [requests], requests <= 8192
+ * table        int32 [requests, table_width], rows table_stride apart: the entries of new pages are written, -1 where
+ *              the free list has run out; columns beyond the table are dropped
+ * free_pages   int32 [free_count]; taken int32 [1]
+ * slots        int64 [tokens], positions int32 [tokens]: of the new tokens, request by request; a token without a page
+ *              has the slot -1, and what lies behind the last token has both -1
+ * starts       int32 [requests + 1]: where a request's tokens begin
+ * lengths_after int32 [requests] = lengths + new_lengths; taken_after int32 [1], at most free_count
+ * No output may overlap an input other than the table itself.  Sums of new tokens below 2^31.
+ */
+int oq_kv_assign(const int32_t *lengths, const int32_t *new_lengths, int64_t requests, int32_t *table,
+                 int64_t table_stride, int64_t table_width, const int32_t *free_pages, int64_t free_count,
+                 const int32_t *taken, int64_t page_size, int64_t tokens, int64_t *slots, int32_t *positions,
+                 int32_t *starts, int32_t *lengths_after, int32_t *taken_after, void *stream);
+
+/*
+ * Keys and values [tokens, kv_heads, D] of dtype into the cache at slots[token]; slots that are negative or beyond the
+ * last page are skipped.  No slot twice in one call.  Strides in elements; the last dimension is contiguous.
+ */
+int oq_kv_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens, const oq_kv_cache *cache,
+                void *stream);
+
+/* What the cache holds at slots[token], as [tokens, kv_heads, D] of dtype, contiguous, 16-byte aligned; zeros for slots
+ * that are negative or beyond the last page. */
+int oq_kv_read(const int64_t *slots, int64_t tokens, const oq_kv_cache *cache, void *k, void *v, int dtype, void *stream);
+
+/*
+ * Attention of q [tokens, heads, D] over the cache; heads a multiple of kv_heads, head h reads key head h / (heads /
+ * kv_heads).  Request r holds lengths[r] tokens (new ones included, already written), at the pages of its row of the
+ * block table, and its queries are the last of them: tokens starts[r] .. starts[r+1] - 1 of q, or token r where starts is
+ * NULL (tokens = requests then).  A query at position p sees the cached positions <= p (causal) or all of them, of these
+ * the last `window` if window > 0 (causal only), and none whose page is missing (-1, or not one of the cache's).
+ *
+ *   out = sum_t softmax_t(scale * q . k^_t) v^_t        of q's dtype, [tokens, heads, D], contiguous, 16-byte aligned
+ *   lse = ln sum_t e^(scale * q . k^_t)                 NULL or fp32 [tokens, heads]
+ * A query that sees nothing, and a token that belongs to no request, gets zeros (lse -inf).  starts[0] is 0.
+ *
+ * max_length   the longest of the lengths as far as the caller knows, -1 if it does not; max_new likewise the largest number of
+ *              a request's queries (1 without starts).  They choose launch shapes: a wrong one costs time, never a result's correctness.
+ * workspace    NULL, or oq_kv_attend_workspace_bytes(...) bytes, 16-byte aligned: the keys are then cut into parts where
+ *              there are few rows.  Without it (or with less) the call runs uncut.
+ */
+int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride,
+                 int64_t q_head_stride, const oq_kv_cache *cache, const int32_t *table, int64_t table_stride,
+                 int64_t table_width, const int32_t *lengths, const int32_t *starts, int64_t requests, int causal,
+                 int64_t window, float scale, int64_t max_length, int64_t max_new, void *out, float *lse,
+                 void *workspace, uint64_t workspace_bytes, void *stream);
+uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                      int64_t page_size, int64_t table_width, int64_t requests, int has_starts,
+                                      int64_t window, int64_t max_length, int64_t max_new);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ EXPORTS = (
     "oq_packed_linear", "oq_packed_linear_group", "oq_packed_linear_mapped", "oq_quantized_linear", "oq_quantized_linear_group", "oq_quantized_linear_static", "oq_matmul_packed_weight", "oq_matmul_packed_adaln_int4", "oq_quantize_adaln_weight", "oq_unpack_lowbit", "oq_pack_lowbit",
     "oq_dequantize_packed_weight", "oq_packed_linear_workspace_bytes", "oq_matmul_packed_weight_workspace_bytes",
     "oq_packed_linear_int8", "oq_packed_linear_int8_workspace_bytes", "oq_packed_linear_least_workspace_bytes",
+    "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes",
 )
 
 _lib = None
@@ -33,6 +34,13 @@ _warned = False
 
 class OrbitQuantHipError(RuntimeError):
     pass
+
+
+class KvCacheStruct(ctypes.Structure):
+    """`oq_kv_cache`."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "k_scales", "v_codes", "v_scales", "signs")] + [
+        (name, ctypes.c_int64) for name in ("pages", "kv_heads", "page_size", "head_dim")]
 
 
 def load() -> ctypes.CDLL:
@@ -107,6 +115,18 @@ def load() -> ctypes.CDLL:
     lib.oq_dequantize_packed_weight.argtypes = [vp, c_int, vp, vp, c_i64, c_i64, vp, c_int, vp]
     lib.oq_unpack_lowbit.restype = c_int
     lib.oq_unpack_lowbit.argtypes = [vp, c_int, c_i64, vp, vp]
+    cache = ctypes.POINTER(KvCacheStruct)
+    lib.oq_kv_assign.restype = c_int
+    lib.oq_kv_assign.argtypes = [vp, vp, c_i64, vp, c_i64, c_i64, vp, c_i64, vp, c_i64, c_i64, vp, vp, vp, vp, vp, vp]
+    lib.oq_kv_write.restype = c_int
+    lib.oq_kv_write.argtypes = [vp, c_i64, c_i64, vp, c_i64, c_i64, c_int, vp, c_i64, cache, vp]
+    lib.oq_kv_read.restype = c_int
+    lib.oq_kv_read.argtypes = [vp, c_i64, cache, vp, vp, c_int, vp]
+    lib.oq_kv_attend.restype = c_int
+    lib.oq_kv_attend.argtypes = [vp, c_int, c_i64, c_i64, c_i64, c_i64, cache, vp, c_i64, c_i64, vp, vp, c_i64, c_int, c_i64, c_f, c_i64, c_i64,
+                                 vp, vp, vp, c_u64, vp]
+    lib.oq_kv_attend_workspace_bytes.restype = c_u64
+    lib.oq_kv_attend_workspace_bytes.argtypes = [c_i64] * 7 + [c_int] + [c_i64] * 3
     _lib = lib
     if hasattr(_torch_ops, "bind"):
         _bind(lib)

@@ -3,8 +3,9 @@
 
     python -m orbitquant_amd.build
 
-hipcc cross-compiles for gfx950 without a GPU.  The rotate+quantize kernel is
-built without FMA contraction (its results must match the CPU statement of the
+hipcc cross-compiles for gfx950 without a GPU.  The rotate+quantize kernel and
+what writes and reads the key/value cache are
+built without FMA contraction (their results must match the CPU statement of the
 algorithm bit for bit); packed fp32 VALU instructions are disabled everywhere.
 
     python -m orbitquant_amd.build --variant stamps --flags=-DOQ_GEMM_STAMPS --only packed_gemm.hip
@@ -58,6 +59,11 @@ SOURCES = {
     "token_linear_w2.hip": [],
     "token_linear_w3.hip": [],
     "token_linear_w4.hip": [],
+    "kv_cache.hip": ["-ffp-contract=off"],
+    "kv_attend.hip": [],
+    "kv_attend_d64.hip": [],
+    "kv_attend_d128.hip": [],
+    "kv_attend_d256.hip": [],
 }
 
 

@@ -10,6 +10,7 @@
 
 #include "dense_gemm.h"
 #include "gemm_epilogue.h"
+#include "kv_cache.h"
 #include "rotate_plan.h"
 
 namespace oq {
@@ -573,6 +574,155 @@ int oq_dequantize_packed_weight(const uint8_t *packed_weight, int bits, const ui
   if (N > 0 && K > 0 && (packed_weight == nullptr || row_norms == nullptr || centroids == nullptr || out == nullptr))
     return fail(OQ_ERR_INVALID, "dequantize_packed_weight: null pointer");
   return dequantize_dispatch(packed_weight, bits, row_norms, centroids, N, K, out, out_dtype, as_stream(stream));
+}
+
+// ---- the 4-bit key/value cache ----
+
+namespace {
+int log2_exact(int64_t v) { return v > 0 && (v & (v - 1)) == 0 ? __builtin_ctzll(static_cast<unsigned long long>(v)) : -1; }
+bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+bool known_dtype(int dt) { return dt == OQ_F32 || dt == OQ_F16 || dt == OQ_BF16; }
+bool known_head_dim(int64_t d) { return d == 64 || d == 128 || d == 256; }
+int page_shift_of(int64_t page_size) { return page_size < oq::kKvMinPage || page_size > oq::kKvMaxPage ? -1 : log2_exact(page_size); }
+
+// The cache as the kernels take it; an error status where it is none.
+int kv_cache_of(const char *what, const oq_kv_cache *c, oq::KvCache &out) {
+  if (c == nullptr) return fail(OQ_ERR_INVALID, "%s: no cache", what);
+  if (!known_head_dim(c->head_dim)) return fail(OQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (64, 128 or 256)", what, (long long)c->head_dim);
+  const int shift = page_shift_of(c->page_size);
+  if (shift < 0) return fail(OQ_ERR_UNSUPPORTED, "%s: page_size=%lld (a power of two, 16 to 1024)", what, (long long)c->page_size);
+  if (c->pages < 1 || c->pages > 0x7fffffffLL || c->kv_heads < 1 || c->kv_heads > 65535)
+    return fail(OQ_ERR_INVALID, "%s: pages=%lld kv_heads=%lld", what, (long long)c->pages, (long long)c->kv_heads);
+  if (c->k_codes == nullptr || c->k_scales == nullptr || c->v_codes == nullptr || c->v_scales == nullptr || c->signs == nullptr)
+    return fail(OQ_ERR_INVALID, "%s: null pointer in the cache", what);
+  if (!aligned(c->k_codes, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_codes, 16) || !aligned(c->v_scales, 16) || !aligned(c->signs, 8))
+    return fail(OQ_ERR_INVALID, "%s: the cache is not aligned to 16 bytes", what);
+  out.k_codes = c->k_codes; out.v_codes = c->v_codes; out.k_scales = c->k_scales; out.v_scales = c->v_scales; out.signs = c->signs;
+  out.pages = c->pages; out.heads = static_cast<int>(c->kv_heads); out.page_shift = shift;
+  return OQ_OK;
+}
+
+bool vectors_wide(const void *p, int64_t token_stride, int64_t head_stride, int dtype) {
+  const int64_t per = 16 / oq::dtype_size(dtype);
+  return aligned(p, 16) && token_stride % per == 0 && head_stride % per == 0;
+}
+
+// A launch of eight values a lane, 256 lanes a workgroup, over keys and values.
+int kv_vectors_fit(const char *what, int64_t tokens, const oq_kv_cache *c) {
+  if (tokens < 0) return fail(OQ_ERR_INVALID, "%s: tokens=%lld", what, (long long)tokens);
+  if (tokens > (1LL << 40) || tokens * c->kv_heads > (1LL << 32)) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld exceed the grid", what, (long long)tokens);
+  return OQ_OK;
+}
+
+int kv_attend_shape(oq::KvAttendArgs &a, int64_t tokens, int64_t heads, int64_t table_width, int64_t requests, int64_t window) {
+  const int64_t kv_heads = a.cache.heads;
+  if (tokens < 0 || heads < 1 || heads % kv_heads != 0 || requests < 0 || table_width < 0 || window < 0)
+    return fail(OQ_ERR_INVALID, "kv_attend: tokens=%lld heads=%lld kv_heads=%lld requests=%lld table_width=%lld window=%lld", (long long)tokens,
+                (long long)heads, (long long)kv_heads, (long long)requests, (long long)table_width, (long long)window);
+  if (tokens > 0x3fffffffLL || requests > 0x3fffffffLL || heads > 65535 || tokens * heads > 0x7fffffffLL ||
+      (tokens * heads / 64 + (requests + 1) * kv_heads) > 0x7fffffffLL || table_width > (1LL << 30) >> a.cache.page_shift)
+    return fail(OQ_ERR_UNSUPPORTED, "kv_attend: tokens=%lld heads=%lld requests=%lld table_width=%lld exceed the grid", (long long)tokens,
+                (long long)heads, (long long)requests, (long long)table_width);
+  a.tokens = tokens; a.heads = static_cast<int>(heads); a.group = static_cast<int>(heads / kv_heads); a.requests = static_cast<int>(requests);
+  a.table_width = static_cast<int>(table_width); a.window = static_cast<int>(window < 0x3fffffffLL ? window : 0x3fffffffLL);
+  return OQ_OK;
+}
+
+int64_t most_queries(int64_t tokens, bool has_starts, int64_t max_new) { return !has_starts ? 1 : max_new >= 1 && max_new < tokens ? max_new : tokens; }
+}  // namespace
+
+int oq_kv_assign(const int32_t *lengths, const int32_t *new_lengths, int64_t requests, int32_t *table, int64_t table_stride,
+                 int64_t table_width, const int32_t *free_pages, int64_t free_count, const int32_t *taken, int64_t page_size,
+                 int64_t tokens, int64_t *slots, int32_t *positions, int32_t *starts, int32_t *lengths_after, int32_t *taken_after,
+                 void *stream) {
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return fail(OQ_ERR_UNSUPPORTED, "kv_assign: page_size=%lld (a power of two, 16 to 1024)", (long long)page_size);
+  if (requests < 0 || tokens < 0 || table_width < 0 || free_count < 0 || (requests > 1 && table_stride < table_width))
+    return fail(OQ_ERR_INVALID, "kv_assign: requests=%lld tokens=%lld table_width=%lld table_stride=%lld free_count=%lld", (long long)requests,
+                (long long)tokens, (long long)table_width, (long long)table_stride, (long long)free_count);
+  if (requests > oq::kKvMaxRequests || tokens > 0x7fffffffLL || table_width > 0x7fffffffLL || free_count > 0x7fffffffLL)
+    return fail(OQ_ERR_UNSUPPORTED, "kv_assign: requests=%lld (at most %d) tokens=%lld", (long long)requests, oq::kKvMaxRequests, (long long)tokens);
+  if ((requests > 0 && (lengths == nullptr || new_lengths == nullptr || lengths_after == nullptr)) ||
+      (requests > 0 && table_width > 0 && table == nullptr) || (free_count > 0 && free_pages == nullptr) || taken == nullptr ||
+      (tokens > 0 && (slots == nullptr || positions == nullptr)) || starts == nullptr || taken_after == nullptr)
+    return fail(OQ_ERR_INVALID, "kv_assign: null pointer");
+  oq::KvAssignArgs a{};
+  a.lengths = lengths; a.new_lengths = new_lengths; a.free_pages = free_pages; a.taken = taken; a.table = table; a.table_stride = table_stride;
+  a.table_width = static_cast<int>(table_width); a.requests = static_cast<int>(requests); a.free_count = static_cast<int>(free_count);
+  a.page_shift = shift; a.tokens = tokens; a.slots = slots; a.positions = positions; a.starts = starts; a.lengths_after = lengths_after;
+  a.taken_after = taken_after;
+  return oq::kv_assign_dispatch(a, as_stream(stream));
+}
+
+int oq_kv_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                int dtype, const int64_t *slots, int64_t tokens, const oq_kv_cache *cache, void *stream) {
+  oq::KvWriteArgs a{};
+  if (const int status = kv_cache_of("kv_write", cache, a.cache)) return status;
+  if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "kv_write: dtype=%d", dtype);
+  if (const int status = kv_vectors_fit("kv_write", tokens, cache)) return status;
+  if (tokens == 0) return OQ_OK;
+  if (k == nullptr || v == nullptr || slots == nullptr) return fail(OQ_ERR_INVALID, "kv_write: null pointer");
+  a.k = k; a.v = v; a.slots = slots; a.tokens = tokens;
+  a.k_token_stride = k_token_stride; a.k_head_stride = k_head_stride; a.v_token_stride = v_token_stride; a.v_head_stride = v_head_stride;
+  a.k_wide = vectors_wide(k, k_token_stride, k_head_stride, dtype);
+  a.v_wide = vectors_wide(v, v_token_stride, v_head_stride, dtype);
+  return oq::kv_write_dispatch(a, static_cast<int>(cache->head_dim), dtype, as_stream(stream));
+}
+
+int oq_kv_read(const int64_t *slots, int64_t tokens, const oq_kv_cache *cache, void *k, void *v, int dtype, void *stream) {
+  oq::KvReadArgs a{};
+  if (const int status = kv_cache_of("kv_read", cache, a.cache)) return status;
+  if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "kv_read: dtype=%d", dtype);
+  if (const int status = kv_vectors_fit("kv_read", tokens, cache)) return status;
+  if (tokens == 0) return OQ_OK;
+  if (k == nullptr || v == nullptr || slots == nullptr) return fail(OQ_ERR_INVALID, "kv_read: null pointer");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(OQ_ERR_INVALID, "kv_read: the outputs are not aligned to 16 bytes");
+  a.slots = slots; a.k = k; a.v = v; a.tokens = tokens;
+  return oq::kv_read_dispatch(a, static_cast<int>(cache->head_dim), dtype, as_stream(stream));
+}
+
+int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
+                 const oq_kv_cache *cache, const int32_t *table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                 const int32_t *starts, int64_t requests, int causal, int64_t window, float scale, int64_t max_length, int64_t max_new,
+                 void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream) {
+  oq::KvAttendArgs a{};
+  if (const int status = kv_cache_of("kv_attend", cache, a.cache)) return status;
+  if (!known_dtype(q_dtype)) return fail(OQ_ERR_INVALID, "kv_attend: q_dtype=%d", q_dtype);
+  if (const int status = kv_attend_shape(a, tokens, heads, table_width, requests, window)) return status;
+  if (starts == nullptr && tokens != requests) return fail(OQ_ERR_INVALID, "kv_attend: tokens=%lld requests=%lld and no starts", (long long)tokens, (long long)requests);
+  if (window > 0 && !causal) return fail(OQ_ERR_INVALID, "kv_attend: a window needs causal attention");
+  if (requests > 1 && table_stride < table_width) return fail(OQ_ERR_INVALID, "kv_attend: table_stride=%lld table_width=%lld", (long long)table_stride, (long long)table_width);
+  if (tokens == 0) return OQ_OK;
+  if (q == nullptr || out == nullptr || (requests > 0 && lengths == nullptr) || (requests > 0 && table_width > 0 && table == nullptr))
+    return fail(OQ_ERR_INVALID, "kv_attend: null pointer");
+  if (!aligned(out, 16) || !aligned(workspace, 16)) return fail(OQ_ERR_INVALID, "kv_attend: the output or the workspace is not aligned to 16 bytes");
+  const int dim = static_cast<int>(cache->head_dim);
+  a.q = q; a.q_dtype = q_dtype; a.q_token_stride = q_token_stride; a.q_head_stride = q_head_stride;
+  a.q_wide = vectors_wide(q, q_token_stride, q_head_stride, q_dtype);
+  a.table = table; a.table_stride = table_stride; a.lengths = lengths; a.starts = starts; a.causal = causal != 0; a.scale = scale;
+  a.out = out; a.lse = lse;
+  max_new = most_queries(tokens, starts != nullptr, max_new);
+  const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, max_new);
+  if (needed > 0 && workspace != nullptr && workspace_bytes >= needed) {
+    a.part_out = static_cast<float *>(workspace);
+    a.part_lse = a.part_out + static_cast<int64_t>(a.parts) * tokens * heads * dim;
+  } else {
+    a.parts = 1;
+  }
+  return oq::kv_attend_dispatch(a, dim, max_new, as_stream(stream));
+}
+
+uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                      int64_t table_width, int64_t requests, int has_starts, int64_t window, int64_t max_length,
+                                      int64_t max_new) {
+  static const int32_t some = 0;
+  oq::KvAttendArgs a{};
+  a.cache.page_shift = page_shift_of(page_size);
+  if (a.cache.page_shift < 0 || !known_head_dim(head_dim) || kv_heads < 1 || kv_heads > 65535) return 0;
+  a.cache.heads = static_cast<int>(kv_heads);
+  if (kv_attend_shape(a, tokens, heads, table_width, requests, window) != OQ_OK || tokens == 0) return 0;
+  a.starts = has_starts ? &some : nullptr;  // (asked whether it is there, not read)
+  return oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new));
 }
 
 }  // extern "C"

@@ -1,0 +1,58 @@
+// What the entry points hand to the kernels of the 4-bit key/value cache.
+#pragma once
+
+#include "kv_format.h"
+
+namespace oq {
+
+struct KvAssignArgs {
+  const int32_t *lengths, *new_lengths, *free_pages, *taken;
+  int32_t *table;
+  int64_t table_stride;
+  int table_width, requests, free_count, page_shift;
+  int64_t tokens;
+  int64_t *slots;
+  int32_t *positions, *starts, *lengths_after, *taken_after;
+};
+
+struct KvWriteArgs {
+  KvCache cache;
+  const void *k, *v;
+  const int64_t *slots;
+  int64_t tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride;  // strides in elements
+  bool k_wide, v_wide;  // every vector begins on 16 bytes
+};
+
+struct KvReadArgs {
+  KvCache cache;
+  const int64_t *slots;
+  void *k, *v;  // [tokens, heads, D], 16-byte aligned
+  int64_t tokens;
+};
+
+struct KvAttendArgs {
+  KvCache cache;
+  const void *q;
+  int q_dtype;
+  int64_t tokens, q_token_stride, q_head_stride;
+  bool q_wide;
+  int heads, group, requests;         // query heads, query heads of a key head
+  const int32_t *table, *lengths, *starts;  // starts: NULL for one query a request
+  int64_t table_stride;
+  int table_width, window;            // window: 0 for none
+  bool causal;
+  float scale;
+  int tiles, parts, part_steps;       // tiles of rows, parts of the keys, steps of 64 keys in a part
+  void *out;
+  float *lse;                         // NULL or [tokens, heads]
+  float *part_out, *part_lse;         // [parts, tokens, heads, D] and [parts, tokens, heads], where parts > 1
+};
+
+int kv_assign_dispatch(const KvAssignArgs &a, hipStream_t stream);
+int kv_write_dispatch(const KvWriteArgs &a, int dim, int dtype, hipStream_t stream);
+int kv_read_dispatch(const KvReadArgs &a, int dim, int dtype, hipStream_t stream);
+// Sets tiles, parts and part_steps; the bytes of part_out and part_lse that they need (0: none).
+uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new);
+int kv_attend_dispatch(KvAttendArgs &a, int dim, int64_t max_new, hipStream_t stream);
+
+}  // namespace oq

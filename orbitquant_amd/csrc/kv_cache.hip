@@ -1,0 +1,266 @@
+// Around the 4-bit key/value cache: pages and slots for new tokens, keys and values into it, and back out of it.
+// (No counterpart in the reference, which has no cache.)
+#include "kv_cache.h"
+
+namespace oq {
+namespace {
+
+// ---- pages and slots ---------------------------------------------------------------------------------------------
+// Request r holds before[r] tokens in have = ceil(before / page) pages and gets new[r] more: fresh = ceil((before + new) /
+// page) - have pages, taken from the free list in request order.  Everything follows from two running sums over the
+// requests (new tokens, fresh pages), which every workgroup makes for itself in LDS: a few thousand requests are some KB, and one launch
+// without a grid-wide wait is what a call of some microseconds can afford.  A token finds its request by bisection.
+// Nothing that one workgroup writes is read by another: the page of a new token is in the old part of the table or in the free list.
+constexpr int kAssignThreads = 256, kAssignTokens = 4;  // tokens a thread
+
+__device__ __forceinline__ int last_not_above(const int *sums, int count, int value) {  // largest r with sums[r] <= value
+  int low = 0, high = count;  // sums[0] = 0 <= value
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (sums[mid] <= value) low = mid; else high = mid;
+  }
+  return low;
+}
+
+__global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs a) {
+  extern __shared__ int lds[];
+  __shared__ uint64_t wave_sum[kAssignThreads / 64];
+  int *starts = lds, *upto = lds + a.requests + 1, *before = lds + 2 * (a.requests + 1);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int page = 1 << a.page_shift;
+  uint64_t carry = 0;  // new tokens in the low half, fresh pages in the high half
+  for (int base = 0; base < a.requests; base += kAssignThreads) {
+    const int r = base + tid;
+    int was = 0, more = 0;
+    if (r < a.requests) {
+      was = max(a.lengths[r], 0);
+      more = max(a.new_lengths[r], 0);
+    }
+    const int fresh = static_cast<int>((static_cast<uint32_t>(was) + more + page - 1) >> a.page_shift) -
+                      static_cast<int>((static_cast<uint32_t>(was) + page - 1) >> a.page_shift);
+    const uint64_t own = static_cast<uint32_t>(more) | (static_cast<uint64_t>(fresh) << 32);
+    uint64_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint64_t below = __shfl_up(static_cast<unsigned long long>(sum), d, 64);
+      if (lane >= d) sum += below;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    uint64_t ahead = carry;
+#pragma unroll
+    for (int w = 0; w < kAssignThreads / 64; ++w) {
+      if (w < wave) ahead += wave_sum[w];
+      carry += wave_sum[w];
+    }
+    if (r < a.requests) {
+      const uint64_t exclusive = ahead + sum - own;
+      starts[r] = static_cast<int>(exclusive);
+      upto[r] = static_cast<int>(exclusive >> 32);
+      before[r] = was;
+      if (blockIdx.x == 0) {
+        a.starts[r] = static_cast<int>(exclusive);
+        a.lengths_after[r] = was + more;
+      }
+    }
+    __syncthreads();
+  }
+  const int total = static_cast<int>(carry), total_fresh = static_cast<int>(carry >> 32);
+  const int taken = max(*a.taken, 0);
+  if (tid == 0) {
+    starts[a.requests] = total;
+    upto[a.requests] = total_fresh;
+    if (blockIdx.x == 0) {
+      a.starts[a.requests] = total;
+      *a.taken_after = static_cast<int>(min(static_cast<int64_t>(taken) + total_fresh, static_cast<int64_t>(a.free_count)));
+    }
+  }
+  __syncthreads();
+  const auto free_page = [&](int64_t index) { return index < a.free_count ? a.free_pages[index] : -1; };
+  for (int64_t f = static_cast<int64_t>(blockIdx.x) * kAssignThreads + tid; f < total_fresh; f += static_cast<int64_t>(gridDim.x) * kAssignThreads) {
+    const int r = last_not_above(upto, a.requests, static_cast<int>(f));
+    const int column = ((before[r] + page - 1) >> a.page_shift) + static_cast<int>(f) - upto[r];
+    if (column < a.table_width) a.table[r * a.table_stride + column] = free_page(taken + f);
+  }
+#pragma unroll
+  for (int i = 0; i < kAssignTokens; ++i) {
+    const int64_t t = (static_cast<int64_t>(blockIdx.x) * kAssignTokens + i) * kAssignThreads + tid;
+    if (t >= a.tokens) break;
+    int64_t slot = -1;
+    int position = -1;
+    if (t < total) {
+      const int r = last_not_above(starts, a.requests, static_cast<int>(t));
+      position = before[r] + static_cast<int>(t) - starts[r];
+      const int column = position >> a.page_shift, have = (before[r] + page - 1) >> a.page_shift;
+      int at = -1;
+      if (column < a.table_width) at = column < have ? a.table[r * a.table_stride + column] : free_page(static_cast<int64_t>(taken) + upto[r] + column - have);
+      if (at >= 0) slot = (static_cast<int64_t>(at) << a.page_shift) + (position & (page - 1));
+    }
+    a.slots[t] = slot;
+    a.positions[t] = position;
+  }
+}
+
+// ---- into the cache and back -----------------------------------------------------------------------------------------
+// Eight values a lane, so a vector is D / 8 lanes and a wavefront holds 512 / D of them.
+template <int DT>
+__device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float (&y)[8]) {
+  if (wide) {
+    if constexpr (DT == OQ_F32) {
+      const float4 lo = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[0], hi = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[1];
+      y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w; y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = dyn_bits_to_f32((v[i / 2] >> (16 * (i & 1))) & 0xffffu, DT);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = load_as_f32<DT>(p, at + i);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void *p, int64_t at, const float (&y)[8]) {  // 16-byte aligned
+  if constexpr (DT == OQ_F32) {
+    reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[0] = make_float4(y[0], y[1], y[2], y[3]);
+    reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[1] = make_float4(y[4], y[5], y[6], y[7]);
+  } else {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = DT == OQ_F16 ? f32_to_f16_bits(y[2 * i]) : f32_to_bf16_bits(y[2 * i]);
+      const uint32_t hi = DT == OQ_F16 ? f32_to_f16_bits(y[2 * i + 1]) : f32_to_bf16_bits(y[2 * i + 1]);
+      v[i] = lo | hi << 16;
+    }
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void times_signs(float (&y)[8], const int8_t *signs, int part) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= static_cast<float>(signs[8 * part + i]);
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs a) {
+  const int lane = threadIdx.x & 63, part = lane & (D / 8 - 1);
+  const int64_t vectors = 2 * a.tokens * a.cache.heads;
+  const int64_t index = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / (D / 8);
+  if (index >= vectors) return;  // (whole vectors)
+  const bool value = index >= vectors / 2;
+  const int64_t rest = value ? index - vectors / 2 : index;
+  const int64_t token = rest / a.cache.heads;
+  const int head = static_cast<int>(rest - token * a.cache.heads);
+  const int64_t slot = a.slots[token];
+  if (slot < 0 || slot >= a.cache.pages << a.cache.page_shift) return;
+  float y[8];
+  if (value) load8<DT>(a.v, token * a.v_token_stride + head * a.v_head_stride + 8 * part, a.v_wide, y);
+  else load8<DT>(a.k, token * a.k_token_stride + head * a.k_head_stride + 8 * part, a.k_wide, y);
+  times_signs<D>(y, a.cache.signs, part);
+  kv_butterflies<D>(y, lane);
+  uint16_t scale;
+  const uint32_t codes = kv_encode<D>(y, scale);
+  const int shift = a.cache.page_shift;
+  const int64_t block = (slot >> shift) * a.cache.heads + head;  // of one page and head
+  const int64_t place = slot & ((1 << shift) - 1);
+  if (value) {
+    uint8_t *to = a.cache.v_codes + ((block * (D / 2) + 4 * part) << shift) + place;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) to[static_cast<int64_t>(b) << shift] = static_cast<uint8_t>(codes >> (8 * b));
+    if (part == 0) a.cache.v_scales[(block << shift) + place] = scale;
+  } else {
+    reinterpret_cast<uint32_t *>(a.cache.k_codes)[((block << shift) + place) * (D / 8) + part] = codes;
+    if (part == 0) a.cache.k_scales[(block << shift) + place] = scale;
+  }
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
+  const int lane = threadIdx.x & 63, part = lane & (D / 8 - 1);
+  const int64_t vectors = 2 * a.tokens * a.cache.heads;
+  const int64_t index = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / (D / 8);
+  if (index >= vectors) return;
+  const bool value = index >= vectors / 2;
+  const int64_t rest = value ? index - vectors / 2 : index;
+  const int64_t token = rest / a.cache.heads;
+  const int head = static_cast<int>(rest - token * a.cache.heads);
+  const int64_t slot = a.slots[token];
+  float y[8] = {};
+  if (slot >= 0 && slot < a.cache.pages << a.cache.page_shift) {
+    const int shift = a.cache.page_shift;
+    const int64_t block = (slot >> shift) * a.cache.heads + head;
+    const int64_t place = slot & ((1 << shift) - 1);
+    uint32_t codes = 0;
+    float scale;
+    if (value) {
+      const uint8_t *from = a.cache.v_codes + ((block * (D / 2) + 4 * part) << shift) + place;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) codes |= static_cast<uint32_t>(from[static_cast<int64_t>(b) << shift]) << (8 * b);
+      scale = bf16_bits_to_f32(a.cache.v_scales[(block << shift) + place]);
+    } else {
+      codes = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[((block << shift) + place) * (D / 8) + part];
+      scale = bf16_bits_to_f32(a.cache.k_scales[(block << shift) + place]);
+    }
+    const kv_f16x8 c = kv_decode8(codes);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(c[i]) * scale;
+    kv_butterflies<D>(y, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= 1.0f / D;
+    times_signs<D>(y, a.cache.signs, part);
+  }
+  store8<DT>(value ? a.v : a.k, rest * D + 8 * part, y);
+}
+
+template <template <int, int> class Run, typename Args>
+int by_type(const Args &a, int dim, int dtype, hipStream_t stream) {
+  const auto with = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (dtype == OQ_F32) Run<D, OQ_F32>::go(a, stream);
+    else if (dtype == OQ_F16) Run<D, OQ_F16>::go(a, stream);
+    else Run<D, OQ_BF16>::go(a, stream);
+  };
+  if (dim == 64) with(std::integral_constant<int, 64>{});
+  else if (dim == 128) with(std::integral_constant<int, 128>{});
+  else with(std::integral_constant<int, 256>{});
+  return OQ_OK;
+}
+
+inline dim3 vector_grid(int64_t tokens, int heads, int dim) {
+  return dim3(static_cast<unsigned>((2 * tokens * heads * (dim / 8) + 255) / 256));
+}
+template <int D, int DT>
+struct RunWrite {
+  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, vector_grid(a.tokens, a.cache.heads, D), dim3(256), 0, s, a); }
+};
+template <int D, int DT>
+struct RunRead {
+  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, vector_grid(a.tokens, a.cache.heads, D), dim3(256), 0, s, a); }
+};
+
+}  // namespace
+
+int kv_assign_dispatch(const KvAssignArgs &a, hipStream_t stream) {
+  const size_t lds = sizeof(int) * (3 * static_cast<size_t>(a.requests) + 2);
+  if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kv_assign_kernel), lds))
+    return fail(OQ_ERR_LAUNCH, "kv_assign: no LDS for %d requests", a.requests);
+  constexpr int64_t per_block = kAssignThreads * kAssignTokens;
+  const int64_t blocks = (a.tokens + per_block - 1) / per_block;
+  launch_kernel(kv_assign_kernel, dim3(static_cast<unsigned>(blocks > 1 ? blocks : 1)), dim3(kAssignThreads), lds, stream, a);
+  return check_launch("kv_assign");
+}
+
+int kv_write_dispatch(const KvWriteArgs &a, int dim, int dtype, hipStream_t stream) {
+  by_type<RunWrite>(a, dim, dtype, stream);
+  return check_launch("kv_write");
+}
+
+int kv_read_dispatch(const KvReadArgs &a, int dim, int dtype, hipStream_t stream) {
+  by_type<RunRead>(a, dim, dtype, stream);
+  return check_launch("kv_read");
+}
+
+}  // namespace oq

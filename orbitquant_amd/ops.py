@@ -780,3 +780,6 @@ def unpack_lowbit(packed: torch.Tensor, bits: int, length: int) -> torch.Tensor:
                                   _stream(packed))
     _lib.check(rc, "oq_unpack_lowbit")
     return out
+
+
+from .kv_cache import kv_assign, kv_attend, kv_read, kv_write  # noqa: E402,F401  (the cache's wrappers, which use the helpers above)
