@@ -620,7 +620,7 @@ int kv_attend_shape(oq::KvAttendArgs &a, int64_t tokens, int64_t heads, int64_t 
     return fail(OQ_ERR_INVALID, "kv_attend: tokens=%lld heads=%lld kv_heads=%lld requests=%lld table_width=%lld window=%lld", (long long)tokens,
                 (long long)heads, (long long)kv_heads, (long long)requests, (long long)table_width, (long long)window);
   if (tokens > 0x3fffffffLL || requests > 0x3fffffffLL || heads > 65535 || tokens * heads > 0x7fffffffLL ||
-      (tokens * heads / 64 + (requests + 1) * kv_heads) > 0x7fffffffLL || table_width > (1LL << 30) >> a.cache.page_shift)
+      (tokens * heads + (requests + 2) * kv_heads * (heads / kv_heads / 16 + 4)) > 0x7fffffffLL || table_width > (1LL << 30) >> a.cache.page_shift)
     return fail(OQ_ERR_UNSUPPORTED, "kv_attend: tokens=%lld heads=%lld requests=%lld table_width=%lld exceed the grid", (long long)tokens,
                 (long long)heads, (long long)requests, (long long)table_width);
   a.tokens = tokens; a.heads = static_cast<int>(heads); a.group = static_cast<int>(heads / kv_heads); a.requests = static_cast<int>(requests);
@@ -701,15 +701,14 @@ int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int6
   a.q_wide = vectors_wide(q, q_token_stride, q_head_stride, q_dtype);
   a.table = table; a.table_stride = table_stride; a.lengths = lengths; a.starts = starts; a.causal = causal != 0; a.scale = scale;
   a.out = out; a.lse = lse;
-  max_new = most_queries(tokens, starts != nullptr, max_new);
-  const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, max_new);
+  const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, most_queries(tokens, starts != nullptr, max_new));
   if (needed > 0 && workspace != nullptr && workspace_bytes >= needed) {
     a.part_out = static_cast<float *>(workspace);
-    a.part_lse = a.part_out + static_cast<int64_t>(a.parts) * tokens * heads * dim;
+    a.part_stats = reinterpret_cast<float2 *>(a.part_out + static_cast<int64_t>(a.parts) * tokens * heads * dim);
   } else {
     a.parts = 1;
   }
-  return oq::kv_attend_dispatch(a, dim, max_new, as_stream(stream));
+  return oq::kv_attend_dispatch(a, dim, as_stream(stream));
 }
 
 uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,

@@ -3,16 +3,9 @@
 
 namespace oq {
 
-void kv_attend_128(const KvAttendArgs &a, int rt, int split, hipStream_t stream) {
-  if (rt == 2) {
-    if (split == 0) kv_attend_launch<128, 2, 0>(a, stream);
-    else if (split == 1) kv_attend_launch<128, 2, 1>(a, stream);
-    else kv_attend_launch<128, 2, 2>(a, stream);
-    return;
-  }
-  if (split == 0) kv_attend_launch<128, 1, 0>(a, stream);
-  else if (split == 1) kv_attend_launch<128, 1, 1>(a, stream);
-  else kv_attend_launch<128, 1, 2>(a, stream);
+bool kv_attend_128(const KvAttendArgs &a, int split, hipStream_t stream) {
+  if (split == 0) return kv_attend_launch<128, 0>(a, stream);
+  return split == 1 ? kv_attend_launch<128, 1>(a, stream) : kv_attend_launch<128, 2>(a, stream);
 }
 
 }  // namespace oq

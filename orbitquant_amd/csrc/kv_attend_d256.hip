@@ -3,11 +3,9 @@
 
 namespace oq {
 
-void kv_attend_256(const KvAttendArgs &a, int rt, int split, hipStream_t stream) {
-  (void)rt;  // (always one)
-  if (split == 0) kv_attend_launch<256, 1, 0>(a, stream);
-  else if (split == 1) kv_attend_launch<256, 1, 1>(a, stream);
-  else kv_attend_launch<256, 1, 2>(a, stream);
+bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream) {
+  if (split == 0) return kv_attend_launch<256, 0>(a, stream);
+  return split == 1 ? kv_attend_launch<256, 1>(a, stream) : kv_attend_launch<256, 2>(a, stream);
 }
 
 }  // namespace oq

@@ -3,16 +3,9 @@
 
 namespace oq {
 
-void kv_attend_64(const KvAttendArgs &a, int rt, int split, hipStream_t stream) {
-  if (rt == 2) {
-    if (split == 0) kv_attend_launch<64, 2, 0>(a, stream);
-    else if (split == 1) kv_attend_launch<64, 2, 1>(a, stream);
-    else kv_attend_launch<64, 2, 2>(a, stream);
-    return;
-  }
-  if (split == 0) kv_attend_launch<64, 1, 0>(a, stream);
-  else if (split == 1) kv_attend_launch<64, 1, 1>(a, stream);
-  else kv_attend_launch<64, 1, 2>(a, stream);
+bool kv_attend_64(const KvAttendArgs &a, int split, hipStream_t stream) {
+  if (split == 0) return kv_attend_launch<64, 0>(a, stream);
+  return split == 1 ? kv_attend_launch<64, 1>(a, stream) : kv_attend_launch<64, 2>(a, stream);
 }
 
 }  // namespace oq

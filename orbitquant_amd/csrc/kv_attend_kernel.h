@@ -3,28 +3,34 @@
 //   s[i, t] = scale * q_i . k^_t = (scale / D) * (H (signs * q_i)) . (a_t c_t)          c: the codes' values, a: their scale
 //   o_i     = sum_t e^(s[i, t] - m_i) v^_t / l_i = signs * H (sum_t e^(s[i, t] - m_i) b_t c'_t) / (D l_i)
 //
-// so a query is rotated once, the output is rotated back once, and in between the codes are used as they are: neither keys nor values are ever
-// rotated back.  Query i of a request that holds `length` tokens, new of them now, stands at position length - new + i and sees the
-// positions up to its own (causal), the last `window` of them if there is a window.
+// so a query is rotated once, the output is rotated back once, and in between the codes are used as they are: neither keys nor
+// values are ever rotated back.  Query i of a request that holds `length` tokens, new of them now, stands at position length -
+// new + i and sees the positions up to its own (causal), the last `window` of them if there is a window.
 //
-// A wavefront holds RT tiles of sixteen query rows (a row: one token and one of the `group` heads that share a key head) and
-// walks the keys in steps of 64.  Both products run transposed, keys and dimensions as the matrix instruction's rows,
-// queries as its columns:
+// A wavefront holds tiles of sixteen query rows (a row: one token and one of the `group` heads that share a key head) and walks
+// the keys in steps of 64.  Both products run transposed, keys and dimensions as the matrix instruction's rows, queries as
+// its columns:
 //   S^T = K Q^T:  lane (n = lane & 15, g = lane >> 4) of the A operand holds key row n and D / 4 dimensions from g * D / 4 on:
-//                 one contiguous piece of the cache.  Row n of tile a is key 16 * (n >> 2) + 4 * a + (n & 3) of the step.
-//   the result:   lane (n, g) has query n and keys 16 * g + 4 * a + r, r = 0..3: sixteen keys in a row over the four tiles.
+//                 one contiguous piece of the cache.  Row n of tile k is key 16 * (n >> 2) + 4 * k + (n & 3) of the step.
+//   the result:   lane (n, g) has query n and keys 16 * g + 4 * k + r, r = 0..3: sixteen keys in a row over the four tiles.
 //   O^T = V^T P^T: the B operand wants query n and eight keys a lane, and any order of the keys does as long as V has the
 //                 same: lane (n, g) has just the sixteen it needs, so the weights go from one product to the other inside their
 //                 registers.  V^T's lane (n, g) reads the bytes of dimensions 32 j + 2 n, 32 j + 2 n + 1 and the tokens
 //                 16 g .. 16 g + 15, sixteen bytes, whose halves are regrouped by token pair.
-// So there is no LDS and no barrier on the way; pages may be as small as sixteen tokens.
+// So pages may be as small as sixteen tokens.
 //
-// Precision.  The codes are exact in fp16.  A rotated query is scaled by a power of two to use fp16's range and rounded to its eleven bits, and so are
-// the weights e^(s - R) b_t; SPLIT 1 (fp16 inputs) keeps a second fp16 part of the query, SPLIT 2 (fp32 inputs) of both, which
-// leaves 22 bits.  Sums, maxima and exponentials are fp32.
-// The reference R of a row is not its maximum: it is raised when a weight could pass 2^15, to where the largest is about 2^10.  Rows are so rescaled a
-// few times in all, no maximum is exchanged between lanes in between, and the fp16 weights have 24 binary digits below their
-// largest before they lose any.  R holds the exponent of the largest value scale too (b_t is anything), bounded so that l stays finite.
+// Precision.  The codes are exact in fp16.  A rotated query is scaled by a power of two to use fp16's range and rounded to its
+// eleven bits, and so are the weights e^(s - R) b_t; SPLIT 1 (fp16 inputs) keeps a second fp16 part of the query, SPLIT 2 (fp32
+// inputs) of both, which leaves 22 bits.  Sums, maxima and exponentials are fp32.
+// The reference R of a row is not its maximum: it is raised when a weight could pass 2^15, to where the largest is about 2^10.
+// Rows are so rescaled a few times in all, no maximum is exchanged between lanes in between, and the fp16 weights have 24
+// binary digits below their largest before they lose any.  R holds the exponent of the largest value scale too (b_t is
+// anything), bounded so that l stays finite.
+//
+// Two kernels.  Few rows (single tokens, at most kKvFewRows of a request): four wavefronts share the keys of sixteen rows, every
+// one decodes for itself, and the launch is bound by the cache's bytes.  Many rows (a prompt): the wavefronts have rows of
+// their own and the same keys, which they decode once for all of them into LDS; bound by the vector instructions around the
+// products.
 #pragma once
 
 #include "kv_cache.h"
@@ -32,18 +38,36 @@
 namespace oq {
 
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key: e^(-inf - R) is 0, any key raises it
-
-// Row tiles of a workgroup: four wavefronts with RT * 16 rows each.  A tile with few rows has its wavefronts share the keys instead.
-template <int RT>
-constexpr int kv_tile_rows() { return 64 * RT; }
+constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
+constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
+constexpr int kKvManyRows = 128;        // rows of a workgroup of the second
 
 // Tiles in front of request r when its rows begin at `row`: enough for every request's last, unfilled tile.
-__host__ __device__ inline int64_t kv_tile_base(int64_t row, int64_t r, int tile_rows) { return row / tile_rows + r; }
+__host__ __device__ inline int64_t kv_tile_base(int64_t row, int64_t r) { return row / kKvManyRows + r; }
 
+__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The butterflies between lanes X apart (16 or 32), two registers at a time: a swap of lane groups puts the two operands of
+// every result into one lane, and a second one the results back.
+template <int X>
+__device__ __forceinline__ void kv_lane_butterfly(float &a, float &b) {
+  const auto swap = [](float x, float y) -> kv_u32x2 {
+    if constexpr (X == 16) return __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    else return __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  };
+  const kv_u32x2 in = swap(a, b);
+  const float x = __uint_as_float(in[0]), y = __uint_as_float(in[1]);
+  const kv_u32x2 out = swap(x + y, x - y);
+  a = __uint_as_float(out[0]);
+  b = __uint_as_float(out[1]);
+}
+
+// D / 4 values a lane.  Every pair of dimensions that differ in one bit meets once: which bits are registers and which lanes
+// does not matter.
 template <int D>
-__device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4], int lane) {  // D / 4 dimensions a lane from (lane >> 4) * D / 4 on
+__device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4]) {
 #pragma unroll
   for (int d = 1; d < D / 4; d *= 2) {
 #pragma unroll
@@ -56,146 +80,282 @@ __device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4], int lane) {  /
     }
   }
 #pragma unroll
-  for (int x = 16; x < 64; x *= 2) {
-    const bool upper = (lane & x) != 0;
+  for (int i = 0; i < D / 4; i += 2) kv_lane_butterfly<16>(y[i], y[i + 1]);
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      const float other = __shfl_xor(y[i], x, 64);
-      y[i] = upper ? other - y[i] : y[i] + other;
+  for (int i = 0; i < D / 4; i += 2) kv_lane_butterfly<32>(y[i], y[i + 1]);
+}
+
+// Over the four lanes that hold a row (lane & 15 the same).
+template <typename Op>
+__device__ __forceinline__ float kv_over_groups(float x, Op op) {
+  const kv_u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const kv_u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float kv_max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float kv_sum_of(float a, float b) { return a + b; }
+
+// A run of rows of one request.
+struct KvRows {
+  int request, start, fresh, length;  // its first token in q, its queries, its cached tokens
+  int first, rows;                    // the run
+  int last_key;
+  __device__ __forceinline__ int position(int token) const { return length - fresh + token; }
+};
+
+__device__ __forceinline__ int kv_start_of(const KvAttendArgs &a, int request) {  // the tokens behind the last request's are a request of their own, without keys
+  return request <= a.requests ? min(max(a.starts[request], 0), static_cast<int>(a.tokens)) : static_cast<int>(a.tokens);
+}
+
+__device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r) {
+  r.length = r.request < a.requests ? max(a.lengths[r.request], 0) : 0;
+  const int64_t reach = static_cast<int64_t>(a.table_width) << a.cache.page_shift;  // what lies behind the table is not there
+  r.last_key = static_cast<int>(min(static_cast<int64_t>(r.length), reach)) - 1;
+}
+
+// What rows [first, first + rows) of the run see: some row the keys lowest..highest, every row the keys all_low..all_high.
+struct KvSpan {
+  int lowest, highest, all_low, all_high;
+};
+__device__ __forceinline__ KvSpan kv_span_of(const KvAttendArgs &a, const KvRows &r, int first, int rows) {
+  const int from = r.position(first / a.group), to = r.position((first + rows - 1) / a.group);
+  KvSpan s;
+  s.highest = a.causal ? min(to, r.last_key) : r.last_key;
+  s.all_high = a.causal ? min(from, r.last_key) : r.last_key;
+  s.lowest = a.window != 0 ? max(from - a.window + 1, 0) : 0;
+  s.all_low = a.window != 0 ? max(to - a.window + 1, 0) : 0;
+  return s;
+}
+
+__device__ __forceinline__ int kv_page_at(const KvAttendArgs &a, const int32_t *table, int key) {  // -1: not there
+  const int column = key >> a.cache.page_shift;
+  const int page = column < a.table_width ? table[column] : -1;
+  return page < a.cache.pages ? page : -1;
+}
+
+// One row a lane (n = lane & 15; the four lanes of a row have a quarter of its dimensions each).
+struct KvRow {
+  int token, head, low, high;  // token -1: none
+};
+__device__ __forceinline__ KvRow kv_row_of(const KvAttendArgs &a, const KvRows &r, int kv_head, int row, bool there) {
+  const int i = row / a.group;
+  KvRow k;
+  k.token = there ? r.start + i : -1;
+  k.head = kv_head * a.group + row - i * a.group;
+  const int position = r.position(i);
+  k.high = there ? (a.causal ? min(position, r.last_key) : r.last_key) : -1;
+  k.low = a.window != 0 ? max(position - a.window + 1, 0) : 0;
+  return k;
+}
+
+template <int D>
+__device__ __forceinline__ void kv_load_query(const KvAttendArgs &a, const KvRow &row, int g, float (&y)[D / 4]) {
+  if (row.token >= 0) {
+    const int64_t at = row.token * a.q_token_stride + row.head * a.q_head_stride + g * (D / 4);
+    if (a.q_wide && a.q_dtype != OQ_F32) {
+#pragma unroll
+      for (int i = 0; i < D / 4; i += 8) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[i + e] = dyn_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu, a.q_dtype);
+      }
+    } else if (a.q_wide) {
+#pragma unroll
+      for (int i = 0; i < D / 4; i += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + i);
+        y[i] = v.x; y[i + 1] = v.y; y[i + 2] = v.z; y[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) y[i] = load_dyn_f32(a.q, a.q_dtype, at + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) y[i] = 0.0f;
+  }
+}
+
+// Rotates a row's quarter; gives the largest magnitude of the row.
+template <int D>
+__device__ __forceinline__ float kv_rotate_query(const KvAttendArgs &a, int g, float (&y)[D / 4]) {
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i) y[i] *= static_cast<float>(a.cache.signs[g * (D / 4) + i]);
+  kv_rotate_lane<D>(y);
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(y[i]));
+  return kv_over_groups(top, kv_max_of);
+}
+
+// The power of two 2^-exponent puts `top` into [2^10, 2^11).
+__device__ __forceinline__ int kv_query_exponent(float top) {
+  return top > 0.0f && top < INFINITY ? min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10, -110), 117) : 0;
+}
+__device__ __forceinline__ float kv_power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+template <int D, int SPLIT>
+__device__ __forceinline__ void kv_query_parts(const float (&y)[D / 4], float down, kv_f16x8 (&q)[D / 32], kv_f16x8 (&rest)[SPLIT > 0 ? D / 32 : 1]) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = y[8 * c + e] * down;
+      q[c][e] = static_cast<_Float16>(v);
+      if constexpr (SPLIT > 0) rest[c][e] = static_cast<_Float16>(v - static_cast<float>(q[c][e]));
     }
   }
 }
 
-__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// Scores become weights, for one tile of sixteen rows and the sixteen keys of a lane.
+struct KvState {
+  float ref, sum;
+  float limit;  // of a score above R: kKvNothing until the row has seen a key, so that the first one sets R
+  __device__ __forceinline__ void begin() { ref = 0.0f; sum = 0.0f; limit = kKvNothing; }
+  __device__ __forceinline__ float reference() const { return limit < 0.0f ? kKvNothing : ref; }
+};
 
-template <int D, int RT, int SPLIT>
-__global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvAttendArgs a) {
-  constexpr int C = D / 32;                 // matrix instructions along the dimensions
-  constexpr int W = D / 32;                 // dwords of codes a lane has of a key
-  constexpr int kOutRegs = RT * (D / 4);
-  __shared__ float join[2][kOutRegs + 2 * RT][64];
+// x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.
+template <int D>
+__device__ __forceinline__ void kv_keep_in_range(float (&x)[16], float top_exponent, KvState &st, kv_f32x4 (&o)[D / 16]) {
+  float best = fmaxf(x[0], x[1]);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) best = fmaxf(best, fmaxf(x[i], x[i + 1]));
+  best += top_exponent;
+  if (__builtin_amdgcn_ballot_w64(best > st.limit) != 0) {
+    best = kv_over_groups(best, kv_max_of);
+    const bool raise = best > st.limit;
+    const float up = raise ? best - 10.0f : 0.0f, by = kv_exp2(fminf(-up, 0.0f));  // (down only where nothing is summed up yet)
+    st.ref += up;
+    st.sum *= by;
+    st.limit = raise ? 15.0f : st.limit;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[j] *= by;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] -= up;
+  }
+}
+
+// Weights as the B operand: entries of tiles 2 * half and 2 * half + 1 side by side.
+template <int SPLIT>
+__device__ __forceinline__ void kv_weights(const float (&x)[16], const float (&vs)[16], float &sum, kv_f16x8 (&p)[2], kv_f16x8 (&rest)[SPLIT > 1 ? 2 : 1]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = 8 * half + 4 * k + r, at = 2 * r + k;
+        const float e = kv_exp2(x[i]);
+        sum += e;
+        const float w = e * vs[i];
+        p[half][at] = static_cast<_Float16>(w);
+        if constexpr (SPLIT > 1) rest[half][at] = static_cast<_Float16>(w - static_cast<float>(p[half][at]));
+      }
+    }
+  }
+}
+
+// Keys that a row does not see, or that are not there.  A weight of 0 does not undo a scale that is NaN: where a value's is, the
+// rows that see it get theirs through the score; what lies behind the last key may be anything.
+__device__ __forceinline__ float kv_masked_score(float x, float vs, int key, bool there, const KvRow &row) {
+  const bool seen = there && key <= row.high && key >= row.low;
+  return seen ? (vs != vs ? NAN : x) : -INFINITY;
+}
+
+__device__ __forceinline__ float kv_exponent_above(const float (&vs)[16]) {  // every scale is below 2^this
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(vs[i]));
+  return static_cast<float>(min(max(static_cast<int>(top >> 23) - 126, -80), 80));
+}
+
+// Sixteen token bytes of two dimensions -> the A operands of the even and the odd one, tiles 2 * half and 2 * half + 1 side by side.
+__device__ __forceinline__ void kv_decode_values(uint32_t x, uint32_t y, kv_f16x8 &even, kv_f16x8 &odd) {
+  even = kv_decode8((x & 0x0f0f0f0fu) | ((y & 0x0f0f0f0fu) << 4));
+  odd = kv_decode8(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u));
+}
+
+// A row's result: rotated back, and stored as the output, or as a part of it.
+template <int D>
+__device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &row, int g, int part, const KvState &st, const kv_f32x4 (&o)[D / 16]) {
+  const float l = kv_over_groups(st.sum, kv_sum_of);
+  const bool parts = a.parts > 1;
+  const float by = parts ? 1.0f / D : l != 0.0f ? (1.0f / D) / l : 0.0f;  // (no key: zeros)
+  // dimension 32 j + 8 g + 2 r + parity is in o[2 j + parity][r]
+  float y[D / 4];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y[8 * j + 2 * r] = o[2 * j][r] * by;
+      y[8 * j + 2 * r + 1] = o[2 * j + 1][r] * by;
+    }
+  }
+  kv_rotate_lane<D>(y);
+  if (row.token < 0) return;
+  const int64_t index = static_cast<int64_t>(row.token) * a.heads + row.head;
+  const int64_t in_parts = static_cast<int64_t>(part) * a.tokens * a.heads + index;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    const uint2 sign = *reinterpret_cast<const uint2 *>(a.cache.signs + 32 * j + 8 * g);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(__float_as_uint(y[8 * j + e]) ^ (((e < 4 ? sign.x : sign.y) << (24 - 8 * (e & 3))) & 0x80000000u));
+    const int at = 32 * j + 8 * g;
+    if (parts || a.q_dtype == OQ_F32) {
+      float *to = parts ? a.part_out + in_parts * D + at : static_cast<float *>(a.out) + index * D + at;
+      reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = a.q_dtype == OQ_F16 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
+                                   : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
+      }
+      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + index * D + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  if (g != 0) return;
+  if (parts) a.part_stats[in_parts] = make_float2(st.reference(), l);
+  else if (a.lse != nullptr) a.lse[index] = l != 0.0f ? (st.ref + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------
+// Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS.  A step's
+// keys, scales and values (8.4 KB at D = 128) are requested a step ahead into the registers of the ones just used.
+template <int D, int SPLIT>
+__global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
+  constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
+  __shared__ float join[2][D / 4 + 2][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int kv_head = blockIdx.x % a.cache.heads, part = blockIdx.y;  // neighbours in the grid: heads of the same rows
-  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x / a.cache.heads);  // a prompt's last rows see the most keys: they begin first
+  const int kv_head = blockIdx.x % a.cache.heads, part = blockIdx.y;
+  const int tile = blockIdx.x / a.cache.heads;
 
-  // which rows
-  int request, first_row, rows, start, length, fresh;
-  if (a.starts == nullptr) {
-    const int each = (a.group + kv_tile_rows<RT>() - 1) / kv_tile_rows<RT>();
-    request = tile / each;
-    first_row = (tile - request * each) * kv_tile_rows<RT>();
-    start = request;
-    fresh = 1;
-  } else {
-    const int tokens = static_cast<int>(a.tokens);
-    const auto start_of = [&](int r) { return min(max(a.starts[r], 0), tokens); };
-    int low = 0, high = a.requests + 1;     // the rows behind the last request's are a request of their own, without keys
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (kv_tile_base(static_cast<int64_t>(start_of(mid)) * a.group, mid, kv_tile_rows<RT>()) <= tile) low = mid; else high = mid;
-    }
-    request = low;
-    start = start_of(request);
-    fresh = max((request < a.requests ? start_of(request + 1) : tokens) - start, 0);
-    const int64_t ahead = tile - kv_tile_base(static_cast<int64_t>(start) * a.group, request, kv_tile_rows<RT>());
-    first_row = static_cast<int>(min(ahead * kv_tile_rows<RT>(), static_cast<int64_t>(0x7fffffff)));
+  KvRows r;
+  r.request = tile / a.few_tiles;
+  r.first = (tile - r.request * a.few_tiles) * 16;
+  r.start = r.request;
+  r.fresh = 1;
+  if (a.starts != nullptr) {
+    r.start = kv_start_of(a, r.request);
+    r.fresh = max(kv_start_of(a, r.request + 1) - r.start, 0);
+    if (static_cast<int64_t>(r.fresh) * a.group > kKvFewRows) return;
   }
-  if (first_row >= static_cast<int64_t>(fresh) * a.group) return;
-  rows = min(static_cast<int>(min(static_cast<int64_t>(fresh) * a.group - first_row, static_cast<int64_t>(kv_tile_rows<RT>()))), kv_tile_rows<RT>());
-  length = request < a.requests ? max(a.lengths[request], 0) : 0;
-  const int64_t reach = static_cast<int64_t>(a.table_width) << a.cache.page_shift;  // what lies behind the table is not there
-  const int last_key = static_cast<int>(min(static_cast<int64_t>(length), reach)) - 1;
-
-  // rows and keys of this wavefront
-  const int sets = (rows + 16 * RT - 1) / (16 * RT);        // of RT tiles
-  const int sharing = sets == 1 ? 4 : sets == 2 ? 2 : 1;    // wavefronts on the same rows
-  const int set = wave / sharing, rank = wave - set * sharing;
-  int token[RT], head[RT], low[RT], high[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int in_tile = (set * RT + t) * 16 + n, row = first_row + in_tile;
-    const int i = row / a.group;
-    token[t] = in_tile < rows ? start + i : -1;
-    head[t] = kv_head * a.group + row - i * a.group;
-    const int position = length - fresh + i;
-    high[t] = in_tile < rows ? (a.causal ? min(position, last_key) : last_key) : -1;
-    low[t] = a.window != 0 ? max(position - a.window + 1, 0) : 0;
-  }
-  const int first_i = first_row / a.group, last_i = (first_row + rows - 1) / a.group;
-  const int highest = a.causal ? min(length - fresh + last_i, last_key) : last_key;
-  const int lowest = a.window != 0 ? max(length - fresh + first_i - a.window + 1, 0) : 0;
-  // every row of the tile sees the keys in between
-  const int all_high = a.causal ? min(length - fresh + first_i, last_key) : last_key;
-  const int all_low = a.window != 0 ? max(length - fresh + last_i - a.window + 1, 0) : 0;
-  int step = (lowest >> 6) + part * a.part_steps;
-  int end = highest >= lowest ? (highest >> 6) + 1 : 0;
+  r.rows = min(r.fresh * a.group - r.first, 16);
+  if (r.rows <= 0) return;
+  kv_keys_of(a, r);
+  const KvSpan span = kv_span_of(a, r, r.first, r.rows);
+  int step = (span.lowest >> 6) + part * a.part_steps;
+  int end = span.highest >= span.lowest ? (span.highest >> 6) + 1 : 0;
   if (part + 1 < a.parts) end = min(end, step + a.part_steps);
-
-  // queries, rotated, as the B operand
-  kv_f16x8 q[RT][C], q_rest[SPLIT > 0 ? RT : 1][C];
-  float factor[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    float y[D / 4];
-    if (token[t] >= 0) {
-      const int64_t at = token[t] * a.q_token_stride + head[t] * a.q_head_stride + g * (D / 4);
-      if (a.q_wide && a.q_dtype != OQ_F32) {
-#pragma unroll
-        for (int i = 0; i < D / 4; i += 8) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at + i);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[i + e] = dyn_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu, a.q_dtype);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i) y[i] = load_dyn_f32(a.q, a.q_dtype, at + i);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) y[i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) y[i] *= static_cast<float>(a.cache.signs[g * (D / 4) + i]);
-    kv_rotate_lane<D>(y, lane);
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(y[i]));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // a power of two that puts the largest entry into [2^10, 2^11)
-    const int exponent = top > 0.0f && top < INFINITY ? min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10, -110), 117) : 0;
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
-    factor[t] = a.scale * (1.44269504088896f / D) * __uint_as_float(static_cast<uint32_t>(127 + exponent) << 23);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = y[8 * c + e] * down;
-        q[t][c][e] = static_cast<_Float16>(v);
-        if constexpr (SPLIT > 0) q_rest[t][c][e] = static_cast<_Float16>(v - static_cast<float>(q[t][c][e]));
-      }
-    }
-  }
-
-  kv_f32x4 o[RT][D / 16];
-  float sum[RT], ref[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    sum[t] = 0.0f;
-    ref[t] = kKvNothing;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) o[t][j] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  step += wave;
 
   const int shift = a.cache.page_shift;
-  const int32_t *table = a.table + request * a.table_stride;
-  const auto page_at = [&](int key) {  // -1: not there
-    const int column = key >> shift;
-    const int page = column < a.table_width ? table[column] : -1;
-    return page < a.cache.pages ? page : -1;
-  };
+  const int32_t *table = a.table + r.request * a.table_stride;
   uint32_t k_raw[4][W];
   uint4 v_raw[D / 32], k_scale[2], v_scale[2];
   const auto load_keys = [&](int s, int page) {
@@ -232,248 +392,354 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvAttendArgs a) {
     v_scale[0] = v_from[0]; v_scale[1] = v_from[1];
   };
 
-  if (set < sets) {
-    step += rank;
-    int page_k = -1, page_v = -1, next_k = -1, next_v = -1;
-    if (step < end) {
-      page_k = page_at(step * 64 + 16 * (n >> 2));
-      page_v = page_at(step * 64 + 16 * g);
-      load_keys(step, page_k);
-      load_scales(step, page_v);
-      load_values(step, page_v);
-      next_k = page_at((step + sharing) * 64 + 16 * (n >> 2));
-      next_v = page_at((step + sharing) * 64 + 16 * g);
-    }
-    for (; step < end; step += sharing) {
-      const int ahead = min(step + sharing, end - 1);  // (the last step asks for itself or an earlier one again)
-      const bool more = step + sharing < end;
-      // scores
-      kv_f32x4 s[RT][4];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[t][k] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const kv_f16x8 codes = kv_decode8(k_raw[k][c]);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            if constexpr (SPLIT > 0) s[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[t][c], s[t][k], 0, 0, 0);
-            s[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[t][c], s[t][k], 0, 0, 0);
-          }
-        }
-      }
-      float ks[16], vs[16];
-      uint32_t top_scale = 0;
-      {
-        const uint32_t kw[8] = {k_scale[0].x, k_scale[0].y, k_scale[0].z, k_scale[0].w, k_scale[1].x, k_scale[1].y, k_scale[1].z, k_scale[1].w};
-        const uint32_t vw[8] = {v_scale[0].x, v_scale[0].y, v_scale[0].z, v_scale[0].w, v_scale[1].x, v_scale[1].y, v_scale[1].z, v_scale[1].w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ks[2 * i] = __uint_as_float(kw[i] << 16);
-          ks[2 * i + 1] = __uint_as_float(kw[i] & 0xffff0000u);
-          vs[2 * i] = __uint_as_float(vw[i] << 16);
-          vs[2 * i + 1] = __uint_as_float(vw[i] & 0xffff0000u);
-        }
-      }
-      const int here_v = page_v;
-      if (more) {
-        load_keys(ahead, next_k);
-        load_scales(ahead, next_v);
-      }
-      // masks: only where the step has keys that some row does not see, or that are not there
-      const int first = step * 64;
-      const bool masked = first + 63 > all_high || first < all_low || __builtin_amdgcn_ballot_w64(here_v < 0) != 0;
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = first + 16 * g + i;
-          const bool there = key <= last_key && here_v >= 0;
-          // A weight of 0 does not undo a scale that is NaN.  Where a value's is, the rows that see it get theirs through the
-          // score; what lies behind the last key may be anything.
-          const bool broken = vs[i] != vs[i];
-          if (broken || !there) vs[i] = 0.0f;
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const bool seen = there && key <= high[t] && key >= low[t];
-            const float score = broken ? NAN : s[t][i >> 2][i & 3] * (ks[i] * factor[t]);
-            s[t][i >> 2][i & 3] = seen ? score : -INFINITY;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i >> 2][i & 3] *= ks[i] * factor[t];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top_scale = max(top_scale, __float_as_uint(vs[i]));
-      const float top_exponent = static_cast<float>(min(max(static_cast<int>(top_scale >> 23) - 126, -80), 80));  // b_t < 2^this
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        float best = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          best = fmaxf(best, s[t][i >> 2][i & 3]);
-        }
-        best += top_exponent;
-        if (__builtin_amdgcn_ballot_w64(best - ref[t] > 15.0f) != 0) {
-          best = fmaxf(best, __shfl_xor(best, 16, 64));
-          best = fmaxf(best, __shfl_xor(best, 32, 64));
-          const float to = fmaxf(ref[t], best - 10.0f), by = kv_exp2(ref[t] - to);
-          ref[t] = to;
-          sum[t] *= by;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) o[t][j] *= by;
-        }
-      }
-      kv_f16x8 p[RT][2], p_rest[SPLIT > 1 ? RT : 1][2];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = kv_exp2(s[t][i >> 2][i & 3] - ref[t]);
-          sum[t] += e;
-          const float w = e * vs[i];
-          const int half = i >> 3, at = 2 * (i & 3) + ((i >> 2) & 1);  // tiles 2 * half and 2 * half + 1 side by side
-          p[t][half][at] = static_cast<_Float16>(w);
-          if constexpr (SPLIT > 1) p_rest[t][half][at] = static_cast<_Float16>(w - static_cast<float>(p[t][half][at]));
-        }
-      }
-      // outputs
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint32_t w[4] = {v_raw[j].x, v_raw[j].y, v_raw[j].z, v_raw[j].w};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t x = w[2 * half], y = w[2 * half + 1];
-          const kv_f16x8 even = kv_decode8((x & 0x0f0f0f0fu) | ((y & 0x0f0f0f0fu) << 4));
-          const kv_f16x8 odd = kv_decode8(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u));
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            if constexpr (SPLIT > 1) {
-              o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p_rest[t][half], o[t][2 * j], 0, 0, 0);
-              o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p_rest[t][half], o[t][2 * j + 1], 0, 0, 0);
-            }
-            o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[t][half], o[t][2 * j], 0, 0, 0);
-            o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[t][half], o[t][2 * j + 1], 0, 0, 0);
-          }
-        }
-      }
-      if (more) load_values(ahead, next_v);
-      page_v = next_v;
-      next_k = page_at((step + 2 * sharing) * 64 + 16 * (n >> 2));
-      next_v = page_at((step + 2 * sharing) * 64 + 16 * g);
-    }
+  // the first step is on its way while the queries are rotated
+  int page_v = -1, next_k = -1, next_v = -1;
+  if (step < end) {
+    const int page_k = kv_page_at(a, table, step * 64 + 16 * (n >> 2));
+    page_v = kv_page_at(a, table, step * 64 + 16 * g);
+    next_k = kv_page_at(a, table, (step + 4) * 64 + 16 * (n >> 2));
+    next_v = kv_page_at(a, table, (step + 4) * 64 + 16 * g);
+    load_keys(step, page_k);
+    load_scales(step, page_v);
+    load_values(step, page_v);
   }
 
-  // the wavefronts that shared the keys: neighbours first, then the two pairs, in this order
-  const auto give = [&](int place) {
+  const KvRow row = kv_row_of(a, r, kv_head, r.first + n, n < r.rows);
+  kv_f16x8 q[W], q_rest[SPLIT > 0 ? W : 1];
+  float factor;
+  {
+    float y[D / 4];
+    kv_load_query<D>(a, row, g, y);
+    const int exponent = kv_query_exponent(kv_rotate_query<D>(a, g, y));
+    factor = a.scale * (1.44269504088896f / D) * kv_power_of_two(exponent);
+    kv_query_parts<D, SPLIT>(y, kv_power_of_two(-exponent), q, q_rest);
+  }
+
+  KvState st;
+  st.begin();
+  kv_f32x4 o[D / 16];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      join[place][2 * t][lane] = ref[t];
-      join[place][2 * t + 1][lane] = sum[t];
+  for (int j = 0; j < D / 16; ++j) o[j] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (; step < end; step += 4) {
+    const bool more = step + 4 < end;
+    float x[16], vs[16];
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
+    for (int k = 0; k < 4; ++k) {
+      kv_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) join[place][2 * RT + (t * (D / 16) + j) * 4 + r][lane] = o[t][j][r];
+      for (int c = 0; c < W; ++c) {
+        const kv_f16x8 codes = kv_decode8(k_raw[k][c]);
+        if constexpr (SPLIT > 0) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[c], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[c], s, 0, 0, 0);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * k + i] = s[i];
+    }
+    {
+      const uint32_t kw[8] = {k_scale[0].x, k_scale[0].y, k_scale[0].z, k_scale[0].w, k_scale[1].x, k_scale[1].y, k_scale[1].z, k_scale[1].w};
+      const uint32_t vw[8] = {v_scale[0].x, v_scale[0].y, v_scale[0].z, v_scale[0].w, v_scale[1].x, v_scale[1].y, v_scale[1].z, v_scale[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[2 * i] = fmaf(x[2 * i], __uint_as_float(kw[i] << 16) * factor, -st.ref);
+        x[2 * i + 1] = fmaf(x[2 * i + 1], __uint_as_float(kw[i] & 0xffff0000u) * factor, -st.ref);
+        vs[2 * i] = __uint_as_float(vw[i] << 16);
+        vs[2 * i + 1] = __uint_as_float(vw[i] & 0xffff0000u);
+      }
+    }
+    const bool here = page_v >= 0;
+    if (more) {
+      load_keys(step + 4, next_k);
+      load_scales(step + 4, next_v);
+    }
+    const int first = step * 64;
+    if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = first + 16 * g + i;
+        const bool there = here && key <= r.last_key;
+        x[i] = kv_masked_score(x[i], vs[i], key, there, row);
+        vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
+      }
+    }
+    kv_keep_in_range<D>(x, kv_exponent_above(vs), st, o);
+    kv_f16x8 p[2], p_rest[SPLIT > 1 ? 2 : 1];
+    kv_weights<SPLIT>(x, vs, st.sum, p, p_rest);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint32_t w[4] = {v_raw[j].x, v_raw[j].y, v_raw[j].z, v_raw[j].w};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        kv_f16x8 even, odd;
+        kv_decode_values(w[2 * half], w[2 * half + 1], even, odd);
+        if constexpr (SPLIT > 1) {
+          o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p_rest[half], o[2 * j], 0, 0, 0);
+          o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p_rest[half], o[2 * j + 1], 0, 0, 0);
+        }
+        o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[half], o[2 * j], 0, 0, 0);
+        o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[half], o[2 * j + 1], 0, 0, 0);
+      }
+    }
+    if (more) load_values(step + 4, next_v);
+    page_v = next_v;
+    next_k = kv_page_at(a, table, (step + 8) * 64 + 16 * (n >> 2));
+    next_v = kv_page_at(a, table, (step + 8) * 64 + 16 * g);
+  }
+  st.ref = st.reference();
+
+  // the four wavefronts: neighbours first, then the two pairs, in this order
+  const auto give = [&](int place) {
+    join[place][0][lane] = st.ref;
+    join[place][1][lane] = st.sum;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) join[place][2 + 4 * j + i][lane] = o[j][i];
     }
   };
   const auto take = [&](int place) {
+    const float theirs = join[place][0][lane], both = fmaxf(st.ref, theirs);
+    const float mine = kv_exp2(st.ref - both), other = kv_exp2(theirs - both);
+    st.ref = both;
+    st.sum = st.sum * mine + join[place][1][lane] * other;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const float theirs = join[place][2 * t][lane], both = fmaxf(ref[t], theirs);
-      const float mine = kv_exp2(ref[t] - both), other = kv_exp2(theirs - both);
-      ref[t] = both;
-      sum[t] = sum[t] * mine + join[place][2 * t + 1][lane] * other;
+    for (int j = 0; j < D / 16; ++j) {
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[t][j][r] = o[t][j][r] * mine + join[place][2 * RT + (t * (D / 16) + j) * 4 + r][lane] * other;
-      }
+      for (int i = 0; i < 4; ++i) o[j][i] = o[j][i] * mine + join[place][2 + 4 * j + i][lane] * other;
     }
   };
-  if (sharing > 1) {
-    if (rank & 1) give(wave >> 1);
-    __syncthreads();
-    if ((rank & 1) == 0) take(wave >> 1);
-    if (sharing == 4) {
-      __syncthreads();
-      if (rank == 2) give(1);
-      __syncthreads();
-      if (rank == 0) take(1);
-    }
-  }
-  if (rank != 0 || set >= sets) return;
-
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    float l = sum[t];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    const float by = l != 0.0f ? (1.0f / D) / l : 0.0f;  // (no key: zeros)
-    // dimension 32 j + 8 g + 2 r + parity is in o[2 j + parity][r]
-    float y[D / 4];
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        y[8 * j + 2 * r] = o[t][2 * j][r] * by;
-        y[8 * j + 2 * r + 1] = o[t][2 * j + 1][r] * by;
-      }
-    }
-    kv_rotate_lane<D>(y, lane);  // (its order of the dimensions over lanes and registers does not matter: every pair of bits takes part once)
-    if (token[t] < 0) continue;
-    const int64_t row = static_cast<int64_t>(token[t]) * a.heads + head[t];
-    const float log_sum = l != 0.0f ? (ref[t] + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
-    if (a.parts > 1) {
-      const int64_t at = static_cast<int64_t>(part) * a.tokens * a.heads + row;
-      float *to = a.part_out + at * D + 8 * g;
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint2 sign = *reinterpret_cast<const uint2 *>(a.cache.signs + 32 * j + 8 * g);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = ((e < 4 ? sign.x : sign.y) >> (8 * (e & 3) + 7)) & 1 ? -y[8 * j + e] : y[8 * j + e];
-        reinterpret_cast<float4 *>(to + 32 * j)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(to + 32 * j)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
-      if (g == 0) a.part_lse[at] = log_sum;
-      continue;
-    }
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const uint2 sign = *reinterpret_cast<const uint2 *>(a.cache.signs + 32 * j + 8 * g);
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = ((e < 4 ? sign.x : sign.y) >> (8 * (e & 3) + 7)) & 1 ? -y[8 * j + e] : y[8 * j + e];
-      const int64_t at = row * D + 32 * j + 8 * g;
-      if (a.q_dtype == OQ_F32) {
-        reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = a.q_dtype == OQ_F16 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
-                                     : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
-        }
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-    if (a.lse != nullptr && g == 0) a.lse[row] = log_sum;
-  }
+  if (wave & 1) give(wave >> 1);
+  __syncthreads();
+  if ((wave & 1) == 0) take(wave >> 1);
+  __syncthreads();
+  if (wave == 2) give(1);
+  __syncthreads();
+  if (wave != 0) return;
+  take(1);
+  st.limit = 1.0f;  // (what R says is all there is to know now)
+  kv_finish<D>(a, row, g, part, st, o);
 }
 
-template <int D, int RT, int SPLIT>
-void kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
-  launch_kernel(kv_attend_kernel<D, RT, SPLIT>, dim3(static_cast<unsigned>(a.cache.heads) * a.tiles, static_cast<unsigned>(a.parts)), dim3(256), 0,
-                stream, a);
+// ---- many rows -----------------------------------------------------------------------------------------------------
+// 128 rows a workgroup, 16 * RT a wavefront, all on the same keys.  Decoding a step costs as many vector instructions as the softmax
+// of 32 rows: each wavefront decodes a part of it into LDS, in the order of the operands (conflict-free on both sides), for the next step while
+// this one's products run; one barrier a step.
+template <int D>
+constexpr int kv_many_waves() { return D == 256 ? 8 : 4; }
+
+template <int D, int SPLIT>
+__global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_kernel(KvAttendArgs a) {
+  constexpr int WAVES = kv_many_waves<D>(), RT = kKvManyRows / 16 / WAVES;
+  constexpr int C = D / 32;
+  constexpr int KD = D * 2 / (16 * WAVES), VD = KD;  // dwords of a step's keys and values that a lane decodes
+  struct Step {
+    kv_f16x8 k[4][C][64];         // [tile][dimensions][lane]
+    kv_f16x8 v[D / 32][2][2][64]; // [dimensions][half of the keys][even, odd][lane]
+    float ks[64], vs[64];         // times the scale of the scores; as it is
+  };
+  extern __shared__ char lds[];
+  Step *steps = reinterpret_cast<Step *>(lds);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int kv_head = blockIdx.x % a.cache.heads, part = blockIdx.y;
+  const int tile = a.many_tiles - 1 - static_cast<int>(blockIdx.x / a.cache.heads);  // a prompt's last rows see the most keys: they begin first
+
+  KvRows r;
+  {
+    int low = 0, high = a.requests + 1;
+    while (high - low > 1) {
+      const int mid = (low + high) >> 1;
+      if (kv_tile_base(static_cast<int64_t>(kv_start_of(a, mid)) * a.group, mid) <= tile) low = mid; else high = mid;
+    }
+    r.request = low;
+    r.start = kv_start_of(a, low);
+    r.fresh = max(kv_start_of(a, low + 1) - r.start, 0);
+    const int64_t first = (tile - kv_tile_base(static_cast<int64_t>(r.start) * a.group, low)) * kKvManyRows, all = static_cast<int64_t>(r.fresh) * a.group;
+    if (first >= all || all <= a.few_rows) return;
+    r.first = static_cast<int>(first);
+    r.rows = static_cast<int>(min(all - first, static_cast<int64_t>(kKvManyRows)));
+  }
+  kv_keys_of(a, r);
+  const KvSpan span = kv_span_of(a, r, r.first, r.rows);
+  int step = (span.lowest >> 6) + part * a.part_steps;
+  int end = span.highest >= span.lowest ? (span.highest >> 6) + 1 : 0;
+  if (part + 1 < a.parts) end = min(end, step + a.part_steps);
+
+  // what this wavefront decodes: keys of one tile, all or half of their dimensions; values of one j, both halves of the keys or one
+  const int shift = a.cache.page_shift;
+  const int32_t *table = a.table + r.request * a.table_stride;
+  const int k_tile = WAVES == 8 ? wave >> 1 : wave, k_from = WAVES == 8 ? (wave & 1) * KD : 0;
+  const int v_j = VD == 2 ? wave >> 1 : wave, v_from = VD == 2 ? wave & 1 : 0;
+  uint32_t k_raw[KD], v_raw[VD], scale_raw = 0;
+  const auto load = [&](int s, int page_k, int page_v) {
+    const int64_t k_block = static_cast<int64_t>(max(page_k, 0)) * a.cache.heads + kv_head, v_block = static_cast<int64_t>(max(page_v, 0)) * a.cache.heads + kv_head;
+    const int in_page = (1 << shift) - 1;
+    const uint32_t *k_at = reinterpret_cast<const uint32_t *>(a.cache.k_codes) +
+                           ((k_block << shift) + ((s * 64 + 16 * (n >> 2)) & in_page) + 4 * k_tile + (n & 3)) * (D / 8) + g * (D / 32) + k_from;
+    const uint8_t *v_at = a.cache.v_codes + ((v_block * (D / 2) + 16 * v_j + n) << shift) + ((s * 64 + 16 * g) & in_page) + 8 * v_from;
+    if constexpr (KD == 2) {
+      const uint2 k = *reinterpret_cast<const uint2 *>(k_at), v = *reinterpret_cast<const uint2 *>(v_at);
+      k_raw[0] = k.x; k_raw[1] = k.y; v_raw[0] = v.x; v_raw[1] = v.y;
+    } else {
+      const uint4 k = *reinterpret_cast<const uint4 *>(k_at), v = *reinterpret_cast<const uint4 *>(v_at);
+      k_raw[0] = k.x; k_raw[1] = k.y; k_raw[2] = k.z; k_raw[3] = k.w; v_raw[0] = v.x; v_raw[1] = v.y; v_raw[2] = v.z; v_raw[3] = v.w;
+    }
+    if (wave < 2) scale_raw = (wave == 0 ? a.cache.k_scales : a.cache.v_scales)[(v_block << shift) + ((s * 64 + 16 * g) & in_page) + n];
+  };
+  int page_v = -1, next_k = -1, next_v = -1, later_k = -1, later_v = -1;  // of the step that is computed (v: whether its keys are there), requested, and after it
+  if (step < end) {
+    const int page_k = kv_page_at(a, table, step * 64 + 16 * (n >> 2));
+    page_v = kv_page_at(a, table, step * 64 + 16 * g);
+    next_k = kv_page_at(a, table, (step + 1) * 64 + 16 * (n >> 2));
+    next_v = kv_page_at(a, table, (step + 1) * 64 + 16 * g);
+    load(step, page_k, page_v);
+  }
+
+  KvRow row[RT];
+  kv_f16x8 q[RT][C], q_rest[RT][SPLIT > 0 ? C : 1];
+  float factor;
+  {
+    float y[RT][D / 4], top = 0.0f;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int at = (wave * RT + t) * 16 + n;
+      row[t] = kv_row_of(a, r, kv_head, r.first + at, at < r.rows);
+      kv_load_query<D>(a, row[t], g, y[t]);
+      const float own_top = kv_rotate_query<D>(a, g, y[t]);
+      top = own_top < INFINITY ? fmaxf(top, own_top) : top;  // (a broken row is its own affair)
+    }
+    // one power of two for the workgroup's rows: its factor goes into the keys' scales
+#pragma unroll
+    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+    float *tops = steps[1].ks;  // (the first step decodes into steps[0])
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
+    const int exponent = kv_query_exponent(top);
+    factor = a.scale * (1.44269504088896f / D) * kv_power_of_two(exponent);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) kv_query_parts<D, SPLIT>(y[t], kv_power_of_two(-exponent), q[t], q_rest[t]);
+  }
+  const int wave_first = wave * RT * 16, wave_rows = min(r.rows - wave_first, RT * 16);  // rows of this wavefront, if any
+  const KvSpan own = kv_span_of(a, r, r.first + min(wave_first, r.rows - 1), max(wave_rows, 1));
+
+  const auto decode = [&](Step &to) {
+#pragma unroll
+    for (int i = 0; i < KD; ++i) to.k[k_tile][k_from + i][lane] = kv_decode8(k_raw[i]);
+#pragma unroll
+    for (int i = 0; i < VD / 2; ++i) {
+      kv_f16x8 even, odd;
+      kv_decode_values(v_raw[2 * i], v_raw[2 * i + 1], even, odd);
+      to.v[v_j][v_from + i][0][lane] = even;
+      to.v[v_j][v_from + i][1][lane] = odd;
+    }
+    const float scale = __uint_as_float(scale_raw << 16);  // of key 16 * g + n: lane
+    if (wave == 0) to.ks[lane] = scale * factor;
+    else if (wave == 1) to.vs[lane] = scale;
+  };
+
+  KvState st[RT];
+  kv_f32x4 o[RT][D / 16];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    st[t].begin();
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[t][j] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  if (step < end) {
+    decode(steps[0]);
+    if (step + 1 < end) load(step + 1, next_k, next_v);
+    later_k = kv_page_at(a, table, (step + 2) * 64 + 16 * (n >> 2));
+    later_v = kv_page_at(a, table, (step + 2) * 64 + 16 * g);
+  }
+  for (int now = 0; step < end; ++step, now ^= 1) {
+    __syncthreads();  // this step is decoded, and nobody reads the one before it any more
+    const Step &from = steps[now];
+    const bool here = page_v >= 0;
+    if (step + 1 < end) {
+      decode(steps[now ^ 1]);
+      if (step + 2 < end) load(step + 2, later_k, later_v);
+    }
+    page_v = next_v; next_k = later_k; next_v = later_v;
+    later_k = kv_page_at(a, table, (step + 3) * 64 + 16 * (n >> 2));
+    later_v = kv_page_at(a, table, (step + 3) * 64 + 16 * g);
+    const int first = step * 64;
+    if (wave_rows <= 0 || first > own.highest || first + 63 < own.lowest) continue;
+
+    float x[RT][16], vs[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      kv_f32x4 s[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const kv_f16x8 codes = from.k[k][c][lane];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if constexpr (SPLIT > 0) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[t][c], s[t], 0, 0, 0);
+          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[t][c], s[t], 0, 0, 0);
+        }
+      }
+      const kv_f32x4 ks = *reinterpret_cast<const kv_f32x4 *>(&from.ks[16 * g + 4 * k]), v = *reinterpret_cast<const kv_f32x4 *>(&from.vs[16 * g + 4 * k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vs[4 * k + i] = v[i];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) x[t][4 * k + i] = fmaf(s[t][i], ks[i], -st[t].ref);
+      }
+    }
+    if (first + 63 > own.all_high || first < own.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = first + 16 * g + i;
+        const bool there = here && key <= r.last_key;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) x[t][i] = kv_masked_score(x[t][i], vs[i], key, there, row[t]);
+        vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
+      }
+    }
+    const float top_exponent = kv_exponent_above(vs);
+    kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      kv_keep_in_range<D>(x[t], top_exponent, st[t], o[t]);
+      kv_weights<SPLIT>(x[t], vs, st[t].sum, p[t], p_rest[t]);
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const kv_f16x8 even = from.v[j][half][0][lane], odd = from.v[j][half][1][lane];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if constexpr (SPLIT > 1) {
+            o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p_rest[t][half], o[t][2 * j], 0, 0, 0);
+            o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p_rest[t][half], o[t][2 * j + 1], 0, 0, 0);
+          }
+          o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[t][half], o[t][2 * j], 0, 0, 0);
+          o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[t][half], o[t][2 * j + 1], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) kv_finish<D>(a, row[t], g, part, st[t], o[t]);
+}
+
+template <int D>
+constexpr size_t kv_many_lds() { return 2 * (4 * (D / 32) * 64 * 16 + (D / 32) * 4 * 64 * 16 + 512); }
+
+template <int D, int SPLIT>
+bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
+  const unsigned heads = static_cast<unsigned>(a.cache.heads), parts = static_cast<unsigned>(a.parts);
+  if (a.many_tiles > 0) {
+    if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kv_attend_many_kernel<D, SPLIT>), kv_many_lds<D>())) return false;
+    launch_kernel(kv_attend_many_kernel<D, SPLIT>, dim3(heads * a.many_tiles, parts), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
+  }
+  if (a.few_requests > 0) launch_kernel(kv_attend_few_kernel<D, SPLIT>, dim3(heads * a.few_requests * a.few_tiles, parts), dim3(256), 0, stream, a);
+  return true;
 }
 
 }  // namespace oq

@@ -42,17 +42,20 @@ struct KvAttendArgs {
   int table_width, window;            // window: 0 for none
   bool causal;
   float scale;
-  int tiles, parts, part_steps;       // tiles of rows, parts of the keys, steps of 64 keys in a part
+  // How the work is cut: tiles of the kernel for many rows (0: not launched); requests (0 likewise) and tiles of each for the one for
+  // few; the rows of a request up to which the latter has it; parts of the keys, and steps of 64 keys in one.
+  int many_tiles, few_requests, few_tiles, few_rows, parts, part_steps;
   void *out;
   float *lse;                         // NULL or [tokens, heads]
-  float *part_out, *part_lse;         // [parts, tokens, heads, D] and [parts, tokens, heads], where parts > 1
+  float *part_out;                    // where parts > 1: [parts, tokens, heads, D], and of each row R and l
+  float2 *part_stats;
 };
 
 int kv_assign_dispatch(const KvAssignArgs &a, hipStream_t stream);
 int kv_write_dispatch(const KvWriteArgs &a, int dim, int dtype, hipStream_t stream);
 int kv_read_dispatch(const KvReadArgs &a, int dim, int dtype, hipStream_t stream);
-// Sets tiles, parts and part_steps; the bytes of part_out and part_lse that they need (0: none).
+// Cuts the work; the bytes of part_out and part_stats (0: none).
 uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new);
-int kv_attend_dispatch(KvAttendArgs &a, int dim, int64_t max_new, hipStream_t stream);
+int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream);
 
 }  // namespace oq
