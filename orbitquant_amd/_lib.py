@@ -135,7 +135,7 @@ def load() -> ctypes.CDLL:
 
 def _bind(lib: ctypes.CDLL) -> None:
     names = ("oq_quantized_linear", "oq_quantized_linear_group", "oq_packed_linear_workspace_bytes", "oq_rotate_plan_bytes",
-             "oq_matmul_packed_adaln_int4")
+             "oq_matmul_packed_adaln_int4", "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes")
     _torch_ops.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names})
 
 

@@ -6,7 +6,8 @@
 hipcc cross-compiles for gfx950 without a GPU.  The rotate+quantize kernel and
 what writes and reads the key/value cache are
 built without FMA contraction (their results must match the CPU statement of the
-algorithm bit for bit); packed fp32 VALU instructions are disabled everywhere.
+algorithm bit for bit), and so is the attention over it (contracted into the conversion, a product and its
+rounding to fp16 are not what the remainder in a second fp16 is taken from); packed fp32 VALU instructions are disabled everywhere.
 
     python -m orbitquant_amd.build --variant stamps --flags=-DOQ_GEMM_STAMPS --only packed_gemm.hip
 
@@ -61,9 +62,9 @@ SOURCES = {
     "token_linear_w4.hip": [],
     "kv_cache.hip": ["-ffp-contract=off"],
     "kv_attend.hip": [],
-    "kv_attend_d64.hip": [],
-    "kv_attend_d128.hip": [],
-    "kv_attend_d256.hip": [],
+    "kv_attend_d64.hip": ["-ffp-contract=off"],
+    "kv_attend_d128.hip": ["-ffp-contract=off"],
+    "kv_attend_d256.hip": ["-ffp-contract=off"],
 }
 
 

@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
@@ -28,6 +29,11 @@ struct Library {
   decltype(&oq_packed_linear_workspace_bytes) workspace_bytes = nullptr;
   decltype(&oq_rotate_plan_bytes) plan_bytes = nullptr;
   decltype(&oq_matmul_packed_adaln_int4) adaln = nullptr;
+  decltype(&oq_kv_assign) kv_assign = nullptr;
+  decltype(&oq_kv_write) kv_write = nullptr;
+  decltype(&oq_kv_read) kv_read = nullptr;
+  decltype(&oq_kv_attend) kv_attend = nullptr;
+  decltype(&oq_kv_attend_workspace_bytes) kv_attend_workspace_bytes = nullptr;
 } lib;
 
 int dtype_code(at::ScalarType t) {
@@ -259,6 +265,143 @@ pybind11::object quantized_linear_group(const Tensor &x, const Tensor &permutati
   return pybind11::cast(outs);
 }
 
+// ---- the 4-bit key/value cache: `kv_cache.py`'s functions for the usual call; None or False: the Python side ----
+
+// The address of a tensor of this type that lies densely on `device`.
+bool dense(const Tensor &t, const at::Device &device, at::ScalarType type) {
+  return t.defined() && t.device() == device && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous() && !faked(t);
+}
+
+bool cache_usable(const pybind11::handle &cache, const at::Device &device, oq_kv_cache &c) {
+  if (!PyTuple_Check(cache.ptr()) || PyTuple_GET_SIZE(cache.ptr()) != 5) return false;
+  const Tensor *t[5];
+  for (int i = 0; i < 5; ++i) {
+    PyObject *item = PyTuple_GET_ITEM(cache.ptr(), i);
+    if (!THPVariable_Check(item)) return false;
+    t[i] = &THPVariable_Unpack(item);
+  }
+  const Tensor &k = *t[0], &ks = *t[1], &v = *t[2], &vs = *t[3], &signs = *t[4];
+  if (!dense(k, device, at::kByte) || k.dim() != 4 || !dense(ks, device, at::kBFloat16) || !dense(v, device, at::kByte) || !dense(vs, device, at::kBFloat16) ||
+      !dense(signs, device, at::kChar))
+    return false;
+  const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), half = k.size(3);
+  const int64_t scales[3] = {pages, heads, page}, values[4] = {pages, heads, half, page};
+  if (!ks.sizes().equals(scales) || !vs.sizes().equals(scales) || !v.sizes().equals(values) || signs.dim() != 1 || signs.size(0) != 2 * half) return false;
+  c.k_codes = static_cast<uint8_t *>(data(k));
+  c.k_scales = static_cast<uint16_t *>(data(ks));
+  c.v_codes = static_cast<uint8_t *>(data(v));
+  c.v_scales = static_cast<uint16_t *>(data(vs));
+  c.signs = static_cast<const int8_t *>(data(signs));
+  c.pages = pages;
+  c.kv_heads = heads;
+  c.page_size = page;
+  c.head_dim = 2 * half;
+  return true;
+}
+
+// [tokens, heads, D] whose last dimension is contiguous, on a GPU.
+bool rows_usable(const Tensor &x, int64_t dim) {
+  return x.defined() && x.device().is_cuda() && x.layout() == at::kStrided && x.dim() == 3 && x.size(0) > 0 && x.size(2) == dim && x.stride(2) == 1 &&
+         dtype_code(x.scalar_type()) >= 0 && !faked(x) && !x.is_conj() && !x.is_neg();
+}
+
+bool table_usable(const Tensor &t, const at::Device &device, int64_t requests) {
+  return t.defined() && t.device() == device && t.scalar_type() == at::kInt && t.layout() == at::kStrided && t.dim() == 2 && t.size(0) == requests &&
+         t.size(1) > 0 && t.stride(1) == 1 && (requests == 1 || t.stride(0) >= t.size(1)) && !faked(t);
+}
+
+void *stream_of(const at::Device &device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+
+// A tensor over part of another's memory.
+Tensor part_of(const Tensor &buffer, at::ScalarType type, int64_t byte, at::IntArrayRef sizes) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), caffe2::TypeMeta::fromScalarType(type));
+  impl->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
+  impl->set_sizes_contiguous(sizes);
+  return Tensor(std::move(impl));
+}
+
+pybind11::object kv_assign(const Tensor &lengths, const Tensor &new_lengths, const Tensor &table, const Tensor &free_pages, const Tensor &taken,
+                           int64_t page_size, int64_t tokens) {
+  if (lib.kv_assign == nullptr || !lengths.defined() || !lengths.device().is_cuda() || tokens < 0 || tokens > 0x7fffffff) return pybind11::none();
+  const at::Device device = lengths.device();
+  const int64_t requests = lengths.numel();
+  if (requests < 1 || !dense(lengths, device, at::kInt) || !dense(new_lengths, device, at::kInt) || new_lengths.numel() != requests ||
+      !dense(free_pages, device, at::kInt) || !dense(taken, device, at::kInt) || taken.numel() != 1 || !table_usable(table, device, requests))
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(device);
+  const Tensor buffer = at::empty({8 * tokens + 4 * (tokens + 2 * requests + 2)}, lengths.options().dtype(at::kByte));
+  if (faked(buffer)) return pybind11::none();
+  char *at = static_cast<char *>(buffer.data_ptr());
+  const int64_t positions = 8 * tokens, starts = positions + 4 * tokens, after = starts + 4 * (requests + 1), taken_after = after + 4 * requests;
+  const auto i32 = [&](int64_t byte) { return reinterpret_cast<int32_t *>(at + byte); };
+  const int rc = lib.kv_assign(static_cast<const int32_t *>(data(lengths)), static_cast<const int32_t *>(data(new_lengths)), requests,
+                               static_cast<int32_t *>(data(table)), table.stride(0), table.size(1), static_cast<const int32_t *>(data(free_pages)),
+                               free_pages.numel(), static_cast<const int32_t *>(data(taken)), page_size, tokens, reinterpret_cast<int64_t *>(at),
+                               i32(positions), i32(starts), i32(after), i32(taken_after), stream_of(device));
+  if (rc != OQ_OK) return pybind11::none();
+  return pybind11::make_tuple(part_of(buffer, at::kLong, 0, {tokens}), part_of(buffer, at::kInt, positions, {tokens}),
+                              part_of(buffer, at::kInt, starts, {requests + 1}), part_of(buffer, at::kInt, after, {requests}),
+                              part_of(buffer, at::kInt, taken_after, {1}));
+}
+
+bool kv_write(const Tensor &k, const Tensor &v, const Tensor &slots, const pybind11::object &cache) {
+  oq_kv_cache c;
+  if (lib.kv_write == nullptr || !k.defined() || !k.device().is_cuda() || !cache_usable(cache, k.device(), c)) return false;
+  const at::Device device = k.device();
+  if (!rows_usable(k, c.head_dim) || !rows_usable(v, c.head_dim) || k.size(1) != c.kv_heads || v.size(1) != c.kv_heads || v.size(0) != k.size(0) ||
+      v.device() != device || v.scalar_type() != k.scalar_type() || !dense(slots, device, at::kLong) || slots.numel() != k.size(0))
+    return false;
+  const c10::OptionalDeviceGuard guard(device);
+  return lib.kv_write(data(k), k.stride(0), k.stride(1), data(v), v.stride(0), v.stride(1), dtype_code(k.scalar_type()),
+                      static_cast<const int64_t *>(data(slots)), k.size(0), &c, stream_of(device)) == OQ_OK;
+}
+
+pybind11::object kv_read(const Tensor &slots, const pybind11::object &cache, const pybind11::object &dtype) {
+  oq_kv_cache c;
+  if (lib.kv_read == nullptr || !THPDtype_Check(dtype.ptr()) || !slots.defined() || !slots.device().is_cuda() || !dense(slots, slots.device(), at::kLong) ||
+      !cache_usable(cache, slots.device(), c))
+    return pybind11::none();
+  const at::ScalarType type = reinterpret_cast<THPDtype *>(dtype.ptr())->scalar_type;
+  const int code = dtype_code(type);
+  const int64_t tokens = slots.numel();
+  if (code < 0 || tokens < 1) return pybind11::none();
+  const c10::OptionalDeviceGuard guard(slots.device());
+  const Tensor k = at::empty({tokens, c.kv_heads, c.head_dim}, slots.options().dtype(type)), v = at::empty_like(k);
+  if (faked(k) || faked(v)) return pybind11::none();
+  const int rc = lib.kv_read(static_cast<const int64_t *>(data(slots)), tokens, &c, data(k), data(v), code, stream_of(slots.device()));
+  return rc == OQ_OK ? pybind11::object(pybind11::make_tuple(k, v)) : pybind11::object(pybind11::none());
+}
+
+pybind11::object kv_attend(const Tensor &q, const pybind11::object &cache, const Tensor &table, const Tensor &lengths, const OptTensor &starts,
+                           int64_t max_new, int64_t max_length, bool causal, int64_t window, double scale, bool want_lse) {
+  oq_kv_cache c;
+  if (lib.kv_attend == nullptr || !q.defined() || !q.device().is_cuda() || !cache_usable(cache, q.device(), c) || !rows_usable(q, c.head_dim))
+    return pybind11::none();
+  const at::Device device = q.device();
+  const int64_t tokens = q.size(0), heads = q.size(1), requests = lengths.defined() ? lengths.numel() : 0;
+  if (requests < 1 || heads < 1 || heads % c.kv_heads != 0 || !dense(lengths, device, at::kInt) || !table_usable(table, device, requests) ||
+      (present(starts) ? !dense(*starts, device, at::kInt) || starts->numel() != requests + 1 : requests != tokens))
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(device);
+  try {
+    const Tensor out = at::empty(q.sizes(), q.options());
+    const Tensor lse = want_lse ? at::empty({tokens, heads}, q.options().dtype(at::kFloat)) : Tensor();
+    const uint64_t need = lib.kv_attend_workspace_bytes(tokens, heads, c.kv_heads, c.head_dim, c.page_size, table.size(1), requests, present(starts), window,
+                                                        max_length, max_new);
+    const Tensor workspace = need > 0 ? bytes_like(q, static_cast<int64_t>(need)) : Tensor();
+    if (faked(out)) return pybind11::none();
+    const int rc = lib.kv_attend(data(q), dtype_code(q.scalar_type()), tokens, heads, q.stride(0), q.stride(1), &c, static_cast<const int32_t *>(data(table)),
+                                 table.stride(0), table.size(1), static_cast<const int32_t *>(data(lengths)), static_cast<const int32_t *>(data(starts)),
+                                 requests, causal, window, static_cast<float>(scale), max_length, max_new, data(out),
+                                 want_lse ? static_cast<float *>(data(lse)) : nullptr, need > 0 ? data(workspace) : nullptr, need, stream_of(device));
+    if (rc != OQ_OK) return pybind11::none();
+    if (want_lse) return pybind11::make_tuple(out, lse);
+    return pybind11::cast(out);
+  } catch (const c10::OutOfMemoryError &) {  // the Python side knows what a call can do without
+  }
+  return pybind11::none();
+}
+
 template <typename F>
 void bind_one(F &entry, const pybind11::dict &addresses, const char *name) {
   entry = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
@@ -278,6 +421,15 @@ PYBIND11_MODULE(_torch_ops, m) {
     bind_one(lib.plan_bytes, addresses, "oq_rotate_plan_bytes");
     bind_one(lib.adaln, addresses, "oq_matmul_packed_adaln_int4");
     bind_one(lib.quantized_linear, addresses, "oq_quantized_linear");
+    bind_one(lib.kv_assign, addresses, "oq_kv_assign");
+    bind_one(lib.kv_write, addresses, "oq_kv_write");
+    bind_one(lib.kv_read, addresses, "oq_kv_read");
+    bind_one(lib.kv_attend, addresses, "oq_kv_attend");
+    bind_one(lib.kv_attend_workspace_bytes, addresses, "oq_kv_attend_workspace_bytes");
   });
   m.def("quantized_linear_group", quantized_linear_group);
+  m.def("kv_assign", kv_assign);
+  m.def("kv_write", kv_write);
+  m.def("kv_read", kv_read);
+  m.def("kv_attend", kv_attend);
 }

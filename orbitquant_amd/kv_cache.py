@@ -13,7 +13,6 @@ Queries are rotated by the attention itself, and its outputs back: what goes in 
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple
 
 import torch
@@ -78,6 +77,15 @@ class KVAssignment(NamedTuple):
     taken: torch.Tensor
 
 
+def _module():
+    """The compiled module (csrc/torch_ops.cpp), which has the usual calls of these functions without Python in between (a cached
+    token's slot 13.5 -> MODULE_US us); None where it is not built.  What it does not take, errors among it, it leaves to the Python below."""
+    module = _lib.torch_ops()
+    if module is None:
+        _lib.warn_without_torch_ops()
+    return module
+
+
 def _cache_struct(cache, like: torch.Tensor) -> _lib.KvCacheStruct:
     """The cache as the library takes it.  Its tensors are written to, so none is ever copied: what is not contiguous is refused."""
     k_codes, k_scales, v_codes, v_scales, signs = cache
@@ -121,6 +129,11 @@ def kv_assign(lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: tor
     `kv_attend` does not see.  `tokens`: the number of new tokens, as the caller's arrays have them; what `new_lengths` leaves of
     it gets slot and position -1.  lengths, new_lengths int32 [requests], block_table int32 [requests, width] (changed in
     place), free_pages int32 [any], taken int32 [1]."""
+    module = _module()
+    if module is not None:
+        got = module.kv_assign(lengths, new_lengths, block_table, free_pages, taken, int(page_size), int(tokens))
+        if got is not None:
+            return KVAssignment._make(got)
     _require_gpu(lengths, "lengths")
     requests = lengths.numel()
     lengths = _operand(lengths, "lengths", lengths, dtype=torch.int32)
@@ -148,6 +161,9 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Orbit
     """Keys and values [tokens, heads, D] into the cache at `slots` int64 [tokens] (`oq_kv_write`).  Slots that are negative or
     beyond the last page are skipped; no slot may occur twice.  k and v: one floating type, any strides whose last is 1 (parts of
     a fused projection's output need no copy)."""
+    module = _module()
+    if module is not None and module.kv_write(k, v, slots, cache):
+        return
     _require_gpu(k, "k")
     struct = _cache_struct(cache, k)
     heads, dim = struct.kv_heads, struct.head_dim
@@ -164,6 +180,11 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Orbit
 def kv_read(slots: torch.Tensor, cache: OrbitKVCache, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """What the cache holds at `slots` int64 [tokens], as keys and values [tokens, heads, D] of `dtype` (`oq_kv_read`); zeros for
     slots that are negative or beyond the last page."""
+    module = _module()
+    if module is not None:
+        got = module.kv_read(slots, cache, dtype)
+        if got is not None:
+            return got
     _require_gpu(slots, "slots")
     struct = _cache_struct(cache, slots)
     slots = _operand(slots, "slots", slots, dtype=torch.int64)
@@ -194,6 +215,17 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
 
     A query that sees no token, and a token behind the last request's, gets zeros (lse -inf).  Accumulation, scores and softmax
     are fp32; queries and weights enter the matrix units as fp16 (as two fp16 parts of float32 queries)."""
+    if window is not None and (window < 1 or not causal):
+        raise ValueError("a window is at least 1 and needs causal attention")
+    window = 0 if window is None else int(window)
+    max_length = -1 if max_length is None else int(max_length)
+    max_new = -1 if max_new is None else int(max_new)
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    module = _module()
+    if module is not None:
+        got = module.kv_attend(q, cache, block_table, lengths, starts, max_new, max_length, bool(causal), window, scale, bool(return_lse))
+        if got is not None:
+            return got
     _require_gpu(q, "q")
     struct = _cache_struct(cache, q)
     q = _rows(q, "q", None, struct.head_dim)
@@ -206,11 +238,6 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
     if starts is None and requests != tokens:
         raise ValueError(f"{tokens} queries for {requests} requests: starts is needed")
     table = _table(block_table, q, requests)
-    if window is not None and (window < 1 or not causal):
-        raise ValueError("a window is at least 1 and needs causal attention")
-    window = 0 if window is None else int(window)
-    max_length = -1 if max_length is None else int(max_length)
-    max_new = -1 if max_new is None else int(max_new)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
     lib = _lib.load()
@@ -219,8 +246,7 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
     workspace, nbytes, _keep = _workspace(needed, q, lambda: (0,))
     with _OnDevice(q):
         rc = lib.oq_kv_attend(q.data_ptr(), _dt(q), tokens, heads, q.stride(0), q.stride(1), ctypes.byref(struct), table.data_ptr(),
-                              table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(starts), requests, bool(causal), window,
-                              float(1.0 / math.sqrt(dim) if scale is None else scale), max_length, max_new, out.data_ptr(), _ptr(lse),
+                              table.stride(0), table.shape[1], lengths.data_ptr(), _ptr(starts), requests, bool(causal), window, scale, max_length, max_new, out.data_ptr(), _ptr(lse),
                               workspace, nbytes, _stream(q))
     _lib.check(rc, "oq_kv_attend")
     return out if lse is None else (out, lse)
