@@ -607,7 +607,7 @@ bool vectors_wide(const void *p, int64_t token_stride, int64_t head_stride, int 
   return aligned(p, 16) && token_stride % per == 0 && head_stride % per == 0;
 }
 
-// A launch of eight values a lane, 256 lanes a workgroup, over keys and values.
+// A launch of a workgroup for every head of sixteen tokens.
 int kv_vectors_fit(const char *what, int64_t tokens, const oq_kv_cache *c) {
   if (tokens < 0) return fail(OQ_ERR_INVALID, "%s: tokens=%lld", what, (long long)tokens);
   if (tokens > (1LL << 40) || tokens * c->kv_heads > (1LL << 32)) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld exceed the grid", what, (long long)tokens);

@@ -38,7 +38,6 @@
 namespace oq {
 
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
 constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
@@ -48,21 +47,6 @@ constexpr int kKvManyRows = 128;        // rows of a workgroup of the second
 __host__ __device__ inline int64_t kv_tile_base(int64_t row, int64_t r) { return row / kKvManyRows + r; }
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// The butterflies between lanes X apart (16 or 32), two registers at a time: a swap of lane groups puts the two operands of
-// every result into one lane, and a second one the results back.
-template <int X>
-__device__ __forceinline__ void kv_lane_butterfly(float &a, float &b) {
-  const auto swap = [](float x, float y) -> kv_u32x2 {
-    if constexpr (X == 16) return __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
-    else return __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
-  };
-  const kv_u32x2 in = swap(a, b);
-  const float x = __uint_as_float(in[0]), y = __uint_as_float(in[1]);
-  const kv_u32x2 out = swap(x + y, x - y);
-  a = __uint_as_float(out[0]);
-  b = __uint_as_float(out[1]);
-}
 
 // D / 4 values a lane.  Every pair of dimensions that differ in one bit meets once: which bits are registers and which lanes
 // does not matter.
@@ -88,9 +72,9 @@ __device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4]) {
 // Over the four lanes that hold a row (lane & 15 the same).
 template <typename Op>
 __device__ __forceinline__ float kv_over_groups(float x, Op op) {
-  const kv_u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const kv_u32x2 a = kv_swap<16>(__float_as_uint(x), __float_as_uint(x));
   x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const kv_u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const kv_u32x2 b = kv_swap<32>(__float_as_uint(x), __float_as_uint(x));
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float kv_max_of(float a, float b) { return fmaxf(a, b); }
@@ -345,12 +329,65 @@ __device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &ro
   else if (a.lse != nullptr) a.lse[index] = l != 0.0f ? (st.ref + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
 }
 
+// A step's keys, scales and values as they come from the cache, for a wavefront that decodes all of them.
+template <int D>
+struct KvRaw {
+  uint32_t k[4][D / 32];
+  uint4 v[D / 32], k_scale[2], v_scale[2];
+  bool here;  // the page of the lane's sixteen keys is there
+};
+struct KvPages {  // of key rows (n >> 2) and of values and scales (g)
+  int k, v;
+};
+__device__ __forceinline__ KvPages kv_pages_of(const KvAttendArgs &a, const int32_t *table, int n, int g, int step) {
+  return {kv_page_at(a, table, step * 64 + 16 * (n >> 2)), kv_page_at(a, table, step * 64 + 16 * g)};
+}
+template <int D>
+__device__ __forceinline__ void kv_request_keys(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
+  constexpr int W = D / 32;
+  const int shift = a.cache.page_shift, in_page = (1 << shift) - 1;
+  const int64_t k_block = static_cast<int64_t>(max(page.k, 0)) * a.cache.heads + kv_head, v_block = static_cast<int64_t>(max(page.v, 0)) * a.cache.heads + kv_head;
+  const uint32_t *from = reinterpret_cast<const uint32_t *>(a.cache.k_codes) + ((k_block << shift) + ((s * 64 + 16 * (n >> 2)) & in_page) + (n & 3)) * (D / 8) + g * W;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (W == 2) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(from + 4 * t * (D / 8));
+      to.k[t][0] = v.x; to.k[t][1] = v.y;
+    } else {
+#pragma unroll
+      for (int w = 0; w < W; w += 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(from + 4 * t * (D / 8) + w);
+        to.k[t][w] = v.x; to.k[t][w + 1] = v.y; to.k[t][w + 2] = v.z; to.k[t][w + 3] = v.w;
+      }
+    }
+  }
+  const int64_t scales = (v_block << shift) + ((s * 64 + 16 * g) & in_page);
+  const uint4 *k_from = reinterpret_cast<const uint4 *>(a.cache.k_scales + scales), *v_from = reinterpret_cast<const uint4 *>(a.cache.v_scales + scales);
+  to.k_scale[0] = k_from[0]; to.k_scale[1] = k_from[1];
+  to.v_scale[0] = v_from[0]; to.v_scale[1] = v_from[1];
+  to.here = page.v >= 0;
+}
+template <int D>
+__device__ __forceinline__ void kv_request_values(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
+  const int shift = a.cache.page_shift;
+  const int64_t block = static_cast<int64_t>(max(page.v, 0)) * a.cache.heads + kv_head;
+  const uint8_t *from = a.cache.v_codes + ((block * (D / 2) + n) << shift) + ((s * 64 + 16 * g) & ((1 << shift) - 1));
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) to.v[j] = *reinterpret_cast<const uint4 *>(from + (static_cast<int64_t>(16 * j) << shift));
+}
+template <int D>
+__device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
+  kv_request_keys<D>(a, kv_head, n, g, s, page, to);
+  kv_request_values<D>(a, kv_head, n, g, s, page, to);
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS.  A step's
-// keys, scales and values (8.4 KB at D = 128) are requested a step ahead into the registers of the ones just used.
+// keys, scales and values (8.4 KB at D = 128) are requested DEPTH of the wavefront's steps ahead, into the registers of the ones just used.
 template <int D, int SPLIT>
 __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
+  constexpr int DEPTH = D == 256 ? 1 : 2;  // (of heads of 256 two steps do not fit the registers)
   __shared__ float join[2][D / 4 + 2][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -376,55 +413,16 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   if (part + 1 < a.parts) end = min(end, step + a.part_steps);
   step += wave;
 
-  const int shift = a.cache.page_shift;
   const int32_t *table = a.table + r.request * a.table_stride;
-  uint32_t k_raw[4][W];
-  uint4 v_raw[D / 32], k_scale[2], v_scale[2];
-  const auto load_keys = [&](int s, int page) {
-    const int64_t block = static_cast<int64_t>(max(page, 0)) * a.cache.heads + kv_head;
-    const int place = (s * 64 + 16 * (n >> 2)) & ((1 << shift) - 1);
-    const uint32_t *from = reinterpret_cast<const uint32_t *>(a.cache.k_codes) + ((block << shift) + place + (n & 3)) * (D / 8) + g * W;
+  KvRaw<D> raw[DEPTH];
+  KvPages pages[DEPTH];  // of the steps that are requested next
+  // the first steps are on their way while the queries are rotated
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if constexpr (W == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(from + 4 * t * (D / 8));
-        k_raw[t][0] = v.x; k_raw[t][1] = v.y;
-      } else {
-#pragma unroll
-        for (int w = 0; w < W; w += 4) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(from + 4 * t * (D / 8) + w);
-          k_raw[t][w] = v.x; k_raw[t][w + 1] = v.y; k_raw[t][w + 2] = v.z; k_raw[t][w + 3] = v.w;
-        }
-      }
-    }
-  };
-  const auto load_values = [&](int s, int page) {
-    const int64_t block = static_cast<int64_t>(max(page, 0)) * a.cache.heads + kv_head;
-    const int place = (s * 64 + 16 * g) & ((1 << shift) - 1);
-    const uint8_t *from = a.cache.v_codes + ((block * (D / 2) + n) << shift) + place;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) v_raw[j] = *reinterpret_cast<const uint4 *>(from + (static_cast<int64_t>(16 * j) << shift));
-  };
-  const auto load_scales = [&](int s, int page) {
-    const int64_t block = static_cast<int64_t>(max(page, 0)) * a.cache.heads + kv_head;
-    const int place = (s * 64 + 16 * g) & ((1 << shift) - 1);
-    const uint4 *k_from = reinterpret_cast<const uint4 *>(a.cache.k_scales + (block << shift) + place);
-    const uint4 *v_from = reinterpret_cast<const uint4 *>(a.cache.v_scales + (block << shift) + place);
-    k_scale[0] = k_from[0]; k_scale[1] = k_from[1];
-    v_scale[0] = v_from[0]; v_scale[1] = v_from[1];
-  };
-
-  // the first step is on its way while the queries are rotated
-  int page_v = -1, next_k = -1, next_v = -1;
-  if (step < end) {
-    const int page_k = kv_page_at(a, table, step * 64 + 16 * (n >> 2));
-    page_v = kv_page_at(a, table, step * 64 + 16 * g);
-    next_k = kv_page_at(a, table, (step + 4) * 64 + 16 * (n >> 2));
-    next_v = kv_page_at(a, table, (step + 4) * 64 + 16 * g);
-    load_keys(step, page_k);
-    load_scales(step, page_v);
-    load_values(step, page_v);
+  for (int i = 0; i < DEPTH; ++i) {
+    if (step + 4 * i < end) kv_request<D>(a, kv_head, n, g, step + 4 * i, kv_pages_of(a, table, n, g, step + 4 * i), raw[i]);
   }
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) pages[i] = kv_pages_of(a, table, n, g, step + 4 * (DEPTH + i));
 
   const KvRow row = kv_row_of(a, r, kv_head, r.first + n, n < r.rows);
   kv_f16x8 q[W], q_rest[SPLIT > 0 ? W : 1];
@@ -443,24 +441,24 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) o[j] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  for (; step < end; step += 4) {
-    const bool more = step + 4 < end;
+  const auto take_step = [&](int s, KvRaw<D> &now, KvPages &next) {
+    const bool more = s + 4 * DEPTH < end;
     float x[16], vs[16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      kv_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+      kv_f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < W; ++c) {
-        const kv_f16x8 codes = kv_decode8(k_raw[k][c]);
-        if constexpr (SPLIT > 0) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[c], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[c], s, 0, 0, 0);
+        const kv_f16x8 codes = kv_decode8(now.k[k][c]);
+        if constexpr (SPLIT > 0) score = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[c], score, 0, 0, 0);
+        score = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[c], score, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * k + i] = s[i];
+      for (int i = 0; i < 4; ++i) x[4 * k + i] = score[i];
     }
     {
-      const uint32_t kw[8] = {k_scale[0].x, k_scale[0].y, k_scale[0].z, k_scale[0].w, k_scale[1].x, k_scale[1].y, k_scale[1].z, k_scale[1].w};
-      const uint32_t vw[8] = {v_scale[0].x, v_scale[0].y, v_scale[0].z, v_scale[0].w, v_scale[1].x, v_scale[1].y, v_scale[1].z, v_scale[1].w};
+      const uint32_t kw[8] = {now.k_scale[0].x, now.k_scale[0].y, now.k_scale[0].z, now.k_scale[0].w, now.k_scale[1].x, now.k_scale[1].y, now.k_scale[1].z, now.k_scale[1].w};
+      const uint32_t vw[8] = {now.v_scale[0].x, now.v_scale[0].y, now.v_scale[0].z, now.v_scale[0].w, now.v_scale[1].x, now.v_scale[1].y, now.v_scale[1].z, now.v_scale[1].w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[2 * i] = fmaf(x[2 * i], __uint_as_float(kw[i] << 16) * factor, -st.ref);
@@ -469,12 +467,9 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
         vs[2 * i + 1] = __uint_as_float(vw[i] & 0xffff0000u);
       }
     }
-    const bool here = page_v >= 0;
-    if (more) {
-      load_keys(step + 4, next_k);
-      load_scales(step + 4, next_v);
-    }
-    const int first = step * 64;
+    const bool here = now.here;
+    if (more) kv_request_keys<D>(a, kv_head, n, g, s + 4 * DEPTH, next, now);
+    const int first = s * 64;
     if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -489,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
     kv_weights<SPLIT>(x, vs, st.sum, p, p_rest);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      const uint32_t w[4] = {v_raw[j].x, v_raw[j].y, v_raw[j].z, v_raw[j].w};
+      const uint32_t w[4] = {now.v[j].x, now.v[j].y, now.v[j].z, now.v[j].w};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         kv_f16x8 even, odd;
@@ -502,10 +497,14 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
         o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[half], o[2 * j + 1], 0, 0, 0);
       }
     }
-    if (more) load_values(step + 4, next_v);
-    page_v = next_v;
-    next_k = kv_page_at(a, table, (step + 8) * 64 + 16 * (n >> 2));
-    next_v = kv_page_at(a, table, (step + 8) * 64 + 16 * g);
+    if (more) kv_request_values<D>(a, kv_head, n, g, s + 4 * DEPTH, next, now);
+    next = kv_pages_of(a, table, n, g, s + 8 * DEPTH);
+  };
+  for (; step < end; step += 4 * DEPTH) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      if (step + 4 * i < end) take_step(step + 4 * i, raw[i], pages[i]);
+    }
   }
   st.ref = st.reference();
 

@@ -102,7 +102,12 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 }
 
 // ---- into the cache and back -----------------------------------------------------------------------------------------
-// Eight values a lane, so a vector is D / 8 lanes and a wavefront holds 512 / D of them.
+// Both are bound by bytes: a workgroup takes one head of sixteen tokens, its lanes eight values each, keys and values all requested at
+// once.  A token's key is D / 2 bytes in a row, but its value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen
+// tokens change places in LDS, and four tokens whose slots follow each other in a page (a prompt's, nearly always) are one dword of
+// a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write and read 31.6 us together; with one byte a store and lanes exchanged through LDS 52.
+constexpr int kKvGroup = 16;  // tokens of a workgroup
+
 template <int DT>
 __device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float (&y)[8]) {
   if (wide) {
@@ -139,80 +144,139 @@ __device__ __forceinline__ void store8(void *p, int64_t at, const float (&y)[8])
 }
 
 template <int D>
-__device__ __forceinline__ void times_signs(float (&y)[8], const int8_t *signs, int part) {
+__device__ __forceinline__ void times_signs(float (&y)[8], uint2 signs) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= static_cast<float>(signs[8 * part + i]);
+  for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(__float_as_uint(y[i]) ^ (((i < 4 ? signs.x : signs.y) << (24 - 8 * (i & 3))) & 0x80000000u));
+}
+
+// The slots of the workgroup's tokens, -1 where there is nothing to do.
+__device__ __forceinline__ void group_slots(int64_t (&slots)[kKvGroup], const int64_t *from, int64_t first, int64_t tokens, int64_t most) {
+  if (threadIdx.x < kKvGroup) {
+    int64_t slot = -1;
+    if (first + threadIdx.x < tokens) slot = from[first + threadIdx.x];
+    slots[threadIdx.x] = slot < most ? slot : -1;
+  }
+}
+
+// Whether four tokens' bytes of a row are one dword.
+__device__ __forceinline__ bool in_a_row(const int64_t *slots, int page_shift) {
+  const int64_t s = slots[0];
+  return s >= 0 && slots[1] == s + 1 && slots[2] == s + 2 && slots[3] == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
 }
 
 template <int D, int DT>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs a) {
-  const int lane = threadIdx.x & 63, part = lane & (D / 8 - 1);
-  const int64_t vectors = 2 * a.tokens * a.cache.heads;
-  const int64_t index = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / (D / 8);
-  if (index >= vectors) return;  // (whole vectors)
-  const bool value = index >= vectors / 2;
-  const int64_t rest = value ? index - vectors / 2 : index;
-  const int64_t token = rest / a.cache.heads;
-  const int head = static_cast<int>(rest - token * a.cache.heads);
-  const int64_t slot = a.slots[token];
-  if (slot < 0 || slot >= a.cache.pages << a.cache.page_shift) return;
-  float y[8];
-  if (value) load8<DT>(a.v, token * a.v_token_stride + head * a.v_head_stride + 8 * part, a.v_wide, y);
-  else load8<DT>(a.k, token * a.k_token_stride + head * a.k_head_stride + 8 * part, a.k_wide, y);
-  times_signs<D>(y, a.cache.signs, part);
-  kv_butterflies<D>(y, lane);
-  uint16_t scale;
-  const uint32_t codes = kv_encode<D>(y, scale);
+  constexpr int AT_ONCE = 2048 / D;                // vectors that the workgroup's lanes hold
+  constexpr int PASSES = 2 * kKvGroup / AT_ONCE;   // keys, then values
+  __shared__ int64_t slots[kKvGroup];
+  __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];  // of the values
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D>(lane);
+  const int head = blockIdx.x % a.cache.heads;
+  const int64_t first = static_cast<int64_t>(blockIdx.x / a.cache.heads) * kKvGroup;
   const int shift = a.cache.page_shift;
-  const int64_t block = (slot >> shift) * a.cache.heads + head;  // of one page and head
-  const int64_t place = slot & ((1 << shift) - 1);
-  if (value) {
-    uint8_t *to = a.cache.v_codes + ((block * (D / 2) + 4 * part) << shift) + place;
+  float y[PASSES][8];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) to[static_cast<int64_t>(b) << shift] = static_cast<uint8_t>(codes >> (8 * b));
-    if (part == 0) a.cache.v_scales[(block << shift) + place] = scale;
-  } else {
-    reinterpret_cast<uint32_t *>(a.cache.k_codes)[((block << shift) + place) * (D / 8) + part] = codes;
-    if (part == 0) a.cache.k_scales[(block << shift) + place] = scale;
+  for (int p = 0; p < PASSES; ++p) {
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane);
+    const int64_t token = min(first + (vector & (kKvGroup - 1)), a.tokens - 1);
+    if (vector >= kKvGroup) load8<DT>(a.v, token * a.v_token_stride + head * a.v_head_stride + 8 * part, a.v_wide, y[p]);
+    else load8<DT>(a.k, token * a.k_token_stride + head * a.k_head_stride + 8 * part, a.k_wide, y[p]);
+  }
+  const uint2 signs = reinterpret_cast<const uint2 *>(a.cache.signs)[part];
+  group_slots(slots, a.slots, first, a.tokens, a.cache.pages << shift);
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane), token = vector & (kKvGroup - 1);
+    times_signs<D>(y[p], signs);
+    kv_butterflies<D>(y[p], lane);
+    uint16_t scale;
+    const uint32_t codes = kv_encode<D>(y[p], scale);
+    const int64_t slot = slots[token];
+    const int64_t at = ((((slot >> shift) * a.cache.heads + head) << shift) + (slot & ((1 << shift) - 1)));
+    if (vector >= kKvGroup) {
+      bytes[token][part] = codes;
+      if (slot >= 0 && part == 0) a.cache.v_scales[at] = scale;
+    } else if (slot >= 0) {
+      reinterpret_cast<uint32_t *>(a.cache.k_codes)[at * (D / 8) + part] = codes;
+      if (part == 0) a.cache.k_scales[at] = scale;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (D / 2) * (kKvGroup / 4); i += 256) {
+    const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
+    uint32_t four[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four[k] = reinterpret_cast<const uint8_t *>(bytes[t + k])[row];
+    const auto place = [&](int64_t slot) { return a.cache.v_codes + ((((slot >> shift) * a.cache.heads + head) * (D / 2) + row) << shift) + (slot & ((1 << shift) - 1)); };
+    if (in_a_row(slots + t, shift)) {
+      const uint32_t word = four[0] | four[1] << 8 | four[2] << 16 | four[3] << 24;
+      __builtin_memcpy(place(slots[t]), &word, 4);  // (a page's tokens may begin anywhere)
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (slots[t + k] >= 0) *place(slots[t + k]) = static_cast<uint8_t>(four[k]);
+      }
+    }
   }
 }
 
 template <int D, int DT>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
-  const int lane = threadIdx.x & 63, part = lane & (D / 8 - 1);
-  const int64_t vectors = 2 * a.tokens * a.cache.heads;
-  const int64_t index = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / (D / 8);
-  if (index >= vectors) return;
-  const bool value = index >= vectors / 2;
-  const int64_t rest = value ? index - vectors / 2 : index;
-  const int64_t token = rest / a.cache.heads;
-  const int head = static_cast<int>(rest - token * a.cache.heads);
-  const int64_t slot = a.slots[token];
-  float y[8] = {};
-  if (slot >= 0 && slot < a.cache.pages << a.cache.page_shift) {
-    const int shift = a.cache.page_shift;
-    const int64_t block = (slot >> shift) * a.cache.heads + head;
-    const int64_t place = slot & ((1 << shift) - 1);
-    uint32_t codes = 0;
-    float scale;
-    if (value) {
-      const uint8_t *from = a.cache.v_codes + ((block * (D / 2) + 4 * part) << shift) + place;
+  constexpr int AT_ONCE = 2048 / D, PASSES = 2 * kKvGroup / AT_ONCE;
+  constexpr int ROWS = (D / 2) * (kKvGroup / 4);   // dwords of the values, turned by LDS
+  __shared__ int64_t slots[kKvGroup];
+  __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D>(lane);
+  const int head = blockIdx.x % a.cache.heads;
+  const int64_t first = static_cast<int64_t>(blockIdx.x / a.cache.heads) * kKvGroup;
+  const int shift = a.cache.page_shift;
+  const uint2 signs = reinterpret_cast<const uint2 *>(a.cache.signs)[part];
+  group_slots(slots, a.slots, first, a.tokens, a.cache.pages << shift);
+  __syncthreads();
+  uint32_t keys[PASSES];
+  float scales[PASSES];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) codes |= static_cast<uint32_t>(from[static_cast<int64_t>(b) << shift]) << (8 * b);
-      scale = bf16_bits_to_f32(a.cache.v_scales[(block << shift) + place]);
-    } else {
-      codes = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[((block << shift) + place) * (D / 8) + part];
-      scale = bf16_bits_to_f32(a.cache.k_scales[(block << shift) + place]);
+  for (int p = 0; p < PASSES; ++p) {
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane);
+    const int64_t slot = slots[vector & (kKvGroup - 1)];
+    const int64_t at = ((((slot >> shift) * a.cache.heads + head) << shift) + (slot & ((1 << shift) - 1)));
+    keys[p] = 0;
+    scales[p] = 0.0f;
+    if (slot >= 0) {
+      if (vector < kKvGroup) keys[p] = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[at * (D / 8) + part];
+      scales[p] = bf16_bits_to_f32((vector < kKvGroup ? a.cache.k_scales : a.cache.v_scales)[at]);
     }
-    const kv_f16x8 c = kv_decode8(codes);
+  }
+  for (int i = threadIdx.x; i < ROWS; i += 256) {
+    const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
+    const auto place = [&](int64_t slot) { return a.cache.v_codes + ((((slot >> shift) * a.cache.heads + head) * (D / 2) + row) << shift) + (slot & ((1 << shift) - 1)); };
+    uint32_t word = 0;
+    if (in_a_row(slots + t, shift)) {
+      __builtin_memcpy(&word, place(slots[t]), 4);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(c[i]) * scale;
+      for (int k = 0; k < 4; ++k) {
+        if (slots[t + k] >= 0) word |= static_cast<uint32_t>(*place(slots[t + k])) << (8 * k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) reinterpret_cast<uint8_t *>(bytes[t + k])[row] = static_cast<uint8_t>(word >> (8 * k));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane), token = vector & (kKvGroup - 1);
+    const kv_f16x8 c = kv_decode8(vector < kKvGroup ? keys[p] : bytes[token][part]);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(c[i]) * scales[p];
     kv_butterflies<D>(y, lane);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] *= 1.0f / D;
-    times_signs<D>(y, a.cache.signs, part);
+    times_signs<D>(y, signs);
+    if (first + token < a.tokens) store8<DT>(vector < kKvGroup ? a.k : a.v, ((first + token) * a.cache.heads + head) * D + 8 * part, y);
   }
-  store8<DT>(value ? a.v : a.k, rest * D + 8 * part, y);
 }
 
 template <template <int, int> class Run, typename Args>
@@ -229,16 +293,14 @@ int by_type(const Args &a, int dim, int dtype, hipStream_t stream) {
   return OQ_OK;
 }
 
-inline dim3 vector_grid(int64_t tokens, int heads, int dim) {
-  return dim3(static_cast<unsigned>((2 * tokens * heads * (dim / 8) + 255) / 256));
-}
+inline dim3 group_grid(int64_t tokens, int heads) { return dim3(static_cast<unsigned>((tokens + kKvGroup - 1) / kKvGroup * heads)); }
 template <int D, int DT>
 struct RunWrite {
-  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, vector_grid(a.tokens, a.cache.heads, D), dim3(256), 0, s, a); }
+  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
 };
 template <int D, int DT>
 struct RunRead {
-  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, vector_grid(a.tokens, a.cache.heads, D), dim3(256), 0, s, a); }
+  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
 };
 
 }  // namespace

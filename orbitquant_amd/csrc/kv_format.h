@@ -27,9 +27,55 @@ struct KvCache {
 constexpr int kKvMaxRequests = 8192;  // of one oq_kv_assign: its two running sums and the lengths sit in LDS
 constexpr int kKvMinPage = 16, kKvMaxPage = 1024;
 
-// Eight values of a vector a lane, the vector's D / 8 lanes side by side: element 8 * lane + i.  Butterfly distances 1, 2
-// and 4 are the lane's own registers, the larger ones exchanges with lane ^ (distance / 8).  One add or subtract for each
-// output and stage: the results do not depend on the schedule.
+// Eight values of a vector a lane: element 8 * part + i in lane `part` of the vector's D / 8.  The parts' bits are lane bits
+// whose exchanges are vector instructions: 0 and 1 (quad permutes), 3 (a rotation of the row by eight; heads of 256 only), 4 (heads of 128 and more) and 5 (swaps of
+// lane groups); the other lane bits tell the wavefront's 512 / D vectors apart.
+template <int D>
+__device__ __forceinline__ int kv_part_of(int lane) {
+  if constexpr (D == 64) return (lane & 3) | (lane >> 5) << 2;
+  else if constexpr (D == 128) return (lane & 3) | (lane >> 4) << 2;
+  else return (lane & 3) | (lane >> 3) << 2;
+}
+template <int D>
+__device__ __forceinline__ int kv_vector_of(int lane) {
+  if constexpr (D == 64) return (lane >> 2) & 7;
+  else if constexpr (D == 128) return (lane >> 2) & 3;
+  else return (lane >> 2) & 1;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t kv_dpp(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kDppXor1 = 0xb1, kDppXor2 = 0x4e, kDppXor8 = 0x128;  // quad permutes, and a row rotated by eight
+typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
+
+template <int X>  // 16 or 32
+__device__ __forceinline__ kv_u32x2 kv_swap(uint32_t a, uint32_t b) {
+  if constexpr (X == 16) return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  else return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+}
+
+// The butterflies between lanes X apart, two registers at a time: a swap of lane groups puts the two operands of
+// every result into one lane, and a second one the results back.
+template <int X>
+__device__ __forceinline__ void kv_lane_butterfly(float &a, float &b) {
+  const kv_u32x2 in = kv_swap<X>(__float_as_uint(a), __float_as_uint(b));
+  const float x = __uint_as_float(in[0]), y = __uint_as_float(in[1]);
+  const kv_u32x2 out = kv_swap<X>(__float_as_uint(x + y), __float_as_uint(x - y));
+  a = __uint_as_float(out[0]);
+  b = __uint_as_float(out[1]);
+}
+
+template <int CTRL>
+__device__ __forceinline__ void kv_dpp_butterflies(float (&y)[8], bool upper) {
+  const float sign = upper ? -1.0f : 1.0f;  // other + y below, other - y above, one rounding
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], sign, __uint_as_float(kv_dpp<CTRL>(__float_as_uint(y[i]))));
+}
+
+// One add or subtract for each output and stage, distances 1, 2, 4, ... in this order: the results are those of any other
+// schedule of the same butterflies.
 template <int D>
 __device__ __forceinline__ void kv_butterflies(float (&y)[8], int lane) {
 #pragma unroll
@@ -43,14 +89,13 @@ __device__ __forceinline__ void kv_butterflies(float (&y)[8], int lane) {
       }
     }
   }
+  kv_dpp_butterflies<kDppXor1>(y, lane & 1);
+  kv_dpp_butterflies<kDppXor2>(y, lane & 2);
+  if constexpr (D == 256) kv_dpp_butterflies<kDppXor8>(y, lane & 8);
 #pragma unroll
-  for (int d = 1; d < D / 8; d *= 2) {
-    const bool upper = (lane & d) != 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor(y[i], d, 64);
-      y[i] = upper ? other - y[i] : y[i] + other;
-    }
+  for (int i = 0; i < 8; i += 2) {
+    if constexpr (D >= 128) kv_lane_butterfly<16>(y[i], y[i + 1]);
+    kv_lane_butterfly<32>(y[i], y[i + 1]);
   }
 }
 
@@ -62,25 +107,28 @@ __device__ __forceinline__ uint32_t kv_encode(const float (&y)[8], uint16_t &sca
   uint32_t top = 0;  // as bits: a NaN is above infinity, infinity above every number
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int d = 1; d < D / 8; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 64)));
-  if (top >= 0x7f800000u) {
-    scale_bits = 0x7fc0u;
-    return 0;
+  top = max(top, kv_dpp<kDppXor1>(top));
+  top = max(top, kv_dpp<kDppXor2>(top));
+  if constexpr (D == 256) top = max(top, kv_dpp<kDppXor8>(top));
+  if constexpr (D >= 128) {
+    const kv_u32x2 both = kv_swap<16>(top, top);
+    top = max(both[0], both[1]);
   }
+  const kv_u32x2 both = kv_swap<32>(top, top);
+  top = max(both[0], both[1]);
+  const bool broken = top >= 0x7f800000u;
   uint16_t a = f32_to_bf16_bits(__uint_as_float(top) * (1.0f / 6.0f));
   if (a < 0x0080u) a = 0;
-  scale_bits = a;
-  const float inv = a != 0 ? 1.0f / bf16_bits_to_f32(a) : 0.0f;
+  scale_bits = broken ? 0x7fc0u : a;
+  const float inv = a != 0 && !broken ? 1.0f / bf16_bits_to_f32(a) : 0.0f;
   uint32_t q = 0;
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[0] * inv, y[1] * inv, 1.0f, 0);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[2] * inv, y[3] * inv, 1.0f, 1);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4] * inv, y[5] * inv, 1.0f, 2);
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[6] * inv, y[7] * inv, 1.0f, 3);
-  return q;
+  return broken ? 0u : q;
 }
 
-typedef float kv_f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 kv_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 kv_f16x8 __attribute__((ext_vector_type(8)));
 
