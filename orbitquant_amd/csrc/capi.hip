@@ -701,13 +701,8 @@ int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int6
   a.q_wide = vectors_wide(q, q_token_stride, q_head_stride, q_dtype);
   a.table = table; a.table_stride = table_stride; a.lengths = lengths; a.starts = starts; a.causal = causal != 0; a.scale = scale;
   a.out = out; a.lse = lse;
-  const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, most_queries(tokens, starts != nullptr, max_new));
-  if (needed > 0 && workspace != nullptr && workspace_bytes >= needed) {
-    a.part_out = static_cast<float *>(workspace);
-    a.part_stats = reinterpret_cast<float2 *>(a.part_out + static_cast<int64_t>(a.parts) * tokens * heads * dim);
-  } else {
-    a.parts = 1;
-  }
+  const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, most_queries(tokens, starts != nullptr, max_new), workspace);
+  if (workspace == nullptr || workspace_bytes < needed) a.few.target = a.many.target = 0;
   return oq::kv_attend_dispatch(a, dim, as_stream(stream));
 }
 
@@ -721,7 +716,7 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
   a.cache.heads = static_cast<int>(kv_heads);
   if (kv_attend_shape(a, tokens, heads, table_width, requests, window) != OQ_OK || tokens == 0) return 0;
   a.starts = has_starts ? &some : nullptr;  // (asked whether it is there, not read)
-  return oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new));
+  return oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new), nullptr);
 }
 
 }  // extern "C"

@@ -11,99 +11,148 @@ bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream);
 
 namespace {
 
-constexpr int kMaxParts = 128;
+// How launches are cut (MI355X, D = 128; a step is 64 keys).
+// Few rows.  One launch and no join up to sixteen steps: 1003 tokens, 32 heads, 10.7 us, cut into fours 11.3.  Above, 512 workgroups or more, two on
+// each compute unit at once: 131101 tokens, 8 heads, 34.6 us (1024: 39.7, 256: 35.0); sixteen requests of up to 4096, 27.2 with the rest of their step (1024: 31).
+// Up to three times as many where a part keeps 80 steps, so that requests of different lengths even out: 64 of up to
+// 16384, 133 us (512 workgroups: 139).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 17.9 us (six: 20).
+constexpr int kFewWhole = 16, kFewGroups = 512, kFewSteps = 80, kFewLeast = 4;
+// Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the chip, and at least 24 steps
+// of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 74 us; 2048 on their own, 264 tiles: 68 -> 97 us if they were cut.
+constexpr int kManyWhole = 384, kManyGroups = 512, kManyLeast = 24;
 
-// out = sum_p 2^(R_p) o_p / sum_p 2^(R_p) l_p.  TPR threads a row: D / 4 of them have the four dimensions each, and as many sets of those
-// as there are take every so many-th part, so that a row of a hundred parts is not a chain of a hundred loads.
-template <int D, int TPR>
-__global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a) {
-  constexpr int SETS = TPR / (D / 4), ROWS = 256 / TPR;
-  __shared__ float2 stats[ROWS][kMaxParts];
+constexpr int kJoinBlocks = 4;  // workgroups of a tile, at most
+
+// The parts of the tiles that a launch has cut: out = sum_p 2^(R_p) o_p / sum_p 2^(R_p) l_p, in the order of the keys.  TPR threads a row:
+// D / 4 of them have four dimensions each, and as many sets of those as there are take every so many-th part, so that a row of
+// a hundred parts is not a chain of a hundred loads.
+template <int D, int TPR, bool MANY>
+__device__ __forceinline__ void join_tile(const KvAttendArgs &a, int block, int blocks) {
+  constexpr int SETS = TPR / (D / 4), ROWS = 256 / TPR, TILE = MANY ? kKvManyRows : 16;
   __shared__ float4 sums[ROWS][SETS][D / 4];
-  const int in_block = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const int64_t rows = a.tokens * a.heads;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + in_block;
-  if (row < rows) {
-    for (int p = t; p < a.parts; p += TPR) stats[in_block][p] = a.part_stats[p * rows + row];
-  }
-  __syncthreads();
-  const int set = t / (D / 4), d = t % (D / 4);
-  float best = kKvNothing, l = 0.0f;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (row < rows) {
-    for (int p = 0; p < a.parts; ++p) best = fmaxf(best, stats[in_block][p].x);
-    for (int p = 0; p < a.parts; ++p) l += kv_exp2(stats[in_block][p].x - best) * stats[in_block][p].y;
+  __shared__ float2 totals[ROWS][SETS];  // of a set: its largest R and its l
+  const KvCut &cut = MANY ? a.many : a.few;
+  const int in_block = threadIdx.x / TPR, t = threadIdx.x % TPR, set = t / (D / 4), d = t % (D / 4);
+  const int in_launch = block / blocks;
+  const int kv_head = in_launch % a.cache.heads, first = in_launch / a.cache.heads;
+  const int2 *maps = cut.map + static_cast<int64_t>(kv_head) * (2 * cut.target + 1);
+  if (first >= maps[2 * cut.target].x) return;  // (the same for the block, as is what follows)
+  const int2 map = maps[first];
+  if (map.x < 0) return;
+  KvRows r;
+  if (!kv_tile<MANY>(a, map.x, r)) return;
+  for (int from = block % blocks * ROWS; from < r.rows; from += blocks * ROWS) {
+    const int in_tile = from + in_block;
+    const bool there = in_tile < r.rows;
+    float best = kKvNothing, l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const auto add = [&](const float2 &stats, const float4 &o) {
+      const float both = fmaxf(best, stats.x), mine = kv_exp2(best - both), theirs = kv_exp2(stats.x - both);
+      best = both;
+      l = fmaf(l, mine, stats.y * theirs);
+      y.x = fmaf(y.x, mine, o.x * theirs); y.y = fmaf(y.y, mine, o.y * theirs);
+      y.z = fmaf(y.z, mine, o.z * theirs); y.w = fmaf(y.w, mine, o.w * theirs);
+    };
+    if (there) {
+      const int64_t place = (static_cast<int64_t>(kv_head) * 2 * cut.target + first) * TILE + in_tile;
 #pragma unroll 4
-    for (int p = set; p < a.parts; p += SETS) {
-      const float w = kv_exp2(stats[in_block][p].x - best);
-      const float4 o = reinterpret_cast<const float4 *>(a.part_out + (p * rows + row) * D)[d];
-      y.x += w * o.x; y.y += w * o.y; y.z += w * o.z; y.w += w * o.w;
+      for (int p = set; p < map.y; p += SETS)
+        add(cut.stats[place + static_cast<int64_t>(p) * TILE], reinterpret_cast<const float4 *>(cut.out + (place + static_cast<int64_t>(p) * TILE) * D)[d]);
     }
-  }
-  sums[in_block][set][d] = y;
-  __syncthreads();
-  if (set != 0 || row >= rows) return;
+    if constexpr (SETS > 1) {
+      sums[in_block][set][d] = y;
+      if (d == 0) totals[in_block][set] = make_float2(best, l);
+      __syncthreads();
+      if (set == 0) {
 #pragma unroll
-  for (int s = 1; s < SETS; ++s) {
-    const float4 o = sums[in_block][s][d];
-    y.x += o.x; y.y += o.y; y.z += o.z; y.w += o.w;
-  }
-  const float by = l != 0.0f ? 1.0f / l : 0.0f;
-  const float v[4] = {y.x * by, y.y * by, y.z * by, y.w * by};
-  const int64_t at = row * D + 4 * d;
-  if (a.q_dtype == OQ_F32) {
-    *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint32_t w[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[e] = a.q_dtype == OQ_F16 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
-                                 : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
+        for (int s = 1; s < SETS; ++s) add(totals[in_block][s], sums[in_block][s][d]);
+      }
+      __syncthreads();
     }
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(w[0], w[1]);
+    if (set != 0 || !there) continue;
+    const KvRow at_row = kv_row_of(a, r, kv_head, r.first + in_tile, true);
+    const int64_t row = static_cast<int64_t>(at_row.token) * a.heads + at_row.head;
+    const float by = l != 0.0f ? 1.0f / l : 0.0f;
+    const float v[4] = {y.x * by, y.y * by, y.z * by, y.w * by};
+    const int64_t at = row * D + 4 * d;
+    if (a.q_dtype == OQ_F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint32_t w[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[e] = a.q_dtype == OQ_F16 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
+                                   : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
+      }
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(w[0], w[1]);
+    }
+    if (a.lse != nullptr && d == 0) a.lse[row] = l != 0.0f ? (best + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
   }
-  if (a.lse != nullptr && d == 0) a.lse[row] = l != 0.0f ? (best + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
+}
+
+// The first `many_blocks` workgroups have the prompts' tiles, the others those of few rows: FEW threads for one of these, `few_blocks` workgroups for a tile.
+template <int D, int FEW>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, int many_blocks, int few_blocks) {
+  const int block = blockIdx.x;
+  if (block < many_blocks) join_tile<D, D / 4, true>(a, block, kJoinBlocks);
+  else join_tile<D, FEW, false>(a, block - many_blocks, few_blocks);
 }
 
 template <int D>
 void join(const KvAttendArgs &a, hipStream_t stream) {
-  const int64_t rows = a.tokens * a.heads;
-  if (a.parts > 8) launch_kernel(kv_join_kernel<D, 256>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a);
-  else launch_kernel(kv_join_kernel<D, 64>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
+  const int many = a.cache.heads * 2 * a.many.target * kJoinBlocks;
+  // Few tiles have many parts each, and a row of them is a workgroup's; many have few.
+  const bool long_rows = static_cast<int64_t>(a.few_requests) * a.few_tiles * a.cache.heads < 256;
+  const int in_tile = long_rows ? a.few_in_tile : (a.few_in_tile + 3) / 4, few_blocks = in_tile < kJoinBlocks ? in_tile : kJoinBlocks;
+  const dim3 grid(static_cast<unsigned>(many + a.cache.heads * 2 * a.few.target * few_blocks));
+  if (long_rows) launch_kernel(kv_join_kernel<D, 256>, grid, dim3(256), 0, stream, a, many, few_blocks);
+  else launch_kernel(kv_join_kernel<D, 64>, grid, dim3(256), 0, stream, a, many, few_blocks);
+}
+
+uint64_t kv_places(KvCut &cut, int heads, int rows, int dim, char *workspace, uint64_t from) {
+  if (cut.target == 0) return from;
+  const uint64_t places = 2ull * cut.target * heads * rows;
+  cut.out = reinterpret_cast<float *>(workspace + from);
+  cut.stats = reinterpret_cast<float2 *>(workspace + from + places * dim * sizeof(float));
+  cut.map = reinterpret_cast<int2 *>(workspace + from + places * (dim + 2) * sizeof(float));
+  return from + places * (dim + 2) * sizeof(float) + (((2ull * cut.target + 1) * heads * sizeof(int2) + 15) & ~15ull);
 }
 
 }  // namespace
 
-uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new) {
+uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new, void *workspace) {
   const int64_t rows = a.tokens * a.group;
-  int64_t busy;  // workgroups with work
+  const int heads = a.cache.heads;
   a.many_tiles = 0;
   a.few_rows = 0;
   if (a.starts == nullptr) {
     a.few_requests = a.requests;
     a.few_tiles = (a.group + 15) / 16;
-    busy = static_cast<int64_t>(a.few_requests) * a.few_tiles;
+    a.few_in_tile = a.group < 16 ? a.group : 16;
   } else {
     // A lone request's rows are known to be many, or few; of several, each may be either.
     const bool many = rows > kKvFewRows, few = !many || a.requests > 1;
     if (many) a.many_tiles = static_cast<int>(kv_tile_base(rows, a.requests)) + 1;
     a.few_requests = few ? a.requests + 1 : 0;
     a.few_tiles = static_cast<int>(((rows < kKvFewRows ? rows : kKvFewRows) + 15) / 16);
+    a.few_in_tile = rows < 16 ? static_cast<int>(rows) : 16;
     a.few_rows = few ? kKvFewRows : 0;
-    busy = many ? (rows + kKvManyRows - 1) / kKvManyRows : a.few_tiles;
   }
-  busy *= a.cache.heads;
   int64_t keys = static_cast<int64_t>(a.table_width) << a.cache.page_shift;
   if (max_length >= 0 && max_length < keys) keys = max_length;
   if (a.window != 0 && keys > a.window + max_new) keys = a.window + max_new + 63;
   const int64_t steps = (keys + 63) / 64;
-  int64_t parts = busy > 0 ? (1024 + busy - 1) / busy : 1;
-  if (parts > steps / 4) parts = steps / 4;
-  if (parts > kMaxParts) parts = kMaxParts;
-  if (parts < 1) parts = 1;
-  a.part_steps = static_cast<int>(steps > 0 ? (steps + parts - 1) / parts : 1);
-  a.parts = static_cast<int>(steps > 0 ? (steps + a.part_steps - 1) / a.part_steps : 1);
-  return a.parts > 1 ? static_cast<uint64_t>(a.parts) * a.tokens * a.heads * (dim + 2) * sizeof(float) : 0;
+  a.few.target = a.many.target = 0;
+  a.few.least = kFewLeast;
+  a.many.least = kManyLeast;
+  if (a.few_requests > 0 && steps > kFewWhole) {
+    const int64_t parts = static_cast<int64_t>(a.requests) * steps * heads / kFewSteps;
+    const int64_t groups = parts < kFewGroups ? kFewGroups : parts > 3 * kFewGroups ? 3 * kFewGroups : parts;
+    a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
+  }
+  if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < kManyWhole) a.many.target = heads < kManyGroups ? kManyGroups / heads : 1;
+  const uint64_t bytes = kv_places(a.few, heads, 16, dim, static_cast<char *>(workspace), 0);
+  return kv_places(a.many, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }
 
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream) {
@@ -111,7 +160,7 @@ int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream) {
   const bool fits = dim == 64 ? kv_attend_64(a, split, stream) : dim == 128 ? kv_attend_128(a, split, stream) : kv_attend_256(a, split, stream);
   if (!fits) return fail(OQ_ERR_LAUNCH, "kv_attend: no LDS for heads of %d", dim);
   const int status = check_launch("kv_attend");
-  if (status != OQ_OK || a.parts == 1) return status;
+  if (status != OQ_OK || (a.few.target == 0 && a.many.target == 0)) return status;
   if (dim == 64) join<64>(a, stream);
   else if (dim == 128) join<128>(a, stream);
   else join<256>(a, stream);

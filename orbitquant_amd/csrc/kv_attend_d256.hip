@@ -3,9 +3,6 @@
 
 namespace oq {
 
-bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream) {
-  if (split == 0) return kv_attend_launch<256, 0>(a, stream);
-  return split == 1 ? kv_attend_launch<256, 1>(a, stream) : kv_attend_launch<256, 2>(a, stream);
-}
+bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream) { return kv_attend_of<256>(a, split, stream); }
 
 }  // namespace oq

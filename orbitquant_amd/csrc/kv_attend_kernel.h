@@ -33,11 +33,16 @@
 // products.
 #pragma once
 
+#include <type_traits>
+
 #include "kv_cache.h"
 
 namespace oq {
 
 typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
+
+template <int SPLIT>
+constexpr int kv_dtype() { return SPLIT == 0 ? OQ_BF16 : SPLIT == 1 ? OQ_F16 : OQ_F32; }
 
 constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
 constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
@@ -112,10 +117,173 @@ __device__ __forceinline__ KvSpan kv_span_of(const KvAttendArgs &a, const KvRows
   return s;
 }
 
-__device__ __forceinline__ int kv_page_at(const KvAttendArgs &a, const int32_t *table, int key) {  // -1: not there
-  const int column = key >> a.cache.page_shift;
-  const int page = column < a.table_width ? table[column] : -1;
-  return page < a.cache.pages ? page : -1;
+// Tile i of a launch: its rows, false where there are none.
+__device__ __forceinline__ bool kv_few_tile(const KvAttendArgs &a, int i, KvRows &r) {
+  r.request = i / a.few_tiles;
+  r.first = (i - r.request * a.few_tiles) * 16;
+  r.start = r.request;
+  r.fresh = 1;
+  if (a.starts != nullptr) {
+    r.start = kv_start_of(a, r.request);
+    r.fresh = max(kv_start_of(a, r.request + 1) - r.start, 0);
+    if (static_cast<int64_t>(r.fresh) * a.group > kKvFewRows) return false;
+  }
+  r.rows = min(r.fresh * a.group - r.first, 16);
+  if (r.rows <= 0) return false;
+  kv_keys_of(a, r);
+  return true;
+}
+
+__device__ __forceinline__ bool kv_many_tile(const KvAttendArgs &a, int i, KvRows &r) {
+  int low = 0, high = a.requests + 1;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (kv_tile_base(static_cast<int64_t>(kv_start_of(a, mid)) * a.group, mid) <= i) low = mid; else high = mid;
+  }
+  r.request = low;
+  r.start = kv_start_of(a, low);
+  r.fresh = max(kv_start_of(a, low + 1) - r.start, 0);
+  const int64_t first = (i - kv_tile_base(static_cast<int64_t>(r.start) * a.group, low)) * kKvManyRows, all = static_cast<int64_t>(r.fresh) * a.group;
+  if (first >= all || all <= a.few_rows) return false;
+  r.first = static_cast<int>(first);
+  r.rows = static_cast<int>(min(all - first, static_cast<int64_t>(kKvManyRows)));
+  kv_keys_of(a, r);
+  return true;
+}
+
+template <bool MANY>
+__device__ __forceinline__ bool kv_tile(const KvAttendArgs &a, int i, KvRows &r) {
+  if constexpr (MANY) return kv_many_tile(a, i, r);
+  else return kv_few_tile(a, i, r);
+}
+
+__device__ __forceinline__ int kv_steps_of(const KvSpan &span) {  // one for a tile without keys: somebody writes its zeros
+  return span.highest >= span.lowest ? (span.highest >> 6) - (span.lowest >> 6) + 1 : 1;
+}
+
+// A workgroup's part of a tile.
+struct KvPart {
+  KvRows rows;
+  int tile, index, count;  // of the tile's parts
+  int place;               // of the part among those of cut tiles
+};
+__device__ __forceinline__ int kv_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int kv_from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// Sums over the lanes up to each: within rows of sixteen, then from row to row.
+__device__ __forceinline__ int kv_sums(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+// Part `group` of the launch's, false behind the last.  Every workgroup counts for itself: the tiles' steps, and from those the parts.
+template <bool MANY, int THREADS>
+__device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  KvRows r = {};
+  const auto steps_of = [&](int i) { return kv_tile<MANY>(a, i, r) ? kv_steps_of(kv_span_of(a, r, r.first, r.rows)) : 0; };
+  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (2 * cut.target + 1);
+  if (tiles <= 64) {  // a lane has a tile, and no wavefront needs another: the first keys are a barrier nearer
+    const int steps = lane < tiles ? steps_of(lane) : 0;
+    const int total = kv_from_lane(kv_sums(steps), 63);  // (below 64 * 2^24)
+    const int longest = max((total + cut.target - 1) / cut.target, cut.least);
+    const int count = (steps + longest - 1) / longest, sum = kv_sums(count);
+    const int in_cut = count > 1 ? count : 0, cut_sum = kv_sums(in_cut);
+    if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(kv_from_lane(cut_sum, 63), 0);
+    const int all = kv_from_lane(sum, 63);
+    if (group >= all) return false;
+    const int at = MANY ? all - 1 - group : group;  // a prompt's last rows see the most keys: they begin first
+    const int found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > at));
+    part.tile = found;
+    part.count = kv_from_lane(count, found);
+    part.index = at - kv_from_lane(sum - count, found);
+    part.place = kv_from_lane(cut_sum - in_cut, found) + part.index;
+    part.rows = {kv_from_lane(r.request, found), kv_from_lane(r.start, found), kv_from_lane(r.fresh, found), kv_from_lane(r.length, found),
+                 kv_from_lane(r.first, found), kv_from_lane(r.rows, found), kv_from_lane(r.last_key, found)};
+  } else {
+    __shared__ int64_t wave_sums[THREADS / 64];
+    __shared__ int2 wave_counts[THREADS / 64];
+    __shared__ int found[4];
+    __shared__ KvRows found_rows;
+    const int chunk = (tiles + THREADS - 1) / THREADS, from = tid * chunk, to = min(from + chunk, tiles);
+    int64_t own = 0;
+    for (int i = from; i < to; ++i) own += steps_of(i);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) own += __shfl_xor(static_cast<long long>(own), d, 64);
+    if (lane == 0) wave_sums[wave] = own;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) total += wave_sums[w];
+    const int longest = static_cast<int>(max((total + cut.target - 1) / cut.target, static_cast<int64_t>(cut.least)));
+    int count = 0, in_cut = 0;
+    for (int i = from; i < to; ++i) {
+      const int n = (steps_of(i) + longest - 1) / longest;
+      count += n;
+      in_cut += n > 1 ? n : 0;
+    }
+    const int sum = kv_sums(count), cut_sum = kv_sums(in_cut);
+    if (lane == 63) wave_counts[wave] = make_int2(sum, cut_sum);
+    __syncthreads();
+    int ahead = sum - count, cut_ahead = cut_sum - in_cut, all = 0, all_cut = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) {
+        ahead += wave_counts[w].x;
+        cut_ahead += wave_counts[w].y;
+      }
+      all += wave_counts[w].x;
+      all_cut += wave_counts[w].y;
+    }
+    if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(all_cut, 0);
+    if (group >= all) return false;
+    const int at = MANY ? all - 1 - group : group;
+    if (at >= ahead && at < ahead + count) {
+      int i = from, n = (steps_of(i) + longest - 1) / longest;
+      while (at >= ahead + n) {
+        ahead += n;
+        cut_ahead += n > 1 ? n : 0;
+        n = (steps_of(++i) + longest - 1) / longest;
+      }
+      found[0] = i;
+      found[1] = n;
+      found[2] = at - ahead;
+      found[3] = cut_ahead + at - ahead;
+      found_rows = r;
+    }
+    __syncthreads();
+    part.tile = kv_uniform(found[0]);
+    part.count = kv_uniform(found[1]);
+    part.index = kv_uniform(found[2]);
+    part.place = kv_uniform(found[3]);
+    part.rows = {kv_uniform(found_rows.request), kv_uniform(found_rows.start), kv_uniform(found_rows.fresh), kv_uniform(found_rows.length),
+                 kv_uniform(found_rows.first), kv_uniform(found_rows.rows), kv_uniform(found_rows.last_key)};
+  }
+  if (part.count > 1 && tid == 0) map[part.place] = part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0);
+  return true;
+}
+
+// The table's entry for a key, as it stands there: it is looked at when the page is asked for, a step later, so that nothing waits for
+// it here (loads come back in order: such a wait is one for everything requested before).  Columns behind the table are clamped;
+// their keys are behind the last one.
+__device__ __forceinline__ int kv_page_at(const KvAttendArgs &a, const int32_t *table, int key) {
+  return table[min(key >> a.cache.page_shift, a.table_width - 1)];
+}
+__device__ __forceinline__ bool kv_page_there(const KvAttendArgs &a, int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.cache.pages); }
+__device__ __forceinline__ int64_t kv_block_of(const KvAttendArgs &a, int page, int kv_head) {  // any that exists, where the page does not
+  return static_cast<int64_t>(kv_page_there(a, page) ? page : 0) * a.cache.heads + kv_head;
+}
+
+// Where pages hold whole steps (64 tokens and more) a step's page is the same for all lanes: its entry is read and its address made by scalar
+// instructions, and lanes add what is theirs.  (Forty vector instructions of a step otherwise, of some three hundred.)
+__device__ __forceinline__ int kv_scalar_page_at(const KvAttendArgs &a, const int32_t *table, int key) {
+  const int column = __builtin_amdgcn_readfirstlane(min(key >> a.cache.page_shift, a.table_width - 1));
+  return *(const __attribute__((address_space(4))) int32_t *)(table + column);
 }
 
 // One row a lane (n = lane & 15; the four lanes of a row have a quarter of its dimensions each).
@@ -133,45 +301,53 @@ __device__ __forceinline__ KvRow kv_row_of(const KvAttendArgs &a, const KvRows &
   return k;
 }
 
-template <int D>
-__device__ __forceinline__ void kv_load_query(const KvAttendArgs &a, const KvRow &row, int g, float (&y)[D / 4]) {
-  if (row.token >= 0) {
-    const int64_t at = row.token * a.q_token_stride + row.head * a.q_head_stride + g * (D / 4);
-    if (a.q_wide && a.q_dtype != OQ_F32) {
+// A row's quarter of a query as it comes, and the signs of its dimensions: requested before the keys, so that it is there before them.
+template <int D, int SPLIT>
+struct KvQuery {
+  static constexpr int WORDS = D / 4 * (SPLIT == 2 ? 4 : 2) / 4;
+  uint32_t raw[WORDS], signs[D / 16];
+
+  __device__ __forceinline__ void request(const KvAttendArgs &a, const KvRow &row, int g) {
 #pragma unroll
-      for (int i = 0; i < D / 4; i += 8) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at + i);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < D / 16; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(a.cache.signs + g * (D / 4) + 4 * i);
+      signs[i] = v.x; signs[i + 1] = v.y; signs[i + 2] = v.z; signs[i + 3] = v.w;
+    }
+    // (a lane without a row reads one that exists, and makes zeros of it)
+    const int64_t at = max(row.token, 0) * a.q_token_stride + row.head * a.q_head_stride + g * (D / 4);
+    if (a.q_wide) {
+      const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q) + at * (SPLIT == 2 ? 4 : 2));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[i + e] = dyn_bits_to_f32((w[e / 2] >> (16 * (e & 1))) & 0xffffu, a.q_dtype);
-      }
-    } else if (a.q_wide) {
-#pragma unroll
-      for (int i = 0; i < D / 4; i += 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + i);
-        y[i] = v.x; y[i + 1] = v.y; y[i + 2] = v.z; y[i + 3] = v.w;
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 v = from[i / 4];
+        raw[i] = v.x; raw[i + 1] = v.y; raw[i + 2] = v.z; raw[i + 3] = v.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) y[i] = load_dyn_f32(a.q, a.q_dtype, at + i);
+      for (int i = 0; i < WORDS; ++i) {
+        if constexpr (SPLIT == 2) raw[i] = static_cast<const uint32_t *>(a.q)[at + i];
+        else raw[i] = static_cast<const uint16_t *>(a.q)[at + 2 * i] | static_cast<uint32_t>(static_cast<const uint16_t *>(a.q)[at + 2 * i + 1]) << 16;
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) y[i] = 0.0f;
   }
-}
 
-// Rotates a row's quarter; gives the largest magnitude of the row.
-template <int D>
-__device__ __forceinline__ float kv_rotate_query(const KvAttendArgs &a, int g, float (&y)[D / 4]) {
+  // Rotated; gives the largest magnitude of the row.
+  __device__ __forceinline__ float rotate(bool there, float (&y)[D / 4]) const {
 #pragma unroll
-  for (int i = 0; i < D / 4; ++i) y[i] *= static_cast<float>(a.cache.signs[g * (D / 4) + i]);
-  kv_rotate_lane<D>(y);
-  float top = 0.0f;
+    for (int i = 0; i < D / 4; ++i) {
+      float v;
+      if constexpr (SPLIT == 2) v = __uint_as_float(raw[i]);
+      else v = dyn_bits_to_f32((raw[i / 2] >> (16 * (i & 1))) & 0xffffu, kv_dtype<SPLIT>());
+      const float sign = static_cast<float>(static_cast<int8_t>(signs[i / 4] >> (8 * (i & 3))));
+      y[i] = there ? v * sign : 0.0f;
+    }
+    kv_rotate_lane<D>(y);
+    float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(y[i]));
-  return kv_over_groups(top, kv_max_of);
-}
+    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(y[i]));
+    return kv_over_groups(top, kv_max_of);
+  }
+};
 
 // The power of two 2^-exponent puts `top` into [2^10, 2^11).
 __device__ __forceinline__ int kv_query_exponent(float top) {
@@ -217,13 +393,23 @@ struct KvState {
   __device__ __forceinline__ float reference() const { return limit < 0.0f ? kKvNothing : ref; }
 };
 
+// (fmaxf of values that come from a branch is two instructions: the compiler first makes sure that a NaN is quiet.)
+__device__ __forceinline__ float kv_max3(float a, float b, float c) {
+  float m;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+  return m;
+}
+
 // x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.
 template <int D>
 __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], float top_exponent, KvState &st, kv_f32x4 (&o)[D / 16]) {
-  float best = fmaxf(x[0], x[1]);
-#pragma unroll
-  for (int i = 2; i < 16; i += 2) best = fmaxf(best, fmaxf(x[i], x[i + 1]));
-  best += top_exponent;
+  float best = kv_max3(x[0], x[1], x[2]), other = kv_max3(x[3], x[4], x[5]);
+  best = kv_max3(best, x[6], x[7]);
+  other = kv_max3(other, x[8], x[9]);
+  best = kv_max3(best, x[10], x[11]);
+  other = kv_max3(other, x[12], x[13]);
+  best = kv_max3(best, x[14], x[15]);
+  best = kv_max3(best, other, other) + top_exponent;
   if (__builtin_amdgcn_ballot_w64(best > st.limit) != 0) {
     best = kv_over_groups(best, kv_max_of);
     const bool raise = best > st.limit;
@@ -283,12 +469,13 @@ __device__ __forceinline__ void kv_decode_values(uint32_t x, uint32_t y, kv_f16x
   odd = kv_decode8(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u));
 }
 
-// A row's result: rotated back, and stored as the output, or as a part of it.
-template <int D>
-__device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &row, int g, int part, const KvState &st, const kv_f32x4 (&o)[D / 16]) {
+// A row's result: rotated back, and stored as the output, or at its place in the parts.
+template <int D, int SPLIT>
+__device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &row, int g, const uint32_t *signs, float *part_out, float2 *part_stats,
+                                          const KvState &st, const kv_f32x4 (&o)[D / 16]) {
   const float l = kv_over_groups(st.sum, kv_sum_of);
-  const bool parts = a.parts > 1;
-  const float by = parts ? 1.0f / D : l != 0.0f ? (1.0f / D) / l : 0.0f;  // (no key: zeros)
+  const bool part = part_out != nullptr;
+  const float by = part ? 1.0f / D : l != 0.0f ? (1.0f / D) / l : 0.0f;  // (no key: zeros)
   // dimension 32 j + 8 g + 2 r + parity is in o[2 j + parity][r]
   float y[D / 4];
 #pragma unroll
@@ -302,30 +489,29 @@ __device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &ro
   kv_rotate_lane<D>(y);
   if (row.token < 0) return;
   const int64_t index = static_cast<int64_t>(row.token) * a.heads + row.head;
-  const int64_t in_parts = static_cast<int64_t>(part) * a.tokens * a.heads + index;
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
-    const uint2 sign = *reinterpret_cast<const uint2 *>(a.cache.signs + 32 * j + 8 * g);
+    const uint2 sign = *reinterpret_cast<const uint2 *>(signs + 8 * j + 2 * g);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(__float_as_uint(y[8 * j + e]) ^ (((e < 4 ? sign.x : sign.y) << (24 - 8 * (e & 3))) & 0x80000000u));
     const int at = 32 * j + 8 * g;
-    if (parts || a.q_dtype == OQ_F32) {
-      float *to = parts ? a.part_out + in_parts * D + at : static_cast<float *>(a.out) + index * D + at;
+    if (SPLIT == 2 || part) {
+      float *to = part ? part_out + at : static_cast<float *>(a.out) + index * D + at;
       reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = a.q_dtype == OQ_F16 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
-                                   : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
+        w[e] = SPLIT == 1 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
+                          : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
       }
       *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + index * D + at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   if (g != 0) return;
-  if (parts) a.part_stats[in_parts] = make_float2(st.reference(), l);
+  if (part) *part_stats = make_float2(st.reference(), l);
   else if (a.lse != nullptr) a.lse[index] = l != 0.0f ? (st.ref + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
 }
 
@@ -339,100 +525,108 @@ struct KvRaw {
 struct KvPages {  // of key rows (n >> 2) and of values and scales (g)
   int k, v;
 };
+template <bool WIDE>
 __device__ __forceinline__ KvPages kv_pages_of(const KvAttendArgs &a, const int32_t *table, int n, int g, int step) {
+  if constexpr (WIDE) {
+    const int page = kv_scalar_page_at(a, table, step * 64);
+    return {page, page};
+  }
   return {kv_page_at(a, table, step * 64 + 16 * (n >> 2)), kv_page_at(a, table, step * 64 + 16 * g)};
 }
-template <int D>
+// Where a step's keys begin, in tokens of the whole cache (all heads): of a lane's group of sixteen, or of the step.
+template <bool WIDE>
+__device__ __forceinline__ int64_t kv_tokens_at(const KvAttendArgs &a, int kv_head, int page, int step, int group) {
+  const int shift = a.cache.page_shift;
+  return (kv_block_of(a, page, kv_head) << shift) + ((step * 64 + (WIDE ? 0 : 16 * group)) & ((1 << shift) - 1));
+}
+template <int D, bool WIDE>
 __device__ __forceinline__ void kv_request_keys(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
   constexpr int W = D / 32;
-  const int shift = a.cache.page_shift, in_page = (1 << shift) - 1;
-  const int64_t k_block = static_cast<int64_t>(max(page.k, 0)) * a.cache.heads + kv_head, v_block = static_cast<int64_t>(max(page.v, 0)) * a.cache.heads + kv_head;
-  const uint32_t *from = reinterpret_cast<const uint32_t *>(a.cache.k_codes) + ((k_block << shift) + ((s * 64 + 16 * (n >> 2)) & in_page) + (n & 3)) * (D / 8) + g * W;
+  const int64_t keys = kv_tokens_at<WIDE>(a, kv_head, page.k, s, n >> 2), scales = kv_tokens_at<WIDE>(a, kv_head, page.v, s, g);
+  const uint32_t in_keys = ((WIDE ? 16 * (n >> 2) : 0) + (n & 3)) * (D / 8) + g * W;  // dwords
+  const uint32_t *from = reinterpret_cast<const uint32_t *>(a.cache.k_codes) + keys * (D / 8);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if constexpr (W == 2) {
-      const uint2 v = *reinterpret_cast<const uint2 *>(from + 4 * t * (D / 8));
+      const uint2 v = *reinterpret_cast<const uint2 *>(from + in_keys + 4 * t * (D / 8));
       to.k[t][0] = v.x; to.k[t][1] = v.y;
     } else {
 #pragma unroll
       for (int w = 0; w < W; w += 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(from + 4 * t * (D / 8) + w);
+        const uint4 v = *reinterpret_cast<const uint4 *>(from + in_keys + 4 * t * (D / 8) + w);
         to.k[t][w] = v.x; to.k[t][w + 1] = v.y; to.k[t][w + 2] = v.z; to.k[t][w + 3] = v.w;
       }
     }
   }
-  const int64_t scales = (v_block << shift) + ((s * 64 + 16 * g) & in_page);
+  const uint32_t in_scales = WIDE ? 2 * g : 0;  // of eight
   const uint4 *k_from = reinterpret_cast<const uint4 *>(a.cache.k_scales + scales), *v_from = reinterpret_cast<const uint4 *>(a.cache.v_scales + scales);
-  to.k_scale[0] = k_from[0]; to.k_scale[1] = k_from[1];
-  to.v_scale[0] = v_from[0]; to.v_scale[1] = v_from[1];
-  to.here = page.v >= 0;
+  to.k_scale[0] = k_from[in_scales]; to.k_scale[1] = k_from[in_scales + 1];
+  to.v_scale[0] = v_from[in_scales]; to.v_scale[1] = v_from[in_scales + 1];
+  to.here = kv_page_there(a, page.v);
 }
-template <int D>
+template <int D, bool WIDE>
 __device__ __forceinline__ void kv_request_values(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
   const int shift = a.cache.page_shift;
-  const int64_t block = static_cast<int64_t>(max(page.v, 0)) * a.cache.heads + kv_head;
-  const uint8_t *from = a.cache.v_codes + ((block * (D / 2) + n) << shift) + ((s * 64 + 16 * g) & ((1 << shift) - 1));
+  const int64_t block = kv_block_of(a, page.v, kv_head);
+  const uint8_t *from = a.cache.v_codes + ((block * (D / 2)) << shift) + ((s * 64 + (WIDE ? 0 : 16 * g)) & ((1 << shift) - 1));
+  const uint32_t in_values = (static_cast<uint32_t>(n) << shift) + (WIDE ? 16 * g : 0);
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) to.v[j] = *reinterpret_cast<const uint4 *>(from + (static_cast<int64_t>(16 * j) << shift));
+  for (int j = 0; j < D / 32; ++j) to.v[j] = *reinterpret_cast<const uint4 *>(from + (static_cast<uint32_t>(16 * j) << shift) + in_values);
 }
-template <int D>
+template <int D, bool WIDE>
 __device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, int n, int g, int s, const KvPages &page, KvRaw<D> &to) {
-  kv_request_keys<D>(a, kv_head, n, g, s, page, to);
-  kv_request_values<D>(a, kv_head, n, g, s, page, to);
+  kv_request_keys<D, WIDE>(a, kv_head, n, g, s, page, to);
+  kv_request_values<D, WIDE>(a, kv_head, n, g, s, page, to);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS.  A step's
-// keys, scales and values (8.4 KB at D = 128) are requested DEPTH of the wavefront's steps ahead, into the registers of the ones just used.
-template <int D, int SPLIT>
+// keys, scales and values (8.4 KB at D = 128) are requested a step of the wavefront's ahead, into the registers of the ones just used.
+template <int D, int SPLIT, bool WIDE>
 __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
-  constexpr int DEPTH = D == 256 ? 1 : 2;  // (of heads of 256 two steps do not fit the registers)
-  __shared__ float join[2][D / 4 + 2][64];
+  __shared__ float join[3][D / 4 + 2][64];
+  __shared__ uint32_t signs[D / 4];
+  if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int kv_head = blockIdx.x % a.cache.heads, part = blockIdx.y;
-  const int tile = blockIdx.x / a.cache.heads;
+  const int kv_head = blockIdx.x % a.cache.heads, group = blockIdx.x / a.cache.heads;
 
-  KvRows r;
-  r.request = tile / a.few_tiles;
-  r.first = (tile - r.request * a.few_tiles) * 16;
-  r.start = r.request;
-  r.fresh = 1;
-  if (a.starts != nullptr) {
-    r.start = kv_start_of(a, r.request);
-    r.fresh = max(kv_start_of(a, r.request + 1) - r.start, 0);
-    if (static_cast<int64_t>(r.fresh) * a.group > kKvFewRows) return;
+  KvPart part;
+  if (a.few.target == 0) {
+    part = {{}, group, 0, 1, 0};
+    if (!kv_few_tile(a, group, part.rows)) return;
+  } else if (!kv_part_of_launch<false, 256>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
+    return;
   }
-  r.rows = min(r.fresh * a.group - r.first, 16);
-  if (r.rows <= 0) return;
-  kv_keys_of(a, r);
+  const KvRows r = part.rows;
   const KvSpan span = kv_span_of(a, r, r.first, r.rows);
-  int step = (span.lowest >> 6) + part * a.part_steps;
-  int end = span.highest >= span.lowest ? (span.highest >> 6) + 1 : 0;
-  if (part + 1 < a.parts) end = min(end, step + a.part_steps);
-  step += wave;
+  const int steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
+  int step = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(steps) * part.index / part.count) + wave;
+  const int end = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(steps) * (part.index + 1) / part.count);
 
   const int32_t *table = a.table + r.request * a.table_stride;
-  KvRaw<D> raw[DEPTH];
-  KvPages pages[DEPTH];  // of the steps that are requested next
-  // the first steps are on their way while the queries are rotated
-#pragma unroll
-  for (int i = 0; i < DEPTH; ++i) {
-    if (step + 4 * i < end) kv_request<D>(a, kv_head, n, g, step + 4 * i, kv_pages_of(a, table, n, g, step + 4 * i), raw[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < DEPTH; ++i) pages[i] = kv_pages_of(a, table, n, g, step + 4 * (DEPTH + i));
-
+  KvRaw<D> raw;
+  KvPages next = {0, 0};
   const KvRow row = kv_row_of(a, r, kv_head, r.first + n, n < r.rows);
   kv_f16x8 q[W], q_rest[SPLIT > 0 ? W : 1];
   float factor;
   {
+    // the first step is on its way while the queries are rotated (in heads of 256 there are no registers for both)
+    KvQuery<D, SPLIT> query;
+    query.request(a, row, g);
+    const auto request = [&] {
+      if (step < end) {
+        kv_request<D, WIDE>(a, kv_head, n, g, step, kv_pages_of<WIDE>(a, table, n, g, step), raw);
+        next = kv_pages_of<WIDE>(a, table, n, g, step + 4);
+      }
+    };
+    if constexpr (D < 256) request();
     float y[D / 4];
-    kv_load_query<D>(a, row, g, y);
-    const int exponent = kv_query_exponent(kv_rotate_query<D>(a, g, y));
+    const int exponent = kv_query_exponent(query.rotate(row.token >= 0, y));
     factor = a.scale * (1.44269504088896f / D) * kv_power_of_two(exponent);
     kv_query_parts<D, SPLIT>(y, kv_power_of_two(-exponent), q, q_rest);
+    if constexpr (D == 256) request();
   }
 
   KvState st;
@@ -441,15 +635,18 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
 #pragma unroll
   for (int j = 0; j < D / 16; ++j) o[j] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const auto take_step = [&](int s, KvRaw<D> &now, KvPages &next) {
-    const bool more = s + 4 * DEPTH < end;
+  // The last step is one of its own: a request that depends on whether there is a next step is one that the compiler cannot count, and it
+  // then waits for all of them.
+  const auto take_step = [&](auto more) {
+    KvPages later = next;
+    if constexpr (more) later = kv_pages_of<WIDE>(a, table, n, g, step + 8);  // (before what is requested next: loads come back in order)
     float x[16], vs[16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       kv_f32x4 score = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < W; ++c) {
-        const kv_f16x8 codes = kv_decode8(now.k[k][c]);
+        const kv_f16x8 codes = kv_decode8(raw.k[k][c]);
         if constexpr (SPLIT > 0) score = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[c], score, 0, 0, 0);
         score = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[c], score, 0, 0, 0);
       }
@@ -457,8 +654,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
       for (int i = 0; i < 4; ++i) x[4 * k + i] = score[i];
     }
     {
-      const uint32_t kw[8] = {now.k_scale[0].x, now.k_scale[0].y, now.k_scale[0].z, now.k_scale[0].w, now.k_scale[1].x, now.k_scale[1].y, now.k_scale[1].z, now.k_scale[1].w};
-      const uint32_t vw[8] = {now.v_scale[0].x, now.v_scale[0].y, now.v_scale[0].z, now.v_scale[0].w, now.v_scale[1].x, now.v_scale[1].y, now.v_scale[1].z, now.v_scale[1].w};
+      const uint32_t kw[8] = {raw.k_scale[0].x, raw.k_scale[0].y, raw.k_scale[0].z, raw.k_scale[0].w, raw.k_scale[1].x, raw.k_scale[1].y, raw.k_scale[1].z, raw.k_scale[1].w};
+      const uint32_t vw[8] = {raw.v_scale[0].x, raw.v_scale[0].y, raw.v_scale[0].z, raw.v_scale[0].w, raw.v_scale[1].x, raw.v_scale[1].y, raw.v_scale[1].z, raw.v_scale[1].w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[2 * i] = fmaf(x[2 * i], __uint_as_float(kw[i] << 16) * factor, -st.ref);
@@ -467,9 +664,13 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
         vs[2 * i + 1] = __uint_as_float(vw[i] & 0xffff0000u);
       }
     }
-    const bool here = now.here;
-    if (more) kv_request_keys<D>(a, kv_head, n, g, s + 4 * DEPTH, next, now);
-    const int first = s * 64;
+    const bool here = raw.here;
+    // The scales' registers are free now; left to itself the compiler takes others and moves them at the end of the step, which
+    // is a wait for all that was just requested.
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(x[i]), "+v"(vs[i])::"memory");
+    if constexpr (more) kv_request_keys<D, WIDE>(a, kv_head, n, g, step + 4, next, raw);
+    const int first = step * 64;
     if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -484,7 +685,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
     kv_weights<SPLIT>(x, vs, st.sum, p, p_rest);
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-      const uint32_t w[4] = {now.v[j].x, now.v[j].y, now.v[j].z, now.v[j].w};
+      const uint32_t w[4] = {raw.v[j].x, raw.v[j].y, raw.v[j].z, raw.v[j].w};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         kv_f16x8 even, odd;
@@ -497,48 +698,47 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
         o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[half], o[2 * j + 1], 0, 0, 0);
       }
     }
-    if (more) kv_request_values<D>(a, kv_head, n, g, s + 4 * DEPTH, next, now);
-    next = kv_pages_of(a, table, n, g, s + 8 * DEPTH);
+    if constexpr (more) kv_request_values<D, WIDE>(a, kv_head, n, g, step + 4, next, raw);
+    next = later;
   };
-  for (; step < end; step += 4 * DEPTH) {
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (step + 4 * i < end) take_step(step + 4 * i, raw[i], pages[i]);
-    }
-  }
+  for (; step + 4 < end; step += 4) take_step(std::true_type{});
+  if (step < end) take_step(std::false_type{});
   st.ref = st.reference();
 
-  // the four wavefronts: neighbours first, then the two pairs, in this order
-  const auto give = [&](int place) {
-    join[place][0][lane] = st.ref;
-    join[place][1][lane] = st.sum;
+  // the four wavefronts, in their order
+  if (wave > 0) {
+    join[wave - 1][0][lane] = st.ref;
+    join[wave - 1][1][lane] = st.sum;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) join[place][2 + 4 * j + i][lane] = o[j][i];
+      for (int i = 0; i < 4; ++i) join[wave - 1][2 + 4 * j + i][lane] = o[j][i];
     }
-  };
-  const auto take = [&](int place) {
-    const float theirs = join[place][0][lane], both = fmaxf(st.ref, theirs);
-    const float mine = kv_exp2(st.ref - both), other = kv_exp2(theirs - both);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    float of[4] = {st.ref, join[0][0][lane], join[1][0][lane], join[2][0][lane]};
+    const float both = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) of[w] = kv_exp2(of[w] - both);
     st.ref = both;
-    st.sum = fmaf(st.sum, mine, join[place][1][lane] * other);
+    st.sum *= of[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) st.sum = fmaf(join[w - 1][1][lane], of[w], st.sum);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
+      if constexpr (D == 256) asm volatile("" ::: "memory");  // (all of it at once does not fit the registers)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[j][i] = fmaf(o[j][i], mine, join[place][2 + 4 * j + i][lane] * other);
+      for (int i = 0; i < 4; ++i) {
+        o[j][i] *= of[0];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) o[j][i] = fmaf(join[w - 1][2 + 4 * j + i][lane], of[w], o[j][i]);
+      }
     }
-  };
-  if (wave & 1) give(wave >> 1);
-  __syncthreads();
-  if ((wave & 1) == 0) take(wave >> 1);
-  __syncthreads();
-  if (wave == 2) give(1);
-  __syncthreads();
-  if (wave != 0) return;
-  take(1);
-  st.limit = 1.0f;  // (what R says is all there is to know now)
-  kv_finish<D>(a, row, g, part, st, o);
+    st.limit = 1.0f;  // (what R says is all there is to know now)
+    const int64_t place = (static_cast<int64_t>(kv_head) * 2 * a.few.target + part.place) * 16 + n;
+    kv_finish<D, SPLIT>(a, row, g, signs, part.count > 1 ? a.few.out + place * D : nullptr, a.few.stats + place, st, o);
+  }
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
@@ -548,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
 template <int D>
 constexpr int kv_many_waves() { return D == 256 ? 8 : 4; }
 
-template <int D, int SPLIT>
+template <int D, int SPLIT, bool WIDE>
 __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_kernel(KvAttendArgs a) {
   constexpr int WAVES = kv_many_waves<D>(), RT = kKvManyRows / 16 / WAVES;
   constexpr int C = D / 32;
@@ -558,62 +758,53 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     kv_f16x8 v[D / 32][2][2][64]; // [dimensions][half of the keys][even, odd][lane]
     float ks[64], vs[64];         // times the scale of the scores; as it is
   };
-  extern __shared__ char lds[];
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ uint32_t signs[D / 4];
+  if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   Step *steps = reinterpret_cast<Step *>(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int kv_head = blockIdx.x % a.cache.heads, part = blockIdx.y;
-  const int tile = a.many_tiles - 1 - static_cast<int>(blockIdx.x / a.cache.heads);  // a prompt's last rows see the most keys: they begin first
+  const int kv_head = blockIdx.x % a.cache.heads, group = blockIdx.x / a.cache.heads;
 
-  KvRows r;
-  {
-    int low = 0, high = a.requests + 1;
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (kv_tile_base(static_cast<int64_t>(kv_start_of(a, mid)) * a.group, mid) <= tile) low = mid; else high = mid;
-    }
-    r.request = low;
-    r.start = kv_start_of(a, low);
-    r.fresh = max(kv_start_of(a, low + 1) - r.start, 0);
-    const int64_t first = (tile - kv_tile_base(static_cast<int64_t>(r.start) * a.group, low)) * kKvManyRows, all = static_cast<int64_t>(r.fresh) * a.group;
-    if (first >= all || all <= a.few_rows) return;
-    r.first = static_cast<int>(first);
-    r.rows = static_cast<int>(min(all - first, static_cast<int64_t>(kKvManyRows)));
+  KvPart part;
+  if (a.many.target == 0) {
+    part = {{}, a.many_tiles - 1 - group, 0, 1, 0};
+    if (!kv_many_tile(a, part.tile, part.rows)) return;
+  } else if (!kv_part_of_launch<true, 64 * WAVES>(a, a.many_tiles, a.many, kv_head, group, part)) {
+    return;
   }
-  kv_keys_of(a, r);
+  const KvRows r = part.rows;
   const KvSpan span = kv_span_of(a, r, r.first, r.rows);
-  int step = (span.lowest >> 6) + part * a.part_steps;
-  int end = span.highest >= span.lowest ? (span.highest >> 6) + 1 : 0;
-  if (part + 1 < a.parts) end = min(end, step + a.part_steps);
+  const int all_steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
+  int step = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(all_steps) * part.index / part.count);
+  const int end = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(all_steps) * (part.index + 1) / part.count);
 
   // what this wavefront decodes: keys of one tile, all or half of their dimensions; values of one j, both halves of the keys or one
   const int shift = a.cache.page_shift;
   const int32_t *table = a.table + r.request * a.table_stride;
   const int k_tile = WAVES == 8 ? wave >> 1 : wave, k_from = WAVES == 8 ? (wave & 1) * KD : 0;
   const int v_j = VD == 2 ? wave >> 1 : wave, v_from = VD == 2 ? wave & 1 : 0;
+  const uint32_t in_keys = ((WIDE ? 16 * (n >> 2) : 0) + 4 * k_tile + (n & 3)) * (D / 8) + g * (D / 32) + k_from;  // dwords
+  const uint32_t in_values = (static_cast<uint32_t>(16 * v_j + n) << shift) + (WIDE ? 16 * g : 0) + 8 * v_from, in_scales = WIDE ? lane : n;
   uint32_t k_raw[KD], v_raw[VD], scale_raw = 0;
-  const auto load = [&](int s, int page_k, int page_v) {
-    const int64_t k_block = static_cast<int64_t>(max(page_k, 0)) * a.cache.heads + kv_head, v_block = static_cast<int64_t>(max(page_v, 0)) * a.cache.heads + kv_head;
-    const int in_page = (1 << shift) - 1;
-    const uint32_t *k_at = reinterpret_cast<const uint32_t *>(a.cache.k_codes) +
-                           ((k_block << shift) + ((s * 64 + 16 * (n >> 2)) & in_page) + 4 * k_tile + (n & 3)) * (D / 8) + g * (D / 32) + k_from;
-    const uint8_t *v_at = a.cache.v_codes + ((v_block * (D / 2) + 16 * v_j + n) << shift) + ((s * 64 + 16 * g) & in_page) + 8 * v_from;
+  const auto load = [&](int s, const KvPages &page) {
+    const int64_t keys = kv_tokens_at<WIDE>(a, kv_head, page.k, s, n >> 2), scales = kv_tokens_at<WIDE>(a, kv_head, page.v, s, g);
+    const uint32_t *k_at = reinterpret_cast<const uint32_t *>(a.cache.k_codes) + keys * (D / 8);
+    const uint8_t *v_at = a.cache.v_codes + ((kv_block_of(a, page.v, kv_head) * (D / 2)) << shift) + ((s * 64 + (WIDE ? 0 : 16 * g)) & ((1 << shift) - 1));
     if constexpr (KD == 2) {
-      const uint2 k = *reinterpret_cast<const uint2 *>(k_at), v = *reinterpret_cast<const uint2 *>(v_at);
+      const uint2 k = *reinterpret_cast<const uint2 *>(k_at + in_keys), v = *reinterpret_cast<const uint2 *>(v_at + in_values);
       k_raw[0] = k.x; k_raw[1] = k.y; v_raw[0] = v.x; v_raw[1] = v.y;
     } else {
-      const uint4 k = *reinterpret_cast<const uint4 *>(k_at), v = *reinterpret_cast<const uint4 *>(v_at);
+      const uint4 k = *reinterpret_cast<const uint4 *>(k_at + in_keys), v = *reinterpret_cast<const uint4 *>(v_at + in_values);
       k_raw[0] = k.x; k_raw[1] = k.y; k_raw[2] = k.z; k_raw[3] = k.w; v_raw[0] = v.x; v_raw[1] = v.y; v_raw[2] = v.z; v_raw[3] = v.w;
     }
-    if (wave < 2) scale_raw = (wave == 0 ? a.cache.k_scales : a.cache.v_scales)[(v_block << shift) + ((s * 64 + 16 * g) & in_page) + n];
+    if (wave < 2) scale_raw = ((wave == 0 ? a.cache.k_scales : a.cache.v_scales) + scales)[in_scales];
   };
-  int page_v = -1, next_k = -1, next_v = -1, later_k = -1, later_v = -1;  // of the step that is computed (v: whether its keys are there), requested, and after it
+  KvPages page = {0, 0}, next = page, later = page;  // of the step that is computed (whether its keys are there), of the one requested, and of the one after it
   if (step < end) {
-    const int page_k = kv_page_at(a, table, step * 64 + 16 * (n >> 2));
-    page_v = kv_page_at(a, table, step * 64 + 16 * g);
-    next_k = kv_page_at(a, table, (step + 1) * 64 + 16 * (n >> 2));
-    next_v = kv_page_at(a, table, (step + 1) * 64 + 16 * g);
-    load(step, page_k, page_v);
+    page = kv_pages_of<WIDE>(a, table, n, g, step);
+    next = kv_pages_of<WIDE>(a, table, n, g, step + 1);
+    load(step, page);
   }
 
   KvRow row[RT];
@@ -625,8 +816,9 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     for (int t = 0; t < RT; ++t) {
       const int at = (wave * RT + t) * 16 + n;
       row[t] = kv_row_of(a, r, kv_head, r.first + at, at < r.rows);
-      kv_load_query<D>(a, row[t], g, y[t]);
-      const float own_top = kv_rotate_query<D>(a, g, y[t]);
+      KvQuery<D, SPLIT> query;
+      query.request(a, row[t], g);
+      const float own_top = query.rotate(row[t].token >= 0, y[t]);
       top = own_top < INFINITY ? fmaxf(top, own_top) : top;  // (a broken row is its own affair)
     }
     // one power of two for the workgroup's rows: its factor goes into the keys' scales
@@ -670,21 +862,20 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   }
   if (step < end) {
     decode(steps[0]);
-    if (step + 1 < end) load(step + 1, next_k, next_v);
-    later_k = kv_page_at(a, table, (step + 2) * 64 + 16 * (n >> 2));
-    later_v = kv_page_at(a, table, (step + 2) * 64 + 16 * g);
+    if (step + 1 < end) load(step + 1, next);
+    later = kv_pages_of<WIDE>(a, table, n, g, step + 2);
   }
   for (int now = 0; step < end; ++step, now ^= 1) {
     __syncthreads();  // this step is decoded, and nobody reads the one before it any more
     const Step &from = steps[now];
-    const bool here = page_v >= 0;
+    const bool here = kv_page_there(a, page.v);
     if (step + 1 < end) {
       decode(steps[now ^ 1]);
-      if (step + 2 < end) load(step + 2, later_k, later_v);
+      if (step + 2 < end) load(step + 2, later);
     }
-    page_v = next_v; next_k = later_k; next_v = later_v;
-    later_k = kv_page_at(a, table, (step + 3) * 64 + 16 * (n >> 2));
-    later_v = kv_page_at(a, table, (step + 3) * 64 + 16 * g);
+    page = next;
+    next = later;
+    later = kv_pages_of<WIDE>(a, table, n, g, step + 3);
     const int first = step * 64;
     if (wave_rows <= 0 || first > own.highest || first + 63 < own.lowest) continue;
 
@@ -746,21 +937,32 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     }
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t) kv_finish<D>(a, row[t], g, part, st[t], o[t]);
+  for (int t = 0; t < RT; ++t) {
+    const int64_t place = (static_cast<int64_t>(kv_head) * 2 * a.many.target + part.place) * kKvManyRows + (wave * RT + t) * 16 + n;
+    kv_finish<D, SPLIT>(a, row[t], g, signs, part.count > 1 ? a.many.out + place * D : nullptr, a.many.stats + place, st[t], o[t]);
+  }
 }
 
 template <int D>
 constexpr size_t kv_many_lds() { return 2 * (4 * (D / 32) * 64 * 16 + (D / 32) * 4 * 64 * 16 + 512); }
 
-template <int D, int SPLIT>
+template <int D, int SPLIT, bool WIDE>
 bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
-  const unsigned heads = static_cast<unsigned>(a.cache.heads), parts = static_cast<unsigned>(a.parts);
+  const unsigned heads = static_cast<unsigned>(a.cache.heads);
   if (a.many_tiles > 0) {
-    if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kv_attend_many_kernel<D, SPLIT>), kv_many_lds<D>())) return false;
-    launch_kernel(kv_attend_many_kernel<D, SPLIT>, dim3(heads * a.many_tiles, parts), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
+    const auto kernel = kv_attend_many_kernel<D, SPLIT, WIDE>;
+    if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kernel), kv_many_lds<D>())) return false;
+    launch_kernel(kernel, dim3(heads * (a.many.target + a.many_tiles)), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
   }
-  if (a.few_requests > 0) launch_kernel(kv_attend_few_kernel<D, SPLIT>, dim3(heads * a.few_requests * a.few_tiles, parts), dim3(256), 0, stream, a);
+  if (a.few_requests > 0) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE>, dim3(heads * (a.few.target + a.few_requests * a.few_tiles)), dim3(256), 0, stream, a);
   return true;
+}
+
+template <int D>
+bool kv_attend_of(const KvAttendArgs &a, int split, hipStream_t stream) {
+  if (a.cache.page_shift >= 6)
+    return split == 0 ? kv_attend_launch<D, 0, true>(a, stream) : split == 1 ? kv_attend_launch<D, 1, true>(a, stream) : kv_attend_launch<D, 2, true>(a, stream);
+  return split == 0 ? kv_attend_launch<D, 0, false>(a, stream) : split == 1 ? kv_attend_launch<D, 1, false>(a, stream) : kv_attend_launch<D, 2, false>(a, stream);
 }
 
 }  // namespace oq

@@ -30,6 +30,16 @@ struct KvReadArgs {
   int64_t tokens;
 };
 
+// How a launch shares its work: for each key head, a tile's steps are cut into equal parts no longer than `longest` = max(least, all
+// tiles' steps / target), a workgroup for each, so that there are about `target` of them however many tiles there are and whatever their lengths.
+struct KvCut {
+  int target, least;  // target 0: nothing is cut
+  // The parts of tiles that are cut, of which there are at most 2 * target (a tile of n > 1 parts has more than (n - 1) * longest steps):
+  float *out;         // [key heads, 2 * target, rows of a tile, D]
+  float2 *stats;      // [key heads, 2 * target, rows of a tile]: R and l
+  int2 *map;          // [key heads, 2 * target + 1]: of a tile's first part, the tile and the number of its parts, (-1, 0) of the others; and their number
+};
+
 struct KvAttendArgs {
   KvCache cache;
   const void *q;
@@ -42,20 +52,18 @@ struct KvAttendArgs {
   int table_width, window;            // window: 0 for none
   bool causal;
   float scale;
-  // How the work is cut: tiles of the kernel for many rows (0: not launched); requests (0 likewise) and tiles of each for the one for
-  // few; the rows of a request up to which the latter has it; parts of the keys, and steps of 64 keys in one.
-  int many_tiles, few_requests, few_tiles, few_rows, parts, part_steps;
+  int few_tiles, few_requests, few_rows, few_in_tile;  // kernel for few rows: tiles of a request, requests (0: not launched), the rows of a request up to which it has it, rows of a tile at most
+  int many_tiles;                     // kernel for many rows (0: not launched)
+  KvCut few, many;
   void *out;
   float *lse;                         // NULL or [tokens, heads]
-  float *part_out;                    // where parts > 1: [parts, tokens, heads, D], and of each row R and l
-  float2 *part_stats;
 };
 
 int kv_assign_dispatch(const KvAssignArgs &a, hipStream_t stream);
 int kv_write_dispatch(const KvWriteArgs &a, int dim, int dtype, hipStream_t stream);
 int kv_read_dispatch(const KvReadArgs &a, int dim, int dtype, hipStream_t stream);
-// Cuts the work; the bytes of part_out and part_stats (0: none).
-uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new);
+// Cuts the work, whose parts go into `workspace`; the bytes that they need.
+uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new, void *workspace);
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream);
 
 }  // namespace oq
