@@ -17,9 +17,10 @@ namespace {
 // Up to three times as many where a part keeps 80 steps, so that requests of different lengths even out: 64 of up to
 // 16384, 133 us (512 workgroups: 139).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 17.9 us (six: 20).
 constexpr int kFewWhole = 16, kFewGroups = 512, kFewSteps = 80, kFewLeast = 4;
-// Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the chip, and at least 24 steps
-// of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 74 us; 2048 on their own, 264 tiles: 68 -> 97 us if they were cut.
-constexpr int kManyWhole = 384, kManyGroups = 512, kManyLeast = 24;
+// Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the workgroups that the chip holds (two on
+// a compute unit, of heads of 256 one), and at least sixteen steps of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us;
+// 2048 on their own, 264 tiles of few steps each: 68 -> 97 us if they were cut.
+constexpr int kManyGroups = 512, kManyLeast = 16;
 
 constexpr int kJoinBlocks = 4;  // workgroups of a tile, at most
 
@@ -150,7 +151,8 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
     const int64_t groups = parts < kFewGroups ? kFewGroups : parts > 3 * kFewGroups ? 3 * kFewGroups : parts;
     a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
   }
-  if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < kManyWhole) a.many.target = heads < kManyGroups ? kManyGroups / heads : 1;
+  const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
+  if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
   const uint64_t bytes = kv_places(a.few, heads, 16, dim, static_cast<char *>(workspace), 0);
   return kv_places(a.many, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }

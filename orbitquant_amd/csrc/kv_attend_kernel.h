@@ -181,6 +181,10 @@ __device__ __forceinline__ int kv_sums(int x) {
   return x;
 }
 
+__device__ __forceinline__ int kv_longer(int longest, int made, int target) {
+  return static_cast<int>(min((static_cast<int64_t>(longest) * made + target - 1) / target, static_cast<int64_t>(0x3fffffff)));
+}
+
 // Part `group` of the launch's, false behind the last.  Every workgroup counts for itself: the tiles' steps, and from those the parts.
 template <bool MANY, int THREADS>
 __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
@@ -191,8 +195,17 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
   if (tiles <= 64) {  // a lane has a tile, and no wavefront needs another: the first keys are a barrier nearer
     const int steps = lane < tiles ? steps_of(lane) : 0;
     const int total = kv_from_lane(kv_sums(steps), 63);  // (below 64 * 2^24)
-    const int longest = max((total + cut.target - 1) / cut.target, cut.least);
-    const int count = (steps + longest - 1) / longest, sum = kv_sums(count);
+    int longest = max((total + cut.target - 1) / cut.target, cut.least);
+    int count = (steps + longest - 1) / longest, sum = kv_sums(count);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // (rounding every tile's parts up makes more of them than meant)
+      const int made = kv_from_lane(sum, 63);
+      if (made > cut.target && longest < total) {
+        longest = kv_longer(longest, made, cut.target);
+        count = (steps + longest - 1) / longest;
+        sum = kv_sums(count);
+      }
+    }
     const int in_cut = count > 1 ? count : 0, cut_sum = kv_sums(in_cut);
     if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(kv_from_lane(cut_sum, 63), 0);
     const int all = kv_from_lane(sum, 63);
@@ -213,6 +226,7 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
     const int chunk = (tiles + THREADS - 1) / THREADS, from = tid * chunk, to = min(from + chunk, tiles);
     int64_t own = 0;
     for (int i = from; i < to; ++i) own += steps_of(i);
+    const int only = static_cast<int>(own);  // (of a thread with one tile)
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) own += __shfl_xor(static_cast<long long>(own), d, 64);
     if (lane == 0) wave_sums[wave] = own;
@@ -220,25 +234,32 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) total += wave_sums[w];
-    const int longest = static_cast<int>(max((total + cut.target - 1) / cut.target, static_cast<int64_t>(cut.least)));
-    int count = 0, in_cut = 0;
-    for (int i = from; i < to; ++i) {
-      const int n = (steps_of(i) + longest - 1) / longest;
-      count += n;
-      in_cut += n > 1 ? n : 0;
-    }
-    const int sum = kv_sums(count), cut_sum = kv_sums(in_cut);
-    if (lane == 63) wave_counts[wave] = make_int2(sum, cut_sum);
-    __syncthreads();
-    int ahead = sum - count, cut_ahead = cut_sum - in_cut, all = 0, all_cut = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-      if (w < wave) {
-        ahead += wave_counts[w].x;
-        cut_ahead += wave_counts[w].y;
+    int longest = static_cast<int>(max((total + cut.target - 1) / cut.target, static_cast<int64_t>(cut.least)));
+    int count, ahead, cut_ahead, all, all_cut;
+    for (int round = 0;; ++round) {
+      count = 0;
+      int in_cut = 0;
+      for (int i = from; i < to; ++i) {
+        const int n = ((chunk == 1 ? only : steps_of(i)) + longest - 1) / longest;
+        count += n;
+        in_cut += n > 1 ? n : 0;
       }
-      all += wave_counts[w].x;
-      all_cut += wave_counts[w].y;
+      const int sum = kv_sums(count), cut_sum = kv_sums(in_cut);
+      __syncthreads();
+      if (lane == 63) wave_counts[wave] = make_int2(sum, cut_sum);
+      __syncthreads();
+      ahead = sum - count; cut_ahead = cut_sum - in_cut; all = 0; all_cut = 0;
+#pragma unroll
+      for (int w = 0; w < THREADS / 64; ++w) {
+        if (w < wave) {
+          ahead += wave_counts[w].x;
+          cut_ahead += wave_counts[w].y;
+        }
+        all += wave_counts[w].x;
+        all_cut += wave_counts[w].y;
+      }
+      if (chunk > 1 || round == 2 || all <= cut.target || longest >= total) break;  // (many tiles even out by themselves)
+      longest = kv_longer(longest, all, cut.target);
     }
     if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(all_cut, 0);
     if (group >= all) return false;
