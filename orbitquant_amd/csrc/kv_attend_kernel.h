@@ -170,17 +170,6 @@ struct KvPart {
 __device__ __forceinline__ int kv_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int kv_from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 
-// Sums over the lanes up to each: within rows of sixteen, then from row to row.
-__device__ __forceinline__ int kv_sums(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-
 __device__ __forceinline__ int kv_longer(int longest, int made, int target) {
   return static_cast<int>(min((static_cast<int64_t>(longest) * made + target - 1) / target, static_cast<int64_t>(0x3fffffff)));
 }
