@@ -4,7 +4,7 @@ Public surface: `OrbitLinear`, `OrbitLinearGroup`, `OrbitQuantConfig`, `recipe`,
 (`get_rpbh_rotation`, `get_codebook`, `pack_lowbit`, `unpack_lowbit`,
 `quantize_weight`), `RTNInt4Linear` (the AdaLN INT4 linear), `load_artifact` / `save_artifact`
 (the reference's on-disk layout), `OrbitKVCache` with `kv_assign`, `kv_write`, `kv_attend` and `kv_read` (a key/value cache in
-four bits and the attention over it) and `ops` (tensor wrappers over the C ABI).
+four bits and the attention over it), `OrbitCachedAttention` (a decoder layer's, on those and the linears) and `ops` (tensor wrappers over the C ABI).
 """
 
 from .codebooks import LloydMaxCodebook, get_codebook
@@ -16,10 +16,11 @@ from . import ops  # noqa: E402
 from .kv_cache import KVAssignment, OrbitKVCache, kv_assign, kv_attend, kv_read, kv_write  # noqa: E402
 from .layers import OrbitLinear, OrbitLinearGroup  # noqa: E402
 from .adaln import RTNInt4Linear, quantize_adaln_weight  # noqa: E402
+from .attention import OrbitCachedAttention  # noqa: E402
 from .artifacts import load_artifact, save_artifact  # noqa: E402
 
 __all__ = [
-    "KVAssignment", "LloydMaxCodebook", "OrbitKVCache", "OrbitLinear", "OrbitLinearGroup", "OrbitQuantConfig", "RPBHRotation", "RTNInt4Linear", "get_codebook",
+    "KVAssignment", "LloydMaxCodebook", "OrbitCachedAttention", "OrbitKVCache", "OrbitLinear", "OrbitLinearGroup", "OrbitQuantConfig", "RPBHRotation", "RTNInt4Linear", "get_codebook",
     "get_rpbh_rotation", "kv_assign", "kv_attend", "kv_read", "kv_write", "load_artifact", "ops", "pack_lowbit", "packed_length", "quantize_adaln_weight",
     "quantize_weight", "recipe", "save_artifact", "unpack_lowbit",
 ]

@@ -77,9 +77,81 @@ class KVAssignment(NamedTuple):
     taken: torch.Tensor
 
 
+# For torch.compile the functions below are opaque ops with fake implementations; eager calls do not go through them.
+_LIB = torch.library.Library("orbitquant_amd", "FRAGMENT")
+_CACHE = "Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, Tensor signs"
+_LIB.define("kv_assign(Tensor lengths, Tensor new_lengths, Tensor(a!) block_table, Tensor free_pages, Tensor taken, SymInt page_size, SymInt tokens) "
+            "-> (Tensor, Tensor)")
+_LIB.define("kv_write(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!) v_codes, Tensor(d!) v_scales, Tensor signs) -> ()")
+_LIB.define(f"kv_read(Tensor slots, {_CACHE}, ScalarType dtype) -> (Tensor, Tensor)")
+_LIB.define(f"kv_attend(Tensor q, {_CACHE}, Tensor block_table, Tensor lengths, Tensor? starts, SymInt max_new, SymInt max_length, bool causal, "
+            "SymInt window, float scale, bool with_lse) -> (Tensor, Tensor)")
+
+
+def _assign_op(lengths, new_lengths, block_table, free_pages, taken, page_size, tokens):
+    """-> slots, and the four int32 results one behind the other (`_assigned` parts them: an op's outputs may not share memory)."""
+    _require_gpu(lengths, "lengths")
+    requests = lengths.numel()
+    lengths = _operand(lengths, "lengths", lengths, dtype=torch.int32)
+    new_lengths = _operand(new_lengths, "new_lengths", lengths, dtype=torch.int32, numel=requests)
+    free_pages = _operand(free_pages, "free_pages", lengths, dtype=torch.int32)
+    taken = _operand(taken, "taken", lengths, dtype=torch.int32, numel=1)
+    table = _table(block_table, lengths, requests)
+    tokens = int(tokens)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    slots, small = _assign_fake(lengths, None, None, None, None, None, tokens)
+    _, positions, starts, after, taken_after = _assigned(slots, small, tokens, requests)
+    with _OnDevice(lengths):
+        rc = _lib.load().oq_kv_assign(
+            lengths.data_ptr(), new_lengths.data_ptr(), requests, table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
+            free_pages.numel(), taken.data_ptr(), int(page_size), tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
+            after.data_ptr(), taken_after.data_ptr(), _stream(lengths))
+    _lib.check(rc, "oq_kv_assign")
+    return slots, small
+
+
+def _assign_fake(lengths, new_lengths, block_table, free_pages, taken, page_size, tokens):
+    return (torch.empty(tokens, dtype=torch.int64, device=lengths.device),
+            torch.empty(tokens + 2 * lengths.numel() + 2, dtype=torch.int32, device=lengths.device))
+
+
+def _assigned(slots, small, tokens, requests) -> KVAssignment:
+    return KVAssignment(slots, *small.split((tokens, requests + 1, requests, 1)))
+
+
+def _write_op(k, v, slots, *cache):
+    kv_write(k, v, slots, OrbitKVCache(*cache))
+
+
+def _read_op(slots, k_codes, k_scales, v_codes, v_scales, signs, dtype):
+    return kv_read(slots, OrbitKVCache(k_codes, k_scales, v_codes, v_scales, signs), dtype)
+
+
+def _read_fake(slots, k_codes, k_scales, v_codes, v_scales, signs, dtype):
+    shape = (slots.numel(), k_codes.shape[1], signs.shape[0])
+    return slots.new_empty(shape, dtype=dtype), slots.new_empty(shape, dtype=dtype)
+
+
+def _attend_op(q, k_codes, k_scales, v_codes, v_scales, signs, block_table, lengths, starts, max_new, max_length, causal, window, scale, with_lse):
+    got = kv_attend(q, OrbitKVCache(k_codes, k_scales, v_codes, v_scales, signs), block_table, lengths, starts=starts, max_new=max_new,
+                    max_length=max_length, causal=causal, window=window or None, scale=scale, return_lse=with_lse)
+    return got if with_lse else (got, q.new_empty((0, q.shape[1]), dtype=torch.float32))
+
+
+def _attend_fake(q, k_codes, k_scales, v_codes, v_scales, signs, block_table, lengths, starts, max_new, max_length, causal, window, scale, with_lse):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0] if with_lse else 0, q.shape[1]), dtype=torch.float32)
+
+
+for _name, _op, _fake in (("kv_assign", _assign_op, _assign_fake), ("kv_write", _write_op, lambda *args: None), ("kv_read", _read_op, _read_fake),
+                          ("kv_attend", _attend_op, _attend_fake)):
+    _LIB.impl(_name, _op, "CUDA")
+    torch.library.register_fake(f"orbitquant_amd::{_name}", _fake, lib=_LIB)
+
+
 def _module():
     """The compiled module (csrc/torch_ops.cpp), which has the usual calls of these functions without Python in between (a cached
-    token's slot 13.5 -> MODULE_US us); None where it is not built.  What it does not take, errors among it, it leaves to the Python below."""
+    token's slot 13.5 -> 5.4 us, one token decoded 19.5 -> 12.2); None where it is not built.  What it does not take, errors among it, it leaves to the Python below."""
     module = _lib.torch_ops()
     if module is None:
         _lib.warn_without_torch_ops()
@@ -129,38 +201,24 @@ def kv_assign(lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: tor
     `kv_attend` does not see.  `tokens`: the number of new tokens, as the caller's arrays have them; what `new_lengths` leaves of
     it gets slot and position -1.  lengths, new_lengths int32 [requests], block_table int32 [requests, width] (changed in
     place), free_pages int32 [any], taken int32 [1]."""
+    if torch.compiler.is_compiling():
+        return _assigned(*torch.ops.orbitquant_amd.kv_assign(lengths, new_lengths, block_table, free_pages, taken, page_size, tokens), tokens,
+                         lengths.numel())
     module = _module()
     if module is not None:
         got = module.kv_assign(lengths, new_lengths, block_table, free_pages, taken, int(page_size), int(tokens))
         if got is not None:
             return KVAssignment._make(got)
-    _require_gpu(lengths, "lengths")
-    requests = lengths.numel()
-    lengths = _operand(lengths, "lengths", lengths, dtype=torch.int32)
-    new_lengths = _operand(new_lengths, "new_lengths", lengths, dtype=torch.int32, numel=requests)
-    free_pages = _operand(free_pages, "free_pages", lengths, dtype=torch.int32)
-    taken = _operand(taken, "taken", lengths, dtype=torch.int32, numel=1)
-    table = _table(block_table, lengths, requests)
-    tokens = int(tokens)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
-    device = lengths.device
-    slots = torch.empty(tokens, dtype=torch.int64, device=device)
-    small = torch.empty(tokens + 2 * requests + 2, dtype=torch.int32, device=device)
-    positions, starts, after, taken_after = small.split((tokens, requests + 1, requests, 1))
-    with _OnDevice(lengths):
-        rc = _lib.load().oq_kv_assign(
-            lengths.data_ptr(), new_lengths.data_ptr(), requests, table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
-            free_pages.numel(), taken.data_ptr(), int(page_size), tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
-            after.data_ptr(), taken_after.data_ptr(), _stream(lengths))
-    _lib.check(rc, "oq_kv_assign")
-    return KVAssignment(slots, positions, starts, after, taken_after)
+    return _assigned(*_assign_op(lengths, new_lengths, block_table, free_pages, taken, page_size, tokens), int(tokens), lengths.numel())
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: OrbitKVCache) -> None:
     """Keys and values [tokens, heads, D] into the cache at `slots` int64 [tokens] (`oq_kv_write`).  Slots that are negative or
     beyond the last page are skipped; no slot may occur twice.  k and v: one floating type, any strides whose last is 1 (parts of
     a fused projection's output need no copy)."""
+    if torch.compiler.is_compiling():
+        torch.ops.orbitquant_amd.kv_write(k, v, slots, *cache)
+        return
     module = _module()
     if module is not None and module.kv_write(k, v, slots, cache):
         return
@@ -180,6 +238,8 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Orbit
 def kv_read(slots: torch.Tensor, cache: OrbitKVCache, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """What the cache holds at `slots` int64 [tokens], as keys and values [tokens, heads, D] of `dtype` (`oq_kv_read`); zeros for
     slots that are negative or beyond the last page."""
+    if torch.compiler.is_compiling():
+        return torch.ops.orbitquant_amd.kv_read(slots, *cache, dtype)
     module = _module()
     if module is not None:
         got = module.kv_read(slots, cache, dtype)
@@ -221,6 +281,9 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
     max_length = -1 if max_length is None else int(max_length)
     max_new = -1 if max_new is None else int(max_new)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.compiler.is_compiling():
+        out, lse = torch.ops.orbitquant_amd.kv_attend(q, *cache, block_table, lengths, starts, max_new, max_length, causal, window, scale, return_lse)
+        return (out, lse) if return_lse else out
     module = _module()
     if module is not None:
         got = module.kv_attend(q, cache, block_table, lengths, starts, max_new, max_length, bool(causal), window, scale, bool(return_lse))
