@@ -36,8 +36,8 @@ __device__ __forceinline__ void join_tile(const KvAttendArgs &a, int block, int 
   const int in_block = threadIdx.x / TPR, t = threadIdx.x % TPR, set = t / (D / 4), d = t % (D / 4);
   const int in_launch = block / blocks;
   const int kv_head = in_launch % a.cache.heads, first = in_launch / a.cache.heads;
-  const int2 *maps = cut.map + static_cast<int64_t>(kv_head) * (2 * cut.target + 1);
-  if (first >= maps[2 * cut.target].x) return;  // (the same for the block, as is what follows)
+  const int2 *maps = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
+  if (first >= maps[cut.places].x) return;  // (the same for the block, as is what follows)
   const int2 map = maps[first];
   if (map.x < 0) return;
   KvRows r;
@@ -55,7 +55,7 @@ __device__ __forceinline__ void join_tile(const KvAttendArgs &a, int block, int 
       y.z = fmaf(y.z, mine, o.z * theirs); y.w = fmaf(y.w, mine, o.w * theirs);
     };
     if (there) {
-      const int64_t place = (static_cast<int64_t>(kv_head) * 2 * cut.target + first) * TILE + in_tile;
+      const int64_t place = (static_cast<int64_t>(kv_head) * cut.places + first) * TILE + in_tile;
 #pragma unroll 4
       for (int p = set; p < map.y; p += SETS)
         add(cut.stats[place + static_cast<int64_t>(p) * TILE], reinterpret_cast<const float4 *>(cut.out + (place + static_cast<int64_t>(p) * TILE) * D)[d]);
@@ -101,22 +101,23 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, int many_b
 
 template <int D>
 void join(const KvAttendArgs &a, hipStream_t stream) {
-  const int many = a.cache.heads * 2 * a.many.target * kJoinBlocks;
+  const int many = a.cache.heads * a.many.places * kJoinBlocks;
   // Few tiles have many parts each, and a row of them is a workgroup's; many have few.
   const bool long_rows = static_cast<int64_t>(a.few_requests) * a.few_tiles * a.cache.heads < 256;
   const int in_tile = long_rows ? a.few_in_tile : (a.few_in_tile + 3) / 4, few_blocks = in_tile < kJoinBlocks ? in_tile : kJoinBlocks;
-  const dim3 grid(static_cast<unsigned>(many + a.cache.heads * 2 * a.few.target * few_blocks));
+  const dim3 grid(static_cast<unsigned>(many + a.cache.heads * a.few.places * few_blocks));
   if (long_rows) launch_kernel(kv_join_kernel<D, 256>, grid, dim3(256), 0, stream, a, many, few_blocks);
   else launch_kernel(kv_join_kernel<D, 64>, grid, dim3(256), 0, stream, a, many, few_blocks);
 }
 
-uint64_t kv_places(KvCut &cut, int heads, int rows, int dim, char *workspace, uint64_t from) {
+uint64_t kv_places(KvCut &cut, int places_a_head, int heads, int rows, int dim, char *workspace, uint64_t from) {
+  cut.places = cut.target == 0 ? 0 : places_a_head;
   if (cut.target == 0) return from;
-  const uint64_t places = 2ull * cut.target * heads * rows;
+  const uint64_t places = static_cast<uint64_t>(places_a_head) * heads * rows;
   cut.out = reinterpret_cast<float *>(workspace + from);
   cut.stats = reinterpret_cast<float2 *>(workspace + from + places * dim * sizeof(float));
   cut.map = reinterpret_cast<int2 *>(workspace + from + places * (dim + 2) * sizeof(float));
-  return from + places * (dim + 2) * sizeof(float) + (((2ull * cut.target + 1) * heads * sizeof(int2) + 15) & ~15ull);
+  return from + places * (dim + 2) * sizeof(float) + (((places_a_head + 1ull) * heads * sizeof(int2) + 15) & ~15ull);
 }
 
 }  // namespace
@@ -153,8 +154,8 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   }
   const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
   if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
-  const uint64_t bytes = kv_places(a.few, heads, 16, dim, static_cast<char *>(workspace), 0);
-  return kv_places(a.many, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
+  const uint64_t bytes = kv_places(a.few, 2 * a.few.target, heads, 16, dim, static_cast<char *>(workspace), 0);
+  return kv_places(a.many, a.many.target, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }
 
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream) {

@@ -47,6 +47,7 @@ constexpr int kv_dtype() { return SPLIT == 0 ? OQ_BF16 : SPLIT == 1 ? OQ_F16 : O
 constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
 constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
 constexpr int kKvManyRows = 128;        // rows of a workgroup of the second
+constexpr int kKvCutTiles = 384;        // tiles of a launch of the second that is cut, at most
 
 // Tiles in front of request r when its rows begin at `row`: enough for every request's last, unfilled tile.
 __host__ __device__ inline int64_t kv_tile_base(int64_t row, int64_t r) { return row / kKvManyRows + r; }
@@ -97,11 +98,13 @@ __device__ __forceinline__ int kv_start_of(const KvAttendArgs &a, int request) {
   return request <= a.requests ? min(max(a.starts[request], 0), static_cast<int>(a.tokens)) : static_cast<int>(a.tokens);
 }
 
-__device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r) {
-  r.length = r.request < a.requests ? max(a.lengths[r.request], 0) : 0;
+__device__ __forceinline__ int kv_length_of(const KvAttendArgs &a, int request) { return request < a.requests ? max(a.lengths[request], 0) : 0; }
+__device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r, int length) {
+  r.length = length;
   const int64_t reach = static_cast<int64_t>(a.table_width) << a.cache.page_shift;  // what lies behind the table is not there
   r.last_key = static_cast<int>(min(static_cast<int64_t>(r.length), reach)) - 1;
 }
+__device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r) { kv_keys_of(a, r, kv_length_of(a, r.request)); }
 
 // What rows [first, first + rows) of the run see: some row the keys lowest..highest, every row the keys all_low..all_high.
 struct KvSpan {
@@ -134,19 +137,31 @@ __device__ __forceinline__ bool kv_few_tile(const KvAttendArgs &a, int i, KvRows
   return true;
 }
 
-__device__ __forceinline__ bool kv_many_tile(const KvAttendArgs &a, int i, KvRows &r) {
+// The request that tile i belongs to; start_of(r): where its tokens begin.
+template <typename Starts>
+__device__ __forceinline__ int kv_request_of(const KvAttendArgs &a, int i, const Starts &start_of) {
   int low = 0, high = a.requests + 1;
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
-    if (kv_tile_base(static_cast<int64_t>(kv_start_of(a, mid)) * a.group, mid) <= i) low = mid; else high = mid;
+    if (kv_tile_base(static_cast<int64_t>(start_of(mid)) * a.group, mid) <= i) low = mid; else high = mid;
   }
-  r.request = low;
-  r.start = kv_start_of(a, low);
-  r.fresh = max(kv_start_of(a, low + 1) - r.start, 0);
-  const int64_t first = (i - kv_tile_base(static_cast<int64_t>(r.start) * a.group, low)) * kKvManyRows, all = static_cast<int64_t>(r.fresh) * a.group;
+  return low;
+}
+
+// Its rows, r.request, r.start and r.fresh known.
+__device__ __forceinline__ bool kv_rows_of(const KvAttendArgs &a, int i, KvRows &r) {
+  const int64_t first = (i - kv_tile_base(static_cast<int64_t>(r.start) * a.group, r.request)) * kKvManyRows, all = static_cast<int64_t>(r.fresh) * a.group;
   if (first >= all || all <= a.few_rows) return false;
   r.first = static_cast<int>(first);
   r.rows = static_cast<int>(min(all - first, static_cast<int64_t>(kKvManyRows)));
+  return true;
+}
+
+__device__ __forceinline__ bool kv_many_tile(const KvAttendArgs &a, int i, KvRows &r) {
+  r.request = kv_request_of(a, i, [&](int request) { return kv_start_of(a, request); });
+  r.start = kv_start_of(a, r.request);
+  r.fresh = max(kv_start_of(a, r.request + 1) - r.start, 0);
+  if (!kv_rows_of(a, i, r)) return false;
   kv_keys_of(a, r);
   return true;
 }
@@ -160,12 +175,14 @@ __device__ __forceinline__ bool kv_tile(const KvAttendArgs &a, int i, KvRows &r)
 __device__ __forceinline__ int kv_steps_of(const KvSpan &span) {  // one for a tile without keys: somebody writes its zeros
   return span.highest >= span.lowest ? (span.highest >> 6) - (span.lowest >> 6) + 1 : 1;
 }
+__device__ __forceinline__ int kv_counted_steps(const KvSpan &span) { return min(kv_steps_of(span), 1 << 22); }  // sums of some hundred tiles stay below 2^31
 
 // A workgroup's part of a tile.
 struct KvPart {
   KvRows rows;
   int tile, index, count;  // of the tile's parts
   int place;               // of the part among those of cut tiles
+  __device__ __forceinline__ int from(int steps, int i) const { return steps / count * i + min(steps % count, i); }  // where part i begins
 };
 __device__ __forceinline__ int kv_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int kv_from_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
@@ -175,15 +192,15 @@ __device__ __forceinline__ int kv_longer(int longest, int made, int target) {
 }
 
 // Part `group` of the launch's, false behind the last.  Every workgroup counts for itself: the tiles' steps, and from those the parts.
-template <bool MANY, int THREADS>
-__device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
+template <int THREADS>
+__device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   KvRows r = {};
-  const auto steps_of = [&](int i) { return kv_tile<MANY>(a, i, r) ? kv_steps_of(kv_span_of(a, r, r.first, r.rows)) : 0; };
-  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (2 * cut.target + 1);
+  const auto steps_of = [&](int i) { return kv_few_tile(a, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0; };
+  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
   if (tiles <= 64) {  // a lane has a tile, and no wavefront needs another: the first keys are a barrier nearer
     const int steps = lane < tiles ? steps_of(lane) : 0;
-    const int total = kv_from_lane(kv_sums(steps), 63);  // (below 64 * 2^24)
+    const int total = kv_from_lane(kv_sums(steps), 63);
     int longest = max((total + cut.target - 1) / cut.target, cut.least);
     int count = (steps + longest - 1) / longest, sum = kv_sums(count);
 #pragma unroll
@@ -196,14 +213,13 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
       }
     }
     const int in_cut = count > 1 ? count : 0, cut_sum = kv_sums(in_cut);
-    if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(kv_from_lane(cut_sum, 63), 0);
+    if (group == 0 && tid == 0) map[cut.places] = make_int2(kv_from_lane(cut_sum, 63), 0);
     const int all = kv_from_lane(sum, 63);
     if (group >= all) return false;
-    const int at = MANY ? all - 1 - group : group;  // a prompt's last rows see the most keys: they begin first
-    const int found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > at));
+    const int found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > group));
     part.tile = found;
     part.count = kv_from_lane(count, found);
-    part.index = at - kv_from_lane(sum - count, found);
+    part.index = group - kv_from_lane(sum - count, found);
     part.place = kv_from_lane(cut_sum - in_cut, found) + part.index;
     part.rows = {kv_from_lane(r.request, found), kv_from_lane(r.start, found), kv_from_lane(r.fresh, found), kv_from_lane(r.length, found),
                  kv_from_lane(r.first, found), kv_from_lane(r.rows, found), kv_from_lane(r.last_key, found)};
@@ -250,20 +266,19 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
       if (chunk > 1 || round == 2 || all <= cut.target || longest >= total) break;  // (many tiles even out by themselves)
       longest = kv_longer(longest, all, cut.target);
     }
-    if (group == 0 && tid == 0) map[2 * cut.target] = make_int2(all_cut, 0);
+    if (group == 0 && tid == 0) map[cut.places] = make_int2(all_cut, 0);
     if (group >= all) return false;
-    const int at = MANY ? all - 1 - group : group;
-    if (at >= ahead && at < ahead + count) {
+    if (group >= ahead && group < ahead + count) {
       int i = from, n = (steps_of(i) + longest - 1) / longest;
-      while (at >= ahead + n) {
+      while (group >= ahead + n) {
         ahead += n;
         cut_ahead += n > 1 ? n : 0;
         n = (steps_of(++i) + longest - 1) / longest;
       }
       found[0] = i;
       found[1] = n;
-      found[2] = at - ahead;
-      found[3] = cut_ahead + at - ahead;
+      found[2] = group - ahead;
+      found[3] = cut_ahead + group - ahead;
       found_rows = r;
     }
     __syncthreads();
@@ -274,6 +289,135 @@ __device__ __forceinline__ bool kv_part_of_launch(const KvAttendArgs &a, int til
     part.rows = {kv_uniform(found_rows.request), kv_uniform(found_rows.start), kv_uniform(found_rows.fresh), kv_uniform(found_rows.length),
                  kv_uniform(found_rows.first), kv_uniform(found_rows.rows), kv_uniform(found_rows.last_key)};
   }
+  if (part.count > 1 && tid == 0) map[part.place] = part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0);
+  return true;
+}
+
+// The same for the many rows of a launch that is cut, whose tiles are fewer than its parts (so that `target` parts are enough).  Parts
+// of one tile are equal, but those of different tiles are not, some half of the others, and two workgroups share a compute unit: the first
+// half of the launch has the long ones, the longest first, the second the short ones, the shortest first, and so a long one's
+// neighbour is short.  (Parts of 19 to 46 steps, 480 of them, D = 64, fp16: 103 -> 87 us
+// with as many parts as there are places for; 532 parts before, whose last twenty began when the others ended.)
+struct KvCounted {
+  int starts[kKvCutTiles + 2], lengths[kKvCutTiles + 2];  // of the requests
+  int steps[kKvCutTiles], requests[kKvCutTiles];          // of the tiles
+};
+template <int THREADS>
+__device__ __forceinline__ bool kv_many_part(const KvAttendArgs &a, int kv_head, int group, KvCounted &counted, KvPart &part) {
+  constexpr int HELD = kKvCutTiles / 64, CLASSES = 8;
+  const int tid = threadIdx.x, lane = tid & 63, tiles = a.many_tiles;
+  const KvCut &cut = a.many;
+  for (int i = tid; i <= a.requests + 1; i += THREADS) {
+    counted.starts[i] = kv_start_of(a, i);
+    counted.lengths[i] = kv_length_of(a, i);
+  }
+  __syncthreads();
+  const auto rows_of = [&](int request, int i, KvRows &r) {
+    r.request = request;
+    r.start = counted.starts[request];
+    r.fresh = max(counted.starts[request + 1] - r.start, 0);
+    kv_keys_of(a, r, counted.lengths[request]);
+    return kv_rows_of(a, i, r);
+  };
+  for (int i = tid; i < tiles; i += THREADS) {
+    KvRows r;
+    const int request = kv_request_of(a, i, [&](int request) { return counted.starts[request]; });
+    counted.steps[i] = rows_of(request, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0;
+    counted.requests[i] = request;
+  }
+  __syncthreads();
+  // From here on every wavefront counts for itself: a lane has `held` tiles.
+  const int held = (tiles + 63) >> 6;
+  int steps[HELD], count[HELD], total = 0;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    steps[h] = h < held && lane * held + h < tiles ? counted.steps[lane * held + h] : 0;
+    total += steps[h];
+  }
+  total = kv_from_lane(kv_sums(total), 63);
+  // No more parts than meant, and rounding every tile's up makes half a part more of each.  Four times total / target is enough
+  // whatever the tiles, as they are fewer than three quarters of the parts.
+  int longest = max(static_cast<int>(static_cast<float>(total) / (static_cast<float>(cut.target) - 0.5f * static_cast<float>(tiles))) + 1, cut.least);
+  const int enough = max(static_cast<int>(min(4 * ((static_cast<int64_t>(total) + cut.target - 1) / cut.target), static_cast<int64_t>(0x3fffffff))), longest);
+  int all, in_lane, in_cut;
+  for (int round = 0;; ++round) {
+    const float by = 1.0f / static_cast<float>(longest);
+    in_lane = in_cut = 0;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      if (h < held) {
+        int n = static_cast<int>(static_cast<float>(steps[h]) * by);  // (below 2^12, so one off at most)
+        n += n * longest < steps[h] ? 1 : 0;
+        n += n * longest < steps[h] ? 1 : 0;
+        n -= n > 0 && (n - 1) * longest >= steps[h] ? 1 : 0;
+        count[h] = n;
+        in_lane += n;
+        in_cut += n > 1 ? n : 0;
+      } else {
+        count[h] = 0;
+      }
+    }
+    all = kv_from_lane(kv_sums(in_lane), 63);
+    if (all <= cut.target || longest >= enough) break;
+    longest = round < 6 ? min(kv_longer(longest, all, cut.target), enough) : enough;
+  }
+  // Parts by length, in classes of longest / 16, all below half of it in the last; two classes' sums in one number (each below 2^16).
+  int classes[CLASSES / 2] = {}, kind[HELD];
+  const float by = 2.0f * CLASSES / static_cast<float>(longest);
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    kind[h] = CLASSES;
+    if (h < held) {
+      const float length = static_cast<float>(steps[h]) * __builtin_amdgcn_rcpf(static_cast<float>(max(count[h], 1)));
+      kind[h] = max(min(static_cast<int>(2.0f * CLASSES - length * by), CLASSES - 1), 0);
+#pragma unroll
+      for (int c = 0; c < CLASSES / 2; ++c) classes[c] += kind[h] >> 1 == c ? count[h] << (16 * (kind[h] & 1)) : 0;
+    }
+  }
+  const int cut_sum = kv_sums(in_cut);
+  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
+  if (group == 0 && tid == 0) map[cut.places] = make_int2(kv_from_lane(cut_sum, 63), 0);
+  if (group >= all) return false;
+  const int half = (cut.target + 1) >> 1;
+  int at = group < half ? group : all - 1 - (group - half), found = 0, found_kind = CLASSES;
+#pragma unroll
+  for (int c = 0; c < CLASSES; c += 2) {
+    const int sums = kv_sums(classes[c >> 1]), sum = kv_from_lane(sums, 63);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int up_to = sums >> (16 * e) & 0xffff, its = sum >> (16 * e) & 0xffff;
+      if (found_kind == CLASSES) {
+        if (at < its) {
+          found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up_to > at));
+          at -= kv_from_lane(up_to - (classes[c >> 1] >> (16 * e) & 0xffff), found);
+          found_kind = c + e;
+        } else {
+          at -= its;
+        }
+      }
+    }
+  }
+  part.place = kv_from_lane(cut_sum - in_cut, found);
+  part.tile = -1;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    if (h < held && part.tile < 0) {
+      const int n = kv_from_lane(count[h], found), of_kind = kv_from_lane(kind[h], found);
+      if (of_kind == found_kind && at < n) {
+        part.tile = found * held + h;
+        part.count = n;
+      } else {
+        at -= of_kind == found_kind ? n : 0;
+        part.place += n > 1 ? n : 0;
+      }
+    }
+  }
+  part.index = at;
+  part.place += at;
+  rows_of(counted.requests[part.tile], part.tile, part.rows);
+  part.rows = {kv_uniform(part.rows.request), kv_uniform(part.rows.start), kv_uniform(part.rows.fresh), kv_uniform(part.rows.length),
+               kv_uniform(part.rows.first), kv_uniform(part.rows.rows), kv_uniform(part.rows.last_key)};
+  __syncthreads();  // (the memory is somebody else's from here on)
   if (part.count > 1 && tid == 0) map[part.place] = part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0);
   return true;
 }
@@ -606,14 +750,14 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   if (a.few.target == 0) {
     part = {{}, group, 0, 1, 0};
     if (!kv_few_tile(a, group, part.rows)) return;
-  } else if (!kv_part_of_launch<false, 256>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
+  } else if (!kv_few_part<256>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
     return;
   }
   const KvRows r = part.rows;
   const KvSpan span = kv_span_of(a, r, r.first, r.rows);
   const int steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
-  int step = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(steps) * part.index / part.count) + wave;
-  const int end = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(steps) * (part.index + 1) / part.count);
+  int step = (span.lowest >> 6) + part.from(steps, part.index) + wave;
+  const int end = (span.lowest >> 6) + part.from(steps, part.index + 1);
 
   const int32_t *table = a.table + r.request * a.table_stride;
   KvRaw<D> raw;
@@ -746,7 +890,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
       }
     }
     st.limit = 1.0f;  // (what R says is all there is to know now)
-    const int64_t place = (static_cast<int64_t>(kv_head) * 2 * a.few.target + part.place) * 16 + n;
+    const int64_t place = (static_cast<int64_t>(kv_head) * a.few.places + part.place) * 16 + n;
     kv_finish<D, SPLIT>(a, row, g, signs, part.count > 1 ? a.few.out + place * D : nullptr, a.few.stats + place, st, o);
   }
 }
@@ -780,14 +924,14 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   if (a.many.target == 0) {
     part = {{}, a.many_tiles - 1 - group, 0, 1, 0};
     if (!kv_many_tile(a, part.tile, part.rows)) return;
-  } else if (!kv_part_of_launch<true, 64 * WAVES>(a, a.many_tiles, a.many, kv_head, group, part)) {
+  } else if (!kv_many_part<64 * WAVES>(a, kv_head, group, *reinterpret_cast<KvCounted *>(lds), part)) {
     return;
   }
   const KvRows r = part.rows;
   const KvSpan span = kv_span_of(a, r, r.first, r.rows);
   const int all_steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
-  int step = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(all_steps) * part.index / part.count);
-  const int end = (span.lowest >> 6) + static_cast<int>(static_cast<int64_t>(all_steps) * (part.index + 1) / part.count);
+  int step = (span.lowest >> 6) + part.from(all_steps, part.index);
+  const int end = (span.lowest >> 6) + part.from(all_steps, part.index + 1);
 
   // what this wavefront decodes: keys of one tile, all or half of their dimensions; values of one j, both halves of the keys or one
   const int shift = a.cache.page_shift;
@@ -810,6 +954,14 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     }
     if (wave < 2) scale_raw = ((wave == 0 ? a.cache.k_scales : a.cache.v_scales) + scales)[in_scales];
   };
+  KvRow row[RT];
+  KvQuery<D, SPLIT> query[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int at = (wave * RT + t) * 16 + n;
+    row[t] = kv_row_of(a, r, kv_head, r.first + at, at < r.rows);
+    query[t].request(a, row[t], g);
+  }
   KvPages page = {0, 0}, next = page, later = page;  // of the step that is computed (whether its keys are there), of the one requested, and of the one after it
   if (step < end) {
     page = kv_pages_of<WIDE>(a, table, n, g, step);
@@ -817,18 +969,13 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     load(step, page);
   }
 
-  KvRow row[RT];
   kv_f16x8 q[RT][C], q_rest[RT][SPLIT > 0 ? C : 1];
   float factor;
   {
     float y[RT][D / 4], top = 0.0f;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int at = (wave * RT + t) * 16 + n;
-      row[t] = kv_row_of(a, r, kv_head, r.first + at, at < r.rows);
-      KvQuery<D, SPLIT> query;
-      query.request(a, row[t], g);
-      const float own_top = query.rotate(row[t].token >= 0, y[t]);
+      const float own_top = query[t].rotate(row[t].token >= 0, y[t]);
       top = own_top < INFINITY ? fmaxf(top, own_top) : top;  // (a broken row is its own affair)
     }
     // one power of two for the workgroup's rows: its factor goes into the keys' scales
@@ -948,7 +1095,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const int64_t place = (static_cast<int64_t>(kv_head) * 2 * a.many.target + part.place) * kKvManyRows + (wave * RT + t) * 16 + n;
+    const int64_t place = (static_cast<int64_t>(kv_head) * a.many.places + part.place) * kKvManyRows + (wave * RT + t) * 16 + n;
     kv_finish<D, SPLIT>(a, row[t], g, signs, part.count > 1 ? a.many.out + place * D : nullptr, a.many.stats + place, st[t], o[t]);
   }
 }
@@ -962,7 +1109,7 @@ bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
   if (a.many_tiles > 0) {
     const auto kernel = kv_attend_many_kernel<D, SPLIT, WIDE>;
     if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kernel), kv_many_lds<D>())) return false;
-    launch_kernel(kernel, dim3(heads * (a.many.target + a.many_tiles)), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
+    launch_kernel(kernel, dim3(heads * (a.many.target != 0 ? a.many.target : a.many_tiles)), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
   }
   if (a.few_requests > 0) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE>, dim3(heads * (a.few.target + a.few_requests * a.few_tiles)), dim3(256), 0, stream, a);
   return true;

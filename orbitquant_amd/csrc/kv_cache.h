@@ -31,13 +31,14 @@ struct KvReadArgs {
 };
 
 // How a launch shares its work: for each key head, a tile's steps are cut into equal parts no longer than `longest` = max(least, all
-// tiles' steps / target), a workgroup for each, so that there are about `target` of them however many tiles there are and whatever their lengths.
+// tiles' steps / target), a workgroup for each, so that there are about `target` of them however many tiles there are and whatever their lengths
+// (of many rows, where a launch is cut only if it has fewer tiles than that, no more than `target`).
 struct KvCut {
   int target, least;  // target 0: nothing is cut
-  // The parts of tiles that are cut, of which there are at most 2 * target (a tile of n > 1 parts has more than (n - 1) * longest steps):
-  float *out;         // [key heads, 2 * target, rows of a tile, D]
-  float2 *stats;      // [key heads, 2 * target, rows of a tile]: R and l
-  int2 *map;          // [key heads, 2 * target + 1]: of a tile's first part, the tile and the number of its parts, (-1, 0) of the others; and their number
+  int places;         // for the parts of tiles that are cut: of few rows 2 * target (a tile of n > 1 parts has more than (n - 1) * longest steps), of many target
+  float *out;         // [key heads, places, rows of a tile, D]
+  float2 *stats;      // [key heads, places, rows of a tile]: R and l
+  int2 *map;          // [key heads, places + 1]: of a tile's first part, the tile and the number of its parts, (-1, 0) of the others; and their number
 };
 
 struct KvAttendArgs {
