@@ -14,9 +14,9 @@ namespace {
 // How launches are cut (MI355X, D = 128; a step is 64 keys).
 // Few rows.  One launch and no join up to sixteen steps: 1003 tokens, 32 heads, 10.7 us, cut into fours 11.3.  Above, 512 workgroups or more, two on
 // each compute unit at once: 131101 tokens, 8 heads, 34.6 us (1024: 39.7, 256: 35.0); sixteen requests of up to 4096, 27.2 with the rest of their step (1024: 31).
-// Up to three times as many where a part keeps 80 steps, so that requests of different lengths even out: 64 of up to
-// 16384, 133 us (512 workgroups: 139).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 17.9 us (six: 20).
-constexpr int kFewWhole = 16, kFewGroups = 512, kFewSteps = 80, kFewLeast = 4;
+// Up to three times as many where a part keeps 60 steps, so that requests of different lengths even out, the longest parts first: 64 of up to
+// 16384, 130 us (512 workgroups: 139; four times: 132), 128 of up to 4096, 81 us (80 steps: 83).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 17.9 us (six: 20).
+constexpr int kFewWhole = 16, kFewGroups = 512, kFewSteps = 60, kFewLeast = 4;
 // Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the workgroups that the chip holds (two on
 // a compute unit, of heads of 256 one), and at least sixteen steps of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us;
 // 2048 on their own, 264 tiles of few steps each: 68 -> 97 us if they were cut.
@@ -145,11 +145,13 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   if (a.window != 0 && keys > a.window + max_new) keys = a.window + max_new + 63;
   const int64_t steps = (keys + 63) / 64;
   a.few.target = a.many.target = 0;
+  a.few.sorted = false;
   a.few.least = kFewLeast;
   a.many.least = kManyLeast;
   if (a.few_requests > 0 && steps > kFewWhole) {
     const int64_t parts = static_cast<int64_t>(a.requests) * steps * heads / kFewSteps;
     const int64_t groups = parts < kFewGroups ? kFewGroups : parts > 3 * kFewGroups ? 3 * kFewGroups : parts;
+    a.few.sorted = groups > kFewGroups;
     a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
   }
   const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;

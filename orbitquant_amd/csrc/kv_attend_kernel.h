@@ -192,37 +192,150 @@ __device__ __forceinline__ int kv_longer(int longest, int made, int target) {
 }
 
 // Part `group` of the launch's, false behind the last.  Every workgroup counts for itself: the tiles' steps, and from those the parts.
+//
+// Up to kKvCutTiles tiles every wavefront does so, a lane for `held` tiles in a row.  Parts of one tile are equal, but those of different tiles are
+// not, some half of the others, so the long ones come first where there are more than the chip holds at once (64 requests of 3300 to 16384
+// tokens: 134 -> 130 us; where there are not, it would cost 0.4).
+// Many rows have no more parts than the chip holds at once, two on a compute unit: there the second half of the launch goes the other
+// way, and a long one's neighbour is short (parts of 19 to 46 steps, 480 of them, D = 64, fp16: 103 -> 87 us with both;
+// 532 parts before, whose last twenty began when the others ended).
+struct KvPick {
+  int tile, lane, all_cut;  // (the lane whose tile it is; the number of all parts of cut tiles)
+};
+template <bool MANY, int HELD>
+__device__ __forceinline__ bool kv_pick(const KvCut &cut, int tiles, int held, const int (&steps)[HELD], int group, KvPart &part, KvPick &pick) {
+  constexpr int CLASSES = 8;
+  int total = 0;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) total += steps[h];
+  total = kv_from_lane(kv_sums(total), 63);
+  int longest = max((total + cut.target - 1) / cut.target, cut.least), enough = total, rounds = 2;
+  if constexpr (MANY) {
+    // No more parts than `target`, and rounding every tile's up makes half a part more of each.  Four times total / target is enough
+    // whatever the tiles, as they are fewer than three quarters of the parts.
+    const int share = (total + cut.target - 1) / cut.target;
+    longest = max(static_cast<int>(static_cast<float>(total) / (static_cast<float>(cut.target) - 0.5f * static_cast<float>(tiles))) + 1, cut.least);
+    enough = max(static_cast<int>(min(4 * static_cast<int64_t>(share), static_cast<int64_t>(0x3fffffff))), longest);
+    rounds = 6;
+  }
+  int count[HELD], all, in_lane, in_cut;
+  for (int round = 0;; ++round) {
+    const float by = 1.0f / static_cast<float>(longest);
+    in_lane = in_cut = 0;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      count[h] = 0;
+      if (h < held) {
+        int n = static_cast<int>(static_cast<float>(steps[h]) * by);  // (below 2^12, so one off at most)
+        n += n * longest < steps[h] ? 1 : 0;
+        n += n * longest < steps[h] ? 1 : 0;
+        n -= n > 0 && (n - 1) * longest >= steps[h] ? 1 : 0;
+        count[h] = n;
+        in_lane += n;
+        in_cut += n > 1 ? n : 0;
+      }
+    }
+    all = kv_from_lane(kv_sums(in_lane), 63);
+    if (all <= cut.target || longest >= enough || (!MANY && round == rounds)) break;
+    longest = MANY && round >= rounds ? enough : min(kv_longer(longest, all, cut.target), enough);
+  }
+  const int cut_sum = kv_sums(in_cut);
+  pick.all_cut = kv_from_lane(cut_sum, 63);
+  if (group >= all) return false;
+  int at, found = 0, found_kind = CLASSES, kind[HELD] = {};
+  if (!MANY && !cut.sorted) {
+    const int sums = kv_sums(in_lane);
+    found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sums > group));
+    at = group - kv_from_lane(sums - in_lane, found);
+    found_kind = 0;
+  } else {
+    // Parts by length, in classes of longest / 16, all below half of it in the last; two classes' sums in one number (each below 2^16).
+    int classes[CLASSES / 2] = {};
+    const float by = 2.0f * CLASSES / static_cast<float>(longest);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      kind[h] = CLASSES;
+      if (h < held) {
+        const float length = static_cast<float>(steps[h]) * __builtin_amdgcn_rcpf(static_cast<float>(max(count[h], 1)));
+        kind[h] = max(min(static_cast<int>(2.0f * CLASSES - length * by), CLASSES - 1), 0);
+#pragma unroll
+        for (int c = 0; c < CLASSES / 2; ++c) classes[c] += kind[h] >> 1 == c ? count[h] << (16 * (kind[h] & 1)) : 0;
+      }
+    }
+    const int half = (cut.target + 1) >> 1;
+    at = !MANY || group < half ? group : all - 1 - (group - half);
+#pragma unroll
+    for (int c = 0; c < CLASSES; c += 2) {
+      const int sums = kv_sums(classes[c >> 1]), sum = kv_from_lane(sums, 63);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int up_to = sums >> (16 * e) & 0xffff, its = sum >> (16 * e) & 0xffff;
+        if (found_kind == CLASSES) {
+          if (at < its) {
+            found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up_to > at));
+            at -= kv_from_lane(up_to - (classes[c >> 1] >> (16 * e) & 0xffff), found);
+            found_kind = c + e;
+          } else {
+            at -= its;
+          }
+        }
+      }
+    }
+  }
+  part.place = kv_from_lane(cut_sum - in_cut, found);
+  pick.lane = found;
+  pick.tile = -1;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    if (h < held && pick.tile < 0) {
+      const int n = kv_from_lane(count[h], found), of_kind = kv_from_lane(kind[h], found);
+      if (of_kind == found_kind && at < n) {
+        pick.tile = found * held + h;
+        part.count = n;
+      } else {
+        at -= of_kind == found_kind ? n : 0;
+        part.place += n > 1 ? n : 0;
+      }
+    }
+  }
+  part.tile = pick.tile;
+  part.index = at;
+  part.place += at;
+  return true;
+}
+__device__ __forceinline__ KvRows kv_uniform(const KvRows &r) {
+  return {kv_uniform(r.request), kv_uniform(r.start), kv_uniform(r.fresh), kv_uniform(r.length), kv_uniform(r.first), kv_uniform(r.rows), kv_uniform(r.last_key)};
+}
+__device__ __forceinline__ int2 *kv_map_of(const KvCut &cut, int kv_head) { return cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1); }
+__device__ __forceinline__ int2 kv_map_entry(const KvPart &part) { return part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0); }
+
 template <int THREADS>
 __device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   KvRows r = {};
   const auto steps_of = [&](int i) { return kv_few_tile(a, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0; };
-  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
-  if (tiles <= 64) {  // a lane has a tile, and no wavefront needs another: the first keys are a barrier nearer
-    const int steps = lane < tiles ? steps_of(lane) : 0;
-    const int total = kv_from_lane(kv_sums(steps), 63);
-    int longest = max((total + cut.target - 1) / cut.target, cut.least);
-    int count = (steps + longest - 1) / longest, sum = kv_sums(count);
+  int2 *const map = kv_map_of(cut, kv_head);
+  if (tiles <= kKvCutTiles) {  // no wavefront needs another: the first keys are a barrier nearer
+    bool there;
+    KvPick pick;
+    if (tiles <= 64) {
+      const int steps[1] = {lane < tiles ? steps_of(lane) : 0};
+      there = kv_pick<false>(cut, tiles, 1, steps, group, part, pick);
+      if (there) part.rows = {kv_from_lane(r.request, pick.lane), kv_from_lane(r.start, pick.lane), kv_from_lane(r.fresh, pick.lane), kv_from_lane(r.length, pick.lane),
+                              kv_from_lane(r.first, pick.lane), kv_from_lane(r.rows, pick.lane), kv_from_lane(r.last_key, pick.lane)};
+    } else {
+      const int held = (tiles + 63) >> 6;
+      int steps[kKvCutTiles / 64];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // (rounding every tile's parts up makes more of them than meant)
-      const int made = kv_from_lane(sum, 63);
-      if (made > cut.target && longest < total) {
-        longest = kv_longer(longest, made, cut.target);
-        count = (steps + longest - 1) / longest;
-        sum = kv_sums(count);
+      for (int h = 0; h < kKvCutTiles / 64; ++h) steps[h] = h < held && lane * held + h < tiles ? steps_of(lane * held + h) : 0;
+      there = kv_pick<false>(cut, tiles, held, steps, group, part, pick);
+      if (there) {
+        kv_few_tile(a, part.tile, r);
+        part.rows = kv_uniform(r);
       }
     }
-    const int in_cut = count > 1 ? count : 0, cut_sum = kv_sums(in_cut);
-    if (group == 0 && tid == 0) map[cut.places] = make_int2(kv_from_lane(cut_sum, 63), 0);
-    const int all = kv_from_lane(sum, 63);
-    if (group >= all) return false;
-    const int found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > group));
-    part.tile = found;
-    part.count = kv_from_lane(count, found);
-    part.index = group - kv_from_lane(sum - count, found);
-    part.place = kv_from_lane(cut_sum - in_cut, found) + part.index;
-    part.rows = {kv_from_lane(r.request, found), kv_from_lane(r.start, found), kv_from_lane(r.fresh, found), kv_from_lane(r.length, found),
-                 kv_from_lane(r.first, found), kv_from_lane(r.rows, found), kv_from_lane(r.last_key, found)};
+    if (group == 0 && tid == 0) map[cut.places] = make_int2(pick.all_cut, 0);
+    if (!there) return false;
   } else {
     __shared__ int64_t wave_sums[THREADS / 64];
     __shared__ int2 wave_counts[THREADS / 64];
@@ -286,27 +399,21 @@ __device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, co
     part.count = kv_uniform(found[1]);
     part.index = kv_uniform(found[2]);
     part.place = kv_uniform(found[3]);
-    part.rows = {kv_uniform(found_rows.request), kv_uniform(found_rows.start), kv_uniform(found_rows.fresh), kv_uniform(found_rows.length),
-                 kv_uniform(found_rows.first), kv_uniform(found_rows.rows), kv_uniform(found_rows.last_key)};
+    part.rows = kv_uniform(found_rows);
   }
-  if (part.count > 1 && tid == 0) map[part.place] = part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0);
+  if (part.count > 1 && tid == 0) map[part.place] = kv_map_entry(part);
   return true;
 }
 
-// The same for the many rows of a launch that is cut, whose tiles are fewer than its parts (so that `target` parts are enough).  Parts
-// of one tile are equal, but those of different tiles are not, some half of the others, and two workgroups share a compute unit: the first
-// half of the launch has the long ones, the longest first, the second the short ones, the shortest first, and so a long one's
-// neighbour is short.  (Parts of 19 to 46 steps, 480 of them, D = 64, fp16: 103 -> 87 us
-// with as many parts as there are places for; 532 parts before, whose last twenty began when the others ended.)
+// For many rows requests and tiles are looked up once a workgroup.
 struct KvCounted {
   int starts[kKvCutTiles + 2], lengths[kKvCutTiles + 2];  // of the requests
   int steps[kKvCutTiles], requests[kKvCutTiles];          // of the tiles
 };
 template <int THREADS>
 __device__ __forceinline__ bool kv_many_part(const KvAttendArgs &a, int kv_head, int group, KvCounted &counted, KvPart &part) {
-  constexpr int HELD = kKvCutTiles / 64, CLASSES = 8;
+  constexpr int HELD = kKvCutTiles / 64;
   const int tid = threadIdx.x, lane = tid & 63, tiles = a.many_tiles;
-  const KvCut &cut = a.many;
   for (int i = tid; i <= a.requests + 1; i += THREADS) {
     counted.starts[i] = kv_start_of(a, i);
     counted.lengths[i] = kv_length_of(a, i);
@@ -319,106 +426,26 @@ __device__ __forceinline__ bool kv_many_part(const KvAttendArgs &a, int kv_head,
     kv_keys_of(a, r, counted.lengths[request]);
     return kv_rows_of(a, i, r);
   };
+  KvRows r;
   for (int i = tid; i < tiles; i += THREADS) {
-    KvRows r;
     const int request = kv_request_of(a, i, [&](int request) { return counted.starts[request]; });
     counted.steps[i] = rows_of(request, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0;
     counted.requests[i] = request;
   }
   __syncthreads();
-  // From here on every wavefront counts for itself: a lane has `held` tiles.
   const int held = (tiles + 63) >> 6;
-  int steps[HELD], count[HELD], total = 0;
+  int steps[HELD];
 #pragma unroll
-  for (int h = 0; h < HELD; ++h) {
-    steps[h] = h < held && lane * held + h < tiles ? counted.steps[lane * held + h] : 0;
-    total += steps[h];
-  }
-  total = kv_from_lane(kv_sums(total), 63);
-  // No more parts than meant, and rounding every tile's up makes half a part more of each.  Four times total / target is enough
-  // whatever the tiles, as they are fewer than three quarters of the parts.
-  int longest = max(static_cast<int>(static_cast<float>(total) / (static_cast<float>(cut.target) - 0.5f * static_cast<float>(tiles))) + 1, cut.least);
-  const int enough = max(static_cast<int>(min(4 * ((static_cast<int64_t>(total) + cut.target - 1) / cut.target), static_cast<int64_t>(0x3fffffff))), longest);
-  int all, in_lane, in_cut;
-  for (int round = 0;; ++round) {
-    const float by = 1.0f / static_cast<float>(longest);
-    in_lane = in_cut = 0;
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      if (h < held) {
-        int n = static_cast<int>(static_cast<float>(steps[h]) * by);  // (below 2^12, so one off at most)
-        n += n * longest < steps[h] ? 1 : 0;
-        n += n * longest < steps[h] ? 1 : 0;
-        n -= n > 0 && (n - 1) * longest >= steps[h] ? 1 : 0;
-        count[h] = n;
-        in_lane += n;
-        in_cut += n > 1 ? n : 0;
-      } else {
-        count[h] = 0;
-      }
-    }
-    all = kv_from_lane(kv_sums(in_lane), 63);
-    if (all <= cut.target || longest >= enough) break;
-    longest = round < 6 ? min(kv_longer(longest, all, cut.target), enough) : enough;
-  }
-  // Parts by length, in classes of longest / 16, all below half of it in the last; two classes' sums in one number (each below 2^16).
-  int classes[CLASSES / 2] = {}, kind[HELD];
-  const float by = 2.0f * CLASSES / static_cast<float>(longest);
-#pragma unroll
-  for (int h = 0; h < HELD; ++h) {
-    kind[h] = CLASSES;
-    if (h < held) {
-      const float length = static_cast<float>(steps[h]) * __builtin_amdgcn_rcpf(static_cast<float>(max(count[h], 1)));
-      kind[h] = max(min(static_cast<int>(2.0f * CLASSES - length * by), CLASSES - 1), 0);
-#pragma unroll
-      for (int c = 0; c < CLASSES / 2; ++c) classes[c] += kind[h] >> 1 == c ? count[h] << (16 * (kind[h] & 1)) : 0;
-    }
-  }
-  const int cut_sum = kv_sums(in_cut);
-  int2 *const map = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
-  if (group == 0 && tid == 0) map[cut.places] = make_int2(kv_from_lane(cut_sum, 63), 0);
-  if (group >= all) return false;
-  const int half = (cut.target + 1) >> 1;
-  int at = group < half ? group : all - 1 - (group - half), found = 0, found_kind = CLASSES;
-#pragma unroll
-  for (int c = 0; c < CLASSES; c += 2) {
-    const int sums = kv_sums(classes[c >> 1]), sum = kv_from_lane(sums, 63);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int up_to = sums >> (16 * e) & 0xffff, its = sum >> (16 * e) & 0xffff;
-      if (found_kind == CLASSES) {
-        if (at < its) {
-          found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up_to > at));
-          at -= kv_from_lane(up_to - (classes[c >> 1] >> (16 * e) & 0xffff), found);
-          found_kind = c + e;
-        } else {
-          at -= its;
-        }
-      }
-    }
-  }
-  part.place = kv_from_lane(cut_sum - in_cut, found);
-  part.tile = -1;
-#pragma unroll
-  for (int h = 0; h < HELD; ++h) {
-    if (h < held && part.tile < 0) {
-      const int n = kv_from_lane(count[h], found), of_kind = kv_from_lane(kind[h], found);
-      if (of_kind == found_kind && at < n) {
-        part.tile = found * held + h;
-        part.count = n;
-      } else {
-        at -= of_kind == found_kind ? n : 0;
-        part.place += n > 1 ? n : 0;
-      }
-    }
-  }
-  part.index = at;
-  part.place += at;
-  rows_of(counted.requests[part.tile], part.tile, part.rows);
-  part.rows = {kv_uniform(part.rows.request), kv_uniform(part.rows.start), kv_uniform(part.rows.fresh), kv_uniform(part.rows.length),
-               kv_uniform(part.rows.first), kv_uniform(part.rows.rows), kv_uniform(part.rows.last_key)};
+  for (int h = 0; h < HELD; ++h) steps[h] = h < held && lane * held + h < tiles ? counted.steps[lane * held + h] : 0;
+  KvPick pick;
+  const bool there = kv_pick<true>(a.many, tiles, held, steps, group, part, pick);
+  int2 *const map = kv_map_of(a.many, kv_head);
+  if (group == 0 && tid == 0) map[a.many.places] = make_int2(pick.all_cut, 0);
+  if (!there) return false;
+  rows_of(counted.requests[part.tile], part.tile, r);
+  part.rows = kv_uniform(r);
   __syncthreads();  // (the memory is somebody else's from here on)
-  if (part.count > 1 && tid == 0) map[part.place] = part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0);
+  if (part.count > 1 && tid == 0) map[part.place] = kv_map_entry(part);
   return true;
 }
 

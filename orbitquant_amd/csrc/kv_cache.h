@@ -35,6 +35,7 @@ struct KvReadArgs {
 // (of many rows, where a launch is cut only if it has fewer tiles than that, no more than `target`).
 struct KvCut {
   int target, least;  // target 0: nothing is cut
+  bool sorted;        // few rows: the longest parts first (for more parts than the chip holds at once)
   int places;         // for the parts of tiles that are cut: of few rows 2 * target (a tile of n > 1 parts has more than (n - 1) * longest steps), of many target
   float *out;         // [key heads, places, rows of a tile, D]
   float2 *stats;      // [key heads, places, rows of a tile]: R and l
