@@ -200,7 +200,7 @@ __device__ __forceinline__ int kv_longer(int longest, int made, int target) {
 // way, and a long one's neighbour is short (parts of 19 to 46 steps, 480 of them, D = 64, fp16: 103 -> 87 us with both;
 // 532 parts before, whose last twenty began when the others ended).
 struct KvPick {
-  int tile, lane, all_cut;  // (the lane whose tile it is; the number of all parts of cut tiles)
+  int tile, all_cut;  // (the number of all parts of cut tiles)
 };
 template <bool MANY, int HELD>
 __device__ __forceinline__ bool kv_pick(const KvCut &cut, int tiles, int held, const int (&steps)[HELD], int group, KvPart &part, KvPick &pick) {
@@ -283,7 +283,6 @@ __device__ __forceinline__ bool kv_pick(const KvCut &cut, int tiles, int held, c
     }
   }
   part.place = kv_from_lane(cut_sum - in_cut, found);
-  pick.lane = found;
   pick.tile = -1;
 #pragma unroll
   for (int h = 0; h < HELD; ++h) {
@@ -315,24 +314,41 @@ __device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, co
   KvRows r = {};
   const auto steps_of = [&](int i) { return kv_few_tile(a, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0; };
   int2 *const map = kv_map_of(cut, kv_head);
-  if (tiles <= kKvCutTiles) {  // no wavefront needs another: the first keys are a barrier nearer
+  if (tiles <= 64 && !cut.sorted) {  // a tile a lane, and the order is theirs: a short launch notices every instruction
+    const int steps = lane < tiles ? steps_of(lane) : 0;
+    const int total = kv_from_lane(kv_sums(steps), 63);
+    int longest = max((total + cut.target - 1) / cut.target, cut.least);
+    int count = (steps + longest - 1) / longest, sum = kv_sums(count);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // (rounding every tile's parts up makes more of them than meant)
+      const int made = kv_from_lane(sum, 63);
+      if (made > cut.target && longest < total) {
+        longest = kv_longer(longest, made, cut.target);
+        count = (steps + longest - 1) / longest;
+        sum = kv_sums(count);
+      }
+    }
+    const int in_cut = count > 1 ? count : 0, cut_sum = kv_sums(in_cut);
+    if (group == 0 && tid == 0) map[cut.places] = make_int2(kv_from_lane(cut_sum, 63), 0);
+    if (group >= kv_from_lane(sum, 63)) return false;
+    const int found = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > group));
+    part.tile = found;
+    part.count = kv_from_lane(count, found);
+    part.index = group - kv_from_lane(sum - count, found);
+    part.place = kv_from_lane(cut_sum - in_cut, found) + part.index;
+    part.rows = {kv_from_lane(r.request, found), kv_from_lane(r.start, found), kv_from_lane(r.fresh, found), kv_from_lane(r.length, found),
+                 kv_from_lane(r.first, found), kv_from_lane(r.rows, found), kv_from_lane(r.last_key, found)};
+  } else if (tiles <= kKvCutTiles) {  // no wavefront needs another: the first keys are a barrier nearer
     bool there;
     KvPick pick;
-    if (tiles <= 64) {
-      const int steps[1] = {lane < tiles ? steps_of(lane) : 0};
-      there = kv_pick<false>(cut, tiles, 1, steps, group, part, pick);
-      if (there) part.rows = {kv_from_lane(r.request, pick.lane), kv_from_lane(r.start, pick.lane), kv_from_lane(r.fresh, pick.lane), kv_from_lane(r.length, pick.lane),
-                              kv_from_lane(r.first, pick.lane), kv_from_lane(r.rows, pick.lane), kv_from_lane(r.last_key, pick.lane)};
-    } else {
-      const int held = (tiles + 63) >> 6;
-      int steps[kKvCutTiles / 64];
+    const int held = (tiles + 63) >> 6;
+    int steps[kKvCutTiles / 64];
 #pragma unroll
-      for (int h = 0; h < kKvCutTiles / 64; ++h) steps[h] = h < held && lane * held + h < tiles ? steps_of(lane * held + h) : 0;
-      there = kv_pick<false>(cut, tiles, held, steps, group, part, pick);
-      if (there) {
-        kv_few_tile(a, part.tile, r);
-        part.rows = kv_uniform(r);
-      }
+    for (int h = 0; h < kKvCutTiles / 64; ++h) steps[h] = h < held && lane * held + h < tiles ? steps_of(lane * held + h) : 0;
+    there = kv_pick<false>(cut, tiles, held, steps, group, part, pick);
+    if (there) {
+      kv_few_tile(a, part.tile, r);
+      part.rows = kv_uniform(r);
     }
     if (group == 0 && tid == 0) map[cut.places] = make_int2(pick.all_cut, 0);
     if (!there) return false;

@@ -16,6 +16,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.compiler import is_compiling
 
 from . import _lib
 from .ops import _DTYPES, _dt, _OnDevice, _operand, _ptr, _require_gpu, _stream, _workspace
@@ -149,13 +150,18 @@ for _name, _op, _fake in (("kv_assign", _assign_op, _assign_fake), ("kv_write", 
     torch.library.register_fake(f"orbitquant_amd::{_name}", _fake, lib=_LIB)
 
 
+_host = None   # what `_module` has found, to be looked at without a call
+
+
 def _module():
     """The compiled module (csrc/torch_ops.cpp), which has the usual calls of these functions without Python in between (a cached
-    token's slot 13.5 -> 5.4 us, one token decoded 19.5 -> 12.2); None where it is not built.  What it does not take, errors among it, it leaves to the Python below."""
-    module = _lib.torch_ops()
-    if module is None:
+    token's slot 13.5 -> 5.4 us, one token decoded 19.5 -> 12.2); None where it is not built.  What it does not take, errors among it, it
+    leaves to the Python below."""
+    global _host
+    _host = _lib.torch_ops()
+    if _host is None:
         _lib.warn_without_torch_ops()
-    return module
+    return _host
 
 
 def _cache_struct(cache, like: torch.Tensor) -> _lib.KvCacheStruct:
@@ -201,10 +207,10 @@ def kv_assign(lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: tor
     `kv_attend` does not see.  `tokens`: the number of new tokens, as the caller's arrays have them; what `new_lengths` leaves of
     it gets slot and position -1.  lengths, new_lengths int32 [requests], block_table int32 [requests, width] (changed in
     place), free_pages int32 [any], taken int32 [1]."""
-    if torch.compiler.is_compiling():
+    if is_compiling():
         return _assigned(*torch.ops.orbitquant_amd.kv_assign(lengths, new_lengths, block_table, free_pages, taken, page_size, tokens), tokens,
                          lengths.numel())
-    module = _module()
+    module = _host or _module()
     if module is not None:
         got = module.kv_assign(lengths, new_lengths, block_table, free_pages, taken, int(page_size), int(tokens))
         if got is not None:
@@ -216,10 +222,10 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Orbit
     """Keys and values [tokens, heads, D] into the cache at `slots` int64 [tokens] (`oq_kv_write`).  Slots that are negative or
     beyond the last page are skipped; no slot may occur twice.  k and v: one floating type, any strides whose last is 1 (parts of
     a fused projection's output need no copy)."""
-    if torch.compiler.is_compiling():
+    if is_compiling():
         torch.ops.orbitquant_amd.kv_write(k, v, slots, *cache)
         return
-    module = _module()
+    module = _host or _module()
     if module is not None and module.kv_write(k, v, slots, cache):
         return
     _require_gpu(k, "k")
@@ -238,9 +244,9 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Orbit
 def kv_read(slots: torch.Tensor, cache: OrbitKVCache, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """What the cache holds at `slots` int64 [tokens], as keys and values [tokens, heads, D] of `dtype` (`oq_kv_read`); zeros for
     slots that are negative or beyond the last page."""
-    if torch.compiler.is_compiling():
+    if is_compiling():
         return torch.ops.orbitquant_amd.kv_read(slots, *cache, dtype)
-    module = _module()
+    module = _host or _module()
     if module is not None:
         got = module.kv_read(slots, cache, dtype)
         if got is not None:
@@ -281,10 +287,10 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
     max_length = -1 if max_length is None else int(max_length)
     max_new = -1 if max_new is None else int(max_new)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if torch.compiler.is_compiling():
+    if is_compiling():
         out, lse = torch.ops.orbitquant_amd.kv_attend(q, *cache, block_table, lengths, starts, max_new, max_length, causal, window, scale, return_lse)
         return (out, lse) if return_lse else out
-    module = _module()
+    module = _host or _module()
     if module is not None:
         got = module.kv_attend(q, cache, block_table, lengths, starts, max_new, max_length, bool(causal), window, scale, bool(return_lse))
         if got is not None:
