@@ -699,13 +699,36 @@ __device__ __forceinline__ void kv_decode_values(uint32_t x, uint32_t y, kv_f16x
   odd = kv_decode8(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u));
 }
 
+// Eight dimensions of a row's result, rotated back but for the signs, from `at` on: of the output's row `index`, or in the parts.
+template <int D, int SPLIT>
+__device__ __forceinline__ void kv_store8(const KvAttendArgs &a, int64_t index, int at, const uint32_t *signs, float *part_out, const float *y) {
+  const uint2 sign = *reinterpret_cast<const uint2 *>(signs + at / 4);
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(__float_as_uint(y[e]) ^ (((e < 4 ? sign.x : sign.y) << (24 - 8 * (e & 3))) & 0x80000000u));
+  if (SPLIT == 2 || part_out != nullptr) {
+    float *to = part_out != nullptr ? part_out + at : static_cast<float *>(a.out) + index * D + at;
+    reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = SPLIT == 1 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
+                        : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
+    }
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + index * D + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ float kv_share(float l, bool part) { return part ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f; }  // (no key: zeros)
+__device__ __forceinline__ float kv_lse(float ref, float l) { return l != 0.0f ? (ref + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY; }
+
 // A row's result: rotated back, and stored as the output, or at its place in the parts.
 template <int D, int SPLIT>
 __device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &row, int g, const uint32_t *signs, float *part_out, float2 *part_stats,
                                           const KvState &st, const kv_f32x4 (&o)[D / 16]) {
   const float l = kv_over_groups(st.sum, kv_sum_of);
-  const bool part = part_out != nullptr;
-  const float by = part ? 1.0f / D : l != 0.0f ? (1.0f / D) / l : 0.0f;  // (no key: zeros)
+  const float by = kv_share(l, part_out != nullptr) * (1.0f / D);
   // dimension 32 j + 8 g + 2 r + parity is in o[2 j + parity][r]
   float y[D / 4];
 #pragma unroll
@@ -720,29 +743,10 @@ __device__ __forceinline__ void kv_finish(const KvAttendArgs &a, const KvRow &ro
   if (row.token < 0) return;
   const int64_t index = static_cast<int64_t>(row.token) * a.heads + row.head;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    const uint2 sign = *reinterpret_cast<const uint2 *>(signs + 8 * j + 2 * g);
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(__float_as_uint(y[8 * j + e]) ^ (((e < 4 ? sign.x : sign.y) << (24 - 8 * (e & 3))) & 0x80000000u));
-    const int at = 32 * j + 8 * g;
-    if (SPLIT == 2 || part) {
-      float *to = part ? part_out + at : static_cast<float *>(a.out) + index * D + at;
-      reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = SPLIT == 1 ? f32_to_f16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(v[2 * e + 1])) << 16
-                          : f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
-      }
-      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + index * D + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
+  for (int j = 0; j < D / 32; ++j) kv_store8<D, SPLIT>(a, index, 32 * j + 8 * g, signs, part_out, y + 8 * j);
   if (g != 0) return;
-  if (part) *part_stats = make_float2(st.reference(), l);
-  else if (a.lse != nullptr) a.lse[index] = l != 0.0f ? (st.ref + __builtin_amdgcn_logf(l)) * 0.693147180559945f : -INFINITY;
+  if (part_out != nullptr) *part_stats = make_float2(st.reference(), l);
+  else if (a.lse != nullptr) a.lse[index] = kv_lse(st.ref, l);
 }
 
 // A step's keys, scales and values as they come from the cache, for a wavefront that decodes all of them.
@@ -815,7 +819,9 @@ __device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, i
 template <int D, int SPLIT, bool WIDE>
 __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
-  __shared__ float join[3][D / 4 + 2][64];
+  constexpr int PITCH = D + 4;
+  __shared__ __attribute__((aligned(16))) float join[4][16][PITCH];
+  __shared__ float refs[4][16], sums[4][16];
   __shared__ uint32_t signs[D / 4];
   if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -935,39 +941,56 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   if (step < end) take_step(std::false_type{});
   st.ref = st.reference();
 
-  // the four wavefronts, in their order
-  if (wave > 0) {
-    join[wave - 1][0][lane] = st.ref;
-    join[wave - 1][1][lane] = st.sum;
+  // The four wavefronts, in their order.  A lane has eight dimensions of a row now, as it has where vectors are written to the cache,
+  // so that a row's sums and its rotation are many lanes' work: with four rows one wavefront's, eight values a lane instead of 32.
+  const float own_sum = kv_over_groups(st.sum, kv_sum_of);
+  if (n < r.rows) {
+    if (g == 0) {
+      refs[wave][n] = st.ref;
+      sums[wave][n] = own_sum;
+    }
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) join[wave - 1][2 + 4 * j + i][lane] = o[j][i];
+    for (int j = 0; j < D / 32; ++j) {  // dimension 32 j + 8 g + 2 r + parity is in o[2 j + parity][r]
+      float4 *to = reinterpret_cast<float4 *>(&join[wave][n][32 * j + 8 * g]);
+      to[0] = make_float4(o[2 * j][0], o[2 * j + 1][0], o[2 * j][1], o[2 * j + 1][1]);
+      to[1] = make_float4(o[2 * j][2], o[2 * j + 1][2], o[2 * j][3], o[2 * j + 1][3]);
     }
   }
   __syncthreads();
-  if (wave == 0) {
-    float of[4] = {st.ref, join[0][0][lane], join[1][0][lane], join[2][0][lane]};
-    const float both = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+  const bool is_part = part.count > 1;
+  const int dims = 8 * kv_part_of<D>(lane);
+  for (int from = wave * (512 / D); from < r.rows; from += 2048 / D) {
+    const int at = from + kv_vector_of<D>(lane);
+    const bool there = at < r.rows;
+    float of[4], both = kKvNothing, l = 0.0f, y[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) of[w] = kv_exp2(of[w] - both);
-    st.ref = both;
-    st.sum *= of[0];
+    for (int w = 0; w < 4; ++w) of[w] = there ? refs[w][at] : kKvNothing;
+    both = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
 #pragma unroll
-    for (int w = 1; w < 4; ++w) st.sum = fmaf(join[w - 1][1][lane], of[w], st.sum);
+    for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+    if (there) {
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      if constexpr (D == 256) asm volatile("" ::: "memory");  // (all of it at once does not fit the registers)
+      for (int w = 0; w < 4; ++w) {
+        of[w] = kv_exp2(of[w] - both);
+        l = fmaf(sums[w][at], of[w], l);
+        const float4 u = *reinterpret_cast<const float4 *>(&join[w][at][dims]), v = *reinterpret_cast<const float4 *>(&join[w][at][dims + 4]);
+        const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[j][i] *= of[0];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) o[j][i] = fmaf(join[w - 1][2 + 4 * j + i][lane], of[w], o[j][i]);
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], of[w], y[e]);
       }
     }
-    st.limit = 1.0f;  // (what R says is all there is to know now)
-    const int64_t place = (static_cast<int64_t>(kv_head) * a.few.places + part.place) * 16 + n;
-    kv_finish<D, SPLIT>(a, row, g, signs, part.count > 1 ? a.few.out + place * D : nullptr, a.few.stats + place, st, o);
+    const float by = kv_share(l, is_part) * (1.0f / D);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] *= by;
+    kv_butterflies<D>(y, lane);
+    if (!there) continue;
+    const KvRow of_row = kv_row_of(a, r, kv_head, r.first + at, true);
+    const int64_t index = static_cast<int64_t>(of_row.token) * a.heads + of_row.head;
+    const int64_t place = (static_cast<int64_t>(kv_head) * a.few.places + part.place) * 16 + at;
+    kv_store8<D, SPLIT>(a, index, dims, signs, is_part ? a.few.out + place * D : nullptr, y);
+    if (dims != 0) continue;
+    if (is_part) a.few.stats[place] = make_float2(both, l);
+    else if (a.lse != nullptr) a.lse[index] = kv_lse(both, l);
   }
 }
 
