@@ -12,11 +12,14 @@ bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream);
 namespace {
 
 // How launches are cut (MI355X, D = 128; a step is 64 keys).
-// Few rows.  One launch and no join up to sixteen steps: 1003 tokens, 32 heads, 10.7 us, cut into fours 11.3.  Above, 512 workgroups or more, two on
-// each compute unit at once: 131101 tokens, 8 heads, 34.6 us (1024: 39.7, 256: 35.0); sixteen requests of up to 4096, 27.2 with the rest of their step (1024: 31).
+// Few rows.  One launch and no join up to sixteen steps (1003 tokens, 32 heads: 8.9 us), and up to 64 where there are workgroups enough
+// without, four for every step beyond sixteen, of shorter heads fewer, of longer ones more: 64 requests of up to 4096 tokens, 8 key heads, 47 -> 38 us,
+// 16 of up to 2000 15.3 -> 12.9, but 4 of them 11.1 -> 12.5, and 16 of up to 4096, with the rest of their step, 24.8 -> 27.1; D = 64, 16 of up to
+// 2000, 13.2 -> 10.5; D = 256, 4 key heads, 17.7 -> 19.3.  Longer ones could leave one workgroup at work alone for too long, 0.22 us a step.
+// Cut, 512 workgroups or more, two on each compute unit at once: 131101 tokens, 8 heads, 34 us (before the other steps 1024: 39.7, 256: 35.0, 512: 34.6).
 // Up to three times as many where a part keeps 60 steps, so that requests of different lengths even out, the longest parts first: 64 of up to
-// 16384, 130 us (512 workgroups: 139; four times: 132), 128 of up to 4096, 81 us (80 steps: 83).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 17.9 us (six: 20).
-constexpr int kFewWhole = 16, kFewGroups = 512, kFewSteps = 60, kFewLeast = 4;
+// 16384, 130 us (512 workgroups: 139; four times: 132).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 15.5 us.
+constexpr int kFewWhole = 16, kFewWholeMost = 64, kFewGroups = 512, kFewSteps = 60, kFewLeast = 4;
 // Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the workgroups that the chip holds (two on
 // a compute unit, of heads of 256 one), and at least sixteen steps of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us;
 // 2048 on their own, 264 tiles of few steps each: 68 -> 97 us if they were cut.
@@ -148,7 +151,8 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   a.few.sorted = false;
   a.few.least = kFewLeast;
   a.many.least = kManyLeast;
-  if (a.few_requests > 0 && steps > kFewWhole) {
+  const int64_t whole = static_cast<int64_t>(a.few_requests) * a.few_tiles * heads;
+  if (a.few_requests > 0 && steps > kFewWhole && (steps > kFewWholeMost || whole * 32 < (steps - kFewWhole) * dim)) {
     const int64_t parts = static_cast<int64_t>(a.requests) * steps * heads / kFewSteps;
     const int64_t groups = parts < kFewGroups ? kFewGroups : parts > 3 * kFewGroups ? 3 * kFewGroups : parts;
     a.few.sorted = groups > kFewGroups;

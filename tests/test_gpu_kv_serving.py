@@ -30,6 +30,22 @@ def test_attend_many_requests_in_parts(requests, longest, heads, window):
                window=window)
 
 
+@pytest.mark.parametrize("requests,heads", [(40, 16), (65, 8), (300, 2), (400, 1)])
+def test_attend_long_requests_in_parts(requests, heads):
+    """The same where requests are so long that they are always cut: the tiles of a wavefront, of a few a lane, of the
+    whole workgroup, with more parts than the chip holds and with fewer."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(heads)
+    lengths = rng.randint(0, 4300, requests)
+    lengths[rng.rand(requests) < 0.5] //= 40
+    lengths[[0, -1]] = 4300, 4299
+    lengths = lengths.tolist()
+    cache, table = _filled(rng, lengths, heads, 64, 64)
+    q = _queries(rng, requests, heads, 64, torch.float16)
+    _check(kv_attend(q, cache, table, _i32(lengths), return_lse=True), q, cache, table, _i32(lengths))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 128)])
 @pytest.mark.parametrize("requests", [3, 70])
