@@ -114,11 +114,12 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 }
 
 // ---- into the cache and back -----------------------------------------------------------------------------------------
-// Both are bound by bytes: a workgroup takes one head of sixteen tokens, its lanes eight values each, keys and values all requested at
+// A workgroup takes one head of sixteen tokens, its lanes eight values each, keys and values all requested at
 // once.  A token's key is D / 2 bytes in a row, but its value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen
 // tokens change places in LDS, and four tokens whose slots follow each other in a page (a prompt's, nearly always) are one dword of
-// a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write and read 31.6 us together; with 64 tokens a workgroup 37; with one byte a
-// store and lanes exchanged through LDS 52.
+// a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write 18 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a
+// store and lanes exchanged through LDS 52).  Bound by vector instructions, 28 and 25 a value, which issue in nine of ten cycles: eleven of
+// them the seven stages of the transform; the bytes alone take 9.
 constexpr int kKvGroup = 16;  // tokens of a workgroup
 
 template <int DT>
