@@ -473,7 +473,7 @@ typedef struct {
   uint16_t *k_scales;   /* bf16 [pages, kv_heads, page_size]                                                                */
   uint8_t *v_codes;     /* [pages, kv_heads, D/2, page_size]: the same bytes, a page's tokens side by side                 */
   uint16_t *v_scales;   /* bf16 [pages, kv_heads, page_size]                                                                */
-  const int8_t *signs;  /* [D], +1/-1, 8-byte aligned; the four above 16-byte aligned                                       */
+  const int8_t *signs;  /* [D], +1/-1; all five 16-byte aligned                                                               */
   int64_t pages;        /* 1 .. 2^31 - 1                                                                                    */
   int64_t kv_heads;     /* 1 .. 65535                                                                                       */
   int64_t page_size;    /* a power of two, 16 .. 1024                                                                       */

@@ -595,7 +595,7 @@ int kv_cache_of(const char *what, const oq_kv_cache *c, oq::KvCache &out) {
     return fail(OQ_ERR_INVALID, "%s: pages=%lld kv_heads=%lld", what, (long long)c->pages, (long long)c->kv_heads);
   if (c->k_codes == nullptr || c->k_scales == nullptr || c->v_codes == nullptr || c->v_scales == nullptr || c->signs == nullptr)
     return fail(OQ_ERR_INVALID, "%s: null pointer in the cache", what);
-  if (!aligned(c->k_codes, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_codes, 16) || !aligned(c->v_scales, 16) || !aligned(c->signs, 8))
+  if (!aligned(c->k_codes, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_codes, 16) || !aligned(c->v_scales, 16) || !aligned(c->signs, 16))
     return fail(OQ_ERR_INVALID, "%s: the cache is not aligned to 16 bytes", what);
   out.k_codes = c->k_codes; out.v_codes = c->v_codes; out.k_scales = c->k_scales; out.v_scales = c->v_scales; out.signs = c->signs;
   out.pages = c->pages; out.heads = static_cast<int>(c->kv_heads); out.page_shift = shift;

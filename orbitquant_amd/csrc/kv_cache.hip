@@ -114,16 +114,15 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 }
 
 // ---- into the cache and back -----------------------------------------------------------------------------------------
-// A workgroup takes one head of sixteen tokens, its lanes eight values each, keys and values all requested at
-// once.  A token's key is D / 2 bytes in a row, but its value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen
-// tokens change places in LDS, and four tokens whose slots follow each other in a page (a prompt's, nearly always) are one dword of
-// a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write 18 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a
-// store and lanes exchanged through LDS 52).  Bound by vector instructions, 28 and 25 a value, which issue in nine of ten cycles: eleven of
+// A workgroup takes one head of sixteen tokens, keys and values all requested at once.  A token's key is D / 2 bytes in a row, but its
+// value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen tokens change places in LDS, and four tokens
+// whose slots follow each other in a page (a prompt's, nearly always) are one dword of a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write 16 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a
+// store and lanes exchanged through LDS 52).  Bound by vector instructions, some 25 a value, which issue in nine of ten cycles: eleven of
 // them the seven stages of the transform; the bytes alone take 9.
 constexpr int kKvGroup = 16;  // tokens of a workgroup
 
 template <int DT>
-__device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float (&y)[8]) {
+__device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float *y) {
   if (wide) {
     if constexpr (DT == OQ_F32) {
       const float4 lo = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[0], hi = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[1];
@@ -141,7 +140,7 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, floa
 }
 
 template <int DT>
-__device__ __forceinline__ void store8(void *p, int64_t at, const float (&y)[8]) {  // 16-byte aligned
+__device__ __forceinline__ void store8(void *p, int64_t at, const float *y) {  // 16-byte aligned
   if constexpr (DT == OQ_F32) {
     reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[0] = make_float4(y[0], y[1], y[2], y[3]);
     reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[1] = make_float4(y[4], y[5], y[6], y[7]);
@@ -157,121 +156,142 @@ __device__ __forceinline__ void store8(void *p, int64_t at, const float (&y)[8])
   }
 }
 
-template <int D>
-__device__ __forceinline__ void times_signs(float (&y)[8], uint2 signs) {
+template <int E>
+__device__ __forceinline__ void times_signs(float (&y)[E], const uint32_t (&words)[E / 4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(__float_as_uint(y[i]) ^ (((i < 4 ? signs.x : signs.y) << (24 - 8 * (i & 3))) & 0x80000000u));
+  for (int i = 0; i < E; ++i) y[i] = __uint_as_float(__float_as_uint(y[i]) ^ ((words[i / 4] << (24 - 8 * (i & 3))) & 0x80000000u));
 }
 
-// The slots of the workgroup's tokens, -1 where there is nothing to do.
-__device__ __forceinline__ void group_slots(int64_t (&slots)[kKvGroup], const int64_t *from, int64_t first, int64_t tokens, int64_t most) {
+// Where the workgroup's tokens are: `slot` -1 for nothing to do, `key` the vector among those of k_codes and the scales, `value` the
+// first byte of its column in v_codes.
+struct KvPlace {
+  int64_t slot, key, value;
+};
+template <int D>
+__device__ __forceinline__ void group_places(KvPlace (&places)[kKvGroup], const KvCache &cache, const int64_t *from, int64_t first, int64_t tokens, int head) {
   if (threadIdx.x < kKvGroup) {
+    const int shift = cache.page_shift;
     int64_t slot = -1;
     if (first + threadIdx.x < tokens) slot = from[first + threadIdx.x];
-    slots[threadIdx.x] = slot < most ? slot : -1;
+    if (slot < 0 || slot >= cache.pages << shift) slot = -1;
+    const int64_t block = max(slot, static_cast<int64_t>(0)) >> shift, in_page = slot & ((1 << shift) - 1);
+    places[threadIdx.x] = {slot, ((block * cache.heads + head) << shift) + in_page, (((block * cache.heads + head) * (D / 2)) << shift) + in_page};
   }
 }
 
 // Whether four tokens' bytes of a row are one dword.
-__device__ __forceinline__ bool in_a_row(const int64_t *slots, int page_shift) {
-  const int64_t s = slots[0];
-  return s >= 0 && slots[1] == s + 1 && slots[2] == s + 2 && slots[3] == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
+__device__ __forceinline__ bool in_a_row(const KvPlace *places, int page_shift) {
+  const int64_t s = places[0].slot;
+  return s >= 0 && places[1].slot == s + 1 && places[2].slot == s + 2 && places[3].slot == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
 }
 
+// Values of a lane: sixteen on the way in, where a vector's scale is found once for twice as many of them and one stage fewer lies between lanes
+// (write 18.1 -> 16.2 us), eight on the way out (sixteen 16.3 -> 16.8).
+constexpr int kKvWriteEach = 16, kKvReadEach = 8;
+template <int LANES>  // of a vector
+constexpr int kv_group_threads() { return LANES == 4 ? 128 : 256; }
+
 template <int D, int DT>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs a) {
-  constexpr int AT_ONCE = 2048 / D;                // vectors that the workgroup's lanes hold
+__global__ __launch_bounds__(kv_group_threads<D / kKvWriteEach>()) void kv_write_kernel(KvWriteArgs a) {
+  constexpr int E = kKvWriteEach, THREADS = kv_group_threads<D / E>();
+  constexpr int AT_ONCE = THREADS * E / D;         // vectors that the workgroup's lanes hold
   constexpr int PASSES = 2 * kKvGroup / AT_ONCE;   // keys, then values
-  __shared__ int64_t slots[kKvGroup];
+  __shared__ KvPlace places[kKvGroup];
   __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];  // of the values
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D>(lane);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D, E>(lane);
   const int head = blockIdx.x % a.cache.heads;
   const int64_t first = static_cast<int64_t>(blockIdx.x / a.cache.heads) * kKvGroup;
   const int shift = a.cache.page_shift;
-  float y[PASSES][8];
+  float y[PASSES][E];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane);
+    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane);
     const int64_t token = min(first + (vector & (kKvGroup - 1)), a.tokens - 1);
-    if (vector >= kKvGroup) load8<DT>(a.v, token * a.v_token_stride + head * a.v_head_stride + 8 * part, a.v_wide, y[p]);
-    else load8<DT>(a.k, token * a.k_token_stride + head * a.k_head_stride + 8 * part, a.k_wide, y[p]);
+#pragma unroll
+    for (int i = 0; i < E; i += 8) {
+      if (vector >= kKvGroup) load8<DT>(a.v, token * a.v_token_stride + head * a.v_head_stride + E * part + i, a.v_wide, y[p] + i);
+      else load8<DT>(a.k, token * a.k_token_stride + head * a.k_head_stride + E * part + i, a.k_wide, y[p] + i);
+    }
   }
-  const uint2 signs = reinterpret_cast<const uint2 *>(a.cache.signs)[part];
-  group_slots(slots, a.slots, first, a.tokens, a.cache.pages << shift);
+  const uint4 signs = reinterpret_cast<const uint4 *>(a.cache.signs)[part];
+  const uint32_t words[4] = {signs.x, signs.y, signs.z, signs.w};
+  group_places<D>(places, a.cache, a.slots, first, a.tokens, head);
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane), token = vector & (kKvGroup - 1);
-    times_signs<D>(y[p], signs);
+    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane), token = vector & (kKvGroup - 1);
+    times_signs(y[p], words);
     kv_butterflies<D>(y[p], lane);
     uint16_t scale;
-    const uint32_t codes = kv_encode<D>(y[p], scale);
-    const int64_t slot = slots[token];
-    const int64_t at = ((((slot >> shift) * a.cache.heads + head) << shift) + (slot & ((1 << shift) - 1)));
+    uint32_t codes[E / 8];
+    kv_encode<D>(y[p], scale, codes);
+    const bool there = places[token].slot >= 0;
+    const int64_t at = places[token].key;
     if (vector >= kKvGroup) {
-      bytes[token][part] = codes;
-      if (slot >= 0 && part == 0) a.cache.v_scales[at] = scale;
-    } else if (slot >= 0) {
-      reinterpret_cast<uint32_t *>(a.cache.k_codes)[at * (D / 8) + part] = codes;
+#pragma unroll
+      for (int w = 0; w < E / 8; ++w) bytes[token][E / 8 * part + w] = codes[w];
+      if (there && part == 0) a.cache.v_scales[at] = scale;
+    } else if (there) {
+      reinterpret_cast<uint2 *>(a.cache.k_codes)[at * (D / E) + part] = make_uint2(codes[0], codes[1]);
       if (part == 0) a.cache.k_scales[at] = scale;
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < (D / 2) * (kKvGroup / 4); i += 256) {
+  for (int i = threadIdx.x; i < (D / 2) * (kKvGroup / 4); i += THREADS) {
     const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
     uint32_t four[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) four[k] = reinterpret_cast<const uint8_t *>(bytes[t + k])[row];
-    const auto place = [&](int64_t slot) { return a.cache.v_codes + ((((slot >> shift) * a.cache.heads + head) * (D / 2) + row) << shift) + (slot & ((1 << shift) - 1)); };
-    if (in_a_row(slots + t, shift)) {
+    uint8_t *const at_row = a.cache.v_codes + (static_cast<int64_t>(row) << shift);
+    if (in_a_row(places + t, shift)) {
       const uint32_t word = four[0] | four[1] << 8 | four[2] << 16 | four[3] << 24;
-      __builtin_memcpy(place(slots[t]), &word, 4);  // (a page's tokens may begin anywhere)
+      __builtin_memcpy(at_row + places[t].value, &word, 4);  // (a page's tokens may begin anywhere)
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (slots[t + k] >= 0) *place(slots[t + k]) = static_cast<uint8_t>(four[k]);
+        if (places[t + k].slot >= 0) at_row[places[t + k].value] = static_cast<uint8_t>(four[k]);
       }
     }
   }
 }
 
 template <int D, int DT>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
-  constexpr int AT_ONCE = 2048 / D, PASSES = 2 * kKvGroup / AT_ONCE;
+__global__ __launch_bounds__(kv_group_threads<D / kKvReadEach>()) void kv_read_kernel(KvReadArgs a) {
+  constexpr int E = kKvReadEach, THREADS = kv_group_threads<D / E>(), AT_ONCE = THREADS * E / D, PASSES = 2 * kKvGroup / AT_ONCE;
   constexpr int ROWS = (D / 2) * (kKvGroup / 4);   // dwords of the values, turned by LDS
-  __shared__ int64_t slots[kKvGroup];
+  __shared__ KvPlace places[kKvGroup];
   __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D>(lane);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D, E>(lane);
   const int head = blockIdx.x % a.cache.heads;
   const int64_t first = static_cast<int64_t>(blockIdx.x / a.cache.heads) * kKvGroup;
   const int shift = a.cache.page_shift;
   const uint2 signs = reinterpret_cast<const uint2 *>(a.cache.signs)[part];
-  group_slots(slots, a.slots, first, a.tokens, a.cache.pages << shift);
+  const uint32_t words[2] = {signs.x, signs.y};
+  group_places<D>(places, a.cache, a.slots, first, a.tokens, head);
   __syncthreads();
   uint32_t keys[PASSES];
   float scales[PASSES];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane);
-    const int64_t slot = slots[vector & (kKvGroup - 1)];
-    const int64_t at = ((((slot >> shift) * a.cache.heads + head) << shift) + (slot & ((1 << shift) - 1)));
+    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane);
+    const KvPlace &place = places[vector & (kKvGroup - 1)];
     keys[p] = 0;
     scales[p] = 0.0f;
-    if (slot >= 0) {
-      if (vector < kKvGroup) keys[p] = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[at * (D / 8) + part];
-      scales[p] = bf16_bits_to_f32((vector < kKvGroup ? a.cache.k_scales : a.cache.v_scales)[at]);
+    if (place.slot >= 0) {
+      if (vector < kKvGroup) keys[p] = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[place.key * (D / E) + part];
+      scales[p] = bf16_bits_to_f32((vector < kKvGroup ? a.cache.k_scales : a.cache.v_scales)[place.key]);
     }
   }
-  for (int i = threadIdx.x; i < ROWS; i += 256) {
+  for (int i = threadIdx.x; i < ROWS; i += THREADS) {
     const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
-    const auto place = [&](int64_t slot) { return a.cache.v_codes + ((((slot >> shift) * a.cache.heads + head) * (D / 2) + row) << shift) + (slot & ((1 << shift) - 1)); };
+    const uint8_t *const at_row = a.cache.v_codes + (static_cast<int64_t>(row) << shift);
     uint32_t word = 0;
-    if (in_a_row(slots + t, shift)) {
-      __builtin_memcpy(&word, place(slots[t]), 4);
+    if (in_a_row(places + t, shift)) {
+      __builtin_memcpy(&word, at_row + places[t].value, 4);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (slots[t + k] >= 0) word |= static_cast<uint32_t>(*place(slots[t + k])) << (8 * k);
+        if (places[t + k].slot >= 0) word |= static_cast<uint32_t>(at_row[places[t + k].value]) << (8 * k);
       }
     }
 #pragma unroll
@@ -280,16 +300,16 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane), token = vector & (kKvGroup - 1);
+    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane), token = vector & (kKvGroup - 1);
     const kv_f16x8 c = kv_decode8(vector < kKvGroup ? keys[p] : bytes[token][part]);
-    float y[8];
+    float y[E];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(c[i]) * scales[p];
+    for (int i = 0; i < E; ++i) y[i] = static_cast<float>(c[i]) * scales[p];
     kv_butterflies<D>(y, lane);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= 1.0f / D;
-    times_signs<D>(y, signs);
-    if (first + token < a.tokens) store8<DT>(vector < kKvGroup ? a.k : a.v, ((first + token) * a.cache.heads + head) * D + 8 * part, y);
+    for (int i = 0; i < E; ++i) y[i] *= 1.0f / D;
+    times_signs(y, words);
+    if (first + token < a.tokens) store8<DT>(vector < kKvGroup ? a.k : a.v, ((first + token) * a.cache.heads + head) * D + E * part, y);
   }
 }
 
@@ -310,11 +330,11 @@ int by_type(const Args &a, int dim, int dtype, hipStream_t stream) {
 inline dim3 group_grid(int64_t tokens, int heads) { return dim3(static_cast<unsigned>((tokens + kKvGroup - 1) / kKvGroup * heads)); }
 template <int D, int DT>
 struct RunWrite {
-  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
+  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_group_threads<D / kKvWriteEach>()), 0, s, a); }
 };
 template <int D, int DT>
 struct RunRead {
-  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
+  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_group_threads<D / kKvReadEach>()), 0, s, a); }
 };
 
 }  // namespace

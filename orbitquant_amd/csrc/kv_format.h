@@ -27,19 +27,21 @@ struct KvCache {
 constexpr int kKvMaxRequests = 8192;  // of one oq_kv_assign: its two running sums and the lengths sit in LDS
 constexpr int kKvMinPage = 16, kKvMaxPage = 1024;
 
-// Eight values of a vector a lane: element 8 * part + i in lane `part` of the vector's D / 8.  The parts' bits are lane bits
-// whose exchanges are vector instructions: 0 and 1 (quad permutes), 3 (a rotation of the row by eight; heads of 256 only), 4 (heads of 128 and more) and 5 (swaps of
-// lane groups); the other lane bits tell the wavefront's 512 / D vectors apart.
-template <int D>
+// E values of a vector a lane (8 or 16): element E * part + i in lane `part` of the vector's D / E.  The parts' bits are lane bits
+// whose exchanges are vector instructions: 0 and 1 (quad permutes), 3 (a rotation of the row by eight; of 32 lanes only), 4 (of sixteen and more) and 5 (of eight; swaps
+// of lane groups); the other lane bits tell the wavefront's vectors apart.
+template <int D, int E = 8>
 __device__ __forceinline__ int kv_part_of(int lane) {
-  if constexpr (D == 64) return (lane & 3) | (lane >> 5) << 2;
-  else if constexpr (D == 128) return (lane & 3) | (lane >> 4) << 2;
+  if constexpr (D / E == 4) return lane & 3;
+  else if constexpr (D / E == 8) return (lane & 3) | (lane >> 5) << 2;
+  else if constexpr (D / E == 16) return (lane & 3) | (lane >> 4) << 2;
   else return (lane & 3) | (lane >> 3) << 2;
 }
-template <int D>
+template <int D, int E = 8>
 __device__ __forceinline__ int kv_vector_of(int lane) {
-  if constexpr (D == 64) return (lane >> 2) & 7;
-  else if constexpr (D == 128) return (lane >> 2) & 3;
+  if constexpr (D / E == 4) return lane >> 2;
+  else if constexpr (D / E == 8) return (lane >> 2) & 7;
+  else if constexpr (D / E == 16) return (lane >> 2) & 3;
   else return (lane >> 2) & 1;
 }
 
@@ -78,21 +80,22 @@ __device__ __forceinline__ void kv_lane_butterfly(float &a, float &b) {
   b = __uint_as_float(out[1]);
 }
 
-template <int CTRL>
-__device__ __forceinline__ void kv_dpp_butterflies(float (&y)[8], bool upper) {
+template <int CTRL, int E>
+__device__ __forceinline__ void kv_dpp_butterflies(float (&y)[E], bool upper) {
   const float sign = upper ? -1.0f : 1.0f;  // other + y below, other - y above, one rounding
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fmaf(y[i], sign, __uint_as_float(kv_dpp<CTRL>(__float_as_uint(y[i]))));
+  for (int i = 0; i < E; ++i) y[i] = fmaf(y[i], sign, __uint_as_float(kv_dpp<CTRL>(__float_as_uint(y[i]))));
 }
 
 // One add or subtract for each output and stage, distances 1, 2, 4, ... in this order: the results are those of any other
 // schedule of the same butterflies.
-template <int D>
-__device__ __forceinline__ void kv_butterflies(float (&y)[8], int lane) {
+template <int D, int E>
+__device__ __forceinline__ void kv_butterflies(float (&y)[E], int lane) {
+  constexpr int LANES = D / E;
 #pragma unroll
-  for (int d = 1; d < 8; d *= 2) {
+  for (int d = 1; d < E; d *= 2) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < E; ++i) {
       if ((i & d) == 0) {
         const float a = y[i], b = y[i + d];
         y[i] = a + b;
@@ -102,42 +105,55 @@ __device__ __forceinline__ void kv_butterflies(float (&y)[8], int lane) {
   }
   kv_dpp_butterflies<kDppXor1>(y, lane & 1);
   kv_dpp_butterflies<kDppXor2>(y, lane & 2);
-  if constexpr (D == 256) kv_dpp_butterflies<kDppXor8>(y, lane & 8);
+  if constexpr (LANES == 32) kv_dpp_butterflies<kDppXor8>(y, lane & 8);
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    if constexpr (D >= 128) kv_lane_butterfly<16>(y[i], y[i + 1]);
-    kv_lane_butterfly<32>(y[i], y[i + 1]);
+  for (int i = 0; i < E; i += 2) {
+    if constexpr (LANES >= 16) kv_lane_butterfly<16>(y[i], y[i + 1]);
+    if constexpr (LANES >= 8) kv_lane_butterfly<32>(y[i], y[i + 1]);
   }
 }
 
-// Scale (bf16 bits) and the lane's eight codes (a dword, element i in bits 4i) of a rotated vector.
+// Scale (bf16 bits) and the lane's codes (element i in bits 4 (i % 8) of dword i / 8) of a rotated vector.
 //   a = bf16(max|y| * fp32(1/6)), 0 below the smallest normal number; code = E2M1 nearest to y * (1 / a), ties to even
 // A vector with an infinity or a NaN in it gets the scale NaN and codes of zero: what attends to it becomes NaN.
-template <int D>
-__device__ __forceinline__ uint32_t kv_encode(const float (&y)[8], uint16_t &scale_bits) {
-  uint32_t top = 0;  // as bits: a NaN is above infinity, infinity above every number
+template <int D, int E>
+__device__ __forceinline__ void kv_encode(const float (&y)[E], uint16_t &scale_bits, uint32_t (&codes)[E / 8]) {
+  // The largest magnitude as bits: a NaN is above infinity, infinity above every number.  As signed numbers the bits of positive values are in
+  // order, as unsigned ones those of negative values above all others: two maxima, and one sign cleared.
+  constexpr int LANES = D / E;
+  int positive = 0;
+  uint32_t any = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+  for (int i = 0; i < E; ++i) {
+    positive = max(positive, __float_as_int(y[i]));
+    any = max(any, __float_as_uint(y[i]));
+  }
+  uint32_t top = max(static_cast<uint32_t>(positive), any & 0x7fffffffu);
   top = max(top, kv_dpp<kDppXor1>(top));
   top = max(top, kv_dpp<kDppXor2>(top));
-  if constexpr (D == 256) top = max(top, kv_dpp<kDppXor8>(top));
-  if constexpr (D >= 128) {
+  if constexpr (LANES == 32) top = max(top, kv_dpp<kDppXor8>(top));
+  if constexpr (LANES >= 16) {
     const kv_u32x2 both = kv_swap<16>(top, top);
     top = max(both[0], both[1]);
   }
-  const kv_u32x2 both = kv_swap<32>(top, top);
-  top = max(both[0], both[1]);
+  if constexpr (LANES >= 8) {
+    const kv_u32x2 both = kv_swap<32>(top, top);
+    top = max(both[0], both[1]);
+  }
   const bool broken = top >= 0x7f800000u;
   uint16_t a = f32_to_bf16_bits(__uint_as_float(top) * (1.0f / 6.0f));
   if (a < 0x0080u) a = 0;
   scale_bits = broken ? 0x7fc0u : a;
   const float inv = a != 0 && !broken ? 1.0f / bf16_bits_to_f32(a) : 0.0f;
-  uint32_t q = 0;
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[0] * inv, y[1] * inv, 1.0f, 0);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[2] * inv, y[3] * inv, 1.0f, 1);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4] * inv, y[5] * inv, 1.0f, 2);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[6] * inv, y[7] * inv, 1.0f, 3);
-  return broken ? 0u : q;
+#pragma unroll
+  for (int w = 0; w < E / 8; ++w) {
+    uint32_t q = 0;
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[8 * w] * inv, y[8 * w + 1] * inv, 1.0f, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[8 * w + 2] * inv, y[8 * w + 3] * inv, 1.0f, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[8 * w + 4] * inv, y[8 * w + 5] * inv, 1.0f, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[8 * w + 6] * inv, y[8 * w + 7] * inv, 1.0f, 3);
+    codes[w] = broken ? 0u : q;
+  }
 }
 
 typedef _Float16 kv_f16x2 __attribute__((ext_vector_type(2)));
