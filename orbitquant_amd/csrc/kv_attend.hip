@@ -19,6 +19,9 @@ namespace {
 // Cut, 512 workgroups or more, two on each compute unit at once: 131101 tokens, 8 heads, 34 us (before the other steps 1024: 39.7, 256: 35.0, 512: 34.6).
 // Up to three times as many where a part keeps 60 steps, so that requests of different lengths even out, the longest parts first: 64 of up to
 // 16384, 130 us (512 workgroups: 139; four times: 132).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 15.5 us.
+// Short and many: one wavefront a workgroup instead of four that share few steps, where there are enough of them to fill the chip (500 requests of up to 60
+// tokens, 8 heads, 31.5 -> 14.5 us, of up to 500 49 -> 43; 128 of up to 256 13.2 -> 10.1, but 64 of them 8.7 -> 9.4).
+constexpr int kFewAlone = 8;  // steps
 constexpr int kFewWhole = 16, kFewWholeMost = 64, kFewGroups = 512, kFewSteps = 60, kFewLeast = 4;
 // Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the workgroups that the chip holds (two on
 // a compute unit, of heads of 256 one), and at least sixteen steps of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us;
@@ -158,6 +161,7 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
     a.few.sorted = groups > kFewGroups;
     a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
   }
+  a.few_alone = a.few_requests > 0 && steps <= kFewAlone && (steps <= 1 || whole > 128 * steps);
   const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
   if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
   const uint64_t bytes = kv_places(a.few, 2 * a.few.target, heads, 16, dim, static_cast<char *>(workspace), 0);

@@ -814,17 +814,18 @@ __device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, i
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
-// Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS.  A step's
+// Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS (or one
+// wavefront takes them all, where requests are short and many).  A step's
 // keys, scales and values (8.4 KB at D = 128) are requested a step of the wavefront's ahead, into the registers of the ones just used.
 // Long ones are bound by memory: 131101 tokens, 8 heads of 128, 138 MB in 26.6 us; 64 requests, 668 MB in 122 to 126, 5.4 TB/s of the 6.3 that a
 // read of nothing else reaches (vector instructions issue in half of the cycles, the matrix units are busy in 15 %).  Short ones by
 // latency: 1003 tokens 8.9 us, three dependent loads (length, page, keys) and four steps a wavefront.  Eight wavefronts a workgroup: 9.3.
-template <int D, int SPLIT, bool WIDE>
-__global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
+template <int D, int SPLIT, bool WIDE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
   constexpr int PITCH = D + 4;
-  __shared__ __attribute__((aligned(16))) float join[4][16][PITCH];
-  __shared__ float refs[4][16], sums[4][16];
+  __shared__ __attribute__((aligned(16))) float join[WAVES][16][PITCH];
+  __shared__ float refs[WAVES][16], sums[WAVES][16];
   __shared__ uint32_t signs[D / 4];
   if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -835,7 +836,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   if (a.few.target == 0) {
     part = {{}, group, 0, 1, 0};
     if (!kv_few_tile(a, group, part.rows)) return;
-  } else if (!kv_few_part<256>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
+  } else if (!kv_few_part<64 * WAVES>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
     return;
   }
   const KvRows r = part.rows;
@@ -857,7 +858,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
     const auto request = [&] {
       if (step < end) {
         kv_request<D, WIDE>(a, kv_head, n, g, step, kv_pages_of<WIDE>(a, table, n, g, step), raw);
-        next = kv_pages_of<WIDE>(a, table, n, g, step + 4);
+        next = kv_pages_of<WIDE>(a, table, n, g, step + WAVES);
       }
     };
     if constexpr (D < 256) request();
@@ -878,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   // then waits for all of them.
   const auto take_step = [&](auto more) {
     KvPages later = next;
-    if constexpr (more) later = kv_pages_of<WIDE>(a, table, n, g, step + 8);  // (before what is requested next: loads come back in order)
+    if constexpr (more) later = kv_pages_of<WIDE>(a, table, n, g, step + 2 * WAVES);  // (before what is requested next: loads come back in order)
     float x[16], vs[16];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -908,7 +909,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
     // is a wait for all that was just requested.
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(x[i]), "+v"(vs[i])::"memory");
-    if constexpr (more) kv_request_keys<D, WIDE>(a, kv_head, n, g, step + 4, next, raw);
+    if constexpr (more) kv_request_keys<D, WIDE>(a, kv_head, n, g, step + WAVES, next, raw);
     const int first = step * 64;
     if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
 #pragma unroll
@@ -937,14 +938,14 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
         o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[half], o[2 * j + 1], 0, 0, 0);
       }
     }
-    if constexpr (more) kv_request_values<D, WIDE>(a, kv_head, n, g, step + 4, next, raw);
+    if constexpr (more) kv_request_values<D, WIDE>(a, kv_head, n, g, step + WAVES, next, raw);
     next = later;
   };
-  for (; step + 4 < end; step += 4) take_step(std::true_type{});
+  for (; step + WAVES < end; step += WAVES) take_step(std::true_type{});
   if (step < end) take_step(std::false_type{});
   st.ref = st.reference();
 
-  // The four wavefronts, in their order.  A lane has eight dimensions of a row now, as it has where vectors are written to the cache,
+  // The wavefronts, in their order.  A lane has eight dimensions of a row now, as it has where vectors are written to the cache,
   // so that a row's sums and its rotation are many lanes' work: with four rows one wavefront's, eight values a lane instead of 32.
   const float own_sum = kv_over_groups(st.sum, kv_sum_of);
   if (n < r.rows) {
@@ -962,18 +963,20 @@ __global__ __launch_bounds__(256, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   __syncthreads();
   const bool is_part = part.count > 1;
   const int dims = 8 * kv_part_of<D>(lane);
-  for (int from = wave * (512 / D); from < r.rows; from += 2048 / D) {
+  for (int from = wave * (512 / D); from < r.rows; from += WAVES * (512 / D)) {
     const int at = from + kv_vector_of<D>(lane);
     const bool there = at < r.rows;
-    float of[4], both = kKvNothing, l = 0.0f, y[8];
+    float of[WAVES], both = kKvNothing, l = 0.0f, y[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) of[w] = there ? refs[w][at] : kKvNothing;
-    both = fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+    for (int w = 0; w < WAVES; ++w) {
+      of[w] = there ? refs[w][at] : kKvNothing;
+      both = fmaxf(both, of[w]);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = 0.0f;
     if (there) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         of[w] = kv_exp2(of[w] - both);
         l = fmaf(sums[w][at], of[w], l);
         const float4 u = *reinterpret_cast<const float4 *>(&join[w][at][dims]), v = *reinterpret_cast<const float4 *>(&join[w][at][dims + 4]);
@@ -1216,7 +1219,11 @@ bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
     if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kernel), kv_many_lds<D>())) return false;
     launch_kernel(kernel, dim3(heads * (a.many.target != 0 ? a.many.target : a.many_tiles)), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
   }
-  if (a.few_requests > 0) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE>, dim3(heads * (a.few.target + a.few_requests * a.few_tiles)), dim3(256), 0, stream, a);
+  if (a.few_requests > 0) {
+    const dim3 grid(heads * (a.few.target + a.few_requests * a.few_tiles));
+    if (a.few_alone) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 1>, grid, dim3(64), 0, stream, a);
+    else launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 4>, grid, dim3(256), 0, stream, a);
+  }
   return true;
 }
 

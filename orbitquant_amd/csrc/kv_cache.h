@@ -55,6 +55,7 @@ struct KvAttendArgs {
   bool causal;
   float scale;
   int few_tiles, few_requests, few_rows, few_in_tile;  // kernel for few rows: tiles of a request, requests (0: not launched), the rows of a request up to which it has it, rows of a tile at most
+  bool few_alone;                     // in the first: one wavefront a workgroup
   int many_tiles;                     // kernel for many rows (0: not launched)
   KvCut few, many;
   void *out;

@@ -30,6 +30,22 @@ def test_attend_many_requests_in_parts(requests, longest, heads, window):
                window=window)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("requests,longest,window", [(3, 60, None), (140, 120, 50), (530, 480, None)])
+def test_attend_short_and_many(requests, longest, window, dim, page, dtype):
+    """A few steps of very many requests, groups of other sizes than the tile's, none and one token among the lengths."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(requests + dim)
+    lengths = rng.randint(0, longest + 1, requests)
+    lengths[:3] = longest, 0, 1
+    lengths = lengths.tolist()
+    cache, table = _filled(rng, lengths, 2, dim, page, extra_columns=0)
+    q = _queries(rng, requests, 2 * 5, dim, dtype)
+    _check(kv_attend(q, cache, table, _i32(lengths), window=window, max_length=longest, return_lse=True), q, cache, table, _i32(lengths), window=window)
+
+
 @pytest.mark.parametrize("requests,heads", [(40, 16), (65, 8), (300, 2), (400, 1)])
 def test_attend_long_requests_in_parts(requests, heads):
     """The same where requests are so long that they are always cut: the tiles of a wavefront, of a few a lane, of the
