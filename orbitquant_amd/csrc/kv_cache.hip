@@ -116,9 +116,10 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 // ---- into the cache and back -----------------------------------------------------------------------------------------
 // A workgroup takes one head of sixteen tokens, keys and values all requested at once.  A token's key is D / 2 bytes in a row, but its
 // value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen tokens change places in LDS, and four tokens
-// whose slots follow each other in a page (a prompt's, nearly always) are one dword of a row.  MI355X, 8192 tokens of 8 heads of 128 in bf16 (42 MB): write 16 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a
-// store and lanes exchanged through LDS 52).  Bound by vector instructions, some 25 a value, which issue in nine of ten cycles: eleven of
-// them the seven stages of the transform; the bytes alone take 9.
+// whose slots follow each other in a page (a prompt's, nearly always) are one dword of a row.  MI355X, 8192 tokens of 8 heads of 128 in
+// bf16 (42 MB): write 16 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a store and lanes exchanged through LDS 52).
+// Bound by vector instructions, 23 and 25 a value, which issue in 78 and 91 % of the cycles: ten and eleven of them the seven stages of the
+// transform; the bytes alone take 9.
 constexpr int kKvGroup = 16;  // tokens of a workgroup
 
 template <int DT>
@@ -179,15 +180,27 @@ __device__ __forceinline__ void group_places(KvPlace (&places)[kKvGroup], const 
   }
 }
 
+// On the way out, where the slots are waited for, as they are.
+__device__ __forceinline__ void group_slots(int64_t (&slots)[kKvGroup], const int64_t *from, int64_t first, int64_t tokens, int64_t most) {
+  if (threadIdx.x < kKvGroup) {
+    int64_t slot = -1;
+    if (first + threadIdx.x < tokens) slot = from[first + threadIdx.x];
+    slots[threadIdx.x] = slot < most ? slot : -1;
+  }
+}
+
 // Whether four tokens' bytes of a row are one dword.
-__device__ __forceinline__ bool in_a_row(const KvPlace *places, int page_shift) {
-  const int64_t s = places[0].slot;
-  return s >= 0 && places[1].slot == s + 1 && places[2].slot == s + 2 && places[3].slot == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
+__device__ __forceinline__ int64_t slot_of(int64_t slot) { return slot; }
+__device__ __forceinline__ int64_t slot_of(const KvPlace &place) { return place.slot; }
+template <typename Token>
+__device__ __forceinline__ bool in_a_row(const Token *tokens, int page_shift) {
+  const int64_t s = slot_of(tokens[0]);
+  return s >= 0 && slot_of(tokens[1]) == s + 1 && slot_of(tokens[2]) == s + 2 && slot_of(tokens[3]) == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
 }
 
 // Values of a lane: sixteen on the way in, where a vector's scale is found once for twice as many of them and one stage fewer lies between lanes
 // (write 18.1 -> 16.2 us), eight on the way out (sixteen 16.3 -> 16.8).
-constexpr int kKvWriteEach = 16, kKvReadEach = 8;
+constexpr int kKvWriteEach = 16;
 template <int LANES>  // of a vector
 constexpr int kv_group_threads() { return LANES == 4 ? 128 : 256; }
 
@@ -256,42 +269,43 @@ __global__ __launch_bounds__(kv_group_threads<D / kKvWriteEach>()) void kv_write
 }
 
 template <int D, int DT>
-__global__ __launch_bounds__(kv_group_threads<D / kKvReadEach>()) void kv_read_kernel(KvReadArgs a) {
-  constexpr int E = kKvReadEach, THREADS = kv_group_threads<D / E>(), AT_ONCE = THREADS * E / D, PASSES = 2 * kKvGroup / AT_ONCE;
+__global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
+  constexpr int AT_ONCE = 2048 / D, PASSES = 2 * kKvGroup / AT_ONCE;
   constexpr int ROWS = (D / 2) * (kKvGroup / 4);   // dwords of the values, turned by LDS
-  __shared__ KvPlace places[kKvGroup];
+  __shared__ int64_t slots[kKvGroup];
   __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D, E>(lane);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = kv_part_of<D>(lane);
   const int head = blockIdx.x % a.cache.heads;
   const int64_t first = static_cast<int64_t>(blockIdx.x / a.cache.heads) * kKvGroup;
   const int shift = a.cache.page_shift;
   const uint2 signs = reinterpret_cast<const uint2 *>(a.cache.signs)[part];
   const uint32_t words[2] = {signs.x, signs.y};
-  group_places<D>(places, a.cache, a.slots, first, a.tokens, head);
+  group_slots(slots, a.slots, first, a.tokens, a.cache.pages << shift);
   __syncthreads();
   uint32_t keys[PASSES];
   float scales[PASSES];
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane);
-    const KvPlace &place = places[vector & (kKvGroup - 1)];
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane);
+    const int64_t slot = slots[vector & (kKvGroup - 1)];
+    const int64_t at = ((((slot >> shift) * a.cache.heads + head) << shift) + (slot & ((1 << shift) - 1)));
     keys[p] = 0;
     scales[p] = 0.0f;
-    if (place.slot >= 0) {
-      if (vector < kKvGroup) keys[p] = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[place.key * (D / E) + part];
-      scales[p] = bf16_bits_to_f32((vector < kKvGroup ? a.cache.k_scales : a.cache.v_scales)[place.key]);
+    if (slot >= 0) {
+      if (vector < kKvGroup) keys[p] = reinterpret_cast<const uint32_t *>(a.cache.k_codes)[at * (D / 8) + part];
+      scales[p] = bf16_bits_to_f32((vector < kKvGroup ? a.cache.k_scales : a.cache.v_scales)[at]);
     }
   }
-  for (int i = threadIdx.x; i < ROWS; i += THREADS) {
+  for (int i = threadIdx.x; i < ROWS; i += 256) {
     const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
-    const uint8_t *const at_row = a.cache.v_codes + (static_cast<int64_t>(row) << shift);
+    const auto place = [&](int64_t slot) { return a.cache.v_codes + ((((slot >> shift) * a.cache.heads + head) * (D / 2) + row) << shift) + (slot & ((1 << shift) - 1)); };
     uint32_t word = 0;
-    if (in_a_row(places + t, shift)) {
-      __builtin_memcpy(&word, at_row + places[t].value, 4);
+    if (in_a_row(slots + t, shift)) {
+      __builtin_memcpy(&word, place(slots[t]), 4);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (places[t + k].slot >= 0) word |= static_cast<uint32_t>(at_row[places[t + k].value]) << (8 * k);
+        if (slots[t + k] >= 0) word |= static_cast<uint32_t>(*place(slots[t + k])) << (8 * k);
       }
     }
 #pragma unroll
@@ -300,16 +314,16 @@ __global__ __launch_bounds__(kv_group_threads<D / kKvReadEach>()) void kv_read_k
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int vector = p * AT_ONCE + wave * (64 * E / D) + kv_vector_of<D, E>(lane), token = vector & (kKvGroup - 1);
+    const int vector = p * AT_ONCE + wave * (AT_ONCE / 4) + kv_vector_of<D>(lane), token = vector & (kKvGroup - 1);
     const kv_f16x8 c = kv_decode8(vector < kKvGroup ? keys[p] : bytes[token][part]);
-    float y[E];
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = static_cast<float>(c[i]) * scales[p];
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(c[i]) * scales[p];
     kv_butterflies<D>(y, lane);
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] *= 1.0f / D;
+    for (int i = 0; i < 8; ++i) y[i] *= 1.0f / D;
     times_signs(y, words);
-    if (first + token < a.tokens) store8<DT>(vector < kKvGroup ? a.k : a.v, ((first + token) * a.cache.heads + head) * D + E * part, y);
+    if (first + token < a.tokens) store8<DT>(vector < kKvGroup ? a.k : a.v, ((first + token) * a.cache.heads + head) * D + 8 * part, y);
   }
 }
 
@@ -334,7 +348,7 @@ struct RunWrite {
 };
 template <int D, int DT>
 struct RunRead {
-  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_group_threads<D / kKvReadEach>()), 0, s, a); }
+  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
 };
 
 }  // namespace
