@@ -23,10 +23,11 @@ namespace {
 // tokens, 8 heads, 31.5 -> 14.5 us, of up to 500 49 -> 43; 128 of up to 256 13.2 -> 10.1, but 64 of them 8.7 -> 9.4).
 constexpr int kFewAlone = 8;  // steps
 constexpr int kFewWhole = 16, kFewWholeMost = 64, kFewGroups = 512, kFewSteps = 60, kFewLeast = 4;
-// Many rows.  A part is 128 rows of fp32 that are written and read again: only where tiles are too few for the workgroups that the chip holds (two on
-// a compute unit, of heads of 256 one), and at least sixteen steps of them.  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us;
-// 2048 on their own, 264 tiles of few steps each: 68 -> 97 us if they were cut.
-constexpr int kManyGroups = 512, kManyLeast = 16;
+// Many rows.  A part is 128 rows of fp32 that are written and read again: only above sixteen steps (500 behind 300 tokens, 8 heads, 31 -> 36 us), and
+// only where tiles are fewer than the workgroups that the chip holds, two on a compute unit, of heads of 256 one (2048 on their own, 264
+// tiles of few steps each: 68 -> 97 us), into eight steps at least (with sixteen: 1500 in fp32, 4 heads, 58 us, now 50; 64 rows behind 2000 tokens, D = 256, 59
+// and 43; with six these are as often slower).  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us.
+constexpr int kManyGroups = 512, kManyWhole = 16, kManyLeast = 8;
 
 constexpr int kJoinBlocks = 4;  // workgroups of a tile, at most
 
@@ -163,7 +164,7 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   }
   a.few_alone = a.few_requests > 0 && steps <= kFewAlone && (steps <= 1 || whole > 128 * steps);
   const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
-  if (a.many_tiles > 0 && steps > kManyLeast && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
+  if (a.many_tiles > 0 && steps > kManyWhole && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
   const uint64_t bytes = kv_places(a.few, 2 * a.few.target, heads, 16, dim, static_cast<char *>(workspace), 0);
   return kv_places(a.many, a.many.target, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }
