@@ -40,17 +40,19 @@ class OrbitCachedAttention(nn.Module):
         self.rotary = rotary
         self.window = window
 
-    def forward(self, x: torch.Tensor, assignment: KVAssignment, block_table: torch.Tensor, *, max_new: int = 1,
+    def forward(self, x: torch.Tensor, assignment: KVAssignment, block_table: torch.Tensor, *, one_each: bool = False, max_new: int | None = None,
                 max_length: int | None = None) -> torch.Tensor:
-        """`max_new`: 1 where every request has exactly one new token (a decoding step); otherwise the largest number of a request's,
-        as far as it is known.  `max_length` as for `kv_attend`."""
+        """`one_each`: every request has exactly one new token, row r of x is request r's (a decoding step, which then need not look
+        for a request's rows).  Otherwise rows belong to the requests that `assignment.starts` gives them to, and those of no request attend to nothing.
+        `max_new` and `max_length` as for `kv_attend`: hints."""
         tokens, dim = x.shape[0], self.cache.head_dim
+        if one_each and tokens != assignment.lengths.numel():
+            raise ValueError(f"one_each: {tokens} rows for {assignment.lengths.numel()} requests")
         q, k, v = OrbitLinearGroup(self.q, self.k, self.v)(x)
         q, k, v = (t.view(tokens, -1, dim) for t in (q, k, v))
         if self.rotary is not None:
             q, k = self.rotary(q, k, assignment.positions)
         kv_write(k, v, assignment.slots, self.cache)
-        one_each = max_new == 1 and tokens == assignment.lengths.numel()
         attended = kv_attend(q, self.cache, block_table, assignment.lengths, starts=None if one_each else assignment.starts, max_new=max_new,
                              max_length=max_length, window=self.window)
         return self.out(attended.reshape(tokens, -1))

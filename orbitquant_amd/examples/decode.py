@@ -67,7 +67,7 @@ class Decoder(nn.Module):
         self.block_table = counts(requests, width) - 1
         self.free_pages = torch.randperm(requests * width, generator=generator, device=device, dtype=torch.int32)
         self.lengths, self.taken, self.last = counts(requests), counts(1), torch.zeros(requests, dtype=torch.int64, device=device)
-        self.one_each = counts(requests) + 1     # (held here: a graph reads it at every replay)
+        self.one_new = counts(requests) + 1      # (held here: a graph reads it at every replay)
 
     @torch.no_grad()
     def step(self, ids: torch.Tensor, new_lengths: torch.Tensor, **hints) -> torch.Tensor:
@@ -88,11 +88,11 @@ class Decoder(nn.Module):
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            self.step(self.last, self.one_each)
+            self.step(self.last, self.one_new, one_each=True)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            self.step(self.last, self.one_each)
+            self.step(self.last, self.one_new, one_each=True)
         for t, was in zip((self.lengths, self.taken, self.last, self.block_table), state):
             t.copy_(was)
         return graph

@@ -1,0 +1,61 @@
+"""`OrbitCachedAttention` where requests do not have one new token each, and the decoding example's caches, tables and pages."""
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv_cache import _cache, _check, _i32
+from test_gpu_kv_serving import _layer
+
+pytestmark = pytest.mark.gpu
+
+
+def _prompted(window=None):
+    """A layer whose cache holds prompts of three requests."""
+    from orbitquant_amd import kv_assign
+
+    rng = np.random.RandomState(30)
+    cache = _cache(20, 2, 64, 16, fill=0xFF)
+    layer = _layer(cache, 4, 256, window=window)
+    table = torch.full((3, 6), -1, dtype=torch.int32, device="cuda")
+    free = _i32(rng.permutation(20).tolist())
+    got = kv_assign(_i32([0, 0, 0]), _i32([30, 17, 60]), table, free, _i32([0]), page_size=16, tokens=107)
+    layer(_inputs(rng, 107), got, table, max_new=60)
+    return rng, layer, table, free, got
+
+
+def _inputs(rng, tokens):
+    return torch.from_numpy(rng.standard_normal((tokens, 256)).astype(np.float32)).to("cuda", torch.bfloat16)
+
+
+@pytest.mark.parametrize("window", [None, 20])
+@pytest.mark.parametrize("new,tokens", [([1, 0, 1], 3), ([0, 0, 1], 3), ([2, 0, 1], 3), ([2, 1, 0], 3), ([0, 0, 0], 3), ([1, 1, 1], 3), ([1, 1, 0], 2), ([0, 3, 1], 5)])
+@pytest.mark.parametrize("hints", [{}, {"max_new": 1}, {"max_new": 3, "max_length": 90}, {"max_length": 10}])
+def test_rows_belong_to_the_requests_that_starts_names(new, tokens, window, hints):
+    """As many rows as requests does not mean a row each: requests without new tokens in a batch of a fixed size, and several tokens of one."""
+    from orbitquant_amd import kv_assign, kv_attend
+
+    rng, layer, table, free, before = _prompted(window)
+    got = kv_assign(before.lengths, _i32(new), table, free, before.taken, page_size=16, tokens=tokens)
+    x = _inputs(rng, tokens)
+    y = layer(x, got, table, **hints)
+    q = layer.q(x).view(tokens, 4, 64)
+    attended = kv_attend(q, layer.cache, table, got.lengths, starts=got.starts, window=window, return_lse=True)
+    _check(attended, q, layer.cache, table, got.lengths, starts=got.starts, window=window)
+    assert (attended[0][sum(new):] == 0).all()
+    assert torch.equal(y, layer.out(attended[0].reshape(tokens, -1)))
+
+
+def test_one_row_each_where_the_caller_says_so():
+    from orbitquant_amd import kv_assign, kv_attend
+
+    rng, layer, table, free, before = _prompted()
+    got = kv_assign(before.lengths, _i32([1, 1, 1]), table, free, before.taken, page_size=16, tokens=3)
+    x = _inputs(rng, 3)
+    y = layer(x, got, table, one_each=True)
+    q = layer.q(x).view(3, 4, 64)
+    attended = kv_attend(q, layer.cache, table, got.lengths, return_lse=True)
+    _check(attended, q, layer.cache, table, got.lengths)
+    assert torch.equal(y, layer.out(attended[0].reshape(3, -1)))
+    with pytest.raises(ValueError, match="one_each"):
+        layer(_inputs(rng, 2), got, table, one_each=True)
