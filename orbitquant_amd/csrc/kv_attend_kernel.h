@@ -19,8 +19,8 @@
 //                 16 g .. 16 g + 15, sixteen bytes, whose halves are regrouped by token pair.
 // So pages may be as small as sixteen tokens.
 //
-// Precision.  The codes are exact in fp16.  A rotated query is scaled by a power of two to use fp16's range and rounded to its
-// eleven bits, and so are the weights e^(s - R) b_t; SPLIT 1 (fp16 inputs) keeps a second fp16 part of the query, SPLIT 2 (fp32
+// Precision.  The codes are exact in fp16.  A rotated query is scaled by a power of two to use fp16's range (its own, or one that it shares
+// with rows of about its size) and rounded to its eleven bits, and so are the weights e^(s - R) b_t; SPLIT 1 (fp16 inputs) keeps a second fp16 part of the query, SPLIT 2 (fp32
 // inputs) of both, which leaves 22 bits.  Sums, maxima and exponentials are fp32.
 // The reference R of a row is not its maximum: it is raised when a weight could pass 2^15, to where the largest is about 2^10.
 // Rows are so rescaled a few times in all, no maximum is exchanged between lanes in between, and the fp16 weights have 24
@@ -75,6 +75,13 @@ __device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4]) {
   for (int i = 0; i < D / 4; i += 2) kv_lane_butterfly<16>(y[i], y[i + 1]);
 #pragma unroll
   for (int i = 0; i < D / 4; i += 2) kv_lane_butterfly<32>(y[i], y[i + 1]);
+}
+
+typedef short kv_i16x2 __attribute__((ext_vector_type(2)));
+constexpr int kDppHalfMirror = 0x141, kDppMirror = 0x140;  // of eight lanes, of sixteen
+template <int CTRL>
+__device__ __forceinline__ kv_i16x2 kv_row_max(kv_i16x2 x) {
+  return __builtin_elementwise_max(x, __builtin_bit_cast(kv_i16x2, kv_dpp<CTRL>(__builtin_bit_cast(uint32_t, x))));
 }
 
 // Over the four lanes that hold a row (lane & 15 the same).
@@ -583,6 +590,10 @@ struct KvQuery {
 __device__ __forceinline__ int kv_query_exponent(float top) {
   return top > 0.0f && top < INFINITY ? min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10, -110), 117) : 0;
 }
+// How far apart the exponents of rows may be that share one: an entry's last place is then 2^-25 / 2^(10 - spread) of its row's top, and
+// the root of D entries' worth of that stays below a part's own rounding (2^-12, of two parts 2^-22).
+template <int SPLIT>
+constexpr int kv_query_spread() { return SPLIT == 0 ? 16 : 8; }
 __device__ __forceinline__ float kv_power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 // Two fp16 parts of a pair of numbers.  The first is cut off, by an instruction of its own: the conversion that rounds is merged into
@@ -1022,6 +1033,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   };
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint32_t signs[D / 4];
+  __shared__ float own_factors[kKvManyRows];  // (of rows that do not share one; in registers they would be spilled)
   if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   Step *steps = reinterpret_cast<Step *>(lds);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1077,27 +1089,42 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     load(step, page);
   }
 
+  // One power of two for the workgroup's rows, whose factor goes into the keys' scales once a step; where rows are further apart than the format
+  // holds, each has its own, which multiplies its scores: a product more of each, so that is a loop of its own.  (The other one keeps its time: a
+  // prompt of 8192 566 us with and without; with one loop gone through again for each class of sizes 608.)
   kv_f16x8 q[RT][C], q_rest[RT][SPLIT > 0 ? C : 1];
   float factor;
+  bool apart;
   {
-    float y[RT][D / 4], top = 0.0f;
+    constexpr short NONE = -1000;
+    float y[RT][D / 4];
+    int own[RT];
+    kv_i16x2 reach = {NONE, NONE};  // the largest exponent, and what the smallest lacks to 0
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float own_top = query[t].rotate(row[t].token >= 0, y[t]);
-      top = own_top < INFINITY ? fmaxf(top, own_top) : top;  // (a broken row is its own affair)
+      own[t] = kv_query_exponent(own_top);
+      const short e = static_cast<short>(own[t]);
+      if (own_top > 0.0f && own_top < INFINITY) reach = __builtin_elementwise_max(reach, kv_i16x2{e, static_cast<short>(-e)});  // (a broken row is its own affair, zeros have any exponent)
     }
-    // one power of two for the workgroup's rows: its factor goes into the keys' scales
-#pragma unroll
-    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-    float *tops = steps[1].ks;  // (the first step decodes into steps[0])
-    if (lane == 0) tops[wave] = top;
+    reach = kv_row_max<kDppXor1>(reach);
+    reach = kv_row_max<kDppXor2>(reach);
+    reach = kv_row_max<kDppHalfMirror>(reach);
+    reach = kv_row_max<kDppMirror>(reach);
+    kv_i16x2 *reaches = reinterpret_cast<kv_i16x2 *>(steps[1].ks);  // (the first step decodes into steps[0])
+    if (lane == 0) reaches[wave] = reach;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w]);
-    const int exponent = kv_query_exponent(top);
-    factor = a.scale * (1.44269504088896f / D) * kv_power_of_two(exponent);
+    for (int w = 0; w < WAVES; ++w) reach = __builtin_elementwise_max(reach, reaches[w]);
+    const int exponent = kv_uniform(reach[0] != NONE ? reach[0] : 0);
+    apart = kv_uniform(reach[0] + reach[1]) > kv_query_spread<SPLIT>();
+    factor = a.scale * (1.44269504088896f / D) * (apart ? 1.0f : kv_power_of_two(exponent));
 #pragma unroll
-    for (int t = 0; t < RT; ++t) kv_query_parts<D, SPLIT>(y[t], kv_power_of_two(-exponent), q[t], q_rest[t]);
+    for (int t = 0; t < RT; ++t) {
+      const int of_row = apart ? own[t] : exponent;
+      if (apart && g == 0) own_factors[(wave * RT + t) * 16 + n] = kv_power_of_two(of_row);  // (read behind the loop's first barrier)
+      kv_query_parts<D, SPLIT>(y[t], kv_power_of_two(-of_row), q[t], q_rest[t]);
+    }
   }
   const int wave_first = wave * RT * 16, wave_rows = min(r.rows - wave_first, RT * 16);  // rows of this wavefront, if any
   const KvSpan own = kv_span_of(a, r, r.first + min(wave_first, r.rows - 1), max(wave_rows, 1));
@@ -1130,77 +1157,84 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     if (step + 1 < end) load(step + 1, next);
     later = kv_pages_of<WIDE>(a, table, n, g, step + 2);
   }
-  for (int now = 0; step < end; ++step, now ^= 1) {
-    __syncthreads();  // this step is decoded, and nobody reads the one before it any more
-    const Step &from = steps[now];
-    const bool here = kv_page_there(a, page.v);
-    if (step + 1 < end) {
-      decode(steps[now ^ 1]);
-      if (step + 2 < end) load(step + 2, later);
-    }
-    page = next;
-    next = later;
-    later = kv_pages_of<WIDE>(a, table, n, g, step + 3);
-    const int first = step * 64;
-    if (wave_rows <= 0 || first > own.highest || first + 63 < own.lowest) continue;
+  const auto walk = [&](auto each) __attribute__((always_inline)) {
+    for (int now = 0; step < end; ++step, now ^= 1) {
+      __syncthreads();  // this step is decoded, and nobody reads the one before it any more
+      const Step &from = steps[now];
+      const bool here = kv_page_there(a, page.v);
+      if (step + 1 < end) {
+        decode(steps[now ^ 1]);
+        if (step + 2 < end) load(step + 2, later);
+      }
+      page = next;
+      next = later;
+      later = kv_pages_of<WIDE>(a, table, n, g, step + 3);
+      const int first = step * 64;
+      if (wave_rows <= 0 || first > own.highest || first + 63 < own.lowest) continue;
 
-    float x[RT][16], vs[16];
+      float own_factor[RT];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      kv_f32x4 s[RT];
+      for (int t = 0; t < RT; ++t) own_factor[t] = each ? own_factors[(wave * RT + t) * 16 + n] : 1.0f;
+      float x[RT][16], vs[16];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) s[t] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k = 0; k < 4; ++k) {
+        kv_f32x4 s[RT];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const kv_f16x8 codes = from.k[k][c][lane];
+        for (int t = 0; t < RT; ++t) s[t] = kv_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          if constexpr (SPLIT > 0) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[t][c], s[t], 0, 0, 0);
-          s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[t][c], s[t], 0, 0, 0);
-        }
-      }
-      const kv_f32x4 ks = *reinterpret_cast<const kv_f32x4 *>(&from.ks[16 * g + 4 * k]), v = *reinterpret_cast<const kv_f32x4 *>(&from.vs[16 * g + 4 * k]);
+        for (int c = 0; c < C; ++c) {
+          const kv_f16x8 codes = from.k[k][c][lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vs[4 * k + i] = v[i];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) x[t][4 * k + i] = fmaf(s[t][i], ks[i], -st[t].ref);
-      }
-    }
-    if (first + 63 > own.all_high || first < own.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = first + 16 * g + i;
-        const bool there = here && key <= r.last_key;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) x[t][i] = kv_masked_score(x[t][i], vs[i], key, there, row[t]);
-        vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
-      }
-    }
-    const float top_exponent = kv_exponent_above(vs);
-    kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      kv_keep_in_range<D>(x[t], top_exponent, st[t], o[t]);
-      kv_weights<SPLIT>(x[t], vs, st[t].sum, p[t], p_rest[t]);
-    }
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const kv_f16x8 even = from.v[j][half][0][lane], odd = from.v[j][half][1][lane];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          if constexpr (SPLIT > 1) {
-            o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p_rest[t][half], o[t][2 * j], 0, 0, 0);
-            o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p_rest[t][half], o[t][2 * j + 1], 0, 0, 0);
+          for (int t = 0; t < RT; ++t) {
+            if constexpr (SPLIT > 0) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q_rest[t][c], s[t], 0, 0, 0);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q[t][c], s[t], 0, 0, 0);
           }
-          o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[t][half], o[t][2 * j], 0, 0, 0);
-          o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[t][half], o[t][2 * j + 1], 0, 0, 0);
+        }
+        const kv_f32x4 ks = *reinterpret_cast<const kv_f32x4 *>(&from.ks[16 * g + 4 * k]), v = *reinterpret_cast<const kv_f32x4 *>(&from.vs[16 * g + 4 * k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          vs[4 * k + i] = v[i];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) x[t][4 * k + i] = fmaf(s[t][i], each ? ks[i] * own_factor[t] : ks[i], -st[t].ref);
+        }
+      }
+      if (first + 63 > own.all_high || first < own.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = first + 16 * g + i;
+          const bool there = here && key <= r.last_key;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) x[t][i] = kv_masked_score(x[t][i], vs[i], key, there, row[t]);
+          vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
+        }
+      }
+      const float top_exponent = kv_exponent_above(vs);
+      kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        kv_keep_in_range<D>(x[t], top_exponent, st[t], o[t]);
+        kv_weights<SPLIT>(x[t], vs, st[t].sum, p[t], p_rest[t]);
+      }
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const kv_f16x8 even = from.v[j][half][0][lane], odd = from.v[j][half][1][lane];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            if constexpr (SPLIT > 1) {
+              o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p_rest[t][half], o[t][2 * j], 0, 0, 0);
+              o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p_rest[t][half], o[t][2 * j + 1], 0, 0, 0);
+            }
+            o[t][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[t][half], o[t][2 * j], 0, 0, 0);
+            o[t][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[t][half], o[t][2 * j + 1], 0, 0, 0);
+          }
         }
       }
     }
-  }
+  };
+  if (apart) walk(std::true_type{});
+  else walk(std::false_type{});
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int64_t place = (static_cast<int64_t>(kv_head) * a.many.places + part.place) * kKvManyRows + (wave * RT + t) * 16 + n;
