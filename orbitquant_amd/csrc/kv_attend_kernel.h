@@ -24,8 +24,8 @@
 // inputs) of both, which leaves 22 bits.  Sums, maxima and exponentials are fp32.
 // The reference R of a row is not its maximum: it is raised when a weight could pass 2^15, to where the largest is about 2^10.
 // Rows are so rescaled a few times in all, no maximum is exchanged between lanes in between, and the fp16 weights have 24
-// binary digits below their largest before they lose any.  R holds the exponent of the largest value scale too (b_t is
-// anything), bounded so that l stays finite.
+// binary digits below their largest before they lose any.  R holds the exponent of the weightiest keys' value
+// scales too (b_t is anything), bounded so that l stays finite.
 //
 // Two kernels.  Few rows (single tokens, at most kKvFewRows of a request): four wavefronts share the keys of sixteen rows, every
 // one decodes for itself, and the launch is bound by the cache's bytes.  Many rows (a prompt): the wavefronts have rows of
@@ -80,8 +80,11 @@ __device__ __forceinline__ void kv_rotate_lane(float (&y)[D / 4]) {
 typedef short kv_i16x2 __attribute__((ext_vector_type(2)));
 constexpr int kDppHalfMirror = 0x141, kDppMirror = 0x140;  // of eight lanes, of sixteen
 template <int CTRL>
-__device__ __forceinline__ kv_i16x2 kv_row_max(kv_i16x2 x) {
+__device__ __forceinline__ kv_i16x2 kv_dpp_max(kv_i16x2 x) {
   return __builtin_elementwise_max(x, __builtin_bit_cast(kv_i16x2, kv_dpp<CTRL>(__builtin_bit_cast(uint32_t, x))));
+}
+__device__ __forceinline__ kv_i16x2 kv_row_max(kv_i16x2 x) {  // of sixteen lanes
+  return kv_dpp_max<kDppMirror>(kv_dpp_max<kDppHalfMirror>(kv_dpp_max<kDppXor2>(kv_dpp_max<kDppXor1>(x))));
 }
 
 // Over the four lanes that hold a row (lane & 15 the same).
@@ -641,9 +644,33 @@ __device__ __forceinline__ float kv_max3(float a, float b, float c) {
   return m;
 }
 
-// x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.
+__device__ __forceinline__ float kv_exponent_of(int scale) { return static_cast<float>(min(max((scale >> 23) - 126, -80), 80)); }  // the scale (its bits) is below 2^this
+__device__ __forceinline__ int kv_largest_scale(const float (&vs)[16]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(vs[i]));
+  return static_cast<int>(top);
+}
+
+// (These two by instructions of their own: what they give is otherwise found in front of the branch that asks for it, whether it is taken or not.)
+__device__ __forceinline__ int kv_smallest_scale(const float (&vs)[16]) {
+  int low = __float_as_int(vs[15]);
+#pragma unroll
+  for (int i = 1; i < 15; i += 2) asm volatile("v_min3_i32 %0, %0, %1, %2" : "+v"(low) : "v"(vs[i]), "v"(vs[i + 1]));
+  return min(low, __float_as_int(vs[0]));
+}
+__device__ __forceinline__ float kv_exponent_alone(float scale) {
+  int bits;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(bits) : "v"(scale));
+  return kv_exponent_of(bits);
+}
+
+// x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.  The exponent of `top`, the largest of the sixteen scales, belongs to keys
+// that the row may not see or hardly weigh: it tells cheaply that no weight is near 2^15, and where the scales are of about one size, where R goes.
+// Where they are not, each key is taken with its own exponent, so that a large value raises R for the rows that it has weight in, and the
+// others keep their weights' digits.  (Always with its own: a prompt of 2048, D = 64, 46.2 -> 50 us; so 47.7.)
 template <int D>
-__device__ __forceinline__ void kv_keep_in_range(float (&x)[16], float top_exponent, KvState &st, kv_f32x4 (&o)[D / 16]) {
+__device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&vs)[16], int top, float top_exponent, KvState &st, kv_f32x4 (&o)[D / 16]) {
   float best = kv_max3(x[0], x[1], x[2]), other = kv_max3(x[3], x[4], x[5]);
   best = kv_max3(best, x[6], x[7]);
   other = kv_max3(other, x[8], x[9]);
@@ -653,7 +680,14 @@ __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], float top_expon
   best = kv_max3(best, other, other) + top_exponent;
   if (__builtin_amdgcn_ballot_w64(best > st.limit) != 0) {
     best = kv_over_groups(best, kv_max_of);
-    const bool raise = best > st.limit;
+    bool raise = best > st.limit;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top - kv_smallest_scale(vs) >= 4 << 23) != 0, false)) {
+      best = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) best = fmaxf(best, x[i] + kv_exponent_alone(vs[i]));
+      best = kv_over_groups(best, kv_max_of);
+      raise = raise && best > fminf(st.limit, 10.0f);  // (wherever it is above 10, so that the next steps need not look)
+    }
     const float up = raise ? best - 10.0f : 0.0f, by = kv_exp2(fminf(-up, 0.0f));  // (down only where nothing is summed up yet)
     st.ref += up;
     st.sum *= by;
@@ -696,12 +730,9 @@ __device__ __forceinline__ float kv_masked_score(float x, float vs, int key, boo
   const bool seen = there && key <= row.high && key >= row.low;
   return seen ? (vs != vs ? NAN : x) : -INFINITY;
 }
-
-__device__ __forceinline__ float kv_exponent_above(const float (&vs)[16]) {  // every scale is below 2^this
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(vs[i]));
-  return static_cast<float>(min(max(static_cast<int>(top >> 23) - 126, -80), 80));
+// Of a key that is not there, whose scale may be anything, the first one's of the lane stands in (its weight is zero, and it is of the others' size).
+__device__ __forceinline__ float kv_masked_scale(const float (&vs)[16], int i, bool there) {
+  return vs[i] != vs[i] ? 0.0f : there ? vs[i] : i > 0 ? vs[0] : 0.0f;
 }
 
 // Sixteen token bytes of two dimensions -> the A operands of the even and the odd one, tiles 2 * half and 2 * half + 1 side by side.
@@ -928,10 +959,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
         const int key = first + 16 * g + i;
         const bool there = here && key <= r.last_key;
         x[i] = kv_masked_score(x[i], vs[i], key, there, row);
-        vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
+        vs[i] = kv_masked_scale(vs, i, there);
       }
     }
-    kv_keep_in_range<D>(x, kv_exponent_above(vs), st, o);
+    const int top = kv_largest_scale(vs);
+    kv_keep_in_range<D>(x, vs, top, kv_exponent_of(top), st, o);
     kv_f16x8 p[2], p_rest[SPLIT > 1 ? 2 : 1];
     kv_weights<SPLIT>(x, vs, st.sum, p, p_rest);
 #pragma unroll
@@ -1020,6 +1052,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
 // Matrix instructions of 32 x 32 overlap in part but leave too few registers: 576 to 587 us.
 template <int D>
 constexpr int kv_many_waves() { return D == 256 ? 8 : 4; }
+template <int D>
+constexpr size_t kv_many_lds() { return 2 * (4 * (D / 32) * 64 * 16 + (D / 32) * 4 * 64 * 16 + 512); }
 
 template <int D, int SPLIT, bool WIDE>
 __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_kernel(KvAttendArgs a) {
@@ -1031,6 +1065,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     kv_f16x8 v[D / 32][2][2][64]; // [dimensions][half of the keys][even, odd][lane]
     float ks[64], vs[64];         // times the scale of the scores; as it is
   };
+  static_assert(2 * sizeof(Step) == kv_many_lds<D>(), "what the launch reserves");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint32_t signs[D / 4];
   __shared__ float own_factors[kKvManyRows];  // (of rows that do not share one; in registers they would be spilled)
@@ -1107,10 +1142,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
       const short e = static_cast<short>(own[t]);
       if (own_top > 0.0f && own_top < INFINITY) reach = __builtin_elementwise_max(reach, kv_i16x2{e, static_cast<short>(-e)});  // (a broken row is its own affair, zeros have any exponent)
     }
-    reach = kv_row_max<kDppXor1>(reach);
-    reach = kv_row_max<kDppXor2>(reach);
-    reach = kv_row_max<kDppHalfMirror>(reach);
-    reach = kv_row_max<kDppMirror>(reach);
+    reach = kv_row_max(reach);
     kv_i16x2 *reaches = reinterpret_cast<kv_i16x2 *>(steps[1].ks);  // (the first step decodes into steps[0])
     if (lane == 0) reaches[wave] = reach;
     __syncthreads();
@@ -1205,14 +1237,15 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
           const bool there = here && key <= r.last_key;
 #pragma unroll
           for (int t = 0; t < RT; ++t) x[t][i] = kv_masked_score(x[t][i], vs[i], key, there, row[t]);
-          vs[i] = there && vs[i] == vs[i] ? vs[i] : 0.0f;
+          vs[i] = kv_masked_scale(vs, i, there);
         }
       }
-      const float top_exponent = kv_exponent_above(vs);
+      const int top = kv_largest_scale(vs);
+      const float top_exponent = kv_exponent_of(top);
       kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        kv_keep_in_range<D>(x[t], top_exponent, st[t], o[t]);
+        kv_keep_in_range<D>(x[t], vs, top, top_exponent, st[t], o[t]);
         kv_weights<SPLIT>(x[t], vs, st[t].sum, p[t], p_rest[t]);
       }
 #pragma unroll
@@ -1241,9 +1274,6 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     kv_finish<D, SPLIT>(a, row[t], g, signs, part.count > 1 ? a.many.out + place * D : nullptr, a.many.stats + place, st[t], o[t]);
   }
 }
-
-template <int D>
-constexpr size_t kv_many_lds() { return 2 * (4 * (D / 32) * 64 * 16 + (D / 32) * 4 * 64 * 16 + 512); }
 
 template <int D, int SPLIT, bool WIDE>
 bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {

@@ -57,3 +57,65 @@ def test_a_row_is_its_own_in_parts(dtype, factor):
     q[101] /= factor if dtype != torch.float16 else 64
     q = q.to(dtype)
     _check(kv_attend(q, cache, table, _i32(lengths), starts=starts, return_lse=True), q, cache, table, _i32(lengths), starts=starts)
+
+
+# ---------------------------------------------------------------- values of one step
+
+def _check_with_overflow(got, q, cache, table, lengths, **kw):
+    """`_check`, where outputs may pass the largest number of their type: an entry is right to be infinite where what its row may be off (the bound
+    is the row's, whose other entries may be far larger) reaches beyond that number."""
+    want, _, bound = oracle.attend(q, cache, table, lengths, **kw)
+    far = oracle.allowed(bound, want, q.dtype)[0][..., None]
+    out = got[0].double().cpu().numpy()
+    fine = np.isinf(out) & (np.sign(out) * want + far > torch.finfo(q.dtype).max)
+    _check((torch.where(torch.from_numpy(fine), torch.from_numpy(want).to(q.dtype), got[0].cpu()), got[1]), q, cache, table, lengths, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,new,at", [(64, 90, 50), (128, 90, 50), (256, 90, 50), (128, 12, 84), (256, 12, 84), (64, 2, 89)])
+@pytest.mark.parametrize("window", [None, 3, 20])
+def test_a_large_value_changes_only_the_rows_that_see_it(window, dim, new, at, dtype):
+    """By both kernels; with a window the rows behind it see past it again."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(new)
+    cache, table = _filled(rng, [90], 1, dim, 32)
+    cache.v_scales[int(table[0, at // 32]), 0, at % 32] *= 2.0 ** 40
+    starts = _i32([0, new])
+    q = _queries(rng, new, 4, dim, dtype)
+    got = kv_attend(q, cache, table, _i32([90]), starts=starts, window=window, return_lse=True)
+    _check_with_overflow(got, q, cache, table, _i32([90]), starts=starts, window=window)
+
+
+def _by_weights(q, cache, table, length):
+    """One request's last token: out, and the mean of |v| over the weights; a relative error of e in every weight moves out by at most 2 e of that."""
+    kc, ks, vc, vs = oracle.cache_codes(cache)
+    dim = kc.shape[-1]
+    turn = oracle.sylvester(dim) / dim * cache[4].cpu().numpy().astype(np.float64)
+    rows = tuple(np.array(x) for x in zip(*[(int(table[0, t // cache.page_size]), 0, t % cache.page_size) for t in range(length)]))
+    k, v = ((oracle.decode(c[rows]) * s[rows][:, None]) @ turn for c, s in ((kc, ks), (vc, vs)))
+    s = q[0].double().cpu().numpy() @ k.T / math.sqrt(dim)
+    w = np.exp(s - s.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    return w @ v, w @ np.linalg.norm(v, axis=-1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [2.0 ** 15, 2.0 ** 30, 2.0 ** 60])
+def test_a_large_value_without_weight_changes_nothing(size, dtype):
+    from orbitquant_amd import OrbitKVCache, kv_attend, kv_write
+
+    rng = np.random.RandomState(32)
+    cache = OrbitKVCache.empty(3, 1, 64, page_size=32)
+    q = _queries(rng, 1, 1, 64, dtype)
+    k, v = (_queries(rng, 90, 1, 64, torch.float32) for _ in range(2))
+    k[60] = -20 * q[0].float()          # a score 20 |q|^2 / 8, some 160, below the others
+    v[60] *= size
+    kv_write(k, v, torch.arange(90, device="cuda"), cache)
+    table = _i32([[0, 1, 2]])
+    out = kv_attend(q, cache, table, _i32([90]))
+    want, mean = _by_weights(q, cache, table, 90)
+    (size_of, _, count, dim), = (oracle.attend(q, cache, table, _i32([90]))[2],)
+    far, _ = oracle.allowed((size_of, mean[None], count, dim), want[None], dtype)
+    off = np.linalg.norm(out.double().cpu().numpy() - want, axis=-1)
+    assert (off <= far).all(), (off, far)
