@@ -55,9 +55,10 @@ __device__ __forceinline__ void join_tile(const KvAttendArgs &a, int block, int 
     float best = kKvNothing, l = 0.0f;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const auto add = [&](const float2 &stats, const float4 &o) {
-      const float both = fmaxf(best, stats.x), mine = kv_exp2(best - both), theirs = kv_exp2(stats.x - both);
+      const float both = fmaxf(best, stats.x), my_half = kv_half_power(best - both), their_half = kv_half_power(stats.x - both);
+      const float mine = my_half * my_half, theirs = their_half * their_half;
       best = both;
-      l = fmaf(l, mine, stats.y * theirs);
+      l = fmaf(l * my_half, my_half, stats.y * their_half * their_half);
       y.x = fmaf(y.x, mine, o.x * theirs); y.y = fmaf(y.y, mine, o.y * theirs);
       y.z = fmaf(y.z, mine, o.z * theirs); y.w = fmaf(y.w, mine, o.w * theirs);
     };

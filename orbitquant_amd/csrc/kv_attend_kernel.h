@@ -25,7 +25,8 @@
 // The reference R of a row is not its maximum: it is raised when a weight could pass 2^15, to where the largest is about 2^10.
 // Rows are so rescaled a few times in all, no maximum is exchanged between lanes in between, and the fp16 weights have 24
 // binary digits below their largest before they lose any.  R holds the exponent of the weightiest keys' value
-// scales too (b_t is anything), bounded so that l stays finite.
+// scales too (b_t is anything, from 2^-80 on: below it R stays, so that l stays finite; above 2^112 l, whose weights are then
+// 2^-102 and less, has fewer than 24 digits before an fp32 ends).
 //
 // Two kernels.  Few rows (single tokens, at most kKvFewRows of a request): four wavefronts share the keys of sixteen rows, every
 // one decodes for itself, and the launch is bound by the cache's bytes.  Many rows (a prompt): the wavefronts have rows of
@@ -55,6 +56,10 @@ constexpr int kKvCutTiles = 384;        // tiles of a launch of the second that 
 __host__ __device__ inline int64_t kv_tile_base(int64_t row, int64_t r) { return row / kKvManyRows + r; }
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 2^(x / 2).  A sum of weights is taken to another reference in two steps of this: with value scales from 2^-80 to 2^127 in it the references are further
+// apart than the exponents of an fp32 reach, the sums themselves are not.
+__device__ __forceinline__ float kv_half_power(float x) { return kv_exp2(0.5f * x); }
 
 // D / 4 values a lane.  Every pair of dimensions that differ in one bit meets once: which bits are registers and which lanes
 // does not matter.
@@ -644,7 +649,7 @@ __device__ __forceinline__ float kv_max3(float a, float b, float c) {
   return m;
 }
 
-__device__ __forceinline__ float kv_exponent_of(int scale) { return static_cast<float>(min(max((scale >> 23) - 126, -80), 80)); }  // the scale (its bits) is below 2^this
+__device__ __forceinline__ float kv_exponent_of(int scale) { return static_cast<float>(max((scale >> 23) - 126, -80)); }  // the scale (its bits) is below 2^this
 __device__ __forceinline__ int kv_largest_scale(const float (&vs)[16]) {
   uint32_t top = 0;
 #pragma unroll
@@ -688,9 +693,9 @@ __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&v
       best = kv_over_groups(best, kv_max_of);
       raise = raise && best > fminf(st.limit, 10.0f);  // (wherever it is above 10, so that the next steps need not look)
     }
-    const float up = raise ? best - 10.0f : 0.0f, by = kv_exp2(fminf(-up, 0.0f));  // (down only where nothing is summed up yet)
+    const float up = raise ? best - 10.0f : 0.0f, half = kv_half_power(fminf(-up, 0.0f)), by = half * half;  // (down only where nothing is summed up yet)
     st.ref += up;
-    st.sum *= by;
+    st.sum = st.sum * half * half;
     st.limit = raise ? 15.0f : st.limit;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) o[j] *= by;
@@ -1009,23 +1014,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
   for (int from = wave * (512 / D); from < r.rows; from += WAVES * (512 / D)) {
     const int at = from + kv_vector_of<D>(lane);
     const bool there = at < r.rows;
-    float of[WAVES], both = kKvNothing, l = 0.0f, y[8];
+    float half[WAVES], both = kKvNothing, l = 0.0f, y[8];
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      of[w] = there ? refs[w][at] : kKvNothing;
-      both = fmaxf(both, of[w]);
+      half[w] = there ? refs[w][at] : kKvNothing;
+      both = fmaxf(both, half[w]);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = 0.0f;
     if (there) {
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        of[w] = kv_exp2(of[w] - both);
-        l = fmaf(sums[w][at], of[w], l);
+        half[w] = kv_half_power(half[w] - both);
+        const float of = half[w] * half[w];
+        l = fmaf(sums[w][at] * half[w], half[w], l);
         const float4 u = *reinterpret_cast<const float4 *>(&join[w][at][dims]), v = *reinterpret_cast<const float4 *>(&join[w][at][dims + 4]);
         const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], of[w], y[e]);
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], of, y[e]);
       }
     }
     const float by = kv_share(l, is_part) * (1.0f / D);

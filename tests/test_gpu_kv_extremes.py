@@ -119,3 +119,24 @@ def test_a_large_value_without_weight_changes_nothing(size, dtype):
     far, _ = oracle.allowed((size_of, mean[None], count, dim), want[None], dtype)
     off = np.linalg.norm(out.double().cpu().numpy() - want, axis=-1)
     assert (off <= far).all(), (off, far)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("sizes", [(1e22, 1e22), (1e25, 1e25), (1e30, 1e30), (1e33, 1e33), (1.0, 1e30), (1e30, 1.0), (1e-30, 1e25), (1e25, 1e-30), (1e-25, 1e25), (1e-30, 1.0)])
+def test_values_of_any_size(sizes, new, dtype):
+    """Numbers of the types that a value's scale holds, large and small ones side by side: in one step, in different steps, by different wavefronts
+    and in different parts."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(33)
+    for length, first in ((60, 25), (400, 64), (400, 350), (1800, 900)):
+        cache, table = _filled(rng, [length], 1, 64, 64)
+        v = torch.where(torch.arange(cache.page_size * table.shape[1], device="cuda") < first, sizes[0], sizes[1])
+        for column in range(-(-length // 64)):
+            cache.v_scales[int(table[0, column]), 0] *= v[64 * column:64 * column + 64]
+        q = _queries(rng, new, 4, 64, dtype)
+        starts = _i32([0, new])
+        for window in (None, 30):
+            _check(kv_attend(q, cache, table, _i32([length]), starts=starts, window=window, return_lse=True), q, cache, table, _i32([length]), starts=starts,
+                   window=window)
