@@ -667,7 +667,7 @@ __device__ __forceinline__ int kv_smallest_scale(const float (&vs)[16]) {
 __device__ __forceinline__ float kv_exponent_alone(float scale) {
   int bits;
   asm volatile("v_mov_b32 %0, %1" : "=v"(bits) : "v"(scale));
-  return kv_exponent_of(bits);
+  return kv_exponent_of(bits < 0x7f800000 ? bits : 0);  // (a NaN has no part in where R goes)
 }
 
 // x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.  The exponent of `top`, the largest of the sixteen scales, belongs to keys
@@ -729,16 +729,39 @@ __device__ __forceinline__ void kv_weights(const float (&x)[16], const float (&v
   }
 }
 
-// Keys that a row does not see, or that are not there.  A weight of 0 does not undo a scale that is NaN: where a value's is, the
-// rows that see it get theirs through the score; what lies behind the last key may be anything.
-__device__ __forceinline__ float kv_masked_score(float x, float vs, int key, bool there, const KvRow &row) {
-  const bool seen = there && key <= row.high && key >= row.low;
-  return seen ? (vs != vs ? NAN : x) : -INFINITY;
-}
-// Of a key that is not there, whose scale may be anything, the first one's of the lane stands in (its weight is zero, and it is of the others' size).
-__device__ __forceinline__ float kv_masked_scale(const float (&vs)[16], int i, bool there) {
-  return vs[i] != vs[i] ? 0.0f : there ? vs[i] : i > 0 ? vs[0] : 0.0f;
-}
+// Keys that a row does not see, or that are not there.  A weight of 0 does not undo a scale that is NaN, so none is multiplied by one.
+__device__ __forceinline__ bool kv_seen(int key, bool there, const KvRow &row) { return there && key <= row.high && key >= row.low; }
+
+// Where several rows share the scales: in the place of what lies behind the last key, which may be anything, stands the lane's first scale (of the
+// others' size), and of a broken value zero.  Those steps are noted, and the rows that see such a value become NaN in the end, not through
+// their weights, whose sum is a result too and has no value in it.
+struct KvBroken {
+  int from, to;  // steps
+  __device__ __forceinline__ void begin() { from = 0x7fffffff; to = -1; }
+  __device__ __forceinline__ void look(float (&vs)[16], int step) {
+    uint32_t top = __float_as_uint(vs[0]);
+    const float last = vs[15];
+#pragma unroll
+    for (int i = 1; i < 15; i += 2) asm volatile("v_max3_u32 %0, %0, %1, %2" : "+v"(top) : "v"(vs[i]), "v"(vs[i + 1]));  // (as above)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) vs[i] = vs[i] != vs[i] ? 0.0f : vs[i];
+    const bool any = __builtin_amdgcn_ballot_w64(max(top, __float_as_uint(last)) > 0x7f800000u) != 0;  // (a branch here costs the steps without a mask, too)
+    from = any ? min(from, step) : from;
+    to = any ? step : to;
+  }
+  // NaN for a row that sees one of them, otherwise 0.
+  __device__ __forceinline__ float of(const KvAttendArgs &a, const int32_t *table, int last_key, const KvRow &row, int kv_head, int g) const {
+    float found = 0.0f;
+    const int last = min(min(row.high, last_key), 64 * to + 63), in_page = (1 << a.cache.page_shift) - 1;
+    for (int key = max(row.low, 64 * from) + g; key <= last; key += 4) {
+      const int page = table[key >> a.cache.page_shift];
+      if (!kv_page_there(a, page)) continue;
+      const float scale = bf16_bits_to_f32(a.cache.v_scales[(kv_block_of(a, page, kv_head) << a.cache.page_shift) + (key & in_page)]);
+      found = scale != scale ? NAN : found;
+    }
+    return kv_over_groups(found, kv_sum_of);
+  }
+};
 
 // Sixteen token bytes of two dimensions -> the A operands of the even and the odd one, tiles 2 * half and 2 * half + 1 side by side.
 __device__ __forceinline__ void kv_decode_values(uint32_t x, uint32_t y, kv_f16x8 &even, kv_f16x8 &odd) {
@@ -962,9 +985,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = first + 16 * g + i;
-        const bool there = here && key <= r.last_key;
-        x[i] = kv_masked_score(x[i], vs[i], key, there, row);
-        vs[i] = kv_masked_scale(vs, i, there);
+        const bool seen = kv_seen(key, here && key <= r.last_key, row);
+        x[i] = seen ? x[i] : -INFINITY;
+        vs[i] = seen ? vs[i] : 0.0f;
       }
     }
     const int top = kv_largest_scale(vs);
@@ -1195,6 +1218,8 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     if (step + 1 < end) load(step + 1, next);
     later = kv_pages_of<WIDE>(a, table, n, g, step + 2);
   }
+  KvBroken broken;
+  broken.begin();
   const auto walk = [&](auto each) __attribute__((always_inline)) {
     for (int now = 0; step < end; ++step, now ^= 1) {
       __syncthreads();  // this step is decoded, and nobody reads the one before it any more
@@ -1242,9 +1267,11 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
           const int key = first + 16 * g + i;
           const bool there = here && key <= r.last_key;
 #pragma unroll
-          for (int t = 0; t < RT; ++t) x[t][i] = kv_masked_score(x[t][i], vs[i], key, there, row[t]);
-          vs[i] = kv_masked_scale(vs, i, there);
+          for (int t = 0; t < RT; ++t) x[t][i] = kv_seen(key, there, row[t]) ? x[t][i] : -INFINITY;
+          vs[i] = there ? vs[i] : i > 0 ? vs[0] : 0.0f;
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (all masks at once are more than there are scalar registers)
         }
+        broken.look(vs, step);
       }
       const int top = kv_largest_scale(vs);
       const float top_exponent = kv_exponent_of(top);
@@ -1274,6 +1301,14 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   };
   if (apart) walk(std::true_type{});
   else walk(std::false_type{});
+  if (broken.to >= 0) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float nan = broken.of(a, table, r.last_key, row[t], kv_head, g);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) o[t][j] += nan;
+    }
+  }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int64_t place = (static_cast<int64_t>(kv_head) * a.many.places + part.place) * kKvManyRows + (wave * RT + t) * 16 + n;

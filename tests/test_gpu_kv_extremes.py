@@ -140,3 +140,26 @@ def test_values_of_any_size(sizes, new, dtype):
         for window in (None, 30):
             _check(kv_attend(q, cache, table, _i32([length]), starts=starts, window=window, return_lse=True), q, cache, table, _i32([length]), starts=starts,
                    window=window)
+
+
+# ---------------------------------------------------------------- broken values
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,length,new,at", [(64, 90, 90, 50), (128, 200, 100, 130), (256, 90, 90, 10), (128, 300, 1, 20), (64, 300, 1, 299), (256, 300, 12, 290), (64, 1800, 30, 700), (64, 1500, 90, 700)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_a_broken_value_leaves_the_scores_alone(window, dim, length, new, at, dtype):
+    """A NaN among the values makes the outputs NaN that see it; the sum of the weights, which lse is, has no value in it.  In steps that a mask goes through and in
+    others, by both kernels and in parts."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(34)
+    cache, table = _filled(rng, [length], 1, dim, 64)
+    cache.v_scales[int(table[0, at // 64]), 0, at % 64] = float("nan")
+    q = _queries(rng, new, 4, dim, dtype)
+    starts, lengths = _i32([0, new]), _i32([length])
+    out, lse = kv_attend(q, cache, table, lengths, starts=starts, window=window, return_lse=True)
+    want, want_lse, bound = oracle.attend(q, cache, table, lengths, starts=starts, window=window)
+    _check((out, torch.where(torch.from_numpy(np.isnan(want).any(-1)).cuda(), torch.from_numpy(want_lse).float().cuda(), lse)), q, cache, table, lengths, starts=starts,
+           window=window)
+    far = oracle.allowed(bound, want, dtype)[1]
+    assert (np.abs(lse.double().cpu().numpy() - want_lse) <= far).all()
