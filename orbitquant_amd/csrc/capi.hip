@@ -624,7 +624,7 @@ int kv_attend_shape(oq::KvAttendArgs &a, int64_t tokens, int64_t heads, int64_t 
     return fail(OQ_ERR_UNSUPPORTED, "kv_attend: tokens=%lld heads=%lld requests=%lld table_width=%lld exceed the grid", (long long)tokens,
                 (long long)heads, (long long)requests, (long long)table_width);
   a.tokens = tokens; a.heads = static_cast<int>(heads); a.group = static_cast<int>(heads / kv_heads); a.requests = static_cast<int>(requests);
-  a.table_width = static_cast<int>(table_width); a.window = static_cast<int>(window < 0x3fffffffLL ? window : 0x3fffffffLL);
+  a.table_width = static_cast<int>(table_width); a.window = static_cast<int>(window < 0x7fffffffLL ? window : 0x7fffffffLL);
   return OQ_OK;
 }
 

@@ -123,6 +123,10 @@ __device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r, int
 }
 __device__ __forceinline__ void kv_keys_of(const KvAttendArgs &a, KvRows &r) { kv_keys_of(a, r, kv_length_of(a, r.request)); }
 
+__device__ __forceinline__ int kv_low_of(const KvAttendArgs &a, int position) {  // the first key that a query there sees (no sum passes 32 bits: positions may be negative)
+  return a.window != 0 && position >= a.window ? position - a.window + 1 : 0;
+}
+
 // What rows [first, first + rows) of the run see: some row the keys lowest..highest, every row the keys all_low..all_high.
 struct KvSpan {
   int lowest, highest, all_low, all_high;
@@ -132,8 +136,8 @@ __device__ __forceinline__ KvSpan kv_span_of(const KvAttendArgs &a, const KvRows
   KvSpan s;
   s.highest = a.causal ? min(to, r.last_key) : r.last_key;
   s.all_high = a.causal ? min(from, r.last_key) : r.last_key;
-  s.lowest = a.window != 0 ? max(from - a.window + 1, 0) : 0;
-  s.all_low = a.window != 0 ? max(to - a.window + 1, 0) : 0;
+  s.lowest = kv_low_of(a, from);
+  s.all_low = kv_low_of(a, to);
   return s;
 }
 
@@ -511,7 +515,7 @@ __device__ __forceinline__ KvRow kv_row_of(const KvAttendArgs &a, const KvRows &
   k.head = kv_head * a.group + row - i * a.group;
   const int position = r.position(i);
   k.high = there ? (a.causal ? min(position, r.last_key) : r.last_key) : -1;
-  k.low = a.window != 0 ? max(position - a.window + 1, 0) : 0;
+  k.low = kv_low_of(a, position);
   return k;
 }
 

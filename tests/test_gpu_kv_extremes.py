@@ -163,3 +163,23 @@ def test_a_broken_value_leaves_the_scores_alone(window, dim, length, new, at, dt
            window=window)
     far = oracle.allowed(bound, want, dtype)[1]
     assert (np.abs(lse.double().cpu().numpy() - want_lse) <= far).all()
+
+
+# ---------------------------------------------------------------- positions at the end of what a table holds
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("window,sees", [((1 << 30) - 1, 1023), (1 << 30, 1024), ((1 << 30) + 1, 1024), (1 << 31, 1024), (1 << 40, 1024)])
+def test_windows_as_long_as_a_table(window, sees, new):
+    """A request of 2^30 tokens, as many as a table may have, whose pages are missing but for the first: its last token sees that page's, but for
+    the one in front of a window of 2^30 - 1."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(35)
+    cache, _ = _filled(rng, [1024], 1, 64, 1024)
+    first = next(p for p in range(cache.pages) if not torch.isnan(cache.v_scales[p]).any())
+    cache.k_scales[first] = 0                   # all scores are equal: lse is the logarithm of the number of keys
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = first
+    q = _queries(rng, new, 2, 64, torch.bfloat16)
+    out, lse = kv_attend(q, cache, table, _i32([1 << 30]), starts=_i32([0, new]), window=window, return_lse=True)
+    _check((out[-1:], lse[-1:]), q[-1:], cache, _i32([[first]]), _i32([1024]), window=sees)
