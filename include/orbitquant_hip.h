@@ -503,6 +503,7 @@ int oq_kv_assign(const int32_t *lengths, const int32_t *new_lengths, int64_t req
 /*
  * Keys and values [tokens, kv_heads, D] of dtype into the cache at slots[token]; slots that are negative or beyond the
  * last page are skipped.  No slot twice in one call.  Strides in elements; the last dimension is contiguous.
+ * (This call, oq_kv_read and oq_kv_attend are OQ_ERR_UNSUPPORTED where a launch would have 2^32 threads: 2^28 vectors of a head.)
  */
 int oq_kv_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
                 int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens, const oq_kv_cache *cache,

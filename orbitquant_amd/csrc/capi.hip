@@ -607,10 +607,11 @@ bool vectors_wide(const void *p, int64_t token_stride, int64_t head_stride, int 
   return aligned(p, 16) && token_stride % per == 0 && head_stride % per == 0;
 }
 
-// A launch of a workgroup for every head of sixteen tokens.
-int kv_vectors_fit(const char *what, int64_t tokens, const oq_kv_cache *c) {
+// Write and read: a launch of `threads` for every head of sixteen tokens.
+int kv_vectors_fit(const char *what, int64_t tokens, const oq_kv_cache *c, int threads) {
   if (tokens < 0) return fail(OQ_ERR_INVALID, "%s: tokens=%lld", what, (long long)tokens);
-  if (tokens > (1LL << 40) || tokens * c->kv_heads > (1LL << 32)) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld exceed the grid", what, (long long)tokens);
+  if (tokens > (1LL << 40) || (tokens + oq::kKvGroup - 1) / oq::kKvGroup * c->kv_heads > oq::kKvMostThreads / threads)
+    return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld kv_heads=%lld exceed the grid", what, (long long)tokens, (long long)c->kv_heads);
   return OQ_OK;
 }
 
@@ -659,7 +660,7 @@ int oq_kv_write(const void *k, int64_t k_token_stride, int64_t k_head_stride, co
   oq::KvWriteArgs a{};
   if (const int status = kv_cache_of("kv_write", cache, a.cache)) return status;
   if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "kv_write: dtype=%d", dtype);
-  if (const int status = kv_vectors_fit("kv_write", tokens, cache)) return status;
+  if (const int status = kv_vectors_fit("kv_write", tokens, cache, oq::kv_write_threads(cache->head_dim))) return status;
   if (tokens == 0) return OQ_OK;
   if (k == nullptr || v == nullptr || slots == nullptr) return fail(OQ_ERR_INVALID, "kv_write: null pointer");
   a.k = k; a.v = v; a.slots = slots; a.tokens = tokens;
@@ -673,7 +674,7 @@ int oq_kv_read(const int64_t *slots, int64_t tokens, const oq_kv_cache *cache, v
   oq::KvReadArgs a{};
   if (const int status = kv_cache_of("kv_read", cache, a.cache)) return status;
   if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "kv_read: dtype=%d", dtype);
-  if (const int status = kv_vectors_fit("kv_read", tokens, cache)) return status;
+  if (const int status = kv_vectors_fit("kv_read", tokens, cache, oq::kv_read_threads(cache->head_dim))) return status;
   if (tokens == 0) return OQ_OK;
   if (k == nullptr || v == nullptr || slots == nullptr) return fail(OQ_ERR_INVALID, "kv_read: null pointer");
   if (!aligned(k, 16) || !aligned(v, 16)) return fail(OQ_ERR_INVALID, "kv_read: the outputs are not aligned to 16 bytes");
@@ -702,6 +703,7 @@ int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int6
   a.table = table; a.table_stride = table_stride; a.lengths = lengths; a.starts = starts; a.causal = causal != 0; a.scale = scale;
   a.out = out; a.lse = lse;
   const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, most_queries(tokens, starts != nullptr, max_new), workspace);
+  if (!oq::kv_attend_fits(a, dim)) return fail(OQ_ERR_UNSUPPORTED, "kv_attend: tokens=%lld heads=%lld requests=%lld exceed the grid", (long long)tokens, (long long)heads, (long long)requests);
   if (workspace == nullptr || workspace_bytes < needed) a.few.target = a.many.target = 0;
   return oq::kv_attend_dispatch(a, dim, as_stream(stream));
 }
@@ -716,7 +718,8 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
   a.cache.heads = static_cast<int>(kv_heads);
   if (kv_attend_shape(a, tokens, heads, table_width, requests, window) != OQ_OK || tokens == 0) return 0;
   a.starts = has_starts ? &some : nullptr;  // (asked whether it is there, not read)
-  return oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new), nullptr);
+  const uint64_t bytes = oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new), nullptr);
+  return oq::kv_attend_fits(a, static_cast<int>(head_dim)) ? bytes : 0;
 }
 
 }  // extern "C"

@@ -170,6 +170,13 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   return kv_places(a.many, a.many.target, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }
 
+bool kv_attend_fits(const KvAttendArgs &a, int dim) {
+  const int64_t heads = a.cache.heads;
+  const int64_t few = a.few_requests > 0 ? heads * (a.few.target + static_cast<int64_t>(a.few_requests) * a.few_tiles) : 0;
+  const int64_t many = a.many_tiles > 0 ? heads * (a.many.target != 0 ? a.many.target : a.many_tiles) : 0;
+  return few <= kKvMostThreads / (a.few_alone ? 64 : 256) && many <= kKvMostThreads / (64 * (dim == 256 ? kv_many_waves<256>() : kv_many_waves<64>()));
+}
+
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream) {
   const int split = a.q_dtype == OQ_F32 ? 2 : a.q_dtype == OQ_F16 ? 1 : 0;
   const bool fits = dim == 64 ? kv_attend_64(a, split, stream) : dim == 128 ? kv_attend_128(a, split, stream) : kv_attend_256(a, split, stream);

@@ -62,11 +62,18 @@ struct KvAttendArgs {
   float *lse;                         // NULL or [tokens, heads]
 };
 
+constexpr int64_t kKvMostThreads = 0xffffffffLL;  // of a launch
+// Write and read: a workgroup has one head of sixteen tokens.
+constexpr int kKvGroup = 16;
+constexpr int kv_write_threads(int64_t dim) { return dim == 64 ? 128 : 256; }
+constexpr int kv_read_threads(int64_t) { return 256; }
+
 int kv_assign_dispatch(const KvAssignArgs &a, hipStream_t stream);
 int kv_write_dispatch(const KvWriteArgs &a, int dim, int dtype, hipStream_t stream);
 int kv_read_dispatch(const KvReadArgs &a, int dim, int dtype, hipStream_t stream);
 // Cuts the work, whose parts go into `workspace`; the bytes that they need.
 uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t max_new, void *workspace);
+bool kv_attend_fits(const KvAttendArgs &a, int dim);  // a planned one's launches
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream);
 
 }  // namespace oq

@@ -120,8 +120,6 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 // bf16 (42 MB): write 16 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a store and lanes exchanged through LDS 52).
 // Bound by vector instructions, 23 and 25 a value, which issue in 78 and 91 % of the cycles: ten and eleven of them the seven stages of the
 // transform; the bytes alone take 9.
-constexpr int kKvGroup = 16;  // tokens of a workgroup
-
 template <int DT>
 __device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float *y) {
   if (wide) {
@@ -201,12 +199,10 @@ __device__ __forceinline__ bool in_a_row(const Token *tokens, int page_shift) {
 // Values of a lane: sixteen on the way in, where a vector's scale is found once for twice as many of them and one stage fewer lies between lanes
 // (write 18.1 -> 16.2 us), eight on the way out (sixteen 16.3 -> 16.8).
 constexpr int kKvWriteEach = 16;
-template <int LANES>  // of a vector
-constexpr int kv_group_threads() { return LANES == 4 ? 128 : 256; }
 
 template <int D, int DT>
-__global__ __launch_bounds__(kv_group_threads<D / kKvWriteEach>()) void kv_write_kernel(KvWriteArgs a) {
-  constexpr int E = kKvWriteEach, THREADS = kv_group_threads<D / E>();
+__global__ __launch_bounds__(kv_write_threads(D)) void kv_write_kernel(KvWriteArgs a) {
+  constexpr int E = kKvWriteEach, THREADS = kv_write_threads(D);
   constexpr int AT_ONCE = THREADS * E / D;         // vectors that the workgroup's lanes hold
   constexpr int PASSES = 2 * kKvGroup / AT_ONCE;   // keys, then values
   __shared__ KvPlace places[kKvGroup];
@@ -269,7 +265,7 @@ __global__ __launch_bounds__(kv_group_threads<D / kKvWriteEach>()) void kv_write
 }
 
 template <int D, int DT>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs a) {
+__global__ __launch_bounds__(kv_read_threads(D)) void kv_read_kernel(KvReadArgs a) {
   constexpr int AT_ONCE = 2048 / D, PASSES = 2 * kKvGroup / AT_ONCE;
   constexpr int ROWS = (D / 2) * (kKvGroup / 4);   // dwords of the values, turned by LDS
   __shared__ int64_t slots[kKvGroup];
@@ -344,11 +340,11 @@ int by_type(const Args &a, int dim, int dtype, hipStream_t stream) {
 inline dim3 group_grid(int64_t tokens, int heads) { return dim3(static_cast<unsigned>((tokens + kKvGroup - 1) / kKvGroup * heads)); }
 template <int D, int DT>
 struct RunWrite {
-  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_group_threads<D / kKvWriteEach>()), 0, s, a); }
+  static void go(const KvWriteArgs &a, hipStream_t s) { launch_kernel(kv_write_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_write_threads(D)), 0, s, a); }
 };
 template <int D, int DT>
 struct RunRead {
-  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(256), 0, s, a); }
+  static void go(const KvReadArgs &a, hipStream_t s) { launch_kernel(kv_read_kernel<D, DT>, group_grid(a.tokens, a.cache.heads), dim3(kv_read_threads(D)), 0, s, a); }
 };
 
 }  // namespace
