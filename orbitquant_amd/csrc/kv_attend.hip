@@ -163,7 +163,7 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
     a.few.sorted = groups > kFewGroups;
     a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
   }
-  a.few_alone = a.few_requests > 0 && steps <= kFewAlone && (steps <= 1 || whole > 128 * steps);
+  a.few_alone = a.few_requests > 0 && a.few.target == 0 && steps <= kFewAlone && (steps <= 1 || whole > 128 * steps);
   const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
   if (a.many_tiles > 0 && steps > kManyWhole && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
   const uint64_t bytes = kv_places(a.few, 2 * a.few.target, heads, 16, dim, static_cast<char *>(workspace), 0);

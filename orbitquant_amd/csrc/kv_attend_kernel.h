@@ -44,9 +44,6 @@ typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv_u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_bf16x8 __attribute__((ext_vector_type(8)));
 
-template <int SPLIT>
-constexpr int kv_dtype() { return SPLIT == 0 ? OQ_BF16 : SPLIT == 1 ? OQ_F16 : OQ_F32; }
-
 constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
 constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
 constexpr int kKvManyRows = 128;        // rows of a workgroup of the second
@@ -907,11 +904,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
   const int kv_head = blockIdx.x % a.cache.heads, group = blockIdx.x / a.cache.heads;
 
   KvPart part;
-  if (a.few.target == 0) {
+  if (WAVES == 1 || a.few.target == 0) {  // (one wavefront: of launches of few steps, which are not cut)
     part = {{}, group, 0, 1, 0};
     if (!kv_few_tile(a, group, part.rows)) return;
-  } else if (!kv_few_part<64 * WAVES>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) {
-    return;
+  } else if constexpr (WAVES > 1) {
+    if (!kv_few_part<64 * WAVES>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) return;
   }
   const KvRows r = part.rows;
   const KvSpan span = kv_span_of(a, r, r.first, r.rows);
