@@ -59,3 +59,28 @@ def test_one_row_each_where_the_caller_says_so():
     assert torch.equal(y, layer.out(attended[0].reshape(3, -1)))
     with pytest.raises(ValueError, match="one_each"):
         layer(_inputs(rng, 2), got, table, one_each=True)
+
+
+def test_decode_example_caches():
+    """After replayed steps every layer's cache holds what the same steps leave there when they are run eagerly, at the same pages."""
+    from orbitquant_amd import kv_read
+    from orbitquant_amd.examples import decode
+
+    prompts = [20, 70, 61]
+    eager, replayed = (decode.Decoder(2, 3, 80) for _ in range(2))
+    ids = torch.randint(0, decode.VOCABULARY, (sum(prompts),), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    for m in (eager, replayed):
+        m.step(ids, _i32(prompts), max_new=max(prompts))
+    graph = replayed.captured_step()
+    for steps in range(1, 6):
+        eager.step(eager.last.clone(), _i32([1, 1, 1]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager.last, replayed.last) and torch.equal(eager.taken, replayed.taken) and torch.equal(eager.block_table, replayed.block_table)
+        assert replayed.lengths.tolist() == [n + steps for n in prompts]
+        held = [int(eager.block_table[r, t // decode.PAGE]) * decode.PAGE + t % decode.PAGE for r, n in enumerate(prompts) for t in range(n + steps)]
+        assert min(held) >= 0 and len(set(held)) == len(held)
+        slots = torch.tensor(held, device="cuda")
+        for a, b in zip(eager.layers, replayed.layers):
+            for x, y in zip(kv_read(slots, a.attention.cache, torch.float32), kv_read(slots, b.attention.cache, torch.float32)):
+                assert torch.equal(x, y) and torch.isfinite(x).all() and x.abs().sum() > 0
