@@ -49,10 +49,10 @@ class OrbitCachedAttention(nn.Module):
         if one_each and tokens != assignment.lengths.numel():
             raise ValueError(f"one_each: {tokens} rows for {assignment.lengths.numel()} requests")
         q, k, v = OrbitLinearGroup(self.q, self.k, self.v)(x)
-        q, k, v = (t.view(tokens, -1, dim) for t in (q, k, v))
+        q, k, v = (t.view(tokens, t.shape[1] // dim, dim) for t in (q, k, v))
         if self.rotary is not None:
             q, k = self.rotary(q, k, assignment.positions)
         kv_write(k, v, assignment.slots, self.cache)
         attended = kv_attend(q, self.cache, block_table, assignment.lengths, starts=None if one_each else assignment.starts, max_new=max_new,
                              max_length=max_length, window=self.window)
-        return self.out(attended.reshape(tokens, -1))
+        return self.out(attended.flatten(1))

@@ -84,3 +84,21 @@ def test_decode_example_caches():
         for a, b in zip(eager.layers, replayed.layers):
             for x, y in zip(kv_read(slots, a.attention.cache, torch.float32), kv_read(slots, b.attention.cache, torch.float32)):
                 assert torch.equal(x, y) and torch.isfinite(x).all() and x.abs().sum() > 0
+
+
+@pytest.mark.parametrize("one_each", [False, True])
+def test_no_rows(one_each):
+    """A step without tokens: of requests that have none, or of no requests."""
+    from orbitquant_amd import kv_assign
+
+    rng, layer, table, free, before = _prompted()
+    if one_each:
+        none = torch.empty(0, dtype=torch.int32, device="cuda")
+        table, got = table[:0], kv_assign(none, none, table[:0], free, before.taken, page_size=16, tokens=0)
+    else:
+        got = kv_assign(before.lengths, _i32([0, 0, 0]), table, free, before.taken, page_size=16, tokens=0)
+    held = [t.clone() for t in layer.cache]
+    y = layer(_inputs(rng, 0), got, table, one_each=one_each)
+    assert y.shape == (0, 256) and y.dtype == torch.bfloat16
+    for was, now in zip(held, layer.cache):
+        assert torch.equal(was.view(torch.uint8), now.view(torch.uint8))
