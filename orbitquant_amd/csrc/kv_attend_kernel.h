@@ -658,6 +658,10 @@ __device__ __forceinline__ int kv_largest_scale(const float (&vs)[16]) {
   return static_cast<int>(top);
 }
 
+// Scales that are further apart than 2^8 are not of about one size.  (A first token's value is often some 2^4 smaller than the others; the weights
+// keep eleven digits down to 2^-16 of the largest where R is 2^8 too high.)
+constexpr int kKvMixed = 8;
+
 // (These two by instructions of their own: what they give is otherwise found in front of the branch that asks for it, whether it is taken or not.)
 __device__ __forceinline__ int kv_smallest_scale(const float (&vs)[16]) {
   int low = __float_as_int(vs[15]);
@@ -671,12 +675,12 @@ __device__ __forceinline__ float kv_exponent_alone(float scale) {
   return kv_exponent_of(bits < 0x7f800000 ? bits : 0);  // (a NaN has no part in where R goes)
 }
 
-// x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.  The exponent of `top`, the largest of the sixteen scales, belongs to keys
+// x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.  The exponent of the largest of the sixteen scales belongs to a key
 // that the row may not see or hardly weigh: it tells cheaply that no weight is near 2^15, and where the scales are of about one size, where R goes.
-// Where they are not, each key is taken with its own exponent, so that a large value raises R for the rows that it has weight in, and the
-// others keep their weights' digits.  (Always with its own: a prompt of 2048, D = 64, 46.2 -> 50 us; so 47.7.)
-template <int D>
-__device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&vs)[16], int top, float top_exponent, KvState &st, kv_f32x4 (&o)[D / 16]) {
+// Where they are not (mixed()), each key is taken with its own exponent, so that a large value raises R for the rows that it has weight in, and the
+// others keep their weights' digits.  (Always with its own: a prompt of 2048, D = 64, 46.0 -> 50 us; so 46.6.)
+template <int D, typename Mixed>
+__device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&vs)[16], float top_exponent, const Mixed &mixed, KvState &st, kv_f32x4 (&o)[D / 16]) {
   float best = kv_max3(x[0], x[1], x[2]), other = kv_max3(x[3], x[4], x[5]);
   best = kv_max3(best, x[6], x[7]);
   other = kv_max3(other, x[8], x[9]);
@@ -687,7 +691,7 @@ __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&v
   if (__builtin_amdgcn_ballot_w64(best > st.limit) != 0) {
     best = kv_over_groups(best, kv_max_of);
     bool raise = best > st.limit;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top - kv_smallest_scale(vs) >= 4 << 23) != 0, false)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(mixed()) != 0, false)) {
       best = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) best = fmaxf(best, x[i] + kv_exponent_alone(vs[i]));
@@ -992,7 +996,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
       }
     }
     const int top = kv_largest_scale(vs);
-    kv_keep_in_range<D>(x, vs, top, kv_exponent_of(top), st, o);
+    kv_keep_in_range<D>(x, vs, kv_exponent_of(top), [&] { return top - kv_smallest_scale(vs) >= kKvMixed << 23; }, st, o);
     kv_f16x8 p[2], p_rest[SPLIT > 1 ? 2 : 1];
     kv_weights<SPLIT>(x, vs, st.sum, p, p_rest);
 #pragma unroll
@@ -1274,12 +1278,17 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
         }
         broken.look(vs, step);
       }
-      const int top = kv_largest_scale(vs);
-      const float top_exponent = kv_exponent_of(top);
+      const float top_exponent = kv_exponent_of(kv_largest_scale(vs));
+      const auto mixed = [&] {  // (a lane for each key, against the first, which is the smaller one if one is)
+        int key = lane;
+        asm volatile("" : "+v"(key));
+        const int scale = __float_as_int(from.vs[key]);
+        return static_cast<uint32_t>(scale - kv_uniform(scale) + (2 << 23)) >= static_cast<uint32_t>(kKvMixed) << 23;
+      };
       kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        kv_keep_in_range<D>(x[t], vs, top, top_exponent, st[t], o[t]);
+        kv_keep_in_range<D>(x[t], vs, top_exponent, mixed, st[t], o[t]);
         kv_weights<SPLIT>(x[t], vs, st[t].sum, p[t], p_rest[t]);
       }
 #pragma unroll
