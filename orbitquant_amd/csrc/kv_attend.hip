@@ -18,7 +18,7 @@ namespace {
 // 2000, 13.2 -> 10.5; D = 256, 4 key heads, 17.7 -> 19.3.  Longer ones could leave one workgroup at work alone for too long, 0.22 us a step.
 // Cut, 512 workgroups or more, two on each compute unit at once: 131101 tokens, 8 heads, 34 us (before the other steps 1024: 39.7, 256: 35.0, 512: 34.6).
 // Up to three times as many where a part keeps 60 steps, so that requests of different lengths even out, the longest parts first: 64 of up to
-// 16384, 130 us (512 workgroups: 139; four times: 132).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 15.5 us.
+// 16384, 130 us (512 workgroups: 139; four times: 132).  Four steps a part at least, one a wavefront: 1500 of 5000 tokens, D = 256, 15.9 us.
 // Short and many: one wavefront a workgroup instead of four that share few steps, where there are enough of them to fill the chip (500 requests of up to 60
 // tokens, 8 heads, 31.5 -> 14.5 us, of up to 500 49 -> 43; 128 of up to 256 13.2 -> 10.1, but 64 of them 8.7 -> 9.4).
 constexpr int kFewAlone = 8;  // steps

@@ -892,7 +892,7 @@ __device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, i
 // Sixteen rows a workgroup; its four wavefronts take every fourth step of the part's keys and are joined through LDS (or one
 // wavefront takes them all, where requests are short and many).  A step's
 // keys, scales and values (8.4 KB at D = 128) are requested a step of the wavefront's ahead, into the registers of the ones just used.
-// Long ones are bound by memory: 131101 tokens, 8 heads of 128, 138 MB in 26.6 us; 64 requests, 668 MB in 122 to 126, 5.4 TB/s of the 6.3 that a
+// Long ones are bound by memory: 131101 tokens, 8 heads of 128, 138 MB in 26.9 us; 64 requests, 668 MB in 127 (least 122), 5.3 TB/s of the 6.3 that a
 // read of nothing else reaches (vector instructions issue in half of the cycles, the matrix units are busy in 15 %).  Short ones by
 // latency: 1003 tokens 8.9 us, three dependent loads (length, page, keys) and four steps a wavefront.  Eight wavefronts a workgroup: 9.3.
 template <int D, int SPLIT, bool WIDE, int WAVES>
@@ -1081,7 +1081,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
 // 128 rows a workgroup, 16 * RT a wavefront, all on the same keys.  Decoding a step costs as many vector instructions as the softmax
 // of 32 rows: each wavefront decodes a part of it into LDS, in the order of the operands (conflict-free on both sides), for the next step while
 // this one's products run; one barrier a step.
-// Bound by instruction issue: 8192 tokens, 32 heads of 128 in bf16, 566 us, 0.97 PFLOP/s (a large product of the library: 1.21); vector
+// Bound by instruction issue: 8192 tokens, 32 heads of 128 in bf16, 565 us, 0.97 PFLOP/s (a large product of the library: 1.21); vector
 // instructions, eight a score and lane, take 56 % of the cycles, the matrix instructions 41 %, and on one SIMD these two do not overlap.
 // Matrix instructions of 32 x 32 overlap in part but leave too few registers: 576 to 587 us.
 template <int D>

@@ -118,8 +118,10 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 // value is spread over the page, one byte in each of D / 2 rows: the bytes of the sixteen tokens change places in LDS, and four tokens
 // whose slots follow each other in a page (a prompt's, nearly always) are one dword of a row.  MI355X, 8192 tokens of 8 heads of 128 in
 // bf16 (42 MB): write 16 us, read 16 (with 64 tokens a workgroup 37 together, with one byte a store and lanes exchanged through LDS 52).
-// Bound by vector instructions, 23 and 25 a value, which issue in 78 and 91 % of the cycles: ten and eleven of them the seven stages of the
-// transform; the bytes alone take 9.
+// Bound by vector instructions, 23 and 25 a value, which issue in 78 and 92 % of the cycles: ten and eleven of them the seven stages of the
+// transform; the bytes alone take 9.  On the way in the order of the sums decides codes.  On the way out it does not: a scale times a code is a
+// multiple of half the scale's last bit, and so is every partial sum, which stays below 2^20 of it and is exact in fp32 in any order.
+
 template <int DT>
 __device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float *y) {
   if (wide) {
