@@ -44,7 +44,7 @@ typedef float kv_f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv_u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 kv_bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float kKvNothing = -1.0e30f;  // R of a row that has seen no key
+constexpr float kKvNothing = -3.402823466e38f;  // R of a row that has seen no key: below every score
 constexpr int kKvFewRows = 64;          // rows of a request that the first kernel takes
 constexpr int kKvManyRows = 128;        // rows of a workgroup of the second
 constexpr int kKvCutTiles = 384;        // tiles of a launch of the second that is cut, at most
@@ -698,7 +698,10 @@ __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&v
       best = kv_over_groups(best, kv_max_of);
       raise = raise && best > fminf(st.limit, 10.0f);  // (wherever it is above 10, so that the next steps need not look)
     }
-    const float up = raise ? best - 10.0f : 0.0f, half = kv_half_power(fminf(-up, 0.0f)), by = half * half;  // (down only where nothing is summed up yet)
+    // (Down only where nothing is summed up yet.  Scores beyond 2^26 are whole powers of two apart: what is meant may be rounded to an R too low.)
+    float up = best - 10.0f;
+    up = raise ? (best - up > 15.0f ? best : up) : 0.0f;
+    const float half = kv_half_power(fminf(-up, 0.0f)), by = half * half;
     st.ref += up;
     st.sum = st.sum * half * half;
     st.limit = raise ? 15.0f : st.limit;

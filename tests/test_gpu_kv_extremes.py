@@ -183,3 +183,34 @@ def test_windows_as_long_as_a_table(window, sees, new):
     q = _queries(rng, new, 2, 64, torch.bfloat16)
     out, lse = kv_attend(q, cache, table, _i32([1 << 30]), starts=_i32([0, new]), window=window, return_lse=True)
     _check((out[-1:], lse[-1:]), q[-1:], cache, _i32([[first]]), _i32([1024]), window=sees)
+
+
+# ---------------------------------------------------------------- scores of any size
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 100), (128, 1), (256, 20), (128, 100)])
+@pytest.mark.parametrize("length", [1, 100, 1500, 9000])
+@pytest.mark.parametrize("one_key", [False, True])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_outputs_are_means_however_large_the_scores_are(sign, one_key, length, dim, new, dtype):
+    """All values are one value, which is then every row's output, whatever its weights: for scores from 1 to what fp32 holds, above and below zero, of
+    keys that are one key or differ.  A weight is rounded once, and the sum of the weights is not."""
+    from orbitquant_amd import OrbitKVCache, kv_attend, kv_write
+
+    rng = np.random.RandomState(36)
+    pages = -(-length // 64) + 1
+    cache = OrbitKVCache.empty(pages, 1, dim, page_size=64, seed=3)
+    k = torch.from_numpy(rng.standard_normal((1 if one_key else 64 * pages, 1, dim)).astype(np.float32)).cuda()
+    v = torch.from_numpy(rng.standard_normal((1, 1, dim)).astype(np.float32)).cuda()
+    kv_write(k.expand(64 * pages, 1, dim), v.expand(64 * pages, 1, dim), torch.arange(64 * pages, device="cuda"), cache)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, -1)
+    heads = 16
+    q = k[:1].expand(new, heads, dim) * sign * 2.0 ** (torch.arange(new * heads, device="cuda").view(new, heads, 1) * (117 / (new * heads)))
+    q = (q * (1 + torch.rand(q.shape[:2], device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))[..., None])).to(dtype)
+    out, lse = kv_attend(q, cache, table, _i32([length]), starts=_i32([0, new]), causal=False, return_lse=True)
+    want, _, (_, largest, _, _) = oracle.attend(q[:1] * 0, cache, table, _i32([1]), starts=_i32([0, 1]), causal=False)
+    zeros = np.zeros((new, heads))
+    far, _ = oracle.allowed((zeros, zeros + largest[0, 0], zeros + length, dim), np.broadcast_to(want[:1], (new, heads, dim)), dtype)
+    off = np.linalg.norm(out.double().cpu().numpy() - want[0, 0], axis=-1)
+    assert (off <= far).all(), (off / far).max()
+    assert torch.isfinite(lse).all()
