@@ -538,6 +538,89 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
                                       int64_t page_size, int64_t table_width, int64_t requests, int has_starts,
                                       int64_t window, int64_t max_length, int64_t max_new);
 
+/*
+ * Norms of queries and keys for each head, and their rotary positions, in one pass (no counterpart in the reference).
+ *
+ * The D values of a head are D/2 pairs: 2p and 2p+1 (interleaved), or p and p + R/2 of the first R and p and p + (D-R)/2 of
+ * the rest (R = rotary_dim, 0 without tables; p and p + D/2 then).  In fp32, every product and sum rounded by itself:
+ *   s  = sum of squares: the two of a pair, then pairs 4, 2, 1 apart of each eight, then eights 1, 2, 4, ... apart
+ *   y  = (x * (1 / sqrt(s * fp32(1/D) + eps))) * w              where norm is set; w = 1 where there is no weight
+ *   (y0, y1) -> (y0 c - y1 s, y1 c + y0 s)                      of the first R/2 pairs; c, s: the position's row of the tables
+ * and rounded once to the output's type.  Squares are fp32: norms are right for values below 2^59.
+ * The struct is host memory, read during the call.
+ */
+typedef struct {
+  const float *cos, *sin;    /* [rows, rotary_dim / 2], contiguous; both NULL: nothing is turned                                   */
+  int64_t rows, rotary_dim;  /* even, 2 .. D                                                                                       */
+  const int32_t *positions;  /* [tokens]: rows of the tables; a token at a negative one is not turned, one behind them becomes NaN.  NULL: token t has row t */
+  const void *q_weight;      /* [D] of weight_dtype, or NULL                                                                       */
+  const void *k_weight;      /* the same                                                                                           */
+  int weight_dtype;
+  int norm;                  /* 0: no norm (and no weights)                                                                        */
+  float eps;                 /* >= 0                                                                                               */
+  int interleaved;
+} oq_qk_norm_rotary_plan;
+
+/*
+ * q [tokens, heads, D] and k [tokens, kv_heads, D] of dtype -> q_out and k_out, contiguous, 16-byte aligned.  D even, 2 .. 512.
+ * Strides in elements; the last dimension is contiguous.  No output may overlap an input.
+ */
+int oq_qk_norm_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t heads, const void *k,
+                      int64_t k_token_stride, int64_t k_head_stride, int64_t kv_heads, int dtype, int64_t tokens,
+                      int64_t head_dim, const oq_qk_norm_rotary_plan *plan, void *q_out, void *k_out, void *stream);
+
+/*
+ * The same for q, and keys and values into the cache at slots[token] as oq_kv_write puts them, the key normed and turned on the
+ * way: its codes are those of the fp32 result, which is not rounded in between.  One launch.
+ */
+int oq_kv_append(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t heads, const void *k,
+                 int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                 int64_t v_head_stride, int dtype, const int64_t *slots, int64_t tokens,
+                 const oq_qk_norm_rotary_plan *plan, const oq_kv_cache *cache, void *q_out, void *stream);
+
+/*
+ * ---- Trees of drafted tokens over the cache ----
+ * A request's new tokens are a tree instead of a chain: token i hangs on token parents[i] < i of the request's new ones, or on what the
+ * request has cached already (negative, or not less than i).
+ *
+ * parents    int32 [tokens]; starts int32 [requests + 1] and lengths int32 [requests] as oq_kv_assign gives them (starts, lengths_after)
+ * positions  int32 [tokens]: of token i, its depth (0 for one that hangs on the cached ones) behind the request's cached tokens
+ * masks      uint64 [tokens, mask_words], mask_words 1 .. 4: bit j % 64 of word j / 64 is set for token i itself and those it hangs on
+ * A request with more new tokens than 64 * mask_words is a prompt: positions one behind the other, masks of zeros (which
+ * oq_kv_attend_tree does not look at).  Tokens of no request have position -1 and zeros.
+ */
+int oq_kv_tree(const int32_t *parents, const int32_t *starts, const int32_t *lengths, int64_t requests, int64_t tokens,
+               int64_t mask_words, int32_t *positions, uint64_t *masks, void *stream);
+
+/*
+ * oq_kv_attend (causal) where a query sees of its request's new tokens those whose bit is set in its mask, whichever these are: any masks will
+ * do, its own token is seen only if its bit is set.  It sees all tokens before the new ones.  Of what it sees, the last `window`
+ * in the cache's order if window > 0.  A request with more new tokens than 64 * mask_words is causal.  masks 8-byte aligned.
+ */
+int oq_kv_attend_tree(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride,
+                      int64_t q_head_stride, const oq_kv_cache *cache, const int32_t *table, int64_t table_stride,
+                      int64_t table_width, const int32_t *lengths, const int32_t *starts, int64_t requests,
+                      const uint64_t *masks, int64_t mask_words, int64_t window, float scale, int64_t max_length,
+                      int64_t max_new, void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * After the step: of each request's new tokens those of an accepted path stay, as if they had been its only ones.
+ *
+ * kept       int32 [requests, most], most <= 256: of the request's new tokens, rising; the list ends at the first entry that does not rise, is
+ *            not one of them (-1, say) or has no slot.  The i-th kept token's entries go to the i-th new token's slot
+ * lengths, starts, slots   as oq_kv_assign gave them for the step (lengths_after, starts, slots [tokens])
+ * caches     host memory: the caches of cache_count layers, of one shape, all moved in one launch (for every 64 of them)
+ * table, free_pages, taken NULL, or as oq_kv_assign left them (taken: taken_after): pages behind the kept tokens go back onto the free
+ *            list, in front of those that it gives out next; the table is not changed, its columns behind the kept pages
+ *            stand for nothing.  Requests <= 8192
+ * lengths_after int32 [requests]: without the forgotten tokens; taken_after int32 [1]
+ * No slot twice in slots.  No output may overlap an input other than the caches and free_pages.
+ */
+int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const int32_t *starts, const int64_t *slots,
+               int64_t requests, int64_t tokens, const oq_kv_cache *caches, int64_t cache_count, const int32_t *table,
+               int64_t table_stride, int64_t table_width, int32_t *free_pages, int64_t free_count,
+               const int32_t *taken, int32_t *lengths_after, int32_t *taken_after, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ EXPORTS = (
     "oq_dequantize_packed_weight", "oq_packed_linear_workspace_bytes", "oq_matmul_packed_weight_workspace_bytes",
     "oq_packed_linear_int8", "oq_packed_linear_int8_workspace_bytes", "oq_packed_linear_least_workspace_bytes",
     "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes",
+    "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_keep",
 )
 
 _lib = None
@@ -41,6 +42,14 @@ class KvCacheStruct(ctypes.Structure):
 
     _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "k_scales", "v_codes", "v_scales", "signs")] + [
         (name, ctypes.c_int64) for name in ("pages", "kv_heads", "page_size", "head_dim")]
+
+
+class QkPlanStruct(ctypes.Structure):
+    """`oq_qk_norm_rotary_plan`."""
+
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("rows", ctypes.c_int64), ("rotary_dim", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int), ("norm", ctypes.c_int), ("eps", ctypes.c_float),
+                ("interleaved", ctypes.c_int)]
 
 
 def load() -> ctypes.CDLL:
@@ -127,6 +136,18 @@ def load() -> ctypes.CDLL:
                                  vp, vp, vp, c_u64, vp]
     lib.oq_kv_attend_workspace_bytes.restype = c_u64
     lib.oq_kv_attend_workspace_bytes.argtypes = [c_i64] * 7 + [c_int] + [c_i64] * 3
+    plan = ctypes.POINTER(QkPlanStruct)
+    lib.oq_qk_norm_rotary.restype = c_int
+    lib.oq_qk_norm_rotary.argtypes = [vp, c_i64, c_i64, c_i64, vp, c_i64, c_i64, c_i64, c_int, c_i64, c_i64, plan, vp, vp, vp]
+    lib.oq_kv_append.restype = c_int
+    lib.oq_kv_append.argtypes = [vp, c_i64, c_i64, c_i64, vp, c_i64, c_i64, vp, c_i64, c_i64, c_int, vp, c_i64, plan, cache, vp, vp]
+    lib.oq_kv_tree.restype = c_int
+    lib.oq_kv_tree.argtypes = [vp, vp, vp, c_i64, c_i64, c_i64, vp, vp, vp]
+    lib.oq_kv_attend_tree.restype = c_int
+    lib.oq_kv_attend_tree.argtypes = [vp, c_int, c_i64, c_i64, c_i64, c_i64, cache, vp, c_i64, c_i64, vp, vp, c_i64, vp, c_i64, c_i64, c_f, c_i64, c_i64,
+                                      vp, vp, vp, c_u64, vp]
+    lib.oq_kv_keep.restype = c_int
+    lib.oq_kv_keep.argtypes = [vp, c_i64, vp, vp, vp, c_i64, c_i64, cache, c_i64, vp, c_i64, c_i64, vp, c_i64, vp, vp, vp, vp]
     _lib = lib
     if hasattr(_torch_ops, "bind"):
         _bind(lib)
@@ -135,7 +156,8 @@ def load() -> ctypes.CDLL:
 
 def _bind(lib: ctypes.CDLL) -> None:
     names = ("oq_quantized_linear", "oq_quantized_linear_group", "oq_packed_linear_workspace_bytes", "oq_rotate_plan_bytes",
-             "oq_matmul_packed_adaln_int4", "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes")
+             "oq_matmul_packed_adaln_int4", "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes",
+             "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_keep")
     _torch_ops.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names})
 
 

@@ -5,7 +5,7 @@
 
 hipcc cross-compiles for gfx950 without a GPU.  The rotate+quantize kernel and
 what writes and reads the key/value cache are
-built without FMA contraction (their results must match the CPU statement of the
+built without FMA contraction, and so are norms and rotary positions (their results must match the CPU statement of the
 algorithm bit for bit), and so is the attention over it (contracted into the conversion, a product and its
 rounding to fp16 are not what the remainder in a second fp16 is taken from); packed fp32 VALU instructions are disabled everywhere.
 
@@ -61,10 +61,16 @@ SOURCES = {
     "token_linear_w3.hip": [],
     "token_linear_w4.hip": [],
     "kv_cache.hip": ["-ffp-contract=off"],
+    "kv_append.hip": ["-ffp-contract=off"],
+    "kv_tree.hip": [],
+    "qk_rotary.hip": ["-ffp-contract=off"],
     "kv_attend.hip": [],
     "kv_attend_d64.hip": ["-ffp-contract=off"],
     "kv_attend_d128.hip": ["-ffp-contract=off"],
     "kv_attend_d256.hip": ["-ffp-contract=off"],
+    "kv_attend_tree_d64.hip": ["-ffp-contract=off"],
+    "kv_attend_tree_d128.hip": ["-ffp-contract=off"],
+    "kv_attend_tree_d256.hip": ["-ffp-contract=off"],
 }
 
 

@@ -11,6 +11,8 @@
 #include "dense_gemm.h"
 #include "gemm_epilogue.h"
 #include "kv_cache.h"
+#include "kv_tree.h"
+#include "qk_rotary_calls.h"
 #include "rotate_plan.h"
 
 namespace oq {
@@ -682,10 +684,11 @@ int oq_kv_read(const int64_t *slots, int64_t tokens, const oq_kv_cache *cache, v
   return oq::kv_read_dispatch(a, static_cast<int>(cache->head_dim), dtype, as_stream(stream));
 }
 
-int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
-                 const oq_kv_cache *cache, const int32_t *table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
-                 const int32_t *starts, int64_t requests, int causal, int64_t window, float scale, int64_t max_length, int64_t max_new,
-                 void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream) {
+namespace {
+int attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride, int64_t q_head_stride, const oq_kv_cache *cache,
+           const int32_t *table, int64_t table_stride, int64_t table_width, const int32_t *lengths, const int32_t *starts, int64_t requests, int causal,
+           const uint64_t *masks, int mask_words, int64_t window, float scale, int64_t max_length, int64_t max_new, void *out, float *lse,
+           void *workspace, uint64_t workspace_bytes, void *stream) {
   oq::KvAttendArgs a{};
   if (const int status = kv_cache_of("kv_attend", cache, a.cache)) return status;
   if (!known_dtype(q_dtype)) return fail(OQ_ERR_INVALID, "kv_attend: q_dtype=%d", q_dtype);
@@ -701,11 +704,32 @@ int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int6
   a.q = q; a.q_dtype = q_dtype; a.q_token_stride = q_token_stride; a.q_head_stride = q_head_stride;
   a.q_wide = vectors_wide(q, q_token_stride, q_head_stride, q_dtype);
   a.table = table; a.table_stride = table_stride; a.lengths = lengths; a.starts = starts; a.causal = causal != 0; a.scale = scale;
+  a.masks = masks; a.mask_words = mask_words;
   a.out = out; a.lse = lse;
   const uint64_t needed = oq::kv_attend_plan(a, dim, max_length, most_queries(tokens, starts != nullptr, max_new), workspace);
   if (!oq::kv_attend_fits(a, dim)) return fail(OQ_ERR_UNSUPPORTED, "kv_attend: tokens=%lld heads=%lld requests=%lld exceed the grid", (long long)tokens, (long long)heads, (long long)requests);
   if (workspace == nullptr || workspace_bytes < needed) a.few.target = a.many.target = 0;
   return oq::kv_attend_dispatch(a, dim, as_stream(stream));
+}
+}  // namespace
+
+int oq_kv_attend(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
+                 const oq_kv_cache *cache, const int32_t *table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                 const int32_t *starts, int64_t requests, int causal, int64_t window, float scale, int64_t max_length, int64_t max_new,
+                 void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream) {
+  return attend(q, q_dtype, tokens, heads, q_token_stride, q_head_stride, cache, table, table_stride, table_width, lengths, starts, requests, causal, nullptr, 0,
+                window, scale, max_length, max_new, out, lse, workspace, workspace_bytes, stream);
+}
+
+int oq_kv_attend_tree(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride, int64_t q_head_stride,
+                      const oq_kv_cache *cache, const int32_t *table, int64_t table_stride, int64_t table_width, const int32_t *lengths,
+                      const int32_t *starts, int64_t requests, const uint64_t *masks, int64_t mask_words, int64_t window, float scale,
+                      int64_t max_length, int64_t max_new, void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream) {
+  if (mask_words < 1) return fail(OQ_ERR_INVALID, "kv_attend_tree: mask_words=%lld", (long long)mask_words);
+  if (mask_words > oq::kKvMaskWords) return fail(OQ_ERR_UNSUPPORTED, "kv_attend_tree: mask_words=%lld (at most %d)", (long long)mask_words, oq::kKvMaskWords);
+  if (tokens > 0 && (masks == nullptr || !aligned(masks, 8))) return fail(OQ_ERR_INVALID, "kv_attend_tree: no masks, or not aligned to 8 bytes");
+  return attend(q, q_dtype, tokens, heads, q_token_stride, q_head_stride, cache, table, table_stride, table_width, lengths, starts, requests, 1, masks,
+                static_cast<int>(mask_words), window, scale, max_length, max_new, out, lse, workspace, workspace_bytes, stream);
 }
 
 uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
@@ -720,6 +744,137 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
   a.starts = has_starts ? &some : nullptr;  // (asked whether it is there, not read)
   const uint64_t bytes = oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new), nullptr);
   return oq::kv_attend_fits(a, static_cast<int>(head_dim)) ? bytes : 0;
+}
+
+// ---- norms and rotary positions ----
+
+namespace {
+// How the pairs of heads of `dim` are normed and turned; an error status where the plan is none.
+int qk_plan_of(const char *what, const oq_qk_norm_rotary_plan *p, int64_t dim, oq::QkNormRotary &how) {
+  if (p == nullptr) return fail(OQ_ERR_INVALID, "%s: no plan", what);
+  if ((p->cos == nullptr) != (p->sin == nullptr)) return fail(OQ_ERR_INVALID, "%s: cosines and sines go together", what);
+  const int64_t rotary = p->cos != nullptr ? p->rotary_dim : 0;
+  if (p->cos != nullptr && (rotary < 2 || rotary % 2 != 0 || rotary > dim || p->rows < 0))
+    return fail(OQ_ERR_INVALID, "%s: rotary_dim=%lld (even, 2 to %lld) rows=%lld", what, (long long)p->rotary_dim, (long long)dim, (long long)p->rows);
+  if (p->rows > 0x7fffffffLL) return fail(OQ_ERR_UNSUPPORTED, "%s: rows=%lld", what, (long long)p->rows);
+  if (!aligned(p->cos, 4) || !aligned(p->sin, 4)) return fail(OQ_ERR_INVALID, "%s: the tables are not aligned to their entries", what);
+  if (p->norm == 0 && (p->q_weight != nullptr || p->k_weight != nullptr)) return fail(OQ_ERR_INVALID, "%s: weights without a norm", what);
+  if ((p->q_weight != nullptr || p->k_weight != nullptr) && !known_dtype(p->weight_dtype)) return fail(OQ_ERR_INVALID, "%s: weight_dtype=%d", what, p->weight_dtype);
+  if (p->norm != 0 && !(p->eps >= 0.0f && p->eps <= 3.402823466e38f)) return fail(OQ_ERR_INVALID, "%s: eps=%g", what, p->eps);
+  how.cos = p->cos; how.sin = p->sin; how.positions = p->positions; how.rows = p->rows;
+  how.half = static_cast<int>(rotary / 2);
+  how.table_wide = how.half % 8 == 0 && aligned(p->cos, 16) && aligned(p->sin, 16);
+  how.weight[0] = p->q_weight; how.weight[1] = p->k_weight; how.weight_dtype = p->weight_dtype;
+  how.norm = p->norm != 0; how.interleaved = p->interleaved != 0; how.eps = p->eps; how.by_dim = static_cast<float>(1.0 / static_cast<double>(dim));
+  how.weight_wide = dim % 16 == 0 && (how.interleaved || how.half % 8 == 0) && aligned(p->q_weight, 16) && aligned(p->k_weight, 16);
+  return OQ_OK;
+}
+
+// One side's tensors, and the workgroups of `threads` that they take.
+int qk_side_of(const char *what, const void *x, int64_t token_stride, int64_t head_stride, int64_t heads, int dtype, int64_t tokens, int64_t dim,
+               const oq::QkNormRotary &how, void *out, int threads, oq::QkSide &side, uint32_t &blocks) {
+  if (tokens < 0 || heads < 1 || heads > 65535) return fail(OQ_ERR_INVALID, "%s: tokens=%lld heads=%lld", what, (long long)tokens, (long long)heads);
+  if (tokens > 0x3fffffffLL || tokens * heads > 0x3fffffffLL) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld heads=%lld exceed the grid", what, (long long)tokens, (long long)heads);
+  if (tokens > 0 && (x == nullptr || out == nullptr)) return fail(OQ_ERR_INVALID, "%s: null pointer", what);
+  if (!aligned(out, 16)) return fail(OQ_ERR_INVALID, "%s: the outputs are not aligned to 16 bytes", what);
+  side.x = x; side.out = out; side.token_stride = token_stride; side.head_stride = head_stride;
+  side.heads = static_cast<int>(heads); side.groups = (side.heads + oq::kQkHeads - 1) / oq::kQkHeads;
+  side.magic = static_cast<uint32_t>(((1ull << 32) + side.groups - 1) / side.groups);
+  side.wide = dim % 16 == 0 && (how.interleaved || how.half % 8 == 0) && vectors_wide(x, token_stride, head_stride, dtype);
+  const int64_t count = oq::qk_blocks(tokens, side.heads, static_cast<int>(dim), threads);
+  if (count > oq::kKvMostThreads / threads / 2) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld heads=%lld exceed the grid", what, (long long)tokens, (long long)heads);
+  blocks = static_cast<uint32_t>(count);
+  return OQ_OK;
+}
+}  // namespace
+
+int oq_qk_norm_rotary(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t heads, const void *k, int64_t k_token_stride,
+                      int64_t k_head_stride, int64_t kv_heads, int dtype, int64_t tokens, int64_t head_dim, const oq_qk_norm_rotary_plan *plan,
+                      void *q_out, void *k_out, void *stream) {
+  oq::QkArgs a{};
+  if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "qk_norm_rotary: dtype=%d", dtype);
+  if (head_dim < 2 || head_dim % 2 != 0) return fail(OQ_ERR_INVALID, "qk_norm_rotary: head_dim=%lld (even)", (long long)head_dim);
+  if (head_dim > oq::kQkMostDim) return fail(OQ_ERR_UNSUPPORTED, "qk_norm_rotary: head_dim=%lld (at most %d)", (long long)head_dim, oq::kQkMostDim);
+  if (const int status = qk_plan_of("qk_norm_rotary", plan, head_dim, a.how)) return status;
+  if (const int status = qk_side_of("qk_norm_rotary", q, q_token_stride, q_head_stride, heads, dtype, tokens, head_dim, a.how, q_out, oq::kQkThreads, a.side[0], a.q_blocks)) return status;
+  if (const int status = qk_side_of("qk_norm_rotary", k, k_token_stride, k_head_stride, kv_heads, dtype, tokens, head_dim, a.how, k_out, oq::kQkThreads, a.side[1], a.k_blocks)) return status;
+  if (tokens == 0) return OQ_OK;
+  a.tokens = tokens;
+  a.dim = static_cast<int>(head_dim);
+  return oq::qk_norm_rotary_dispatch(a, dtype, as_stream(stream));
+}
+
+int oq_kv_append(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t heads, const void *k, int64_t k_token_stride,
+                 int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t *slots,
+                 int64_t tokens, const oq_qk_norm_rotary_plan *plan, const oq_kv_cache *cache, void *q_out, void *stream) {
+  oq::KvAppendArgs a{};
+  if (const int status = kv_cache_of("kv_append", cache, a.write.cache)) return status;
+  if (!known_dtype(dtype)) return fail(OQ_ERR_INVALID, "kv_append: dtype=%d", dtype);
+  const int threads = oq::kv_write_threads(cache->head_dim);
+  if (const int status = kv_vectors_fit("kv_append", tokens, cache, 2 * threads)) return status;
+  if (const int status = qk_plan_of("kv_append", plan, cache->head_dim, a.how)) return status;
+  if (const int status = qk_side_of("kv_append", q, q_token_stride, q_head_stride, heads, dtype, tokens, cache->head_dim, a.how, q_out, threads, a.q, a.q_blocks)) return status;
+  if (tokens == 0) return OQ_OK;
+  if (k == nullptr || v == nullptr || slots == nullptr) return fail(OQ_ERR_INVALID, "kv_append: null pointer");
+  oq::KvWriteArgs &w = a.write;
+  w.k = k; w.v = v; w.slots = slots; w.tokens = tokens;
+  w.k_token_stride = k_token_stride; w.k_head_stride = k_head_stride; w.v_token_stride = v_token_stride; w.v_head_stride = v_head_stride;
+  w.k_wide = (a.how.interleaved || a.how.half % 8 == 0) && vectors_wide(k, k_token_stride, k_head_stride, dtype);
+  w.v_wide = vectors_wide(v, v_token_stride, v_head_stride, dtype);
+  a.kv_blocks = static_cast<uint32_t>((tokens + oq::kKvGroup - 1) / oq::kKvGroup * cache->kv_heads);
+  return oq::kv_append_dispatch(a, static_cast<int>(cache->head_dim), dtype, as_stream(stream));
+}
+
+// ---- trees of drafted tokens ----
+
+int oq_kv_tree(const int32_t *parents, const int32_t *starts, const int32_t *lengths, int64_t requests, int64_t tokens, int64_t mask_words,
+               int32_t *positions, uint64_t *masks, void *stream) {
+  if (requests < 0 || tokens < 0 || mask_words < 1)
+    return fail(OQ_ERR_INVALID, "kv_tree: requests=%lld tokens=%lld mask_words=%lld", (long long)requests, (long long)tokens, (long long)mask_words);
+  if (mask_words > oq::kKvMaskWords || requests > 0xffffff || tokens > 0x3fffffffLL)
+    return fail(OQ_ERR_UNSUPPORTED, "kv_tree: requests=%lld tokens=%lld mask_words=%lld (at most %d)", (long long)requests, (long long)tokens, (long long)mask_words, oq::kKvMaskWords);
+  if (tokens == 0) return OQ_OK;
+  if (parents == nullptr || starts == nullptr || (requests > 0 && lengths == nullptr) || positions == nullptr || masks == nullptr)
+    return fail(OQ_ERR_INVALID, "kv_tree: null pointer");
+  if (!aligned(masks, 8)) return fail(OQ_ERR_INVALID, "kv_tree: the masks are not aligned to 8 bytes");
+  return oq::kv_tree_dispatch({parents, starts, lengths, static_cast<int>(requests), static_cast<int>(mask_words), tokens, positions, masks}, as_stream(stream));
+}
+
+int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const int32_t *starts, const int64_t *slots, int64_t requests, int64_t tokens,
+               const oq_kv_cache *caches, int64_t cache_count, const int32_t *table, int64_t table_stride, int64_t table_width, int32_t *free_pages,
+               int64_t free_count, const int32_t *taken, int32_t *lengths_after, int32_t *taken_after, void *stream) {
+  if (most < 0 || requests < 0 || tokens < 0 || cache_count < 1 || table_width < 0 || free_count < 0 || (table != nullptr && requests > 1 && table_stride < table_width))
+    return fail(OQ_ERR_INVALID, "kv_keep: most=%lld requests=%lld tokens=%lld caches=%lld table_width=%lld table_stride=%lld free_count=%lld", (long long)most,
+                (long long)requests, (long long)tokens, (long long)cache_count, (long long)table_width, (long long)table_stride, (long long)free_count);
+  if (caches == nullptr) return fail(OQ_ERR_INVALID, "kv_keep: no cache");
+  oq::KvCache first{}, other{};
+  if (const int status = kv_cache_of("kv_keep", caches, first)) return status;
+  for (int64_t i = 1; i < cache_count; ++i) {
+    if (const int status = kv_cache_of("kv_keep", caches + i, other)) return status;
+    if (other.pages != first.pages || other.heads != first.heads || other.page_shift != first.page_shift || caches[i].head_dim != caches[0].head_dim)
+      return fail(OQ_ERR_INVALID, "kv_keep: cache %lld is of another shape than the first", (long long)i);
+  }
+  if (most > oq::kKvMostKept || requests > oq::kKvMaxRequests || tokens > 0x3fffffffLL || table_width > 0x7fffffffLL || free_count > 0x7fffffffLL)
+    return fail(OQ_ERR_UNSUPPORTED, "kv_keep: most=%lld (at most %d) requests=%lld (at most %d) tokens=%lld", (long long)most, oq::kKvMostKept, (long long)requests,
+                oq::kKvMaxRequests, (long long)tokens);
+  if ((table == nullptr) != (taken == nullptr) || (taken == nullptr) != (taken_after == nullptr) || (free_count > 0 && free_pages == nullptr))
+    return fail(OQ_ERR_INVALID, "kv_keep: block table, free pages and their count go together");
+  if (requests == 0 && table == nullptr) return OQ_OK;
+  if ((requests > 0 && (lengths == nullptr || starts == nullptr || lengths_after == nullptr || (most > 0 && kept == nullptr))) || (tokens > 0 && slots == nullptr))
+    return fail(OQ_ERR_INVALID, "kv_keep: null pointer");
+  oq::KvKeepArgs a{};
+  a.kept = kept; a.lengths = lengths; a.starts = starts; a.slots = slots; a.tokens = tokens; a.pages = first.pages; a.table_stride = table_stride;
+  a.requests = static_cast<int>(requests); a.most = static_cast<int>(most); a.heads = first.heads; a.page_shift = first.page_shift;
+  a.table_width = static_cast<int>(table_width); a.free_count = static_cast<int>(free_count);
+  a.table = table; a.taken = taken; a.free_pages = free_pages; a.lengths_after = lengths_after; a.taken_after = taken_after;
+  for (int64_t at = 0; at < cache_count; at += oq::kKvKeepCaches) {
+    a.counts = at == 0;
+    a.caches = static_cast<int>(cache_count - at < oq::kKvKeepCaches ? cache_count - at : oq::kKvKeepCaches);
+    for (int i = 0; i < a.caches; ++i) a.cache[i] = {caches[at + i].k_codes, caches[at + i].v_codes, caches[at + i].k_scales, caches[at + i].v_scales};
+    if (oq::kv_keep_blocks(a) > oq::kKvMostThreads / 256) return fail(OQ_ERR_UNSUPPORTED, "kv_keep: requests=%lld kv_heads=%d exceed the grid", (long long)requests, a.heads);
+    if (const int status = oq::kv_keep_dispatch(a, static_cast<int>(caches->head_dim), as_stream(stream))) return status;
+  }
+  return OQ_OK;
 }
 
 }  // extern "C"

@@ -8,6 +8,9 @@ namespace oq {
 bool kv_attend_64(const KvAttendArgs &a, int split, hipStream_t stream);
 bool kv_attend_128(const KvAttendArgs &a, int split, hipStream_t stream);
 bool kv_attend_256(const KvAttendArgs &a, int split, hipStream_t stream);
+bool kv_attend_tree_64(const KvAttendArgs &a, int split, hipStream_t stream);
+bool kv_attend_tree_128(const KvAttendArgs &a, int split, hipStream_t stream);
+bool kv_attend_tree_256(const KvAttendArgs &a, int split, hipStream_t stream);
 
 namespace {
 
@@ -179,7 +182,9 @@ bool kv_attend_fits(const KvAttendArgs &a, int dim) {
 
 int kv_attend_dispatch(const KvAttendArgs &a, int dim, hipStream_t stream) {
   const int split = a.q_dtype == OQ_F32 ? 2 : a.q_dtype == OQ_F16 ? 1 : 0;
-  const bool fits = dim == 64 ? kv_attend_64(a, split, stream) : dim == 128 ? kv_attend_128(a, split, stream) : kv_attend_256(a, split, stream);
+  const bool tree = a.masks != nullptr;
+  const bool fits = tree ? (dim == 64 ? kv_attend_tree_64(a, split, stream) : dim == 128 ? kv_attend_tree_128(a, split, stream) : kv_attend_tree_256(a, split, stream))
+                    : dim == 64 ? kv_attend_64(a, split, stream) : dim == 128 ? kv_attend_128(a, split, stream) : kv_attend_256(a, split, stream);
   if (!fits) return fail(OQ_ERR_LAUNCH, "kv_attend: no LDS for heads of %d", dim);
   const int status = check_launch("kv_attend");
   if (status != OQ_OK || (a.few.target == 0 && a.many.target == 0)) return status;

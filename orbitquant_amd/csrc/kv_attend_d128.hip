@@ -3,6 +3,6 @@
 
 namespace oq {
 
-bool kv_attend_128(const KvAttendArgs &a, int split, hipStream_t stream) { return kv_attend_of<128>(a, split, stream); }
+bool kv_attend_128(const KvAttendArgs &a, int split, hipStream_t stream) { return kv_attend_of<128, false>(a, split, stream); }
 
 }  // namespace oq

@@ -3,6 +3,6 @@
 
 namespace oq {
 
-bool kv_attend_64(const KvAttendArgs &a, int split, hipStream_t stream) { return kv_attend_of<64>(a, split, stream); }
+bool kv_attend_64(const KvAttendArgs &a, int split, hipStream_t stream) { return kv_attend_of<64, false>(a, split, stream); }
 
 }  // namespace oq

@@ -32,11 +32,17 @@
 // one decodes for itself, and the launch is bound by the cache's bytes.  Many rows (a prompt): the wavefronts have rows of
 // their own and the same keys, which they decode once for all of them into LDS; bound by the vector instructions around the
 // products.
+//
+// Drafted tokens (TREE).  A request's new tokens may be a tree instead of a chain: query i then sees what the request held before, and of the new
+// tokens those whose bit is set in its mask.  Keys before the new tokens are everybody's, so the masks are looked at in the last steps
+// alone: sixteen bits for a lane's sixteen keys, cut out of two words that the wavefront has put into LDS before its first step, between words of
+// ones (what was there before) and zeros (behind the last bit).  Kernels of their own: the others stay as they are.
 #pragma once
 
 #include <type_traits>
 
 #include "kv_cache.h"
+#include "kv_tree.h"
 
 namespace oq {
 
@@ -128,7 +134,20 @@ __device__ __forceinline__ int kv_low_of(const KvAttendArgs &a, int position) { 
 struct KvSpan {
   int lowest, highest, all_low, all_high;
 };
+__device__ __forceinline__ bool kv_drafted(const KvAttendArgs &a, const KvRows &r) { return r.fresh <= 64 * a.mask_words; }  // more new tokens than bits are a prompt's
+template <bool TREE = false>
 __device__ __forceinline__ KvSpan kv_span_of(const KvAttendArgs &a, const KvRows &r, int first, int rows) {
+  if constexpr (TREE) {
+    if (kv_drafted(a, r)) {  // whatever the masks are: of a window at least `window` less the new tokens lie before these
+      const int before = r.position(0);
+      KvSpan s;
+      s.highest = r.last_key;
+      s.all_high = min(before - 1, r.last_key);
+      s.lowest = a.window != 0 && before > a.window ? before - a.window : 0;
+      s.all_low = a.window != 0 && before > a.window - min(r.fresh, a.window) ? before - a.window + min(r.fresh, a.window) : 0;
+      return s;
+    }
+  }
   const int from = r.position(first / a.group), to = r.position((first + rows - 1) / a.group);
   KvSpan s;
   s.highest = a.causal ? min(to, r.last_key) : r.last_key;
@@ -326,11 +345,11 @@ __device__ __forceinline__ KvRows kv_uniform(const KvRows &r) {
 __device__ __forceinline__ int2 *kv_map_of(const KvCut &cut, int kv_head) { return cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1); }
 __device__ __forceinline__ int2 kv_map_entry(const KvPart &part) { return part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0); }
 
-template <int THREADS>
+template <int THREADS, bool TREE>
 __device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   KvRows r = {};
-  const auto steps_of = [&](int i) { return kv_few_tile(a, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0; };
+  const auto steps_of = [&](int i) { return kv_few_tile(a, i, r) ? kv_counted_steps(kv_span_of<TREE>(a, r, r.first, r.rows)) : 0; };
   int2 *const map = kv_map_of(cut, kv_head);
   if (tiles <= 64 && !cut.sorted) {  // a tile a lane, and the order is theirs: a short launch notices every instruction
     const int steps = lane < tiles ? steps_of(lane) : 0;
@@ -444,7 +463,7 @@ struct KvCounted {
   int starts[kKvCutTiles + 2], lengths[kKvCutTiles + 2];  // of the requests
   int steps[kKvCutTiles], requests[kKvCutTiles];          // of the tiles
 };
-template <int THREADS>
+template <int THREADS, bool TREE>
 __device__ __forceinline__ bool kv_many_part(const KvAttendArgs &a, int kv_head, int group, KvCounted &counted, KvPart &part) {
   constexpr int HELD = kKvCutTiles / 64;
   const int tid = threadIdx.x, lane = tid & 63, tiles = a.many_tiles;
@@ -463,7 +482,7 @@ __device__ __forceinline__ bool kv_many_part(const KvAttendArgs &a, int kv_head,
   KvRows r;
   for (int i = tid; i < tiles; i += THREADS) {
     const int request = kv_request_of(a, i, [&](int request) { return counted.starts[request]; });
-    counted.steps[i] = rows_of(request, i, r) ? kv_counted_steps(kv_span_of(a, r, r.first, r.rows)) : 0;
+    counted.steps[i] = rows_of(request, i, r) ? kv_counted_steps(kv_span_of<TREE>(a, r, r.first, r.rows)) : 0;
     counted.requests[i] = request;
   }
   __syncthreads();
@@ -514,6 +533,49 @@ __device__ __forceinline__ KvRow kv_row_of(const KvAttendArgs &a, const KvRows &
   k.high = there ? (a.causal ? min(position, r.last_key) : r.last_key) : -1;
   k.low = kv_low_of(a, position);
   return k;
+}
+
+// The masks of a wavefront's rows in LDS: of each a word of ones, its kKvMaskWords, a word of zeros.
+struct KvMasks {
+  uint64_t row[16][kKvMaskWords + 2];
+};
+// Sixteen rows' (lane (n, g): word g of row n; requested before the keys, as queries are), and what of the keys before the new ones a window leaves: with fewer bits than it holds, the last of
+// those; with more, none, and of the bits the last.
+__device__ __forceinline__ uint64_t kv_request_mask(const KvAttendArgs &a, const KvRow &row, int g) {
+  static_assert(kKvMaskWords == 4, "a word for each of a row's lanes");
+  return row.token >= 0 && g < a.mask_words ? a.masks[static_cast<int64_t>(row.token) * a.mask_words + g] : 0;
+}
+__device__ __forceinline__ void kv_place_masks(const KvAttendArgs &a, const KvRows &r, KvRow &row, uint64_t mask, KvMasks &to) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  if (!kv_drafted(a, r)) return;  // (the same for all)
+  const int bits = r.fresh - 64 * g;
+  mask &= bits >= 64 ? ~0ull : bits > 0 ? (1ull << bits) - 1 : 0;
+  const int before = r.position(0);
+  if (row.token >= 0) {
+    row.high = r.last_key;
+    row.low = 0;
+  }
+  if (a.window != 0) {
+    const int own = __popcll(mask);
+    const int words[4] = {__shfl(own, n, 64), __shfl(own, 16 + n, 64), __shfl(own, 32 + n, 64), __shfl(own, 48 + n, 64)};
+    const int all = words[0] + words[1] + words[2] + words[3];
+    const int ahead = (g > 0 ? words[0] : 0) + (g > 1 ? words[1] : 0) + (g > 2 ? words[2] : 0);
+    const int over = max(all - a.window, 0);
+    for (int drop = min(max(over - ahead, 0), own); drop > 0; --drop) mask &= mask - 1;
+    const int left = a.window - (all - over);
+    if (row.token >= 0) row.low = before > left ? before - left : 0;
+  }
+  to.row[n][1 + g] = mask;
+  if (g == 0) to.row[n][0] = ~0ull;
+  if (g == 1) to.row[n][kKvMaskWords + 1] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (read by the same wavefront alone)
+}
+// Of the sixteen keys from `key` on those that row n sees, `begin` being the request's first new token (0x7fffffff where there are no masks).
+__device__ __forceinline__ uint32_t kv_mask_bits(const KvMasks &masks, int n, int begin, int key) {
+  const int at = key - begin, word = at >> 6, bit = at & 63;
+  if (word < -1) return 0xffffu;
+  const uint64_t low = masks.row[n][min(word + 1, kKvMaskWords + 1)], high = masks.row[n][min(word + 2, kKvMaskWords + 1)];
+  return static_cast<uint32_t>(low >> bit | (bit > 48 ? high << (64 - bit) : 0)) & 0xffffu;
 }
 
 // A row's quarter of a query as it comes, and the signs of its dimensions: requested before the keys, so that it is there before them.
@@ -758,12 +820,13 @@ struct KvBroken {
     to = any ? step : to;
   }
   // NaN for a row that sees one of them, otherwise 0.
-  __device__ __forceinline__ float of(const KvAttendArgs &a, const int32_t *table, int last_key, const KvRow &row, int kv_head, int g) const {
+  template <typename Masked>
+  __device__ __forceinline__ float of(const KvAttendArgs &a, const int32_t *table, int last_key, const KvRow &row, int kv_head, int g, const Masked &masked) const {
     float found = 0.0f;
     const int last = min(min(row.high, last_key), 64 * to + 63), in_page = (1 << a.cache.page_shift) - 1;
     for (int key = max(row.low, 64 * from) + g; key <= last; key += 4) {
       const int page = table[key >> a.cache.page_shift];
-      if (!kv_page_there(a, page)) continue;
+      if (!kv_page_there(a, page) || masked(key)) continue;
       const float scale = bf16_bits_to_f32(a.cache.v_scales[(kv_block_of(a, page, kv_head) << a.cache.page_shift) + (key & in_page)]);
       found = scale != scale ? NAN : found;
     }
@@ -898,13 +961,14 @@ __device__ __forceinline__ void kv_request(const KvAttendArgs &a, int kv_head, i
 // Long ones are bound by memory: 131101 tokens, 8 heads of 128, 138 MB in 26.9 us; 64 requests, 668 MB in 127 (least 122), 5.3 TB/s of the 6.3 that a
 // read of nothing else reaches (vector instructions issue in half of the cycles, the matrix units are busy in 15 %).  Short ones by
 // latency: 1003 tokens 8.9 us, three dependent loads (length, page, keys) and four steps a wavefront.  Eight wavefronts a workgroup: 9.3.
-template <int D, int SPLIT, bool WIDE, int WAVES>
+template <int D, int SPLIT, bool WIDE, int WAVES, bool TREE>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendArgs a) {
   constexpr int W = D / 32;  // dwords of codes that a lane has of a key, and matrix instructions along the dimensions
   constexpr int PITCH = D + 4;
   __shared__ __attribute__((aligned(16))) float join[WAVES][16][PITCH];
   __shared__ float refs[WAVES][16], sums[WAVES][16];
   __shared__ uint32_t signs[D / 4];
+  __shared__ KvMasks masks[TREE ? WAVES : 1];
   if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -915,10 +979,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
     part = {{}, group, 0, 1, 0};
     if (!kv_few_tile(a, group, part.rows)) return;
   } else if constexpr (WAVES > 1) {
-    if (!kv_few_part<64 * WAVES>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) return;
+    if (!kv_few_part<64 * WAVES, TREE>(a, a.few_requests * a.few_tiles, a.few, kv_head, group, part)) return;
   }
   const KvRows r = part.rows;
-  const KvSpan span = kv_span_of(a, r, r.first, r.rows);
+  const KvSpan span = kv_span_of<TREE>(a, r, r.first, r.rows);
   const int steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
   int step = (span.lowest >> 6) + part.from(steps, part.index) + wave;
   const int end = (span.lowest >> 6) + part.from(steps, part.index + 1);
@@ -926,7 +990,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
   const int32_t *table = a.table + r.request * a.table_stride;
   KvRaw<D> raw;
   KvPages next = {0, 0};
-  const KvRow row = kv_row_of(a, r, kv_head, r.first + n, n < r.rows);
+  KvRow row = kv_row_of(a, r, kv_head, r.first + n, n < r.rows);
   kv_f16x8 q[W], q_rest[SPLIT > 0 ? W : 1];
   float factor;
   {
@@ -939,7 +1003,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
         next = kv_pages_of<WIDE>(a, table, n, g, step + WAVES);
       }
     };
+    uint64_t mask = 0;
+    if constexpr (TREE) mask = kv_request_mask(a, row, g);
     if constexpr (D < 256) request();
+    if constexpr (TREE) kv_place_masks(a, r, row, mask, masks[wave]);
     float y[D / 4];
     const int exponent = kv_query_exponent(query.rotate(row.token >= 0, y));
     factor = a.scale * (1.44269504088896f / D) * kv_power_of_two(exponent);
@@ -990,10 +1057,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
     if constexpr (more) kv_request_keys<D, WIDE>(a, kv_head, n, g, step + WAVES, next, raw);
     const int first = step * 64;
     if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
+      uint32_t bits = 0xffffu;
+      if constexpr (TREE) bits = kv_mask_bits(masks[wave], n, r.position(0), first + 16 * g);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = first + 16 * g + i;
-        const bool seen = kv_seen(key, here && key <= r.last_key, row);
+        const bool seen = kv_seen(key, here && key <= r.last_key, row) && (!TREE || (bits >> i & 1));
         x[i] = seen ? x[i] : -INFINITY;
         vs[i] = seen ? vs[i] : 0.0f;
       }
@@ -1092,7 +1161,7 @@ constexpr int kv_many_waves() { return D == 256 ? 8 : 4; }
 template <int D>
 constexpr size_t kv_many_lds() { return 2 * (4 * (D / 32) * 64 * 16 + (D / 32) * 4 * 64 * 16 + 512); }
 
-template <int D, int SPLIT, bool WIDE>
+template <int D, int SPLIT, bool WIDE, bool TREE>
 __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_kernel(KvAttendArgs a) {
   constexpr int WAVES = kv_many_waves<D>(), RT = kKvManyRows / 16 / WAVES;
   constexpr int C = D / 32;
@@ -1105,6 +1174,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   static_assert(2 * sizeof(Step) == kv_many_lds<D>(), "what the launch reserves");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint32_t signs[D / 4];
+  __shared__ KvMasks masks[TREE ? kKvManyRows / 16 : 1];
   __shared__ float own_factors[kKvManyRows];  // (of rows that do not share one; in registers they would be spilled)
   if (threadIdx.x < D / 4) signs[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.cache.signs)[threadIdx.x];
   Step *steps = reinterpret_cast<Step *>(lds);
@@ -1116,11 +1186,11 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   if (a.many.target == 0) {
     part = {{}, a.many_tiles - 1 - group, 0, 1, 0};
     if (!kv_many_tile(a, part.tile, part.rows)) return;
-  } else if (!kv_many_part<64 * WAVES>(a, kv_head, group, *reinterpret_cast<KvCounted *>(lds), part)) {
+  } else if (!kv_many_part<64 * WAVES, TREE>(a, kv_head, group, *reinterpret_cast<KvCounted *>(lds), part)) {
     return;
   }
   const KvRows r = part.rows;
-  const KvSpan span = kv_span_of(a, r, r.first, r.rows);
+  const KvSpan span = kv_span_of<TREE>(a, r, r.first, r.rows);
   const int all_steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
   int step = (span.lowest >> 6) + part.from(all_steps, part.index);
   const int end = (span.lowest >> 6) + part.from(all_steps, part.index + 1);
@@ -1153,7 +1223,9 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     const int at = (wave * RT + t) * 16 + n;
     row[t] = kv_row_of(a, r, kv_head, r.first + at, at < r.rows);
     query[t].request(a, row[t], g);
+    if constexpr (TREE) kv_place_masks(a, r, row[t], kv_request_mask(a, row[t], g), masks[wave * RT + t]);
   }
+  const int begin = TREE && kv_drafted(a, r) ? r.position(0) : 0x7fffffff;
   KvPages page = {0, 0}, next = page, later = page;  // of the step that is computed (whether its keys are there), of the one requested, and of the one after it
   if (step < end) {
     page = kv_pages_of<WIDE>(a, table, n, g, step);
@@ -1196,7 +1268,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
     }
   }
   const int wave_first = wave * RT * 16, wave_rows = min(r.rows - wave_first, RT * 16);  // rows of this wavefront, if any
-  const KvSpan own = kv_span_of(a, r, r.first + min(wave_first, r.rows - 1), max(wave_rows, 1));
+  const KvSpan own = kv_span_of<TREE>(a, r, r.first + min(wave_first, r.rows - 1), max(wave_rows, 1));
 
   const auto decode = [&](Step &to) {
 #pragma unroll
@@ -1270,12 +1342,15 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
         }
       }
       if (first + 63 > own.all_high || first < own.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
+        uint32_t bits[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) bits[t] = TREE ? kv_mask_bits(masks[wave * RT + t], n, begin, first + 16 * g) : 0xffffu;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = first + 16 * g + i;
           const bool there = here && key <= r.last_key;
 #pragma unroll
-          for (int t = 0; t < RT; ++t) x[t][i] = kv_seen(key, there, row[t]) ? x[t][i] : -INFINITY;
+          for (int t = 0; t < RT; ++t) x[t][i] = kv_seen(key, there, row[t]) && (!TREE || (bits[t] >> i & 1)) ? x[t][i] : -INFINITY;
           vs[i] = there ? vs[i] : i > 0 ? vs[0] : 0.0f;
           if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (all masks at once are more than there are scalar registers)
         }
@@ -1317,7 +1392,7 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   if (broken.to >= 0) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const float nan = broken.of(a, table, r.last_key, row[t], kv_head, g);
+      const float nan = broken.of(a, table, r.last_key, row[t], kv_head, g, [&](int key) { return TREE && (kv_mask_bits(masks[wave * RT + t], n, begin, key) & 1) == 0; });
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[t][j] += nan;
     }
@@ -1329,27 +1404,27 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
   }
 }
 
-template <int D, int SPLIT, bool WIDE>
+template <int D, int SPLIT, bool WIDE, bool TREE>
 bool kv_attend_launch(const KvAttendArgs &a, hipStream_t stream) {
   const unsigned heads = static_cast<unsigned>(a.cache.heads);
   if (a.many_tiles > 0) {
-    const auto kernel = kv_attend_many_kernel<D, SPLIT, WIDE>;
+    const auto kernel = kv_attend_many_kernel<D, SPLIT, WIDE, TREE>;
     if (!reserve_dynamic_lds(reinterpret_cast<const void *>(kernel), kv_many_lds<D>())) return false;
     launch_kernel(kernel, dim3(heads * (a.many.target != 0 ? a.many.target : a.many_tiles)), dim3(64 * kv_many_waves<D>()), kv_many_lds<D>(), stream, a);
   }
   if (a.few_requests > 0) {
     const dim3 grid(heads * (a.few.target + a.few_requests * a.few_tiles));
-    if (a.few_alone) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 1>, grid, dim3(64), 0, stream, a);
-    else launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 4>, grid, dim3(256), 0, stream, a);
+    if (a.few_alone) launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 1, TREE>, grid, dim3(64), 0, stream, a);
+    else launch_kernel(kv_attend_few_kernel<D, SPLIT, WIDE, 4, TREE>, grid, dim3(256), 0, stream, a);
   }
   return true;
 }
 
-template <int D>
+template <int D, bool TREE>
 bool kv_attend_of(const KvAttendArgs &a, int split, hipStream_t stream) {
   if (a.cache.page_shift >= 6)
-    return split == 0 ? kv_attend_launch<D, 0, true>(a, stream) : split == 1 ? kv_attend_launch<D, 1, true>(a, stream) : kv_attend_launch<D, 2, true>(a, stream);
-  return split == 0 ? kv_attend_launch<D, 0, false>(a, stream) : split == 1 ? kv_attend_launch<D, 1, false>(a, stream) : kv_attend_launch<D, 2, false>(a, stream);
+    return split == 0 ? kv_attend_launch<D, 0, true, TREE>(a, stream) : split == 1 ? kv_attend_launch<D, 1, true, TREE>(a, stream) : kv_attend_launch<D, 2, true, TREE>(a, stream);
+  return split == 0 ? kv_attend_launch<D, 0, false, TREE>(a, stream) : split == 1 ? kv_attend_launch<D, 1, false, TREE>(a, stream) : kv_attend_launch<D, 2, false, TREE>(a, stream);
 }
 
 }  // namespace oq

@@ -53,6 +53,8 @@ struct KvAttendArgs {
   int64_t table_stride;
   int table_width, window;            // window: 0 for none
   bool causal;
+  const uint64_t *masks;              // NULL, or [tokens, mask_words]: of the request's new tokens, which ones a query sees (causal then)
+  int mask_words;
   float scale;
   int few_tiles, few_requests, few_rows, few_in_tile;  // kernel for few rows: tiles of a request, requests (0: not launched), the rows of a request up to which it has it, rows of a tile at most
   bool few_alone;                     // in the first: one wavefront a workgroup

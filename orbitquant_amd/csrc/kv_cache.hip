@@ -1,6 +1,7 @@
 // Around the 4-bit key/value cache: pages and slots for new tokens, keys and values into it, and back out of it.
 // (No counterpart in the reference, which has no cache.)
 #include "kv_cache.h"
+#include "kv_rows.h"
 
 namespace oq {
 namespace {
@@ -122,64 +123,6 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(KvAssignArgs 
 // transform; the bytes alone take 9.  On the way in the order of the sums decides codes.  On the way out it does not: a scale times a code is a
 // multiple of half the scale's last bit, and so is every partial sum, which stays below 2^20 of it and is exact in fp32 in any order.
 
-template <int DT>
-__device__ __forceinline__ void load8(const void *p, int64_t at, bool wide, float *y) {
-  if (wide) {
-    if constexpr (DT == OQ_F32) {
-      const float4 lo = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[0], hi = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at)[1];
-      y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w; y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
-    } else {
-      const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
-      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = dyn_bits_to_f32((v[i / 2] >> (16 * (i & 1))) & 0xffffu, DT);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = load_as_f32<DT>(p, at + i);
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(void *p, int64_t at, const float *y) {  // 16-byte aligned
-  if constexpr (DT == OQ_F32) {
-    reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[0] = make_float4(y[0], y[1], y[2], y[3]);
-    reinterpret_cast<float4 *>(static_cast<float *>(p) + at)[1] = make_float4(y[4], y[5], y[6], y[7]);
-  } else {
-    uint32_t v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = DT == OQ_F16 ? f32_to_f16_bits(y[2 * i]) : f32_to_bf16_bits(y[2 * i]);
-      const uint32_t hi = DT == OQ_F16 ? f32_to_f16_bits(y[2 * i + 1]) : f32_to_bf16_bits(y[2 * i + 1]);
-      v[i] = lo | hi << 16;
-    }
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) = make_uint4(v[0], v[1], v[2], v[3]);
-  }
-}
-
-template <int E>
-__device__ __forceinline__ void times_signs(float (&y)[E], const uint32_t (&words)[E / 4]) {
-#pragma unroll
-  for (int i = 0; i < E; ++i) y[i] = __uint_as_float(__float_as_uint(y[i]) ^ ((words[i / 4] << (24 - 8 * (i & 3))) & 0x80000000u));
-}
-
-// Where the workgroup's tokens are: `slot` -1 for nothing to do, `key` the vector among those of k_codes and the scales, `value` the
-// first byte of its column in v_codes.
-struct KvPlace {
-  int64_t slot, key, value;
-};
-template <int D>
-__device__ __forceinline__ void group_places(KvPlace (&places)[kKvGroup], const KvCache &cache, const int64_t *from, int64_t first, int64_t tokens, int head) {
-  if (threadIdx.x < kKvGroup) {
-    const int shift = cache.page_shift;
-    int64_t slot = -1;
-    if (first + threadIdx.x < tokens) slot = from[first + threadIdx.x];
-    if (slot < 0 || slot >= cache.pages << shift) slot = -1;
-    const int64_t block = max(slot, static_cast<int64_t>(0)) >> shift, in_page = slot & ((1 << shift) - 1);
-    places[threadIdx.x] = {slot, ((block * cache.heads + head) << shift) + in_page, (((block * cache.heads + head) * (D / 2)) << shift) + in_page};
-  }
-}
-
 // On the way out, where the slots are waited for, as they are.
 __device__ __forceinline__ void group_slots(int64_t (&slots)[kKvGroup], const int64_t *from, int64_t first, int64_t tokens, int64_t most) {
   if (threadIdx.x < kKvGroup) {
@@ -187,15 +130,6 @@ __device__ __forceinline__ void group_slots(int64_t (&slots)[kKvGroup], const in
     if (first + threadIdx.x < tokens) slot = from[first + threadIdx.x];
     slots[threadIdx.x] = slot < most ? slot : -1;
   }
-}
-
-// Whether four tokens' bytes of a row are one dword.
-__device__ __forceinline__ int64_t slot_of(int64_t slot) { return slot; }
-__device__ __forceinline__ int64_t slot_of(const KvPlace &place) { return place.slot; }
-template <typename Token>
-__device__ __forceinline__ bool in_a_row(const Token *tokens, int page_shift) {
-  const int64_t s = slot_of(tokens[0]);
-  return s >= 0 && slot_of(tokens[1]) == s + 1 && slot_of(tokens[2]) == s + 2 && slot_of(tokens[3]) == s + 3 && (s >> page_shift) == ((s + 3) >> page_shift);
 }
 
 // Values of a lane: sixteen on the way in, where a vector's scale is found once for twice as many of them and one stage fewer lies between lanes
@@ -248,22 +182,7 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_write_kernel(KvWriteAr
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < (D / 2) * (kKvGroup / 4); i += THREADS) {
-    const int row = i / (kKvGroup / 4), t = i % (kKvGroup / 4) * 4;
-    uint32_t four[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) four[k] = reinterpret_cast<const uint8_t *>(bytes[t + k])[row];
-    uint8_t *const at_row = a.cache.v_codes + (static_cast<int64_t>(row) << shift);
-    if (in_a_row(places + t, shift)) {
-      const uint32_t word = four[0] | four[1] << 8 | four[2] << 16 | four[3] << 24;
-      __builtin_memcpy(at_row + places[t].value, &word, 4);  // (a page's tokens may begin anywhere)
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (places[t + k].slot >= 0) at_row[places[t + k].value] = static_cast<uint8_t>(four[k]);
-      }
-    }
-  }
+  store_values<D, THREADS>(a.cache, places, bytes);
 }
 
 template <int D, int DT>

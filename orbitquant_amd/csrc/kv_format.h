@@ -89,11 +89,13 @@ __device__ __forceinline__ void kv_dpp_butterflies(float (&y)[E], bool upper) {
 
 // One add or subtract for each output and stage, distances 1, 2, 4, ... in this order: the results are those of any other
 // schedule of the same butterflies.
-template <int D, int E>
+// HALVES: of sixteen values a lane has elements 8 * part + i and D / 2 + 8 * part + i, and their distance, the last, between registers.
+template <int D, int E, bool HALVES = false>
 __device__ __forceinline__ void kv_butterflies(float (&y)[E], int lane) {
   constexpr int LANES = D / E;
+  static_assert(!HALVES || E == 16, "two eights");
 #pragma unroll
-  for (int d = 1; d < E; d *= 2) {
+  for (int d = 1; d < (HALVES ? E / 2 : E); d *= 2) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       if ((i & d) == 0) {
@@ -110,6 +112,14 @@ __device__ __forceinline__ void kv_butterflies(float (&y)[E], int lane) {
   for (int i = 0; i < E; i += 2) {
     if constexpr (LANES >= 16) kv_lane_butterfly<16>(y[i], y[i + 1]);
     if constexpr (LANES >= 8) kv_lane_butterfly<32>(y[i], y[i + 1]);
+  }
+  if constexpr (HALVES) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float a = y[i], b = y[i + E / 2];
+      y[i] = a + b;
+      y[i + E / 2] = a - b;
+    }
   }
 }
 

@@ -1,0 +1,230 @@
+// Trees of drafted tokens over the 4-bit cache: positions and masks before the step, the accepted path after it.
+// (No counterpart in the reference, which has no cache.)
+#include "kv_tree.h"
+
+namespace oq {
+namespace {
+
+__device__ __forceinline__ int start_of(const int32_t *starts, int64_t tokens, int r) { return static_cast<int>(min(static_cast<int64_t>(max(starts[r], 0)), tokens)); }
+
+// ---- positions and masks ----------------------------------------------------------------------------------------------
+// Token i of a request's new ones hangs on parents[i] < i, or on what the request has cached already.  mask_i = bit i | mask_parent: every
+// token takes in what its ancestor has gathered and moves on to that one's ancestor, so that a path of 2^n tokens is whole after n
+// rounds.  Its depth is the number of its bits.  A workgroup a request, a thread a token; the last one has the tokens of no request.
+// Bound by latency: three loads one behind the other, and log2(nodes) rounds in LDS.
+template <int WORDS>
+__global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
+  __shared__ uint64_t masks[64 * WORDS][WORDS];
+  __shared__ int up[64 * WORDS];
+  const int r = blockIdx.x, i = threadIdx.x;
+  const int first = start_of(a.starts, a.tokens, r);
+  if (r == a.requests) {
+    for (int64_t t = first + i; t < a.tokens; t += 64 * WORDS) {
+      a.positions[t] = -1;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) a.masks[t * WORDS + w] = 0;
+    }
+    return;
+  }
+  const int count = max(start_of(a.starts, a.tokens, r + 1) - first, 0);
+  const int before = max(a.lengths[r], 0) - count;
+  if (count > 64 * WORDS) {  // more than there are bits: a prompt, one token behind the other
+    for (int t = i; t < count; t += 64 * WORDS) {
+      a.positions[first + t] = before + t;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) a.masks[(static_cast<int64_t>(first) + t) * WORDS + w] = 0;
+    }
+    return;
+  }
+  uint64_t mask[WORDS];
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) mask[w] = i >> 6 == w ? 1ull << (i & 63) : 0;
+  int ancestor = i < count ? a.parents[first + i] : -1;
+  if (ancestor >= i) ancestor = -1;
+  for (int reach = 1; reach < count; reach *= 2) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) masks[i][w] = mask[w];
+    up[i] = ancestor;
+    __syncthreads();
+    if (ancestor >= 0) {
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) mask[w] |= masks[ancestor][w];
+      ancestor = up[ancestor];
+    }
+    __syncthreads();
+  }
+  if (i >= count) return;
+  int depth = 0;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    depth += __popcll(mask[w]);
+    a.masks[(static_cast<int64_t>(first) + i) * WORDS + w] = mask[w];
+  }
+  a.positions[first + i] = before + depth - 1;
+}
+
+// ---- the accepted path -----------------------------------------------------------------------------------------------
+// kept[r] names tokens of request r's new ones in rising order; the i-th becomes its i-th new token, and the others are forgotten.
+// The list ends at its first entry that does not rise, is none of the request's tokens or has no slot.
+//
+// One launch for all layers.  A wavefront takes one head of one request in one cache.  A lane has the same bytes of all
+// entries: a dword of the keys, a row of the values (two of heads of 256), a scale.  So whatever an entry moves onto, its lane has read before:
+// the places rise with the list and are never behind their sources, and of a batch all are read before the first is written.
+// The bytes are few (132 an entry at D = 128): bound by the latency of four loads one behind the other (starts, list, slots, entries).
+constexpr int kKeepThreads = 256, kKeepBatch = 8;
+
+struct Path {
+  int first, fresh;
+};
+__device__ __forceinline__ Path path_of(const KvKeepArgs &a, int r) {
+  const int first = start_of(a.starts, a.tokens, r);
+  return {first, max(start_of(a.starts, a.tokens, r + 1) - first, 0)};
+}
+__device__ __forceinline__ int64_t slot_at(const KvKeepArgs &a, int64_t token) {
+  const int64_t slot = a.slots[token];
+  return slot < a.pages << a.page_shift ? slot : -1;
+}
+
+// Lengths, and the pages behind them onto the free list again, in front of those that it gives out next, in request order.
+__device__ void keep_counts(const KvKeepArgs &a) {
+  __shared__ int wave_sums[kKeepThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int run = (a.requests + kKeepThreads - 1) / kKeepThreads, from = min(tid * run, a.requests), to = min(from + run, a.requests);
+  const auto pages_of = [&](int tokens) { return static_cast<int>(min((static_cast<int64_t>(max(tokens, 0)) + (1 << a.page_shift) - 1) >> a.page_shift, static_cast<int64_t>(a.table_width))); };
+  int own = 0;
+  for (int r = from; r < to; ++r) {
+    const Path path = path_of(a, r);
+    int count = 0, last = -1;
+    for (int i = 0; i < a.most; ++i) {
+      const int k = a.kept[static_cast<int64_t>(r) * a.most + i];
+      if (k <= last || k >= path.fresh || slot_at(a, path.first + k) < 0) break;
+      last = k;
+      ++count;
+    }
+    const int length = max(a.lengths[r], 0), kept = max(length - path.fresh, 0) + count;
+    a.lengths_after[r] = kept;
+    if (a.table == nullptr) continue;
+    for (int column = pages_of(kept); column < pages_of(length); ++column) own += a.table[r * a.table_stride + column] >= 0 ? 1 : 0;
+  }
+  if (a.table == nullptr) return;
+  const int sum = kv_sums(own);
+  if (lane == 63) wave_sums[wave] = sum;
+  __syncthreads();
+  int ahead = sum - own, all = 0;
+#pragma unroll
+  for (int w = 0; w < kKeepThreads / 64; ++w) {
+    ahead += w < wave ? wave_sums[w] : 0;
+    all += wave_sums[w];
+  }
+  const int taken = min(max(*a.taken, 0), a.free_count), begin = taken - all;
+  if (tid == 0) *a.taken_after = max(begin, 0);
+  if (own == 0) return;
+  int at = begin + ahead;
+  for (int r = from; r < to; ++r) {
+    const int kept = a.lengths_after[r];  // (this thread's own)
+    for (int column = pages_of(kept); column < pages_of(max(a.lengths[r], 0)); ++column) {
+      const int page = a.table[r * a.table_stride + column];
+      if (page < 0) continue;
+      if (at >= 0) a.free_pages[at] = page;
+      ++at;
+    }
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepArgs a) {
+  const int counting = a.counts ? 1 : 0;
+  if (blockIdx.x < counting) {
+    keep_counts(a);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x - counting) * (kKeepThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (unit >= static_cast<int64_t>(a.requests) * a.heads * a.caches) return;
+  const int head = static_cast<int>(unit % a.heads), rest = static_cast<int>(unit / a.heads), r = rest % a.requests;
+  const auto &cache = a.cache[rest / a.requests];
+  const Path path = path_of(a, r);
+  const int shift = a.page_shift, in_page = (1 << shift) - 1;
+  int before = -1;  // the last entry of the lanes' batch before
+  for (int base = 0; base < a.most; base += 64) {
+    const int i = base + lane;
+    const int k = i < a.most ? a.kept[static_cast<int64_t>(r) * a.most + i] : -1;
+    const int ahead = __shfl_up(k, 1, 64), last = lane == 0 ? before : ahead;
+    int64_t source = -1, target = -1;
+    if (k > last && k < path.fresh) {
+      source = slot_at(a, static_cast<int64_t>(path.first) + k);
+      target = slot_at(a, static_cast<int64_t>(path.first) + i);  // (i <= k: a token of the request)
+    }
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(source < 0);
+    const int good = bad == 0 ? 64 : __builtin_ctzll(bad);
+    before = __builtin_amdgcn_readlane(k, 63);
+    // vectors of the cache, of codes and scales
+    const auto vector_of = [&](int64_t slot) { return ((((slot >> shift) * a.heads + head) << shift) + (slot & in_page)); };
+    const auto column_of = [&](int64_t slot) { return ((((slot >> shift) * a.heads + head) * (D / 2)) << shift) + (slot & in_page); };
+    const auto of_lane = [&](int64_t x, int from) {
+      return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), from))) |
+                                  static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), from))) << 32);
+    };
+    uint64_t moves = __builtin_amdgcn_ballot_w64(lane < good && source != target && target >= 0);
+    while (moves != 0) {
+      constexpr int ROWS = (D / 2 + 63) / 64;
+      int64_t to[kKeepBatch];
+      uint32_t key[kKeepBatch];
+      uint16_t scale[kKeepBatch];
+      uint8_t value[kKeepBatch][ROWS];
+      int count = 0;
+#pragma unroll
+      for (int b = 0; b < kKeepBatch; ++b) {
+        if (moves == 0) continue;
+        const int from_lane = __builtin_ctzll(moves);
+        moves &= moves - 1;
+        const int64_t from = of_lane(source, from_lane);
+        to[b] = of_lane(target, from_lane);
+        count = b + 1;
+        if (lane < D / 8) key[b] = reinterpret_cast<const uint32_t *>(cache.k_codes)[vector_of(from) * (D / 8) + lane];
+        if (lane < 2) scale[b] = (lane == 0 ? cache.k_scales : cache.v_scales)[vector_of(from)];
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+          if (64 * j + lane < D / 2) value[b][j] = cache.v_codes[column_of(from) + (static_cast<int64_t>(64 * j + lane) << shift)];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kKeepBatch; ++b) {
+        if (b >= count) continue;
+        if (lane < D / 8) reinterpret_cast<uint32_t *>(cache.k_codes)[vector_of(to[b]) * (D / 8) + lane] = key[b];
+        if (lane < 2) (lane == 0 ? cache.k_scales : cache.v_scales)[vector_of(to[b])] = scale[b];
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+          if (64 * j + lane < D / 2) cache.v_codes[column_of(to[b]) + (static_cast<int64_t>(64 * j + lane) << shift)] = value[b][j];
+        }
+      }
+    }
+    if (good < 64) break;
+  }
+}
+
+}  // namespace
+
+int kv_tree_dispatch(const KvTreeArgs &a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.requests + 1));
+  if (a.words == 1) launch_kernel(kv_tree_kernel<1>, grid, dim3(64), 0, stream, a);
+  else if (a.words == 2) launch_kernel(kv_tree_kernel<2>, grid, dim3(128), 0, stream, a);
+  else if (a.words == 3) launch_kernel(kv_tree_kernel<3>, grid, dim3(192), 0, stream, a);
+  else launch_kernel(kv_tree_kernel<4>, grid, dim3(256), 0, stream, a);
+  return check_launch("kv_tree");
+}
+
+int64_t kv_keep_blocks(const KvKeepArgs &a) {
+  const int64_t units = static_cast<int64_t>(a.requests) * a.heads * a.caches, each = kKeepThreads / 64;
+  return (units + each - 1) / each + (a.counts ? 1 : 0);
+}
+
+int kv_keep_dispatch(const KvKeepArgs &a, int dim, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(kv_keep_blocks(a)));
+  if (dim == 64) launch_kernel(kv_keep_kernel<64>, grid, dim3(kKeepThreads), 0, stream, a);
+  else if (dim == 128) launch_kernel(kv_keep_kernel<128>, grid, dim3(kKeepThreads), 0, stream, a);
+  else launch_kernel(kv_keep_kernel<256>, grid, dim3(kKeepThreads), 0, stream, a);
+  return check_launch("kv_keep");
+}
+
+}  // namespace oq

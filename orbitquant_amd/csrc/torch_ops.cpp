@@ -34,6 +34,11 @@ struct Library {
   decltype(&oq_kv_read) kv_read = nullptr;
   decltype(&oq_kv_attend) kv_attend = nullptr;
   decltype(&oq_kv_attend_workspace_bytes) kv_attend_workspace_bytes = nullptr;
+  decltype(&oq_qk_norm_rotary) qk_norm_rotary = nullptr;
+  decltype(&oq_kv_append) kv_append = nullptr;
+  decltype(&oq_kv_tree) kv_tree = nullptr;
+  decltype(&oq_kv_attend_tree) kv_attend_tree = nullptr;
+  decltype(&oq_kv_keep) kv_keep = nullptr;
 } lib;
 
 int dtype_code(at::ScalarType t) {
@@ -373,14 +378,15 @@ pybind11::object kv_read(const Tensor &slots, const pybind11::object &cache, con
 }
 
 pybind11::object kv_attend(const Tensor &q, const pybind11::object &cache, const Tensor &table, const Tensor &lengths, const OptTensor &starts,
-                           int64_t max_new, int64_t max_length, bool causal, int64_t window, double scale, bool want_lse) {
+                           int64_t max_new, int64_t max_length, bool causal, int64_t window, double scale, bool want_lse, const OptTensor &masks) {
   oq_kv_cache c;
-  if (lib.kv_attend == nullptr || !q.defined() || !q.device().is_cuda() || !cache_usable(cache, q.device(), c) || !rows_usable(q, c.head_dim))
+  if (lib.kv_attend == nullptr || lib.kv_attend_tree == nullptr || !q.defined() || !q.device().is_cuda() || !cache_usable(cache, q.device(), c) || !rows_usable(q, c.head_dim))
     return pybind11::none();
   const at::Device device = q.device();
   const int64_t tokens = q.size(0), heads = q.size(1), requests = lengths.defined() ? lengths.numel() : 0;
   if (requests < 1 || heads < 1 || heads % c.kv_heads != 0 || !dense(lengths, device, at::kInt) || !table_usable(table, device, requests) ||
-      (present(starts) ? !dense(*starts, device, at::kInt) || starts->numel() != requests + 1 : requests != tokens))
+      (present(starts) ? !dense(*starts, device, at::kInt) || starts->numel() != requests + 1 : requests != tokens) ||
+      (present(masks) && (!causal || !dense(*masks, device, at::kLong) || masks->dim() != 2 || masks->size(0) != tokens)))
     return pybind11::none();
   const c10::OptionalDeviceGuard guard(device);
   try {
@@ -390,16 +396,142 @@ pybind11::object kv_attend(const Tensor &q, const pybind11::object &cache, const
                                                         max_length, max_new);
     const Tensor workspace = need > 0 ? bytes_like(q, static_cast<int64_t>(need)) : Tensor();
     if (faked(out)) return pybind11::none();
-    const int rc = lib.kv_attend(data(q), dtype_code(q.scalar_type()), tokens, heads, q.stride(0), q.stride(1), &c, static_cast<const int32_t *>(data(table)),
-                                 table.stride(0), table.size(1), static_cast<const int32_t *>(data(lengths)), static_cast<const int32_t *>(data(starts)),
-                                 requests, causal, window, static_cast<float>(scale), max_length, max_new, data(out),
-                                 want_lse ? static_cast<float *>(data(lse)) : nullptr, need > 0 ? data(workspace) : nullptr, need, stream_of(device));
+    const int32_t *const pages = static_cast<const int32_t *>(data(table)), *const held = static_cast<const int32_t *>(data(lengths)),
+                  *const begin = static_cast<const int32_t *>(data(starts));
+    float *const sums = want_lse ? static_cast<float *>(data(lse)) : nullptr;
+    void *const room = need > 0 ? data(workspace) : nullptr;
+    const int type = dtype_code(q.scalar_type());
+    const int rc = present(masks) ? lib.kv_attend_tree(data(q), type, tokens, heads, q.stride(0), q.stride(1), &c, pages, table.stride(0), table.size(1), held, begin,
+                                                       requests, static_cast<const uint64_t *>(data(masks)), masks->size(1), window, static_cast<float>(scale),
+                                                       max_length, max_new, data(out), sums, room, need, stream_of(device))
+                                  : lib.kv_attend(data(q), type, tokens, heads, q.stride(0), q.stride(1), &c, pages, table.stride(0), table.size(1), held, begin,
+                                                  requests, causal, window, static_cast<float>(scale), max_length, max_new, data(out), sums, room, need,
+                                                  stream_of(device));
     if (rc != OQ_OK) return pybind11::none();
     if (want_lse) return pybind11::make_tuple(out, lse);
     return pybind11::cast(out);
   } catch (const c10::OutOfMemoryError &) {  // the Python side knows what a call can do without
   }
   return pybind11::none();
+}
+
+// ---- norms and rotary positions: `qk_rotary.py`'s and `kv_cache.py`'s functions for the usual call ----
+
+// The plan for `q`'s heads, which all of its tensors suit; false: the Python side.
+bool plan_of(const Tensor &q, const OptTensor &cos, const OptTensor &sin, const OptTensor &q_weight, const OptTensor &k_weight, const std::optional<double> &eps,
+             bool interleaved, const OptTensor &positions, oq_qk_norm_rotary_plan &p) {
+  const at::Device device = q.device();
+  const int64_t tokens = q.size(0), dim = q.size(2);
+  p = {};
+  if (present(cos) != present(sin)) return false;
+  if (present(cos)) {
+    if (!dense(*cos, device, at::kFloat) || !dense(*sin, device, at::kFloat) || cos->dim() != 2 || !cos->sizes().equals(sin->sizes()) || cos->size(1) < 1 ||
+        2 * cos->size(1) > dim)
+      return false;
+    p.cos = static_cast<const float *>(data(cos));
+    p.sin = static_cast<const float *>(data(sin));
+    p.rows = cos->size(0);
+    p.rotary_dim = 2 * cos->size(1);
+    if (present(positions)) {
+      if (!dense(*positions, device, at::kInt) || positions->numel() != tokens) return false;
+      p.positions = static_cast<const int32_t *>(data(positions));
+    } else if (p.rows < tokens) {
+      return false;
+    }
+  }
+  if (!eps.has_value() && (present(q_weight) || present(k_weight))) return false;
+  if (present(q_weight) && present(k_weight) && q_weight->scalar_type() != k_weight->scalar_type()) return false;
+  for (const OptTensor *w : {&q_weight, &k_weight}) {
+    if (!present(*w)) continue;
+    const int code = dtype_code((*w)->scalar_type());
+    if (code < 0 || !dense(**w, device, (*w)->scalar_type()) || (*w)->numel() != dim) return false;
+    p.weight_dtype = code;
+  }
+  p.q_weight = data(q_weight);
+  p.k_weight = data(k_weight);
+  p.norm = eps.has_value();
+  p.eps = eps.has_value() ? static_cast<float>(*eps) : 0.0f;
+  p.interleaved = interleaved;
+  return p.eps >= 0.0f && p.eps <= 3.402823466e38f;
+}
+
+pybind11::object qk_norm_rotary(const Tensor &q, const Tensor &k, const OptTensor &cos, const OptTensor &sin, const OptTensor &q_weight, const OptTensor &k_weight,
+                                const std::optional<double> &eps, bool interleaved, const OptTensor &positions) {
+  oq_qk_norm_rotary_plan p;
+  if (lib.qk_norm_rotary == nullptr || !q.defined() || q.dim() != 3 || !rows_usable(q, q.size(2)) || !rows_usable(k, q.size(2)) || q.size(1) < 1 || k.size(1) < 1 ||
+      k.size(0) != q.size(0) || k.device() != q.device() || k.scalar_type() != q.scalar_type() ||
+      !plan_of(q, cos, sin, q_weight, k_weight, eps, interleaved, positions, p))
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(q.device());
+  const Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+  if (faked(q_out) || faked(k_out)) return pybind11::none();
+  const int rc = lib.qk_norm_rotary(data(q), q.stride(0), q.stride(1), q.size(1), data(k), k.stride(0), k.stride(1), k.size(1), dtype_code(q.scalar_type()),
+                                    q.size(0), q.size(2), &p, data(q_out), data(k_out), stream_of(q.device()));
+  return rc == OQ_OK ? pybind11::object(pybind11::make_tuple(q_out, k_out)) : pybind11::object(pybind11::none());
+}
+
+pybind11::object kv_append(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &slots, const pybind11::object &cache, const OptTensor &cos,
+                           const OptTensor &sin, const OptTensor &q_weight, const OptTensor &k_weight, const std::optional<double> &eps, bool interleaved,
+                           const OptTensor &positions) {
+  oq_kv_cache c;
+  oq_qk_norm_rotary_plan p;
+  if (lib.kv_append == nullptr || !q.defined() || !q.device().is_cuda() || !cache_usable(cache, q.device(), c)) return pybind11::none();
+  const at::Device device = q.device();
+  if (!rows_usable(q, c.head_dim) || !rows_usable(k, c.head_dim) || !rows_usable(v, c.head_dim) || q.size(1) < 1 || k.size(1) != c.kv_heads ||
+      v.size(1) != c.kv_heads || k.size(0) != q.size(0) || v.size(0) != q.size(0) || k.device() != device || v.device() != device ||
+      k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || !dense(slots, device, at::kLong) || slots.numel() != q.size(0) ||
+      !plan_of(q, cos, sin, q_weight, k_weight, eps, interleaved, positions, p))
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(device);
+  const Tensor out = at::empty(q.sizes(), q.options());
+  if (faked(out)) return pybind11::none();
+  const int rc = lib.kv_append(data(q), q.stride(0), q.stride(1), q.size(1), data(k), k.stride(0), k.stride(1), data(v), v.stride(0), v.stride(1),
+                               dtype_code(q.scalar_type()), static_cast<const int64_t *>(data(slots)), q.size(0), &p, &c, data(out), stream_of(device));
+  return rc == OQ_OK ? pybind11::cast(out) : pybind11::object(pybind11::none());
+}
+
+// ---- trees of drafted tokens ----
+
+pybind11::object kv_tree(const Tensor &parents, const Tensor &starts, const Tensor &lengths, int64_t words) {
+  if (lib.kv_tree == nullptr || !parents.defined() || !parents.device().is_cuda() || words < 1 || words > 4) return pybind11::none();
+  const at::Device device = parents.device();
+  const int64_t tokens = parents.numel(), requests = lengths.defined() ? lengths.numel() : 0;
+  if (tokens < 1 || requests < 1 || !dense(parents, device, at::kInt) || parents.dim() != 1 || !dense(lengths, device, at::kInt) ||
+      !dense(starts, device, at::kInt) || starts.numel() != requests + 1)
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(device);
+  const Tensor positions = at::empty({tokens}, parents.options()), masks = at::empty({tokens, words}, parents.options().dtype(at::kLong));
+  if (faked(positions) || faked(masks)) return pybind11::none();
+  const int rc = lib.kv_tree(static_cast<const int32_t *>(data(parents)), static_cast<const int32_t *>(data(starts)), static_cast<const int32_t *>(data(lengths)),
+                             requests, tokens, words, static_cast<int32_t *>(data(positions)), static_cast<uint64_t *>(data(masks)), stream_of(device));
+  return rc == OQ_OK ? pybind11::object(pybind11::make_tuple(positions, masks)) : pybind11::object(pybind11::none());
+}
+
+pybind11::object kv_keep(const Tensor &kept, const Tensor &lengths, const Tensor &starts, const Tensor &slots, const pybind11::list &caches, const OptTensor &table,
+                         const OptTensor &free_pages, const OptTensor &taken) {
+  if (lib.kv_keep == nullptr || !lengths.defined() || !lengths.device().is_cuda() || caches.empty()) return pybind11::none();
+  const at::Device device = lengths.device();
+  const int64_t requests = lengths.numel();
+  std::vector<oq_kv_cache> all(caches.size());
+  for (size_t i = 0; i < all.size(); ++i)
+    if (!cache_usable(caches[i], device, all[i])) return pybind11::none();
+  const bool pages = present(taken);
+  if (requests < 1 || !dense(lengths, device, at::kInt) || !dense(kept, device, at::kInt) || kept.dim() != 2 || kept.size(0) != requests ||
+      !dense(starts, device, at::kInt) || starts.numel() != requests + 1 || !dense(slots, device, at::kLong) || present(table) != pages ||
+      present(free_pages) != pages ||
+      (pages && (!table_usable(*table, device, requests) || !dense(*free_pages, device, at::kInt) || free_pages->dim() != 1 || !dense(*taken, device, at::kInt) ||
+                 taken->numel() != 1)))
+    return pybind11::none();
+  const c10::OptionalDeviceGuard guard(device);
+  const Tensor after = at::empty({requests}, lengths.options()), taken_after = pages ? at::empty({1}, lengths.options()) : Tensor();
+  if (faked(after)) return pybind11::none();
+  const int rc = lib.kv_keep(static_cast<const int32_t *>(data(kept)), kept.size(1), static_cast<const int32_t *>(data(lengths)),
+                             static_cast<const int32_t *>(data(starts)), static_cast<const int64_t *>(data(slots)), requests, slots.numel(), all.data(),
+                             static_cast<int64_t>(all.size()), static_cast<const int32_t *>(data(table)), pages ? table->stride(0) : 0, pages ? table->size(1) : 0,
+                             static_cast<int32_t *>(data(free_pages)), pages ? free_pages->numel() : 0, static_cast<const int32_t *>(data(taken)),
+                             static_cast<int32_t *>(data(after)), pages ? static_cast<int32_t *>(data(taken_after)) : nullptr, stream_of(device));
+  if (rc != OQ_OK) return pybind11::none();
+  return pybind11::make_tuple(after, pages ? pybind11::cast(taken_after) : pybind11::object(pybind11::none()));
 }
 
 template <typename F>
@@ -426,10 +558,19 @@ PYBIND11_MODULE(_torch_ops, m) {
     bind_one(lib.kv_read, addresses, "oq_kv_read");
     bind_one(lib.kv_attend, addresses, "oq_kv_attend");
     bind_one(lib.kv_attend_workspace_bytes, addresses, "oq_kv_attend_workspace_bytes");
+    bind_one(lib.qk_norm_rotary, addresses, "oq_qk_norm_rotary");
+    bind_one(lib.kv_append, addresses, "oq_kv_append");
+    bind_one(lib.kv_tree, addresses, "oq_kv_tree");
+    bind_one(lib.kv_attend_tree, addresses, "oq_kv_attend_tree");
+    bind_one(lib.kv_keep, addresses, "oq_kv_keep");
   });
   m.def("quantized_linear_group", quantized_linear_group);
   m.def("kv_assign", kv_assign);
   m.def("kv_write", kv_write);
   m.def("kv_read", kv_read);
   m.def("kv_attend", kv_attend);
+  m.def("qk_norm_rotary", qk_norm_rotary);
+  m.def("kv_append", kv_append);
+  m.def("kv_tree", kv_tree);
+  m.def("kv_keep", kv_keep);
 }

@@ -782,4 +782,5 @@ def unpack_lowbit(packed: torch.Tensor, bits: int, length: int) -> torch.Tensor:
     return out
 
 
-from .kv_cache import kv_assign, kv_attend, kv_read, kv_write  # noqa: E402,F401  (the cache's wrappers, which use the helpers above)
+from .qk_rotary import qk_norm_rotary  # noqa: E402,F401  (these wrappers use the helpers above)
+from .kv_cache import kv_append, kv_assign, kv_attend, kv_keep, kv_read, kv_tree, kv_write  # noqa: E402,F401
