@@ -749,6 +749,14 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
 // ---- norms and rotary positions ----
 
 namespace {
+// No more values at once than 16 bytes hold of the smaller type, or 8, where these vectors begin.
+void qk_fit_piece(oq::QkNormRotary &how, const void *x, int64_t token_stride, int64_t head_stride, int dtype) {
+  for (; how.piece > 1; how.piece = how.piece == 8 ? 4 : 1) {
+    const int bytes = how.piece * oq::dtype_size(dtype) < 16 ? how.piece * oq::dtype_size(dtype) : 16, per = bytes / oq::dtype_size(dtype);
+    if (aligned(x, bytes) && token_stride % per == 0 && head_stride % per == 0) return;
+  }
+}
+
 // How the pairs of heads of `dim` are normed and turned; an error status where the plan is none.
 int qk_plan_of(const char *what, const oq_qk_norm_rotary_plan *p, int64_t dim, oq::QkNormRotary &how) {
   if (p == nullptr) return fail(OQ_ERR_INVALID, "%s: no plan", what);
@@ -766,13 +774,16 @@ int qk_plan_of(const char *what, const oq_qk_norm_rotary_plan *p, int64_t dim, o
   how.table_wide = how.half % 8 == 0 && aligned(p->cos, 16) && aligned(p->sin, 16);
   how.weight[0] = p->q_weight; how.weight[1] = p->k_weight; how.weight_dtype = p->weight_dtype;
   how.norm = p->norm != 0; how.interleaved = p->interleaved != 0; how.eps = p->eps; how.by_dim = static_cast<float>(1.0 / static_cast<double>(dim));
-  how.weight_wide = dim % 16 == 0 && (how.interleaved || how.half % 8 == 0) && aligned(p->q_weight, 16) && aligned(p->k_weight, 16);
+  // Eight values at once where a head's parts are multiples of eight pairs, four where they are of four; the vectors' alignment has its say below.
+  how.piece = dim % 16 == 0 && (how.interleaved || how.half % 8 == 0) ? 8 : dim % 8 == 0 && (how.interleaved || how.half % 4 == 0) ? 4 : 1;
+  qk_fit_piece(how, p->q_weight, 0, 0, p->weight_dtype);
+  qk_fit_piece(how, p->k_weight, 0, 0, p->weight_dtype);
   return OQ_OK;
 }
 
 // One side's tensors, and the workgroups of `threads` that they take.
 int qk_side_of(const char *what, const void *x, int64_t token_stride, int64_t head_stride, int64_t heads, int dtype, int64_t tokens, int64_t dim,
-               const oq::QkNormRotary &how, void *out, int threads, oq::QkSide &side, uint32_t &blocks) {
+               oq::QkNormRotary &how, void *out, int threads, oq::QkSide &side, uint32_t &blocks) {
   if (tokens < 0 || heads < 1 || heads > 65535) return fail(OQ_ERR_INVALID, "%s: tokens=%lld heads=%lld", what, (long long)tokens, (long long)heads);
   if (tokens > 0x3fffffffLL || tokens * heads > 0x3fffffffLL) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld heads=%lld exceed the grid", what, (long long)tokens, (long long)heads);
   if (tokens > 0 && (x == nullptr || out == nullptr)) return fail(OQ_ERR_INVALID, "%s: null pointer", what);
@@ -780,7 +791,7 @@ int qk_side_of(const char *what, const void *x, int64_t token_stride, int64_t he
   side.x = x; side.out = out; side.token_stride = token_stride; side.head_stride = head_stride;
   side.heads = static_cast<int>(heads); side.groups = (side.heads + oq::kQkHeads - 1) / oq::kQkHeads;
   side.magic = static_cast<uint32_t>(((1ull << 32) + side.groups - 1) / side.groups);
-  side.wide = dim % 16 == 0 && (how.interleaved || how.half % 8 == 0) && vectors_wide(x, token_stride, head_stride, dtype);
+  qk_fit_piece(how, x, token_stride, head_stride, dtype);
   const int64_t count = oq::qk_blocks(tokens, side.heads, static_cast<int>(dim), threads);
   if (count > oq::kKvMostThreads / threads / 2) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld heads=%lld exceed the grid", what, (long long)tokens, (long long)heads);
   blocks = static_cast<uint32_t>(count);
@@ -819,7 +830,7 @@ int oq_kv_append(const void *q, int64_t q_token_stride, int64_t q_head_stride, i
   oq::KvWriteArgs &w = a.write;
   w.k = k; w.v = v; w.slots = slots; w.tokens = tokens;
   w.k_token_stride = k_token_stride; w.k_head_stride = k_head_stride; w.v_token_stride = v_token_stride; w.v_head_stride = v_head_stride;
-  w.k_wide = (a.how.interleaved || a.how.half % 8 == 0) && vectors_wide(k, k_token_stride, k_head_stride, dtype);
+  qk_fit_piece(a.how, k, k_token_stride, k_head_stride, dtype);
   w.v_wide = vectors_wide(v, v_token_stride, v_head_stride, dtype);
   a.kv_blocks = static_cast<uint32_t>((tokens + oq::kKvGroup - 1) / oq::kKvGroup * cache->kv_heads);
   return oq::kv_append_dispatch(a, static_cast<int>(cache->head_dim), dtype, as_stream(stream));

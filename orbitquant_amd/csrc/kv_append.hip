@@ -21,7 +21,7 @@ __device__ __forceinline__ void load_vector(const void *p, int64_t at, int part,
 
 // The workgroups of kv_write (one head of sixteen tokens each), whose keys go through the norm and the rotation first, and behind them
 // those of the queries.  A wavefront has keys or values, never both.
-template <int D, int DT, int LAYOUT>
+template <int D, int DT, int LAYOUT, int PIECE>
 __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppendArgs a) {
   constexpr int E = 16, L = D / E, THREADS = kv_write_threads(D);
   constexpr int AT_ONCE = THREADS / L, PASSES = 2 * kKvGroup / AT_ONCE;
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppend
   __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];
   __shared__ __attribute__((aligned(16))) float turned[LAYOUT == THROUGH_LDS ? kKvGroup : 1][LAYOUT == THROUGH_LDS ? D + 4 : 1];
   if (blockIdx.x >= a.kv_blocks) {
-    qk_block<DT, L, THREADS>(a.how, a.q, 0, a.write.tokens, D, blockIdx.x - a.kv_blocks);
+    qk_block<DT, L, PIECE, LAYOUT == IN_A_ROW, THREADS>(a.how, a.q, 0, a.write.tokens, D, blockIdx.x - a.kv_blocks);
     return;
   }
   const KvWriteArgs &w = a.write;
@@ -46,11 +46,14 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppend
     } else {
       const int64_t at = token * w.k_token_stride + head * w.k_head_stride;
       float u[8], v[8], wu[8], wv[8];
-      qk_load_vector<DT>(w.k, at, part, D, a.how, w.k_wide, u, v);
       QkTurn turn;
-      turn.load(a.how, token, part);
-      qk_load_weight(a.how, 1, part, D, wu, wv);
-      qk_apply<L>(a.how, part, wu, wv, turn, u, v);
+      const int64_t position = turn.row_of(a.how, token);
+      QkRaw<DT, PIECE, LAYOUT == IN_A_ROW> raw;
+      raw.request(w.k, at, part, D, a.how);
+      turn.load(a.how, position, part);
+      qk_load_weight<PIECE, LAYOUT == IN_A_ROW>(a.how, 1, part, D, wu, wv);
+      raw.pairs(u, v);
+      qk_apply<L>(a.how, wu, wv, turn, u, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[p][LAYOUT == IN_A_ROW ? 2 * i : i] = u[i];
@@ -110,12 +113,17 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppend
   store_values<D, THREADS>(w.cache, places, bytes);
 }
 
-template <int D, int DT>
+template <int D, int DT, int LAYOUT>
 void launch(const KvAppendArgs &a, hipStream_t stream) {
   const dim3 grid(a.kv_blocks + a.q_blocks), block(kv_write_threads(D));
-  if (a.how.interleaved) launch_kernel(kv_append_kernel<D, DT, IN_A_ROW>, grid, block, 0, stream, a);
-  else if (a.how.half == 0 || a.how.half == D / 2) launch_kernel(kv_append_kernel<D, DT, IN_HALVES>, grid, block, 0, stream, a);
-  else launch_kernel(kv_append_kernel<D, DT, THROUGH_LDS>, grid, block, 0, stream, a);
+  if (a.how.piece == 8) launch_kernel(kv_append_kernel<D, DT, LAYOUT, 8>, grid, block, 0, stream, a);
+  else launch_kernel(kv_append_kernel<D, DT, LAYOUT, 1>, grid, block, 0, stream, a);
+}
+template <int D, int DT>
+void launch(const KvAppendArgs &a, hipStream_t stream) {
+  if (a.how.interleaved) launch<D, DT, IN_A_ROW>(a, stream);
+  else if (a.how.half == 0 || a.how.half == D / 2) launch<D, DT, IN_HALVES>(a, stream);
+  else launch<D, DT, THROUGH_LDS>(a, stream);
 }
 template <int D>
 void launch(const KvAppendArgs &a, int dtype, hipStream_t stream) {

@@ -25,7 +25,7 @@ struct QkNormRotary {
   bool table_wide;             // eight entries begin on 16 bytes
   const void *weight[2];       // of queries and of keys; NULL: ones
   int weight_dtype;
-  bool weight_wide;
+  int piece;                   // values fetched at once, of all that is fetched: 8, 4 or 1
   bool norm, interleaved;
   float eps, by_dim;           // by_dim: 1 / D
 };
@@ -36,7 +36,6 @@ struct QkSide {  // queries, or keys
   int64_t token_stride, head_stride;
   int heads, groups;           // groups of kQkHeads heads
   uint32_t magic;              // of a division by `groups`: ceil(2^32 / groups)
-  bool wide;                   // eight values begin on 16 bytes, in x and in out
 };
 
 constexpr int kQkHeads = 4;    // of a token a lane, which share its entries of the tables and the weights
@@ -87,94 +86,106 @@ __device__ __forceinline__ int2 qk_pair(int p, int dim, const QkNormRotary &how)
   return p < how.half ? make_int2(p, p + how.half) : make_int2(p + how.half, p + dim / 2);
 }
 
-// Eight values that begin on 16 bytes, of a type that is known when the call comes.
-__device__ __forceinline__ void qk_load8(const void *p, int dtype, int64_t at, bool wide, float *y) {
-  if (dtype == OQ_F32) load8<OQ_F32>(p, at, wide, y);
-  else if (dtype == OQ_F16) load8<OQ_F16>(p, at, wide, y);
-  else load8<OQ_BF16>(p, at, wide, y);
-}
-
-// A lane's pairs 8 * part .. of the vector at `at`; `load`: eight values in a row, or one.
-template <typename Load8, typename Load1>
-__device__ __forceinline__ void qk_load_pairs(int part, int dim, const QkNormRotary &how, bool wide, float (&a)[8], float (&b)[8], const Load8 &eight, const Load1 &one) {
-  if (wide) {
-    const bool there = 16 * part < dim;
-    if (how.interleaved) {
-      float v[16];
-      if (there) {
-        eight(16 * part, v);
-        eight(16 * part + 8, v + 8);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = there ? v[2 * i] : 0.0f;
-        b[i] = there ? v[2 * i + 1] : 0.0f;
-      }
-    } else {
-      const int2 at = qk_pair(8 * part, dim, how);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
-      if (there) {
-        eight(at.x, a);
-        eight(at.y, b);
-      }
-    }
+// How a lane's pairs are fetched: PIECE = 8 or 4 values at once, where the first dimensions of the head's parts and its vectors allow it, or one by one.
+constexpr int qk_piece_words(int dt, int piece) { return dt == OQ_F32 ? piece : (piece + 1) / 2; }
+template <int DT, int PIECE>
+__device__ __forceinline__ void qk_fetch(const void *p, int64_t at, uint32_t *w) {
+  if constexpr (PIECE == 1) {
+    if constexpr (DT == OQ_F32) w[0] = static_cast<const uint32_t *>(p)[at];
+    else w[0] = static_cast<const uint16_t *>(p)[at];
   } else {
+    constexpr int WORDS = qk_piece_words(DT, PIECE);
+    const char *from = static_cast<const char *>(p) + at * (DT == OQ_F32 ? 4 : 2);
+    if constexpr (WORDS == 2) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(from);
+      w[0] = v.x; w[1] = v.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int p = 8 * part + i;
-      const int2 at = qk_pair(p, dim, how);
-      a[i] = 2 * p < dim ? one(at.x) : 0.0f;
-      b[i] = 2 * p < dim ? one(at.y) : 0.0f;
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 v = reinterpret_cast<const uint4 *>(from)[i / 4];
+        w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+      }
     }
   }
 }
 
-template <int DT>
-__device__ __forceinline__ void qk_load_vector(const void *x, int64_t at, int part, int dim, const QkNormRotary &how, bool wide, float (&a)[8], float (&b)[8]) {
-  qk_load_pairs(part, dim, how, wide, a, b, [&](int d, float *y) { load8<DT>(x, at + d, true, y); }, [&](int d) { return load_as_f32<DT>(x, at + d); });
+// Sixteen values as they come, requested for all of a lane's heads before the first is looked at.
+template <int DT, int PIECE, bool INTERLEAVED>
+struct QkRaw {
+  static constexpr int EACH = qk_piece_words(DT, PIECE), PIECES = 16 / PIECE;
+  uint32_t w[PIECES * EACH];
+
+  // Halves: the first dimensions of the eight pairs, then the second ones; neighbours: pair by pair.  Zeros behind the last pair.
+  __device__ __forceinline__ void request(const void *x, int64_t at, int part, int dim, const QkNormRotary &how) {
+#pragma unroll
+    for (int i = 0; i < PIECES * EACH; ++i) w[i] = 0;
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+      const int value = (INTERLEAVED ? c : c % (PIECES / 2)) * PIECE;  // of sixteen in a row; of eight first or second ones
+      if (INTERLEAVED) {
+        const int d = 16 * part + value;
+        if (d < dim) qk_fetch<DT, PIECE>(x, at + d, w + c * EACH);
+      } else {
+        const int pair = 8 * part + value;
+        const int2 d = qk_pair(pair, dim, how);
+        if (2 * pair < dim) qk_fetch<DT, PIECE>(x, at + (c < PIECES / 2 ? d.x : d.y), w + c * EACH);
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (DT == OQ_F32) return __uint_as_float(w[i]);
+    else if constexpr (PIECE == 1) return dyn_bits_to_f32(w[i], DT);
+    else if constexpr (DT == OQ_BF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return f16_bits_to_f32(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
+  }
+  __device__ __forceinline__ void pairs(float (&a)[8], float (&b)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = value(INTERLEAVED ? 2 * i : i);
+      b[i] = value(INTERLEAVED ? 2 * i + 1 : 8 + i);
+    }
+  }
+};
+
+template <int DT, int PIECE, bool INTERLEAVED>
+__device__ __forceinline__ void qk_load_pairs(const void *x, int64_t at, int part, int dim, const QkNormRotary &how, float (&a)[8], float (&b)[8]) {
+  QkRaw<DT, PIECE, INTERLEAVED> raw;
+  raw.request(x, at, part, dim, how);
+  raw.pairs(a, b);
 }
+template <int PIECE, bool INTERLEAVED>
 __device__ __forceinline__ void qk_load_weight(const QkNormRotary &how, int side, int part, int dim, float (&a)[8], float (&b)[8]) {
   const void *const w = how.weight[side];
   if (w == nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = b[i] = 1.0f;
+  } else if (how.weight_dtype == OQ_F32) {
+    qk_load_pairs<OQ_F32, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
+  } else if (how.weight_dtype == OQ_F16) {
+    qk_load_pairs<OQ_F16, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
   } else {
-    qk_load_pairs(part, dim, how, how.weight_wide, a, b, [&](int d, float *y) { qk_load8(w, how.weight_dtype, d, true, y); },
-                  [&](int d) { return load_dyn_f32(w, how.weight_dtype, d); });
+    qk_load_pairs<OQ_BF16, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
   }
 }
 
 // A token's row of the tables, eight entries of a lane.  A negative position (a token of no request) turns nothing, one behind the tables makes NaN.
 struct QkTurn {
   float c[8], s[8];
-  bool turns;
-  __device__ __forceinline__ void load(const QkNormRotary &how, int64_t token, int part) {
+  int pairs;  // of the lane's that are turned
+  __device__ __forceinline__ int64_t row_of(const QkNormRotary &how, int64_t token) const { return how.half == 0 ? -1 : how.positions != nullptr ? how.positions[token] : token; }
+  __device__ __forceinline__ void load(const QkNormRotary &how, int64_t row, int part) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = 1.0f;
-      s[i] = 0.0f;
-    }
-    turns = false;
-    if (how.half == 0) return;
-    const int64_t row = how.positions != nullptr ? how.positions[token] : token;
-    if (row < 0) return;
-    turns = true;
-    if (row >= how.rows) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
-      return;
-    }
+    for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
+    pairs = row >= 0 ? min(max(how.half - 8 * part, 0), 8) : 0;
+    if (pairs == 0 || row >= how.rows) return;
     const int64_t at = row * how.half + 8 * part;
     if (how.table_wide) {
-      if (8 * part < how.half) {
-        load8<OQ_F32>(how.cos, at, true, c);
-        load8<OQ_F32>(how.sin, at, true, s);
-      }
+      load8<OQ_F32>(how.cos, at, true, c);
+      load8<OQ_F32>(how.sin, at, true, s);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (8 * part + i < how.half) {
+        if (i < pairs) {
           c[i] = how.cos[at + i];
           s[i] = how.sin[at + i];
         }
@@ -184,7 +195,7 @@ struct QkTurn {
 };
 
 template <int L>
-__device__ __forceinline__ void qk_apply(const QkNormRotary &how, int part, const float (&wa)[8], const float (&wb)[8], const QkTurn &turn, float (&a)[8], float (&b)[8]) {
+__device__ __forceinline__ void qk_apply(const QkNormRotary &how, const float (&wa)[8], const float (&wb)[8], const QkTurn &turn, float (&a)[8], float (&b)[8]) {
   if (how.norm) {
     const float r = 1.0f / sqrtf(qk_square_sum<L>(a, b) * how.by_dim + how.eps);
 #pragma unroll
@@ -193,48 +204,61 @@ __device__ __forceinline__ void qk_apply(const QkNormRotary &how, int part, cons
       b[i] = b[i] * r * wb[i];
     }
   }
+  if (turn.pairs == 0) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float u = a[i] * turn.c[i] - b[i] * turn.s[i], v = b[i] * turn.c[i] + a[i] * turn.s[i];
-    const bool turned = turn.turns && 8 * part + i < how.half;  // (what is not may be an infinity, which a sine of zero does not leave alone)
-    a[i] = turned ? u : a[i];
-    b[i] = turned ? v : b[i];
+    a[i] = i < turn.pairs ? u : a[i];
+    b[i] = i < turn.pairs ? v : b[i];
   }
 }
 
-template <int DT>
-__device__ __forceinline__ void qk_store_vector(void *out, int64_t at, int part, int dim, const QkNormRotary &how, bool wide, const float (&a)[8], const float (&b)[8]) {
-  if (wide) {
-    if (16 * part >= dim) return;
-    if (how.interleaved) {
-      float v[16];
+template <int DT, int PIECE>
+__device__ __forceinline__ void qk_put(void *p, int64_t at, const float *y) {
+  if constexpr (PIECE == 8) {
+    store8<DT>(p, at, y);
+  } else if constexpr (PIECE == 1) {
+    store_from_f32<DT>(p, at, y[0]);
+  } else if constexpr (DT == OQ_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(p) + at) = make_float4(y[0], y[1], y[2], y[3]);
+  } else {
+    uint32_t w[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[2 * i] = a[i];
-        v[2 * i + 1] = b[i];
-      }
-      store8<DT>(out, at + 16 * part, v);
-      store8<DT>(out, at + 16 * part + 8, v + 8);
-    } else {
-      const int2 d = qk_pair(8 * part, dim, how);
-      store8<DT>(out, at + d.x, a);
-      store8<DT>(out, at + d.y, b);
+    for (int i = 0; i < 2; ++i) {
+      w[i] = DT == OQ_F16 ? f32_to_f16_bits(y[2 * i]) | static_cast<uint32_t>(f32_to_f16_bits(y[2 * i + 1])) << 16
+                          : f32_to_bf16_bits(y[2 * i]) | static_cast<uint32_t>(f32_to_bf16_bits(y[2 * i + 1])) << 16;
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = make_uint2(w[0], w[1]);
+  }
+}
+template <int DT, int PIECE, bool INTERLEAVED>
+__device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, int dim, const QkNormRotary &how, const float (&a)[8], const float (&b)[8]) {
+  if constexpr (INTERLEAVED) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[2 * i] = a[i];
+      v[2 * i + 1] = b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += PIECE) {
+      if (16 * part + i < dim) qk_put<DT, PIECE>(out, at + 16 * part + i, v + i);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int p = 8 * part + i;
-      if (2 * p < dim) {
-        const int2 d = qk_pair(p, dim, how);
-        store_from_f32<DT>(out, at + d.x, a[i]);
-        store_from_f32<DT>(out, at + d.y, b[i]);
+    for (int i = 0; i < 8; i += PIECE) {
+      const int pair = 8 * part + i;
+      const int2 d = qk_pair(pair, dim, how);
+      if (2 * pair < dim) {
+        qk_put<DT, PIECE>(out, at + d.x, a + i);
+        qk_put<DT, PIECE>(out, at + d.y, b + i);
       }
     }
   }
 }
 
-// Workgroup `block` of a side: four heads of a token for every L lanes.
-template <int DT, int L, int THREADS>
+// Workgroup `block` of a side: HEADS heads of a token for every L lanes.
+template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS>
 __device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
   constexpr int UNITS = THREADS / L;
   const int lane = threadIdx.x & 63, part = qk_part_of<L>(lane);
@@ -243,21 +267,22 @@ __device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &
   const uint32_t down = groups == 1 ? n : __umulhi(n, side.magic);
   const int64_t token = static_cast<int64_t>(row) + down;
   const int head = static_cast<int>(n - down * groups) * kQkHeads;
-  const bool there = token < tokens;
-  float a[kQkHeads][8], b[kQkHeads][8], wa[8], wb[8];
+  if (token >= tokens) return;  // (all of a unit's lanes)
+  QkRaw<DT, PIECE, INTERLEAVED> raw[kQkHeads];
+  float wa[8], wb[8];
   QkTurn turn;
-  if (there) {
-    const int64_t at = token * side.token_stride;
+  const int64_t position = turn.row_of(how, token), at = token * side.token_stride;
 #pragma unroll
-    for (int h = 0; h < kQkHeads; ++h) qk_load_vector<DT>(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how, side.wide, a[h], b[h]);
-    turn.load(how, token, part);
-    qk_load_weight(how, which, part, dim, wa, wb);
-  }
+  for (int h = 0; h < kQkHeads; ++h) raw[h].request(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how);
+  turn.load(how, position, part);
+  qk_load_weight<PIECE, INTERLEAVED>(how, which, part, dim, wa, wb);
 #pragma unroll
   for (int h = 0; h < kQkHeads; ++h) {
-    if (h > 0 && head + h >= side.heads) break;  // (a unit's lanes agree, and their sums are theirs)
-    qk_apply<L>(how, part, wa, wb, turn, a[h], b[h]);
-    if (there) qk_store_vector<DT>(side.out, (token * side.heads + head + h) * dim, part, dim, how, side.wide, a[h], b[h]);
+    if (h > 0 && head + h >= side.heads) break;
+    float a[8], b[8];
+    raw[h].pairs(a, b);
+    qk_apply<L>(how, wa, wb, turn, a, b);
+    qk_store_pairs<DT, PIECE, INTERLEAVED>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
   }
 }
 

@@ -7,18 +7,29 @@ namespace oq {
 namespace {
 
 // The first workgroups have the queries, the others the keys.
-template <int DT, int L>
+template <int DT, int L, int PIECE, bool INTERLEAVED>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rotary_kernel(QkArgs a) {
   const bool keys = blockIdx.x >= a.q_blocks;
-  qk_block<DT, L, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
+  qk_block<DT, L, PIECE, INTERLEAVED, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
 }
 
+template <int DT, int L, int PIECE>
+void launch(const QkArgs &a, hipStream_t stream) {
+  const dim3 grid(a.q_blocks + a.k_blocks);
+  if (a.how.interleaved) launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, true>, grid, dim3(kQkThreads), 0, stream, a);
+  else launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, false>, grid, dim3(kQkThreads), 0, stream, a);
+}
+template <int DT, int L>
+void launch(const QkArgs &a, hipStream_t stream) {
+  if (a.how.piece == 8) launch<DT, L, 8>(a, stream);
+  else if (a.how.piece == 4) launch<DT, L, 4>(a, stream);
+  else launch<DT, L, 1>(a, stream);
+}
 template <int L>
 void launch(const QkArgs &a, int dtype, hipStream_t stream) {
-  const dim3 grid(a.q_blocks + a.k_blocks);
-  if (dtype == OQ_F32) launch_kernel(qk_norm_rotary_kernel<OQ_F32, L>, grid, dim3(kQkThreads), 0, stream, a);
-  else if (dtype == OQ_F16) launch_kernel(qk_norm_rotary_kernel<OQ_F16, L>, grid, dim3(kQkThreads), 0, stream, a);
-  else launch_kernel(qk_norm_rotary_kernel<OQ_BF16, L>, grid, dim3(kQkThreads), 0, stream, a);
+  if (dtype == OQ_F32) launch<OQ_F32, L>(a, stream);
+  else if (dtype == OQ_F16) launch<OQ_F16, L>(a, stream);
+  else launch<OQ_BF16, L>(a, stream);
 }
 
 }  // namespace
