@@ -596,12 +596,16 @@ int oq_kv_tree(const int32_t *parents, const int32_t *starts, const int32_t *len
  * oq_kv_attend (causal) where a query sees of its request's new tokens those whose bit is set in its mask, whichever these are: any masks will
  * do, its own token is seen only if its bit is set.  It sees all tokens before the new ones.  Of what it sees, the last `window`
  * in the cache's order if window > 0.  A request with more new tokens than 64 * mask_words is causal.  masks 8-byte aligned.
+ * workspace: NULL, or oq_kv_attend_tree_workspace_bytes(...) bytes, as for oq_kv_attend.
  */
 int oq_kv_attend_tree(const void *q, int q_dtype, int64_t tokens, int64_t heads, int64_t q_token_stride,
                       int64_t q_head_stride, const oq_kv_cache *cache, const int32_t *table, int64_t table_stride,
                       int64_t table_width, const int32_t *lengths, const int32_t *starts, int64_t requests,
                       const uint64_t *masks, int64_t mask_words, int64_t window, float scale, int64_t max_length,
                       int64_t max_new, void *out, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
+uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t page_size, int64_t table_width, int64_t requests, int has_starts,
+                                           int64_t mask_words, int64_t window, int64_t max_length, int64_t max_new);
 
 /*
  * After the step: of each request's new tokens those of an accepted path stay, as if they had been its only ones.

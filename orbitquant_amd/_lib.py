@@ -25,7 +25,7 @@ EXPORTS = (
     "oq_dequantize_packed_weight", "oq_packed_linear_workspace_bytes", "oq_matmul_packed_weight_workspace_bytes",
     "oq_packed_linear_int8", "oq_packed_linear_int8_workspace_bytes", "oq_packed_linear_least_workspace_bytes",
     "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes",
-    "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_keep",
+    "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_attend_tree_workspace_bytes", "oq_kv_keep",
 )
 
 _lib = None
@@ -146,6 +146,8 @@ def load() -> ctypes.CDLL:
     lib.oq_kv_attend_tree.restype = c_int
     lib.oq_kv_attend_tree.argtypes = [vp, c_int, c_i64, c_i64, c_i64, c_i64, cache, vp, c_i64, c_i64, vp, vp, c_i64, vp, c_i64, c_i64, c_f, c_i64, c_i64,
                                       vp, vp, vp, c_u64, vp]
+    lib.oq_kv_attend_tree_workspace_bytes.restype = c_u64
+    lib.oq_kv_attend_tree_workspace_bytes.argtypes = [c_int] + [c_i64] * 7 + [c_int] + [c_i64] * 4
     lib.oq_kv_keep.restype = c_int
     lib.oq_kv_keep.argtypes = [vp, c_i64, vp, vp, vp, c_i64, c_i64, cache, c_i64, vp, c_i64, c_i64, vp, c_i64, vp, vp, vp, vp]
     _lib = lib
@@ -157,7 +159,7 @@ def load() -> ctypes.CDLL:
 def _bind(lib: ctypes.CDLL) -> None:
     names = ("oq_quantized_linear", "oq_quantized_linear_group", "oq_packed_linear_workspace_bytes", "oq_rotate_plan_bytes",
              "oq_matmul_packed_adaln_int4", "oq_kv_assign", "oq_kv_write", "oq_kv_read", "oq_kv_attend", "oq_kv_attend_workspace_bytes",
-             "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_keep")
+             "oq_qk_norm_rotary", "oq_kv_append", "oq_kv_tree", "oq_kv_attend_tree", "oq_kv_attend_tree_workspace_bytes", "oq_kv_keep")
     _torch_ops.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names})
 
 

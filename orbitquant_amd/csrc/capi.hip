@@ -732,11 +732,15 @@ int oq_kv_attend_tree(const void *q, int q_dtype, int64_t tokens, int64_t heads,
                 static_cast<int>(mask_words), window, scale, max_length, max_new, out, lse, workspace, workspace_bytes, stream);
 }
 
-uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
-                                      int64_t table_width, int64_t requests, int has_starts, int64_t window, int64_t max_length,
-                                      int64_t max_new) {
+namespace {
+uint64_t attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t table_width, int64_t requests,
+                                int has_starts, int q_dtype, int64_t mask_words, int64_t window, int64_t max_length, int64_t max_new) {
   static const int32_t some = 0;
+  static const uint64_t mask = 0;
   oq::KvAttendArgs a{};
+  a.q_dtype = q_dtype;
+  a.masks = mask_words > 0 ? &mask : nullptr;  // (as the starts)
+  a.mask_words = static_cast<int>(mask_words);
   a.cache.page_shift = page_shift_of(page_size);
   if (a.cache.page_shift < 0 || !known_head_dim(head_dim) || kv_heads < 1 || kv_heads > 65535) return 0;
   a.cache.heads = static_cast<int>(kv_heads);
@@ -744,6 +748,20 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
   a.starts = has_starts ? &some : nullptr;  // (asked whether it is there, not read)
   const uint64_t bytes = oq::kv_attend_plan(a, static_cast<int>(head_dim), max_length, most_queries(tokens, has_starts != 0, max_new), nullptr);
   return oq::kv_attend_fits(a, static_cast<int>(head_dim)) ? bytes : 0;
+}
+}  // namespace
+
+uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                      int64_t table_width, int64_t requests, int has_starts, int64_t window, int64_t max_length,
+                                      int64_t max_new) {
+  return attend_workspace_bytes(tokens, heads, kv_heads, head_dim, page_size, table_width, requests, has_starts, OQ_F32, 0, window, max_length, max_new);
+}
+
+uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                           int64_t table_width, int64_t requests, int has_starts, int64_t mask_words, int64_t window,
+                                           int64_t max_length, int64_t max_new) {
+  if (!known_dtype(q_dtype) || mask_words < 1 || mask_words > oq::kKvMaskWords) return 0;
+  return attend_workspace_bytes(tokens, heads, kv_heads, head_dim, page_size, table_width, requests, has_starts, q_dtype, mask_words, window, max_length, max_new);
 }
 
 // ---- norms and rotary positions ----

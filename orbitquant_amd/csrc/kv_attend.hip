@@ -32,6 +32,23 @@ constexpr int kFewWhole = 16, kFewWholeMost = 64, kFewGroups = 512, kFewSteps = 
 // and 43; with six these are as often slower).  512 queries behind 3584 tokens, 8 heads, 128 tiles: 117 -> 66 us.
 constexpr int kManyGroups = 512, kManyWhole = 16, kManyLeast = 8;
 
+constexpr int many_groups(int dim) { return dim == 256 ? kManyGroups / 2 : kManyGroups; }
+constexpr bool many_cut(int64_t tiles, int64_t heads, int dim) { return tiles * heads < many_groups(dim) * 3 / 4; }
+
+// Drafted tokens, whose rows of a request are a few hundred at most.  The kernel for few rows costs by sixteen of them, the other by 128, of which
+// ragged trees leave much unused: up to 128 rows of a request the first is faster however large the batch (64 requests of up to 26 drafts behind up to
+// 4000 tokens, 32 heads of 128 on 8, 188 -> 111 us; 16 behind up to 16384, 126 -> 108), and up to 256 where there is little work (60 drafts behind
+// a thousand tokens 37 -> 10.5, behind 16000 60 -> 46) or where rows are few on the average (16 requests of up to 40 drafts, 102 -> 86).  Above, it is the
+// second's where that is cut into even parts, heads of 256 excepted (16 of up to 60 behind 16384 tokens 202 -> 178; behind 8192, D = 256, 210 -> 295).
+constexpr int kTreeRows = 256, kTreeAlways = 128, kTreeAverage = 144;
+constexpr int64_t kTreeSmall = 1 << 16;  // steps of sixteen rows of a key head
+
+int tree_few_rows(const KvAttendArgs &a, int dim, int64_t widest, int64_t steps) {
+  const int64_t rows = a.tokens * a.group, heads = a.cache.heads, few = widest < 16 ? 16 : widest < kTreeRows ? (widest + 15) & ~15 : kTreeRows;
+  if (widest <= kTreeAlways || rows / 16 * steps * heads <= kTreeSmall || rows <= static_cast<int64_t>(kTreeAverage) * a.requests) return static_cast<int>(few);
+  return dim == 256 && !many_cut(kv_tile_base(rows, a.requests) + 1, heads, dim) ? static_cast<int>(few) : kKvFewRows;
+}
+
 constexpr int kJoinBlocks = 4;  // workgroups of a tile, at most
 
 // The parts of the tiles that a launch has cut: out = sum_p 2^(R_p) o_p / sum_p 2^(R_p) l_p, in the order of the keys.  TPR threads a row:
@@ -138,37 +155,42 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   const int heads = a.cache.heads;
   a.many_tiles = 0;
   a.few_rows = 0;
+  int64_t keys = static_cast<int64_t>(a.table_width) << a.cache.page_shift;
+  if (max_length >= 0 && max_length < keys) keys = max_length;
+  if (a.window != 0 && keys > a.window + max_new) keys = a.window + max_new + 63;
+  const int64_t steps = (keys + 63) / 64;
+  const int64_t widest = max_new * a.group;  // rows of a request, as the caller says
   if (a.starts == nullptr) {
     a.few_requests = a.requests;
     a.few_tiles = (a.group + 15) / 16;
     a.few_in_tile = a.group < 16 ? a.group : 16;
   } else {
     // A lone request's rows are known to be many, or few; of several, each may be either.
-    const bool many = rows > kKvFewRows, few = !many || a.requests > 1;
+    const int most = a.masks != nullptr ? tree_few_rows(a, dim, widest, steps) : kKvFewRows;
+    const bool many = rows > most, few = !many || a.requests > 1;
     if (many) a.many_tiles = static_cast<int>(kv_tile_base(rows, a.requests)) + 1;
     a.few_requests = few ? a.requests + 1 : 0;
-    a.few_tiles = static_cast<int>(((rows < kKvFewRows ? rows : kKvFewRows) + 15) / 16);
+    a.few_tiles = static_cast<int>(((rows < most ? rows : most) + 15) / 16);
     a.few_in_tile = rows < 16 ? static_cast<int>(rows) : 16;
-    a.few_rows = few ? kKvFewRows : 0;
+    a.few_rows = few ? most : 0;
   }
-  int64_t keys = static_cast<int64_t>(a.table_width) << a.cache.page_shift;
-  if (max_length >= 0 && max_length < keys) keys = max_length;
-  if (a.window != 0 && keys > a.window + max_new) keys = a.window + max_new + 63;
-  const int64_t steps = (keys + 63) / 64;
   a.few.target = a.many.target = 0;
   a.few.sorted = false;
   a.few.least = kFewLeast;
   a.many.least = kManyLeast;
+  // (a drafted step in fp32 costs twice as much: 13 drafts of 7 requests, a window of 1500, D = 256, 37 -> 30 us)
+  const int weight = a.masks != nullptr && a.q_dtype == OQ_F32 ? 2 : 1;
   const int64_t whole = static_cast<int64_t>(a.few_requests) * a.few_tiles * heads;
-  if (a.few_requests > 0 && steps > kFewWhole && (steps > kFewWholeMost || whole * 32 < (steps - kFewWhole) * dim)) {
+  if (a.few_requests > 0 && steps > kFewWhole && (steps > kFewWholeMost || whole * 32 < (steps - kFewWhole) * dim * weight)) {
     const int64_t parts = static_cast<int64_t>(a.requests) * steps * heads / kFewSteps;
     const int64_t groups = parts < kFewGroups ? kFewGroups : parts > 3 * kFewGroups ? 3 * kFewGroups : parts;
     a.few.sorted = groups > kFewGroups;
     a.few.target = groups > heads ? static_cast<int>(groups / heads) : 1;
   }
   a.few_alone = a.few_requests > 0 && a.few.target == 0 && steps <= kFewAlone && (steps <= 1 || whole > 128 * steps);
-  const int many_groups = dim == 256 ? kManyGroups / 2 : kManyGroups;
-  if (a.many_tiles > 0 && steps > kManyWhole && static_cast<int64_t>(a.many_tiles) * heads < many_groups * 3 / 4) a.many.target = heads < many_groups ? many_groups / heads : 1;
+  // (drafted requests of which none should be here are not cut: then nothing has to be joined, and the launch finds nothing)
+  const bool expected = a.masks == nullptr || widest > a.few_rows;
+  if (a.many_tiles > 0 && steps > kManyWhole && expected && many_cut(a.many_tiles, heads, dim)) a.many.target = heads < many_groups(dim) ? many_groups(dim) / heads : 1;
   const uint64_t bytes = kv_places(a.few, 2 * a.few.target, heads, 16, dim, static_cast<char *>(workspace), 0);
   return kv_places(a.many, a.many.target, heads, kKvManyRows, dim, static_cast<char *>(workspace), bytes);
 }

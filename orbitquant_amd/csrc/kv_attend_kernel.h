@@ -166,7 +166,7 @@ __device__ __forceinline__ bool kv_few_tile(const KvAttendArgs &a, int i, KvRows
   if (a.starts != nullptr) {
     r.start = kv_start_of(a, r.request);
     r.fresh = max(kv_start_of(a, r.request + 1) - r.start, 0);
-    if (static_cast<int64_t>(r.fresh) * a.group > kKvFewRows) return false;
+    if (static_cast<int64_t>(r.fresh) * a.group > a.few_rows) return false;
   }
   r.rows = min(r.fresh * a.group - r.first, 16);
   if (r.rows <= 0) return false;
@@ -983,6 +983,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
   }
   const KvRows r = part.rows;
   const KvSpan span = kv_span_of<TREE>(a, r, r.first, r.rows);
+  const int begin = TREE && kv_drafted(a, r) ? r.position(0) : 0x7fffffff;  // of what masks are about
   const int steps = span.highest >= span.lowest ? kv_steps_of(span) : 0;
   int step = (span.lowest >> 6) + part.from(steps, part.index) + wave;
   const int end = (span.lowest >> 6) + part.from(steps, part.index + 1);
@@ -1058,7 +1059,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attend_few_kernel(KvAttendAr
     const int first = step * 64;
     if (first + 63 > span.all_high || first < span.all_low || __builtin_amdgcn_ballot_w64(!here) != 0) {
       uint32_t bits = 0xffffu;
-      if constexpr (TREE) bits = kv_mask_bits(masks[wave], n, r.position(0), first + 16 * g);
+      if constexpr (TREE) bits = kv_mask_bits(masks[wave], n, begin, first + 16 * g);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = first + 16 * g + i;

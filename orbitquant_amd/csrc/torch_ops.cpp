@@ -38,6 +38,7 @@ struct Library {
   decltype(&oq_kv_append) kv_append = nullptr;
   decltype(&oq_kv_tree) kv_tree = nullptr;
   decltype(&oq_kv_attend_tree) kv_attend_tree = nullptr;
+  decltype(&oq_kv_attend_tree_workspace_bytes) kv_attend_tree_workspace_bytes = nullptr;
   decltype(&oq_kv_keep) kv_keep = nullptr;
 } lib;
 
@@ -392,15 +393,17 @@ pybind11::object kv_attend(const Tensor &q, const pybind11::object &cache, const
   try {
     const Tensor out = at::empty(q.sizes(), q.options());
     const Tensor lse = want_lse ? at::empty({tokens, heads}, q.options().dtype(at::kFloat)) : Tensor();
-    const uint64_t need = lib.kv_attend_workspace_bytes(tokens, heads, c.kv_heads, c.head_dim, c.page_size, table.size(1), requests, present(starts), window,
-                                                        max_length, max_new);
+    const int type = dtype_code(q.scalar_type());
+    const uint64_t need = present(masks) ? lib.kv_attend_tree_workspace_bytes(type, tokens, heads, c.kv_heads, c.head_dim, c.page_size, table.size(1), requests,
+                                                                              present(starts), masks->size(1), window, max_length, max_new)
+                                         : lib.kv_attend_workspace_bytes(tokens, heads, c.kv_heads, c.head_dim, c.page_size, table.size(1), requests,
+                                                                         present(starts), window, max_length, max_new);
     const Tensor workspace = need > 0 ? bytes_like(q, static_cast<int64_t>(need)) : Tensor();
     if (faked(out)) return pybind11::none();
     const int32_t *const pages = static_cast<const int32_t *>(data(table)), *const held = static_cast<const int32_t *>(data(lengths)),
                   *const begin = static_cast<const int32_t *>(data(starts));
     float *const sums = want_lse ? static_cast<float *>(data(lse)) : nullptr;
     void *const room = need > 0 ? data(workspace) : nullptr;
-    const int type = dtype_code(q.scalar_type());
     const int rc = present(masks) ? lib.kv_attend_tree(data(q), type, tokens, heads, q.stride(0), q.stride(1), &c, pages, table.stride(0), table.size(1), held, begin,
                                                        requests, static_cast<const uint64_t *>(data(masks)), masks->size(1), window, static_cast<float>(scale),
                                                        max_length, max_new, data(out), sums, room, need, stream_of(device))
@@ -562,6 +565,7 @@ PYBIND11_MODULE(_torch_ops, m) {
     bind_one(lib.kv_append, addresses, "oq_kv_append");
     bind_one(lib.kv_tree, addresses, "oq_kv_tree");
     bind_one(lib.kv_attend_tree, addresses, "oq_kv_attend_tree");
+    bind_one(lib.kv_attend_tree_workspace_bytes, addresses, "oq_kv_attend_tree_workspace_bytes");
     bind_one(lib.kv_keep, addresses, "oq_kv_keep");
   });
   m.def("quantized_linear_group", quantized_linear_group);

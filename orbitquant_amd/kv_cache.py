@@ -409,8 +409,11 @@ def kv_attend(q: torch.Tensor, cache: OrbitKVCache, block_table: torch.Tensor, l
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
     lib = _lib.load()
-    needed = lib.oq_kv_attend_workspace_bytes(tokens, heads, struct.kv_heads, dim, struct.page_size, table.shape[1], requests, starts is not None,
-                                              window, max_length, max_new)
+    shape = (tokens, heads, struct.kv_heads, dim, struct.page_size, table.shape[1], requests, starts is not None)
+    if masks is None:
+        needed = lib.oq_kv_attend_workspace_bytes(*shape, window, max_length, max_new)
+    else:
+        needed = lib.oq_kv_attend_tree_workspace_bytes(_dt(q), *shape, masks.shape[1], window, max_length, max_new)
     workspace, nbytes, _keep = _workspace(needed, q, lambda: (0,))
     which, seen = (lib.oq_kv_attend, (bool(causal),)) if masks is None else (lib.oq_kv_attend_tree, (masks.data_ptr(), masks.shape[1]))
     with _OnDevice(q):

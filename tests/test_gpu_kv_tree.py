@@ -156,7 +156,8 @@ def test_attend_masks_long(dim, page, dtype, window):
 
 
 def test_a_chain_is_causal_attention():
-    """Masks of chains give what no masks give, bit for bit: the same keys in the same order."""
+    """Masks of chains see what no masks see.  (Not bit for bit: the two may be launched otherwise, and then add up in another order.  So both are held
+    to the bound of the same definition.)"""
     from orbitquant_amd import kv_attend, kv_tree
 
     rng = np.random.RandomState(8)
@@ -167,9 +168,10 @@ def test_a_chain_is_causal_attention():
     tree = kv_tree(_i32(_parents(rng, new, "chain")), _i32(starts), _i32(lengths), max_new=200)
     positions = np.concatenate([np.arange(b, b + n) for b, n in zip(before, new)])
     assert tree.positions.tolist() == positions.tolist()
-    for a, b in zip(kv_attend(q, cache, table, _i32(lengths), starts=_i32(starts), masks=tree.masks, return_lse=True),
-                    kv_attend(q, cache, table, _i32(lengths), starts=_i32(starts), return_lse=True)):
-        assert torch.equal(a, b)
+    masks = oracle.tree(_parents(rng, new, "chain"), starts, lengths, 4, starts[-1])[1]
+    for got in (kv_attend(q, cache, table, _i32(lengths), starts=_i32(starts), masks=tree.masks, return_lse=True),
+                kv_attend(q, cache, table, _i32(lengths), starts=_i32(starts), return_lse=True)):
+        _check(got, q, cache, table, lengths, starts, masks)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
