@@ -807,10 +807,11 @@ int qk_side_of(const char *what, const void *x, int64_t token_stride, int64_t he
   if (tokens > 0 && (x == nullptr || out == nullptr)) return fail(OQ_ERR_INVALID, "%s: null pointer", what);
   if (!aligned(out, 16)) return fail(OQ_ERR_INVALID, "%s: the outputs are not aligned to 16 bytes", what);
   side.x = x; side.out = out; side.token_stride = token_stride; side.head_stride = head_stride;
-  side.heads = static_cast<int>(heads); side.groups = (side.heads + oq::kQkHeads - 1) / oq::kQkHeads;
+  side.heads = static_cast<int>(heads); side.each = tokens * heads <= oq::kQkAlone ? 1 : oq::kQkHeads;
+  side.groups = (side.heads + side.each - 1) / side.each;
   side.magic = static_cast<uint32_t>(((1ull << 32) + side.groups - 1) / side.groups);
   qk_fit_piece(how, x, token_stride, head_stride, dtype);
-  const int64_t count = oq::qk_blocks(tokens, side.heads, static_cast<int>(dim), threads);
+  const int64_t count = oq::qk_blocks(tokens, side.groups, static_cast<int>(dim), threads);
   if (count > oq::kKvMostThreads / threads / 2) return fail(OQ_ERR_UNSUPPORTED, "%s: tokens=%lld heads=%lld exceed the grid", what, (long long)tokens, (long long)heads);
   blocks = static_cast<uint32_t>(count);
   return OQ_OK;

@@ -39,14 +39,14 @@ constexpr bool many_cut(int64_t tiles, int64_t heads, int dim) { return tiles * 
 // ragged trees leave much unused: up to 128 rows of a request the first is faster however large the batch (64 requests of up to 26 drafts behind up to
 // 4000 tokens, 32 heads of 128 on 8, 188 -> 111 us; 16 behind up to 16384, 126 -> 108), and up to 256 where there is little work (60 drafts behind
 // a thousand tokens 37 -> 10.5, behind 16000 60 -> 46) or where rows are few on the average (16 requests of up to 40 drafts, 102 -> 86).  Above, it is the
-// second's where that is cut into even parts, heads of 256 excepted (16 of up to 60 behind 16384 tokens 202 -> 178; behind 8192, D = 256, 210 -> 295).
+// second's, few rows and many, where that is cut into even parts, heads of 256 excepted (16 of up to 60 behind 16384 tokens 202 -> 178; behind 8192, D = 256, 210 -> 295).
 constexpr int kTreeRows = 256, kTreeAlways = 128, kTreeAverage = 144;
 constexpr int64_t kTreeSmall = 1 << 16;  // steps of sixteen rows of a key head
 
 int tree_few_rows(const KvAttendArgs &a, int dim, int64_t widest, int64_t steps) {
   const int64_t rows = a.tokens * a.group, heads = a.cache.heads, few = widest < 16 ? 16 : widest < kTreeRows ? (widest + 15) & ~15 : kTreeRows;
   if (widest <= kTreeAlways || rows / 16 * steps * heads <= kTreeSmall || rows <= static_cast<int64_t>(kTreeAverage) * a.requests) return static_cast<int>(few);
-  return dim == 256 && !many_cut(kv_tile_base(rows, a.requests) + 1, heads, dim) ? static_cast<int>(few) : kKvFewRows;
+  return dim == 256 && !many_cut(kv_tile_base(rows, a.requests) + 1, heads, dim) ? static_cast<int>(few) : 0;
 }
 
 constexpr int kJoinBlocks = 4;  // workgroups of a tile, at most
@@ -167,7 +167,7 @@ uint64_t kv_attend_plan(KvAttendArgs &a, int dim, int64_t max_length, int64_t ma
   } else {
     // A lone request's rows are known to be many, or few; of several, each may be either.
     const int most = a.masks != nullptr ? tree_few_rows(a, dim, widest, steps) : kKvFewRows;
-    const bool many = rows > most, few = !many || a.requests > 1;
+    const bool many = rows > most, few = !many || (a.requests > 1 && most > 0);
     if (many) a.many_tiles = static_cast<int>(kv_tile_base(rows, a.requests)) + 1;
     a.few_requests = few ? a.requests + 1 : 0;
     a.few_tiles = static_cast<int>(((rows < most ? rows : most) + 15) / 16);

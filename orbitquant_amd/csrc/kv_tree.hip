@@ -14,8 +14,8 @@ __device__ __forceinline__ int start_of(const int32_t *starts, int64_t tokens, i
 // Bound by latency: three loads one behind the other, and log2(nodes) rounds in LDS.
 template <int WORDS>
 __global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
-  __shared__ uint64_t masks[64 * WORDS][WORDS];
-  __shared__ int up[64 * WORDS];
+  __shared__ uint64_t masks[2][64 * WORDS][WORDS];  // (a round writes one and reads it, the next the other: one barrier a round)
+  __shared__ int up[2][64 * WORDS];
   const int r = blockIdx.x, i = threadIdx.x;
   const int first = start_of(a.starts, a.tokens, r);
   if (r == a.requests) {
@@ -41,17 +41,16 @@ __global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
   for (int w = 0; w < WORDS; ++w) mask[w] = i >> 6 == w ? 1ull << (i & 63) : 0;
   int ancestor = i < count ? a.parents[first + i] : -1;
   if (ancestor >= i) ancestor = -1;
-  for (int reach = 1; reach < count; reach *= 2) {
+  for (int reach = 1, now = 0; reach < count; reach *= 2, now ^= 1) {
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w) masks[i][w] = mask[w];
-    up[i] = ancestor;
+    for (int w = 0; w < WORDS; ++w) masks[now][i][w] = mask[w];
+    up[now][i] = ancestor;
     __syncthreads();
     if (ancestor >= 0) {
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) mask[w] |= masks[ancestor][w];
-      ancestor = up[ancestor];
+      for (int w = 0; w < WORDS; ++w) mask[w] |= masks[now][ancestor][w];
+      ancestor = up[now][ancestor];
     }
-    __syncthreads();
   }
   if (i >= count) return;
   int depth = 0;
@@ -85,26 +84,52 @@ __device__ __forceinline__ int64_t slot_at(const KvKeepArgs &a, int64_t token) {
   return slot < a.pages << a.page_shift ? slot : -1;
 }
 
+// How many entries of a request's list count.  Eight at a time, whose loads do not wait for each other.
+__device__ __forceinline__ int kept_of(const KvKeepArgs &a, int r, const Path &path) {
+  int last = -1;
+  for (int base = 0; base < a.most; base += kKeepBatch) {
+    int k[kKeepBatch];
+    int64_t slot[kKeepBatch];
+#pragma unroll
+    for (int b = 0; b < kKeepBatch; ++b) k[b] = base + b < a.most ? a.kept[static_cast<int64_t>(r) * a.most + base + b] : -1;
+#pragma unroll
+    for (int b = 0; b < kKeepBatch; ++b) slot[b] = k[b] >= 0 && k[b] < path.fresh ? slot_at(a, static_cast<int64_t>(path.first) + k[b]) : -1;
+#pragma unroll
+    for (int b = 0; b < kKeepBatch; ++b) {
+      if (k[b] <= last || slot[b] < 0) return base + b;
+      last = k[b];
+    }
+  }
+  return a.most;
+}
+
 // Lengths, and the pages behind them onto the free list again, in front of those that it gives out next, in request order.
 __device__ void keep_counts(const KvKeepArgs &a) {
   __shared__ int wave_sums[kKeepThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.requests + kKeepThreads - 1) / kKeepThreads, from = min(tid * run, a.requests), to = min(from + run, a.requests);
+  const int taken = a.table != nullptr ? min(max(*a.taken, 0), a.free_count) : 0;
   const auto pages_of = [&](int tokens) { return static_cast<int>(min((static_cast<int64_t>(max(tokens, 0)) + (1 << a.page_shift) - 1) >> a.page_shift, static_cast<int64_t>(a.table_width))); };
+  // each(page) for a request's pages from `column` on, four of them requested at once
+  const auto over_pages = [&](int r, int column, int end, const auto &each) {
+    const int32_t *const row = a.table + r * a.table_stride;
+    for (; column < end; column += 4) {
+      int page[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) page[c] = column + c < end ? row[column + c] : -1;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (page[c] >= 0) each(page[c]);
+      }
+    }
+  };
   int own = 0;
   for (int r = from; r < to; ++r) {
+    const int length = max(a.lengths[r], 0);
     const Path path = path_of(a, r);
-    int count = 0, last = -1;
-    for (int i = 0; i < a.most; ++i) {
-      const int k = a.kept[static_cast<int64_t>(r) * a.most + i];
-      if (k <= last || k >= path.fresh || slot_at(a, path.first + k) < 0) break;
-      last = k;
-      ++count;
-    }
-    const int length = max(a.lengths[r], 0), kept = max(length - path.fresh, 0) + count;
+    const int kept = max(length - path.fresh, 0) + kept_of(a, r, path);
     a.lengths_after[r] = kept;
-    if (a.table == nullptr) continue;
-    for (int column = pages_of(kept); column < pages_of(length); ++column) own += a.table[r * a.table_stride + column] >= 0 ? 1 : 0;
+    if (a.table != nullptr) over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
   }
   if (a.table == nullptr) return;
   const int sum = kv_sums(own);
@@ -116,33 +141,32 @@ __device__ void keep_counts(const KvKeepArgs &a) {
     ahead += w < wave ? wave_sums[w] : 0;
     all += wave_sums[w];
   }
-  const int taken = min(max(*a.taken, 0), a.free_count), begin = taken - all;
+  const int begin = taken - all;
   if (tid == 0) *a.taken_after = max(begin, 0);
   if (own == 0) return;
   int at = begin + ahead;
   for (int r = from; r < to; ++r) {
-    const int kept = a.lengths_after[r];  // (this thread's own)
-    for (int column = pages_of(kept); column < pages_of(max(a.lengths[r], 0)); ++column) {
-      const int page = a.table[r * a.table_stride + column];
-      if (page < 0) continue;
+    over_pages(r, pages_of(a.lengths_after[r]) /* this thread's own */, pages_of(a.lengths[r]), [&](int page) {
       if (at >= 0) a.free_pages[at] = page;
       ++at;
-    }
+    });
   }
 }
 
 template <int D>
 __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepArgs a) {
   const int counting = a.counts ? 1 : 0;
-  if (blockIdx.x < counting) {
+  if (static_cast<int>(blockIdx.x) < counting) {
     keep_counts(a);
     return;
   }
   const int lane = threadIdx.x & 63;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x - counting) * (kKeepThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (unit >= static_cast<int64_t>(a.requests) * a.heads * a.caches) return;
-  const int head = static_cast<int>(unit % a.heads), rest = static_cast<int>(unit / a.heads), r = rest % a.requests;
-  const auto &cache = a.cache[rest / a.requests];
+  // (a launch has fewer than 2^26 of these: 2^32 threads)
+  const uint32_t unit = (blockIdx.x - counting) * (kKeepThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t rest = unit / static_cast<uint32_t>(a.heads), layer = rest / static_cast<uint32_t>(a.requests);
+  if (layer >= static_cast<uint32_t>(a.caches)) return;
+  const int head = static_cast<int>(unit - rest * a.heads), r = static_cast<int>(rest - layer * a.requests);
+  const auto &cache = a.cache[layer];
   const Path path = path_of(a, r);
   const int shift = a.page_shift, in_page = (1 << shift) - 1;
   int before = -1;  // the last entry of the lanes' batch before

@@ -34,11 +34,14 @@ struct QkSide {  // queries, or keys
   const void *x;
   void *out;                   // [tokens, heads, D]
   int64_t token_stride, head_stride;
-  int heads, groups;           // groups of kQkHeads heads
+  int heads, groups, each;     // groups of `each` heads: kQkHeads or 1
   uint32_t magic;              // of a division by `groups`: ceil(2^32 / groups)
 };
 
-constexpr int kQkHeads = 4;    // of a token a lane, which share its entries of the tables and the weights
+// Heads of a token that a lane takes, which share its entries of the tables and the weights; where there are few, one: what a wavefront then waits
+// for is its own instructions (one token, 32 heads and 8, 5.2 -> 3.1 us; 1024 tokens are as fast either way).
+constexpr int kQkHeads = 4;
+constexpr int64_t kQkAlone = 1 << 14;  // heads of all tokens
 
 template <int L>
 __device__ __forceinline__ int qk_part_of(int lane) {
@@ -258,32 +261,38 @@ __device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, 
 }
 
 // Workgroup `block` of a side: HEADS heads of a token for every L lanes.
-template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS>
-__device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
+template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS, int HEADS>
+__device__ __forceinline__ void qk_heads_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
   constexpr int UNITS = THREADS / L;
   const int lane = threadIdx.x & 63, part = qk_part_of<L>(lane);
   const uint32_t first = block * UNITS, local = (threadIdx.x >> 6) * (64 / L) + qk_vector_of<L>(lane);
   const uint32_t groups = side.groups, row = first / groups, n = first - row * groups + local;  // (n < groups + 256: the product by the reciprocal is exact)
   const uint32_t down = groups == 1 ? n : __umulhi(n, side.magic);
   const int64_t token = static_cast<int64_t>(row) + down;
-  const int head = static_cast<int>(n - down * groups) * kQkHeads;
+  const int head = static_cast<int>(n - down * groups) * HEADS;
   if (token >= tokens) return;  // (all of a unit's lanes)
-  QkRaw<DT, PIECE, INTERLEAVED> raw[kQkHeads];
+  QkRaw<DT, PIECE, INTERLEAVED> raw[HEADS];
   float wa[8], wb[8];
   QkTurn turn;
   const int64_t position = turn.row_of(how, token), at = token * side.token_stride;
 #pragma unroll
-  for (int h = 0; h < kQkHeads; ++h) raw[h].request(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how);
+  for (int h = 0; h < HEADS; ++h) raw[h].request(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how);
   turn.load(how, position, part);
   qk_load_weight<PIECE, INTERLEAVED>(how, which, part, dim, wa, wb);
 #pragma unroll
-  for (int h = 0; h < kQkHeads; ++h) {
+  for (int h = 0; h < HEADS; ++h) {
     if (h > 0 && head + h >= side.heads) break;
     float a[8], b[8];
     raw[h].pairs(a, b);
     qk_apply<L>(how, wa, wb, turn, a, b);
     qk_store_pairs<DT, PIECE, INTERLEAVED>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
   }
+}
+
+template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS>
+__device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
+  if (side.each == 1) qk_heads_block<DT, L, PIECE, INTERLEAVED, THREADS, 1>(how, side, which, tokens, dim, block);
+  else qk_heads_block<DT, L, PIECE, INTERLEAVED, THREADS, kQkHeads>(how, side, which, tokens, dim, block);
 }
 
 }  // namespace oq

@@ -29,9 +29,9 @@ constexpr int qk_lanes(int dim) {
   while (16 * lanes < dim) lanes *= 2;
   return lanes;
 }
-inline int64_t qk_blocks(int64_t tokens, int heads, int dim, int threads) {
+inline int64_t qk_blocks(int64_t tokens, int groups, int dim, int threads) {
   const int64_t units = threads / qk_lanes(dim);
-  return (tokens * ((heads + kQkHeads - 1) / kQkHeads) + units - 1) / units;
+  return (tokens * groups + units - 1) / units;
 }
 
 int qk_norm_rotary_dispatch(const QkArgs &a, int dtype, hipStream_t stream);

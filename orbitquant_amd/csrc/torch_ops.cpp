@@ -466,8 +466,20 @@ pybind11::object qk_norm_rotary(const Tensor &q, const Tensor &k, const OptTenso
       !plan_of(q, cos, sin, q_weight, k_weight, eps, interleaved, positions, p))
     return pybind11::none();
   const c10::OptionalDeviceGuard guard(q.device());
-  const Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
-  if (faked(q_out) || faked(k_out)) return pybind11::none();
+  // Small results share one allocation, a microsecond less; large ones can be freed by themselves.
+  constexpr int64_t kShared = 1 << 18;
+  const int64_t q_bytes = (static_cast<int64_t>(q.numel() * q.element_size()) + 15) & ~int64_t{15}, bytes = q_bytes + static_cast<int64_t>(k.numel() * k.element_size());
+  Tensor q_out, k_out;
+  if (bytes <= kShared) {
+    const Tensor both = bytes_like(q, bytes);
+    if (faked(both)) return pybind11::none();
+    q_out = part_of(both, q.scalar_type(), 0, q.sizes());
+    k_out = part_of(both, q.scalar_type(), q_bytes, k.sizes());
+  } else {
+    q_out = at::empty(q.sizes(), q.options());
+    k_out = at::empty(k.sizes(), k.options());
+    if (faked(q_out) || faked(k_out)) return pybind11::none();
+  }
   const int rc = lib.qk_norm_rotary(data(q), q.stride(0), q.stride(1), q.size(1), data(k), k.stride(0), k.stride(1), k.size(1), dtype_code(q.scalar_type()),
                                     q.size(0), q.size(2), &p, data(q_out), data(k_out), stream_of(q.device()));
   return rc == OQ_OK ? pybind11::object(pybind11::make_tuple(q_out, k_out)) : pybind11::object(pybind11::none());
@@ -503,8 +515,9 @@ pybind11::object kv_tree(const Tensor &parents, const Tensor &starts, const Tens
       !dense(starts, device, at::kInt) || starts.numel() != requests + 1)
     return pybind11::none();
   const c10::OptionalDeviceGuard guard(device);
-  const Tensor positions = at::empty({tokens}, parents.options()), masks = at::empty({tokens, words}, parents.options().dtype(at::kLong));
-  if (faked(positions) || faked(masks)) return pybind11::none();
+  const Tensor both = bytes_like(parents, (8 * words + 4) * tokens);
+  if (faked(both)) return pybind11::none();
+  const Tensor masks = part_of(both, at::kLong, 0, {tokens, words}), positions = part_of(both, at::kInt, 8 * words * tokens, {tokens});
   const int rc = lib.kv_tree(static_cast<const int32_t *>(data(parents)), static_cast<const int32_t *>(data(starts)), static_cast<const int32_t *>(data(lengths)),
                              requests, tokens, words, static_cast<int32_t *>(data(positions)), static_cast<uint64_t *>(data(masks)), stream_of(device));
   return rc == OQ_OK ? pybind11::object(pybind11::make_tuple(positions, masks)) : pybind11::object(pybind11::none());

@@ -39,7 +39,7 @@ def linear(inputs: int, outputs: int, generator: torch.Generator, device) -> Orb
 
 
 class Layer(nn.Module):
-    def __init__(self, pages: int, generator: torch.Generator, device) -> None:
+    def __init__(self, pages: int, generator: torch.Generator, device, rotary) -> None:
         super().__init__()
         cache = OrbitKVCache.empty(pages, KV_HEADS, HEAD_DIM, page_size=PAGE, device=device)
         wide, kv = HEADS * HEAD_DIM, KV_HEADS * HEAD_DIM
@@ -54,13 +54,13 @@ class Layer(nn.Module):
 
 
 class Decoder(nn.Module):
-    """`requests` rows of a block table over a pool of pages, and the tokens that they hold."""
+    """`requests` rows of a block table over a pool of pages, and the tokens that they hold.  `rotary`: as OrbitCachedAttention takes it."""
 
-    def __init__(self, layers: int, requests: int, longest: int, device="cuda", seed: int = 0) -> None:
+    def __init__(self, layers: int, requests: int, longest: int, device="cuda", seed: int = 0, rotary=rotary) -> None:
         super().__init__()
         generator = torch.Generator(device=device).manual_seed(seed)
         width = -(-longest // PAGE)
-        self.layers = nn.ModuleList(Layer(requests * width, generator, device) for _ in range(layers))
+        self.layers = nn.ModuleList(Layer(requests * width, generator, device, rotary) for _ in range(layers))
         self.head = linear(HIDDEN, VOCABULARY, generator, device)
         self.embedding = torch.randn(VOCABULARY, HIDDEN, generator=generator, device=device).to(torch.bfloat16)
         counts = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=device)  # noqa: E731

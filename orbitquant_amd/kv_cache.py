@@ -174,7 +174,7 @@ def _append_op(q, k, v, slots, k_codes, k_scales, v_codes, v_scales, signs, cos,
 
 
 def _tree_op(parents, starts, lengths, words):
-    return tuple(kv_tree(parents, starts, lengths, max_new=64 * words))
+    return tuple(_tree(parents, starts, lengths, words))   # (an op's outputs may not share memory)
 
 
 def _tree_fake(parents, starts, lengths, words):
@@ -445,6 +445,10 @@ def kv_tree(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, 
         got = module.kv_tree(parents, starts, lengths, words)
         if got is not None:
             return KVTree._make(got)
+    return _tree(parents, starts, lengths, words)
+
+
+def _tree(parents, starts, lengths, words) -> KVTree:
     _require_gpu(parents, "parents")
     if parents.ndim != 1:
         raise ValueError(f"parents must be [tokens], got {list(parents.shape)}")

@@ -42,7 +42,7 @@ _LIB.define(f"qk_norm_rotary(Tensor q, Tensor k, {_HOW}, Tensor? positions) -> (
 
 
 def _op(q, k, cos, sin, q_weight, k_weight, eps, interleaved, positions):
-    return qk_norm_rotary(q, k, QKNormRotary(cos, sin, q_weight, k_weight, eps, interleaved), positions)
+    return _general(q, k, QKNormRotary(cos, sin, q_weight, k_weight, eps, interleaved), positions)   # (an op's outputs may not share memory)
 
 
 _LIB.impl("qk_norm_rotary", _op, "CUDA")
@@ -113,6 +113,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, how: QKNormRotary, position
         got = module.qk_norm_rotary(q, k, *how, positions)
         if got is not None:
             return got
+    return _general(q, k, how, positions)
+
+
+def _general(q, k, how, positions):
     _require_gpu(q, "q")
     if q.ndim != 3:
         raise ValueError(f"q must be [tokens, heads, D], got {list(q.shape)}")
