@@ -67,14 +67,16 @@ __device__ __forceinline__ void join_tile(const KvAttendArgs &a, int block, int 
   const KvCut &cut = MANY ? a.many : a.few;
   const int in_block = threadIdx.x / TPR, t = threadIdx.x % TPR, set = t / (D / 4), d = t % (D / 4);
   const int in_launch = block / blocks;
-  const int kv_head = in_launch % a.cache.heads, first = in_launch / a.cache.heads;
+  // Every part has `blocks` workgroups, and all of a tile's share its rows: a tile of many parts has a long way to go for each row.
+  const int kv_head = in_launch % a.cache.heads, place_of_part = in_launch / a.cache.heads;
   const int2 *maps = cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1);
-  if (first >= maps[cut.places].x) return;  // (the same for the block, as is what follows)
-  const int2 map = maps[first];
-  if (map.x < 0) return;
+  if (place_of_part >= maps[cut.places].x) return;  // (the same for the block, as is what follows)
+  const int2 own = maps[place_of_part];
+  const int part = own.x < 0 ? -own.x : 0, first = place_of_part - part;
+  const int2 map = part == 0 ? own : maps[first];
   KvRows r;
   if (!kv_tile<MANY>(a, map.x, r)) return;
-  for (int from = block % blocks * ROWS; from < r.rows; from += blocks * ROWS) {
+  for (int from = (part * blocks + block % blocks) * ROWS; from < r.rows; from += map.y * blocks * ROWS) {
     const int in_tile = from + in_block;
     const bool there = in_tile < r.rows;
     float best = kKvNothing, l = 0.0f;

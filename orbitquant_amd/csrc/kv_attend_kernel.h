@@ -343,7 +343,7 @@ __device__ __forceinline__ KvRows kv_uniform(const KvRows &r) {
   return {kv_uniform(r.request), kv_uniform(r.start), kv_uniform(r.fresh), kv_uniform(r.length), kv_uniform(r.first), kv_uniform(r.rows), kv_uniform(r.last_key)};
 }
 __device__ __forceinline__ int2 *kv_map_of(const KvCut &cut, int kv_head) { return cut.map + static_cast<int64_t>(kv_head) * (cut.places + 1); }
-__device__ __forceinline__ int2 kv_map_entry(const KvPart &part) { return part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-1, 0); }
+__device__ __forceinline__ int2 kv_map_entry(const KvPart &part) { return part.index == 0 ? make_int2(part.tile, part.count) : make_int2(-part.index, 0); }
 
 template <int THREADS, bool TREE>
 __device__ __forceinline__ bool kv_few_part(const KvAttendArgs &a, int tiles, const KvCut &cut, int kv_head, int group, KvPart &part) {

@@ -39,7 +39,7 @@ struct KvCut {
   int places;         // for the parts of tiles that are cut: of few rows 2 * target (a tile of n > 1 parts has more than (n - 1) * longest steps), of many target
   float *out;         // [key heads, places, rows of a tile, D]
   float2 *stats;      // [key heads, places, rows of a tile]: R and l
-  int2 *map;          // [key heads, places + 1]: of a tile's first part, the tile and the number of its parts, (-1, 0) of the others; and their number
+  int2 *map;          // [key heads, places + 1]: of a tile's first part, the tile and the number of its parts, of the others (minus how many are before them, 0); and their number
 };
 
 struct KvAttendArgs {
