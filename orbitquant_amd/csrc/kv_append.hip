@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppend
   __shared__ uint32_t bytes[kKvGroup][D / 8 + 1];
   __shared__ __attribute__((aligned(16))) float turned[LAYOUT == THROUGH_LDS ? kKvGroup : 1][LAYOUT == THROUGH_LDS ? D + 4 : 1];
   if (blockIdx.x >= a.kv_blocks) {
-    qk_block<DT, L, PIECE, LAYOUT == IN_A_ROW, THREADS>(a.how, a.q, 0, a.write.tokens, D, blockIdx.x - a.kv_blocks);
+    qk_block<DT, L, qk_form(LAYOUT == IN_A_ROW, L, PIECE), PIECE, THREADS>(a.how, a.q, 0, a.write.tokens, D, blockIdx.x - a.kv_blocks);
     return;
   }
   const KvWriteArgs &w = a.write;
@@ -46,14 +46,15 @@ __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppend
     } else {
       const int64_t at = token * w.k_token_stride + head * w.k_head_stride;
       float u[8], v[8], wu[8], wv[8];
-      QkTurn turn;
+      constexpr int FORM = LAYOUT == IN_A_ROW ? QK_NEIGHBOURS : QK_HALVES, STRIPE = qk_stripe(DT);
+      QkTurn<L, FORM, STRIPE> turn;
       const int64_t position = turn.row_of(a.how, token);
-      QkRaw<DT, PIECE, LAYOUT == IN_A_ROW> raw;
+      QkRaw<DT, L, FORM, PIECE, STRIPE> raw;
       raw.request(w.k, at, part, D, a.how);
       turn.load(a.how, position, part);
-      qk_load_weight<PIECE, LAYOUT == IN_A_ROW>(a.how, 1, part, D, wu, wv);
+      qk_load_weight<L, FORM, PIECE, STRIPE>(a.how, 1, part, D, wu, wv);
       raw.pairs(u, v);
-      qk_apply<L>(a.how, wu, wv, turn, u, v);
+      qk_apply(a.how, wu, wv, turn, u, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[p][LAYOUT == IN_A_ROW ? 2 * i : i] = u[i];

@@ -8,8 +8,10 @@
 // way into the 4-bit cache, when it becomes a code).  s is added up in one order everywhere: the two squares of a pair, then pairs 4, 2, 1
 // apart of each eight, then eights 1, 2, 4, ... apart, zeros behind the last pair.  So a key's codes do not depend on the launch that made them.
 //
-// A lane holds eight pairs, `L` = 1, 2, 4, ... 32 lanes a head: both halves of every pair are in one lane, the rotation needs no other, and
-// the sums need log2(L) exchanges.
+// A lane holds eight pairs, `L` = 1, 2, 4, ... 32 lanes a head: both values of every pair are in one lane, the rotation needs no other, and
+// the sums need log2(L) exchanges.  Bound by memory: 32760 tokens, 40 heads of 128 for queries and keys each, bf16, 1.36 GB, 252 us (halves; neighbours 260),
+// 5.4 TB/s, where a copy of the library reaches 5.2; few tokens by latency, 3.1 us for one.  (Converted as they were fetched, head by head, 344 us; four heads a
+// lane 264.)
 #pragma once
 
 #include "kv_rows.h"
@@ -40,7 +42,7 @@ struct QkSide {  // queries, or keys
 
 // Heads of a token that a lane takes, which share its entries of the tables and the weights; where there are few, one: what a wavefront then waits
 // for is its own instructions (one token, 32 heads and 8, 5.2 -> 3.1 us; 1024 tokens are as fast either way).
-constexpr int kQkHeads = 4;
+constexpr int kQkHeads = 2;
 constexpr int64_t kQkAlone = 1 << 14;  // heads of all tokens
 
 template <int L>
@@ -54,32 +56,67 @@ __device__ __forceinline__ int qk_vector_of(int lane) {
   else return kv_vector_of<8 * L>(lane);
 }
 
-template <int X>
-__device__ __forceinline__ float qk_swap_sum(float x) {
-  const kv_u32x2 both = kv_swap<X>(__float_as_uint(x), __float_as_uint(x));
-  return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+// Which of a head's pairs a lane has (its part of L), and how they are fetched.
+//   QK_HALVES      eight in a row, whose first and whose second values lie in a row
+//   QK_NEIGHBOURS  eight in a row, sixteen values in a row
+//   QK_STRIPES     the same pairs dealt out to the lanes sixteen bytes at a time, so that what all lanes fetch or store at once lies in a row (sixteen values a
+//                  lane in a row: as many bytes in fp32 326 us instead of 258)
+enum QkForm { QK_HALVES, QK_NEIGHBOURS, QK_STRIPES };
+constexpr int qk_form(bool interleaved, int lanes, int piece) { return !interleaved ? QK_HALVES : lanes >= 4 && piece == 8 ? QK_STRIPES : QK_NEIGHBOURS; }
+constexpr int qk_stripe(int dt) { return dt == OQ_F32 ? 4 : 8; }  // values
+
+// The i-th pair of a lane; STRIPE: values of a stripe.
+template <int L, int FORM, int STRIPE>
+__device__ __forceinline__ int qk_pair_of(int part, int i) {
+  if constexpr (FORM == QK_STRIPES) return STRIPE / 2 * (L * (i / (STRIPE / 2)) + part) + i % (STRIPE / 2);
+  else return 8 * part + i;
 }
-template <int CTRL>
-__device__ __forceinline__ float qk_dpp_sum(float x) { return x + __uint_as_float(kv_dpp<CTRL>(__float_as_uint(x))); }
+
+// Plus what the lane has whose part differs in bit BIT.
+template <int L, int BIT>
+__device__ __forceinline__ float qk_exchange_sum(float x) {
+  constexpr int SWAPS = L == 8 ? 1 : L >= 16 ? 2 : 0, FIRST = L == 32 ? 3 : 2;  // the swaps of lane groups are the last exchanges
+  if constexpr ((1 << BIT) >= L) {
+    return x;
+  } else if constexpr (BIT >= FIRST) {
+    constexpr int X = BIT - FIRST == SWAPS - 1 ? 32 : 16;
+    const kv_u32x2 both = kv_swap<X>(__float_as_uint(x), __float_as_uint(x));
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  } else {
+    constexpr int CTRL = BIT == 0 ? kDppXor1 : BIT == 1 ? kDppXor2 : kDppXor8;
+    return x + __uint_as_float(kv_dpp<CTRL>(__float_as_uint(x)));
+  }
+}
 
 // Of a head's squares, in the order above.
-template <int L>
+template <int L, int FORM, int STRIPE>
 __device__ __forceinline__ float qk_square_sum(const float (&a)[8], const float (&b)[8]) {
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = a[i] * a[i] + b[i] * b[i];
+  if constexpr (FORM == QK_STRIPES && STRIPE == 8) {  // pairs 4 apart are in the next lane
 #pragma unroll
-  for (int d = 4; d > 0; d /= 2) {
+    for (int i = 0; i < 8; ++i) s[i] = qk_exchange_sum<L, 0>(s[i]);
 #pragma unroll
-    for (int i = 0; i < d; ++i) s[i] = s[i] + s[i + d];
+    for (int c = 0; c < 8; c += 4) {
+      s[c] = (s[c] + s[c + 2]) + (s[c + 1] + s[c + 3]);
+      s[c] = qk_exchange_sum<L, 4>(qk_exchange_sum<L, 3>(qk_exchange_sum<L, 2>(qk_exchange_sum<L, 1>(s[c]))));
+    }
+    return s[0] + s[4];
+  } else if constexpr (FORM == QK_STRIPES) {  // 4 and 2 apart in other lanes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = qk_exchange_sum<L, 0>(qk_exchange_sum<L, 1>(s[i]));
+#pragma unroll
+    for (int c = 0; c < 8; c += 2) s[c] = qk_exchange_sum<L, 4>(qk_exchange_sum<L, 3>(qk_exchange_sum<L, 2>(s[c] + s[c + 1])));
+    return (s[0] + s[2]) + (s[4] + s[6]);
+  } else {
+#pragma unroll
+    for (int d = 4; d > 0; d /= 2) {
+#pragma unroll
+      for (int i = 0; i < d; ++i) s[i] = s[i] + s[i + d];
+    }
+    return qk_exchange_sum<L, 4>(qk_exchange_sum<L, 3>(qk_exchange_sum<L, 2>(qk_exchange_sum<L, 1>(qk_exchange_sum<L, 0>(s[0])))));
   }
-  float sum = s[0];
-  if constexpr (L >= 2) sum = qk_dpp_sum<kDppXor1>(sum);
-  if constexpr (L >= 4) sum = qk_dpp_sum<kDppXor2>(sum);
-  if constexpr (L == 32) sum = qk_dpp_sum<kDppXor8>(sum);
-  if constexpr (L >= 16) sum = qk_swap_sum<16>(sum);
-  if constexpr (L >= 8) sum = qk_swap_sum<32>(sum);
-  return sum;
 }
 
 // The dimensions of pair p.
@@ -112,107 +149,125 @@ __device__ __forceinline__ void qk_fetch(const void *p, int64_t at, uint32_t *w)
   }
 }
 
-// Sixteen values as they come, requested for all of a lane's heads before the first is looked at.
-template <int DT, int PIECE, bool INTERLEAVED>
+// Sixteen values as they come, requested for all of a lane's heads before the first is looked at.  (STRIPE is the tensors', whatever these values' type.)
+template <int DT, int L, int FORM, int PIECE, int STRIPE>
 struct QkRaw {
-  static constexpr int EACH = qk_piece_words(DT, PIECE), PIECES = 16 / PIECE;
+  static constexpr int AT_ONCE = FORM == QK_STRIPES ? STRIPE : PIECE;
+  static constexpr int EACH = qk_piece_words(DT, AT_ONCE), PIECES = 16 / AT_ONCE;
   uint32_t w[PIECES * EACH];
 
-  // Halves: the first dimensions of the eight pairs, then the second ones; neighbours: pair by pair.  Zeros behind the last pair.
+  // Halves: the first values of the eight pairs, then the second ones; otherwise pair by pair.  Zeros behind the last pair.
   __device__ __forceinline__ void request(const void *x, int64_t at, int part, int dim, const QkNormRotary &how) {
 #pragma unroll
     for (int i = 0; i < PIECES * EACH; ++i) w[i] = 0;
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-      const int value = (INTERLEAVED ? c : c % (PIECES / 2)) * PIECE;  // of sixteen in a row; of eight first or second ones
-      if (INTERLEAVED) {
-        const int d = 16 * part + value;
-        if (d < dim) qk_fetch<DT, PIECE>(x, at + d, w + c * EACH);
-      } else {
-        const int pair = 8 * part + value;
+      if constexpr (FORM == QK_HALVES) {
+        const int pair = 8 * part + c % (PIECES / 2) * AT_ONCE;
         const int2 d = qk_pair(pair, dim, how);
-        if (2 * pair < dim) qk_fetch<DT, PIECE>(x, at + (c < PIECES / 2 ? d.x : d.y), w + c * EACH);
+        if (2 * pair < dim) qk_fetch<DT, AT_ONCE>(x, at + (c < PIECES / 2 ? d.x : d.y), w + c * EACH);
+      } else {
+        const int d = FORM == QK_STRIPES ? STRIPE * (L * c + part) : 16 * part + AT_ONCE * c;
+        if (d < dim) qk_fetch<DT, AT_ONCE>(x, at + d, w + c * EACH);
       }
     }
   }
   __device__ __forceinline__ float value(int i) const {
     if constexpr (DT == OQ_F32) return __uint_as_float(w[i]);
-    else if constexpr (PIECE == 1) return dyn_bits_to_f32(w[i], DT);
+    else if constexpr (AT_ONCE == 1) return dyn_bits_to_f32(w[i], DT);
     else if constexpr (DT == OQ_BF16) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     else return f16_bits_to_f32(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
   }
   __device__ __forceinline__ void pairs(float (&a)[8], float (&b)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      a[i] = value(INTERLEAVED ? 2 * i : i);
-      b[i] = value(INTERLEAVED ? 2 * i + 1 : 8 + i);
+      a[i] = value(FORM == QK_HALVES ? i : 2 * i);
+      b[i] = value(FORM == QK_HALVES ? 8 + i : 2 * i + 1);
     }
   }
 };
 
-template <int DT, int PIECE, bool INTERLEAVED>
-__device__ __forceinline__ void qk_load_pairs(const void *x, int64_t at, int part, int dim, const QkNormRotary &how, float (&a)[8], float (&b)[8]) {
-  QkRaw<DT, PIECE, INTERLEAVED> raw;
-  raw.request(x, at, part, dim, how);
+template <int DT, int L, int FORM, int PIECE, int STRIPE>
+__device__ __forceinline__ void qk_load_pairs(const void *x, int part, int dim, const QkNormRotary &how, float (&a)[8], float (&b)[8]) {
+  QkRaw<DT, L, FORM, PIECE, STRIPE> raw;
+  raw.request(x, 0, part, dim, how);
   raw.pairs(a, b);
 }
-template <int PIECE, bool INTERLEAVED>
+template <int L, int FORM, int PIECE, int STRIPE>
 __device__ __forceinline__ void qk_load_weight(const QkNormRotary &how, int side, int part, int dim, float (&a)[8], float (&b)[8]) {
   const void *const w = how.weight[side];
   if (w == nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = b[i] = 1.0f;
   } else if (how.weight_dtype == OQ_F32) {
-    qk_load_pairs<OQ_F32, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
+    qk_load_pairs<OQ_F32, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
   } else if (how.weight_dtype == OQ_F16) {
-    qk_load_pairs<OQ_F16, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
+    qk_load_pairs<OQ_F16, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
   } else {
-    qk_load_pairs<OQ_BF16, PIECE, INTERLEAVED>(w, 0, part, dim, how, a, b);
+    qk_load_pairs<OQ_BF16, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
   }
 }
 
 // A token's row of the tables, eight entries of a lane.  A negative position (a token of no request) turns nothing, one behind the tables makes NaN.
+template <int L, int FORM, int STRIPE>
 struct QkTurn {
   float c[8], s[8];
-  int pairs;  // of the lane's that are turned
+  uint32_t turned;  // a bit for each pair that is
   __device__ __forceinline__ int64_t row_of(const QkNormRotary &how, int64_t token) const { return how.half == 0 ? -1 : how.positions != nullptr ? how.positions[token] : token; }
   __device__ __forceinline__ void load(const QkNormRotary &how, int64_t row, int part) {
+    turned = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
-    pairs = row >= 0 ? min(max(how.half - 8 * part, 0), 8) : 0;
-    if (pairs == 0 || row >= how.rows) return;
-    const int64_t at = row * how.half + 8 * part;
-    if (how.table_wide) {
-      load8<OQ_F32>(how.cos, at, true, c);
-      load8<OQ_F32>(how.sin, at, true, s);
-    } else {
+    for (int i = 0; i < 8; ++i) {
+      c[i] = s[i] = NAN;
+      turned |= (row >= 0 && qk_pair_of<L, FORM, STRIPE>(part, i) < how.half ? 1u : 0u) << i;
+    }
+    if (row >= how.rows) return;
+    constexpr int IN_ROW = FORM == QK_STRIPES ? STRIPE / 2 : 8;  // pairs
+    const int64_t at = row * how.half;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < pairs) {
-          c[i] = how.cos[at + i];
-          s[i] = how.sin[at + i];
+    for (int i = 0; i < 8; i += IN_ROW) {
+      if (how.table_wide) {
+        if ((turned >> i & 1) == 0) continue;
+        const int64_t from = at + qk_pair_of<L, FORM, STRIPE>(part, i);
+#pragma unroll
+        for (int e = 0; e < IN_ROW; e += IN_ROW < 4 ? 2 : 4) {
+          if constexpr (IN_ROW < 4) {
+            const float2 x = *reinterpret_cast<const float2 *>(how.cos + from), y = *reinterpret_cast<const float2 *>(how.sin + from);
+            c[i] = x.x; c[i + 1] = x.y; s[i] = y.x; s[i + 1] = y.y;
+          } else {
+            const float4 x = *reinterpret_cast<const float4 *>(how.cos + from + e), y = *reinterpret_cast<const float4 *>(how.sin + from + e);
+            c[i + e] = x.x; c[i + e + 1] = x.y; c[i + e + 2] = x.z; c[i + e + 3] = x.w;
+            s[i + e] = y.x; s[i + e + 1] = y.y; s[i + e + 2] = y.z; s[i + e + 3] = y.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < IN_ROW; ++e) {
+          if ((turned >> (i + e) & 1) == 0) continue;
+          c[i + e] = how.cos[at + qk_pair_of<L, FORM, STRIPE>(part, i + e)];
+          s[i + e] = how.sin[at + qk_pair_of<L, FORM, STRIPE>(part, i + e)];
         }
       }
     }
   }
 };
 
-template <int L>
-__device__ __forceinline__ void qk_apply(const QkNormRotary &how, const float (&wa)[8], const float (&wb)[8], const QkTurn &turn, float (&a)[8], float (&b)[8]) {
+template <int L, int FORM, int STRIPE>
+__device__ __forceinline__ void qk_apply(const QkNormRotary &how, const float (&wa)[8], const float (&wb)[8], const QkTurn<L, FORM, STRIPE> &turn, float (&a)[8], float (&b)[8]) {
   if (how.norm) {
-    const float r = 1.0f / sqrtf(qk_square_sum<L>(a, b) * how.by_dim + how.eps);
+    const float r = 1.0f / sqrtf(qk_square_sum<L, FORM, STRIPE>(a, b) * how.by_dim + how.eps);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       a[i] = a[i] * r * wa[i];
       b[i] = b[i] * r * wb[i];
     }
   }
-  if (turn.pairs == 0) return;
+  if (turn.turned == 0) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float u = a[i] * turn.c[i] - b[i] * turn.s[i], v = b[i] * turn.c[i] + a[i] * turn.s[i];
-    a[i] = i < turn.pairs ? u : a[i];
-    b[i] = i < turn.pairs ? v : b[i];
+    a[i] = turn.turned >> i & 1 ? u : a[i];
+    b[i] = turn.turned >> i & 1 ? v : b[i];
   }
 }
 
@@ -234,20 +289,9 @@ __device__ __forceinline__ void qk_put(void *p, int64_t at, const float *y) {
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = make_uint2(w[0], w[1]);
   }
 }
-template <int DT, int PIECE, bool INTERLEAVED>
+template <int DT, int L, int FORM, int PIECE, int STRIPE>
 __device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, int dim, const QkNormRotary &how, const float (&a)[8], const float (&b)[8]) {
-  if constexpr (INTERLEAVED) {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[2 * i] = a[i];
-      v[2 * i + 1] = b[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i += PIECE) {
-      if (16 * part + i < dim) qk_put<DT, PIECE>(out, at + 16 * part + i, v + i);
-    }
-  } else {
+  if constexpr (FORM == QK_HALVES) {
 #pragma unroll
     for (int i = 0; i < 8; i += PIECE) {
       const int pair = 8 * part + i;
@@ -257,13 +301,26 @@ __device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, 
         qk_put<DT, PIECE>(out, at + d.y, b + i);
       }
     }
+  } else {
+    constexpr int AT_ONCE = FORM == QK_STRIPES ? STRIPE : PIECE;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[2 * i] = a[i];
+      v[2 * i + 1] = b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += AT_ONCE) {
+      const int d = FORM == QK_STRIPES ? STRIPE * (L * (i / STRIPE) + part) : 16 * part + i;
+      if (d < dim) qk_put<DT, AT_ONCE>(out, at + d, v + i);
+    }
   }
 }
 
 // Workgroup `block` of a side: HEADS heads of a token for every L lanes.
-template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS, int HEADS>
+template <int DT, int L, int FORM, int PIECE, int THREADS, int HEADS>
 __device__ __forceinline__ void qk_heads_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
-  constexpr int UNITS = THREADS / L;
+  constexpr int UNITS = THREADS / L, STRIPE = qk_stripe(DT);
   const int lane = threadIdx.x & 63, part = qk_part_of<L>(lane);
   const uint32_t first = block * UNITS, local = (threadIdx.x >> 6) * (64 / L) + qk_vector_of<L>(lane);
   const uint32_t groups = side.groups, row = first / groups, n = first - row * groups + local;  // (n < groups + 256: the product by the reciprocal is exact)
@@ -271,28 +328,27 @@ __device__ __forceinline__ void qk_heads_block(const QkNormRotary &how, const Qk
   const int64_t token = static_cast<int64_t>(row) + down;
   const int head = static_cast<int>(n - down * groups) * HEADS;
   if (token >= tokens) return;  // (all of a unit's lanes)
-  QkRaw<DT, PIECE, INTERLEAVED> raw[HEADS];
+  QkRaw<DT, L, FORM, PIECE, STRIPE> raw[HEADS];
   float wa[8], wb[8];
-  QkTurn turn;
+  QkTurn<L, FORM, STRIPE> turn;
   const int64_t position = turn.row_of(how, token), at = token * side.token_stride;
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) raw[h].request(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how);
   turn.load(how, position, part);
-  qk_load_weight<PIECE, INTERLEAVED>(how, which, part, dim, wa, wb);
+  qk_load_weight<L, FORM, PIECE, STRIPE>(how, which, part, dim, wa, wb);
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
     if (h > 0 && head + h >= side.heads) break;
     float a[8], b[8];
     raw[h].pairs(a, b);
-    qk_apply<L>(how, wa, wb, turn, a, b);
-    qk_store_pairs<DT, PIECE, INTERLEAVED>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
+    qk_apply(how, wa, wb, turn, a, b);
+    qk_store_pairs<DT, L, FORM, PIECE, STRIPE>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
   }
 }
-
-template <int DT, int L, int PIECE, bool INTERLEAVED, int THREADS>
+template <int DT, int L, int FORM, int PIECE, int THREADS>
 __device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
-  if (side.each == 1) qk_heads_block<DT, L, PIECE, INTERLEAVED, THREADS, 1>(how, side, which, tokens, dim, block);
-  else qk_heads_block<DT, L, PIECE, INTERLEAVED, THREADS, kQkHeads>(how, side, which, tokens, dim, block);
+  if (side.each == 1) qk_heads_block<DT, L, FORM, PIECE, THREADS, 1>(how, side, which, tokens, dim, block);
+  else qk_heads_block<DT, L, FORM, PIECE, THREADS, kQkHeads>(how, side, which, tokens, dim, block);
 }
 
 }  // namespace oq

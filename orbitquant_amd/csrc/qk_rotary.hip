@@ -10,7 +10,7 @@ namespace {
 template <int DT, int L, int PIECE, bool INTERLEAVED>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rotary_kernel(QkArgs a) {
   const bool keys = blockIdx.x >= a.q_blocks;
-  qk_block<DT, L, PIECE, INTERLEAVED, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
+  qk_block<DT, L, qk_form(INTERLEAVED, L, PIECE), PIECE, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
 }
 
 template <int DT, int L, int PIECE>
