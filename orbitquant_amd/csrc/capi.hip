@@ -887,9 +887,10 @@ int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const 
   if (most > oq::kKvMostKept || requests > oq::kKvMaxRequests || tokens > 0x3fffffffLL || table_width > 0x7fffffffLL || free_count > 0x7fffffffLL)
     return fail(OQ_ERR_UNSUPPORTED, "kv_keep: most=%lld (at most %d) requests=%lld (at most %d) tokens=%lld", (long long)most, oq::kKvMostKept, (long long)requests,
                 oq::kKvMaxRequests, (long long)tokens);
-  if ((table == nullptr) != (taken == nullptr) || (taken == nullptr) != (taken_after == nullptr) || (free_count > 0 && free_pages == nullptr))
+  const bool pages = taken != nullptr;
+  if (pages != (taken_after != nullptr) || (pages ? requests > 0 && table_width > 0 && table == nullptr : table != nullptr) || (free_count > 0 && free_pages == nullptr))
     return fail(OQ_ERR_INVALID, "kv_keep: block table, free pages and their count go together");
-  if (requests == 0 && table == nullptr) return OQ_OK;
+  if (requests == 0 && !pages) return OQ_OK;
   if ((requests > 0 && (lengths == nullptr || starts == nullptr || lengths_after == nullptr || (most > 0 && kept == nullptr))) || (tokens > 0 && slots == nullptr))
     return fail(OQ_ERR_INVALID, "kv_keep: null pointer");
   oq::KvKeepArgs a{};
@@ -901,6 +902,7 @@ int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const 
     a.counts = at == 0;
     a.caches = static_cast<int>(cache_count - at < oq::kKvKeepCaches ? cache_count - at : oq::kKvKeepCaches);
     for (int i = 0; i < a.caches; ++i) a.cache[i] = {caches[at + i].k_codes, caches[at + i].v_codes, caches[at + i].k_scales, caches[at + i].v_scales};
+    if (oq::kv_keep_blocks(a) == 0) break;  // (no requests: the first launch has made the counts)
     if (oq::kv_keep_blocks(a) > oq::kKvMostThreads / 256) return fail(OQ_ERR_UNSUPPORTED, "kv_keep: requests=%lld kv_heads=%d exceed the grid", (long long)requests, a.heads);
     if (const int status = oq::kv_keep_dispatch(a, static_cast<int>(caches->head_dim), as_stream(stream))) return status;
   }

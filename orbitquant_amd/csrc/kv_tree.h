@@ -22,7 +22,7 @@ struct KvKeepArgs {
   const int64_t *slots;
   int64_t tokens, pages, table_stride;
   int requests, most, heads, page_shift, table_width, free_count;
-  const int32_t *table, *taken;    // NULL: no page is given back
+  const int32_t *table, *taken;    // taken NULL: no page is given back
   int32_t *free_pages, *lengths_after, *taken_after;
   bool counts;                     // the launch whose first workgroup makes lengths and free pages
   int caches;

@@ -108,7 +108,7 @@ __device__ void keep_counts(const KvKeepArgs &a) {
   __shared__ int wave_sums[kKeepThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.requests + kKeepThreads - 1) / kKeepThreads, from = min(tid * run, a.requests), to = min(from + run, a.requests);
-  const int taken = a.table != nullptr ? min(max(*a.taken, 0), a.free_count) : 0;
+  const int taken = a.taken != nullptr ? min(max(*a.taken, 0), a.free_count) : 0;
   const auto pages_of = [&](int tokens) { return static_cast<int>(min((static_cast<int64_t>(max(tokens, 0)) + (1 << a.page_shift) - 1) >> a.page_shift, static_cast<int64_t>(a.table_width))); };
   // each(page) for a request's pages from `column` on, four of them requested at once
   const auto over_pages = [&](int r, int column, int end, const auto &each) {
@@ -129,9 +129,9 @@ __device__ void keep_counts(const KvKeepArgs &a) {
     const Path path = path_of(a, r);
     const int kept = max(length - path.fresh, 0) + kept_of(a, r, path);
     a.lengths_after[r] = kept;
-    if (a.table != nullptr) over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
+    if (a.taken != nullptr) over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
   }
-  if (a.table == nullptr) return;
+  if (a.taken == nullptr) return;
   const int sum = kv_sums(own);
   if (lane == 63) wave_sums[wave] = sum;
   __syncthreads();

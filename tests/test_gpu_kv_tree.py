@@ -339,6 +339,19 @@ def test_keep_many_requests_and_caches():
     assert min(held) >= 0 and len(set(held)) == len(held)
 
 
+def test_keep_no_requests():
+    """Nothing moves, the count stays; also with more caches than one launch takes."""
+    from orbitquant_amd import kv_keep
+
+    cache = _cache(2, 1, 64, 16)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    for caches in ([cache], [cache] * 65):
+        got = kv_keep(none.view(0, 3), none, _i32([0]), torch.empty(0, dtype=torch.int64, device="cuda"), caches, block_table=none.view(0, 4), free_pages=_i32([4, 5, 6]),
+                      taken=_i32([2]))
+        assert got.lengths.shape == (0,) and got.taken.tolist() == [2]
+    assert (cache[0] == 0xA5).all()
+
+
 def test_keep_refuses():
     from orbitquant_amd import kv_keep
 
