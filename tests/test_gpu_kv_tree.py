@@ -155,6 +155,56 @@ def test_attend_masks_long(dim, page, dtype, window):
         _check(got, q, cache, table, lengths, starts, masks, window)
 
 
+@pytest.mark.parametrize("dim,page,dtype", [(64, 64, torch.bfloat16), (128, 16, torch.float16), (256, 64, torch.float32)])
+def test_hints_and_windows_of_any_size(dim, page, dtype):
+    """Wrong hints cost time only, windows may be longer than anything, and a call gives the same bits every time."""
+    from orbitquant_amd import kv_attend
+
+    rng = np.random.RandomState(14)
+    new, before = [40, 2, 90], [1300, 0, 2]
+    lengths, starts = [a + b for a, b in zip(new, before)], _starts(new)
+    cache, table = _filled(rng, lengths, 2, dim, page)
+    q = _queries(rng, starts[-1], 6, dim, dtype)
+    masks = _random_masks(rng, new, 2, starts[-1])
+    call = lambda **kw: kv_attend(q, cache, table, _i32(lengths), starts=_i32(starts), masks=_masks(masks), return_lse=True, **kw)  # noqa: E731
+    for hints in ({"max_length": 1}, {"max_length": 10 ** 6, "max_new": 10 ** 6}, {"max_length": 0, "max_new": 0}, {"max_new": 3, "max_length": 1300}):
+        _check(call(**hints), q, cache, table, lengths, starts, masks)
+    for window in (1341, 2 ** 30, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        _check(call(window=window), q, cache, table, lengths, starts, masks, window)
+    first = call(max_new=90)
+    for _ in range(5):
+        for a, b in zip(first, call(max_new=90)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("before", [[1500, 900], [5500, 900]])     # whole by themselves; cut where there is a workspace
+def test_attend_masks_without_workspace(before, dtype):
+    """The library's call without a workspace leaves requests whole; with less than it asks for, too."""
+    import ctypes
+
+    from orbitquant_amd import _lib, kv_cache
+
+    rng = np.random.RandomState(15)
+    new = [30, 70]
+    lengths, starts = [a + b for a, b in zip(new, before)], _starts(new)
+    cache, table = _filled(rng, lengths, 2, 64, 64)
+    q = _queries(rng, 100, 4, 64, dtype)
+    masks = _random_masks(rng, new, 2, 100)
+    held = [_i32(lengths), _i32(starts), _masks(masks), torch.empty(1024, dtype=torch.uint8, device="cuda")]
+    lib, struct = _lib.load(), kv_cache._cache_struct(cache, q)
+    shape = (100, 4, 2, 64, 64, table.shape[1], 2, 1)
+    needed = lib.oq_kv_attend_tree_workspace_bytes(kv_cache._dt(q), *shape, 2, 0, -1, 70)
+    assert needed == 0 if before[0] == 1500 else needed > 1024
+    for workspace, size in ((None, 0), (held[3].data_ptr(), 1024)):
+        out, lse = torch.empty_like(q), torch.empty(100, 4, device="cuda")
+        rc = lib.oq_kv_attend_tree(q.data_ptr(), kv_cache._dt(q), 100, 4, q.stride(0), q.stride(1), ctypes.byref(struct), table.data_ptr(), table.stride(0), table.shape[1],
+                                   held[0].data_ptr(), held[1].data_ptr(), 2, held[2].data_ptr(), 2, 0, 0.125, -1, 70, out.data_ptr(), lse.data_ptr(), workspace, size,
+                                   kv_cache._stream(q))
+        assert rc == 0
+        _check((out, lse), q, cache, table, lengths, starts, masks, scale=0.125)
+
+
 def test_a_chain_is_causal_attention():
     """Masks of chains see what no masks see.  (Not bit for bit: the two may be launched otherwise, and then add up in another order.  So both are held
     to the bound of the same definition.)"""
@@ -337,6 +387,28 @@ def test_keep_many_requests_and_caches():
     again = kv_assign(lengths, _i32(new), table, free, taken, page_size=page, tokens=sum(new))
     held = [int(table[r, c]) for r, n in enumerate(again.lengths.tolist()) for c in range(min(6, -(-n // page)))]
     assert min(held) >= 0 and len(set(held)) == len(held)
+
+
+def test_keep_beyond_32_bits():
+    """Entries whose codes lie behind 4 GiB."""
+    from orbitquant_amd import OrbitKVCache, kv_keep
+
+    cache = OrbitKVCache.empty(5 * 2 ** 13, 16, 128, page_size=128)      # 2^13 pages of 16 heads: 1 GiB of keys
+    slots = torch.tensor([5, 2 ** 20 + 70, 5 * 2 ** 20 - 1, 2 ** 22 + 3], device="cuda")
+    at, place = slots // 128, slots % 128
+    for t in cache[:4]:
+        where = (at, slice(None), place) if t.ndim == 3 or t is cache[0] else (at, slice(None), slice(None), place)
+        t[where] = torch.randint(1, 100, t[where].shape, device="cuda").to(t.dtype)
+    was = _entries(cache, at, place)
+    got = kv_keep(_i32([[0, 2, 3]]), _i32([4]), _i32([0, 4]), slots, [cache])
+    assert got.lengths.tolist() == [3]
+    for x, y in zip(_entries(cache, at, place), was):
+        assert torch.equal(x[[0, 1, 2, 3]], y[[0, 2, 3, 3]])
+
+
+def _entries(cache, at, place):
+    """The entries' codes and scales."""
+    return [cache[0][at, :, place], cache[1][at, :, place], cache[2][at, :, :, place], cache[3][at, :, place]]
 
 
 def test_keep_no_requests():
