@@ -9,9 +9,9 @@
 // apart of each eight, then eights 1, 2, 4, ... apart, zeros behind the last pair.  So a key's codes do not depend on the launch that made them.
 //
 // A lane holds eight pairs, `L` = 1, 2, 4, ... 32 lanes a head: both values of every pair are in one lane, the rotation needs no other, and
-// the sums need log2(L) exchanges.  Bound by memory: 32760 tokens, 40 heads of 128 for queries and keys each, bf16, 1.36 GB, 252 us (halves; neighbours 260),
-// 5.4 TB/s, where a copy of the library reaches 5.2; few tokens by latency, 3.1 us for one.  (Converted as they were fetched, head by head, 344 us; four heads a
-// lane 264.)
+// the sums need log2(L) exchanges.  Bound by memory: 32760 tokens, 40 heads of 128 for queries and keys each, bf16, 1.36 GB, 249 us (neighbours 252, as many
+// bytes in fp32 245), 5.4 TB/s, where a copy of the library reaches 5.2; vector instructions issue in 72 % of the cycles.  Few tokens by latency, 3.1 us for one.
+// (Converted as they were fetched, head by head, 344 us; four heads a lane 260.)
 #pragma once
 
 #include "kv_rows.h"
@@ -150,7 +150,8 @@ __device__ __forceinline__ void qk_fetch(const void *p, int64_t at, uint32_t *w)
 }
 
 // Sixteen values as they come, requested for all of a lane's heads before the first is looked at.  (STRIPE is the tensors', whatever these values' type.)
-template <int DT, int L, int FORM, int PIECE, int STRIPE>
+// FULL: the lanes have nothing behind the last pair (D = 16 L).
+template <int DT, int L, int FORM, int PIECE, int STRIPE, bool FULL>
 struct QkRaw {
   static constexpr int AT_ONCE = FORM == QK_STRIPES ? STRIPE : PIECE;
   static constexpr int EACH = qk_piece_words(DT, AT_ONCE), PIECES = 16 / AT_ONCE;
@@ -158,17 +159,19 @@ struct QkRaw {
 
   // Halves: the first values of the eight pairs, then the second ones; otherwise pair by pair.  Zeros behind the last pair.
   __device__ __forceinline__ void request(const void *x, int64_t at, int part, int dim, const QkNormRotary &how) {
+    if constexpr (!FULL) {
 #pragma unroll
-    for (int i = 0; i < PIECES * EACH; ++i) w[i] = 0;
+      for (int i = 0; i < PIECES * EACH; ++i) w[i] = 0;
+    }
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
       if constexpr (FORM == QK_HALVES) {
         const int pair = 8 * part + c % (PIECES / 2) * AT_ONCE;
         const int2 d = qk_pair(pair, dim, how);
-        if (2 * pair < dim) qk_fetch<DT, AT_ONCE>(x, at + (c < PIECES / 2 ? d.x : d.y), w + c * EACH);
+        if (FULL || 2 * pair < dim) qk_fetch<DT, AT_ONCE>(x, at + (c < PIECES / 2 ? d.x : d.y), w + c * EACH);
       } else {
         const int d = FORM == QK_STRIPES ? STRIPE * (L * c + part) : 16 * part + AT_ONCE * c;
-        if (d < dim) qk_fetch<DT, AT_ONCE>(x, at + d, w + c * EACH);
+        if (FULL || d < dim) qk_fetch<DT, AT_ONCE>(x, at + d, w + c * EACH);
       }
     }
   }
@@ -187,48 +190,64 @@ struct QkRaw {
   }
 };
 
-template <int DT, int L, int FORM, int PIECE, int STRIPE>
-__device__ __forceinline__ void qk_load_pairs(const void *x, int part, int dim, const QkNormRotary &how, float (&a)[8], float (&b)[8]) {
-  QkRaw<DT, L, FORM, PIECE, STRIPE> raw;
-  raw.request(x, 0, part, dim, how);
-  raw.pairs(a, b);
-}
-template <int L, int FORM, int PIECE, int STRIPE>
-__device__ __forceinline__ void qk_load_weight(const QkNormRotary &how, int side, int part, int dim, float (&a)[8], float (&b)[8]) {
-  const void *const w = how.weight[side];
-  if (w == nullptr) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = b[i] = 1.0f;
-  } else if (how.weight_dtype == OQ_F32) {
-    qk_load_pairs<OQ_F32, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
-  } else if (how.weight_dtype == OQ_F16) {
-    qk_load_pairs<OQ_F16, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
-  } else {
-    qk_load_pairs<OQ_BF16, L, FORM, PIECE, STRIPE>(w, part, dim, how, a, b);
+// A norm's weights, as they come and as numbers.  (Their type is looked at twice: what is converted where it is requested is waited for there.)
+template <int L, int FORM, int PIECE, int STRIPE, bool FULL>
+struct QkWeight {
+  QkRaw<OQ_F32, L, FORM, PIECE, STRIPE, FULL> wide;
+  QkRaw<OQ_BF16, L, FORM, PIECE, STRIPE, FULL> narrow;
+  __device__ __forceinline__ void request(const QkNormRotary &how, int side, int part, int dim) {
+    const void *const w = how.weight[side];
+    if (w == nullptr) return;
+    if (how.weight_dtype == OQ_F32) wide.request(w, 0, part, dim, how);
+    else narrow.request(w, 0, part, dim, how);
   }
-}
+  __device__ __forceinline__ void pairs(const QkNormRotary &how, int side, float (&a)[8], float (&b)[8]) const {
+    if (how.weight[side] == nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = b[i] = 1.0f;
+    } else if (how.weight_dtype == OQ_F32) {
+      wide.pairs(a, b);
+    } else if (how.weight_dtype == OQ_BF16) {
+      narrow.pairs(a, b);
+    } else {
+      QkRaw<OQ_F16, L, FORM, PIECE, STRIPE, FULL> half;
+#pragma unroll
+      for (int i = 0; i < narrow.PIECES * narrow.EACH; ++i) half.w[i] = narrow.w[i];
+      half.pairs(a, b);
+    }
+  }
+};
 
-// A token's row of the tables, eight entries of a lane.  A negative position (a token of no request) turns nothing, one behind the tables makes NaN.
+// A token's row of the tables, eight entries of a lane.  A negative position (a token of no request) turns nothing, one behind the tables makes NaN;
+// both read a row that exists, so that no load is in a branch of some lanes.
 template <int L, int FORM, int STRIPE>
 struct QkTurn {
   float c[8], s[8];
   uint32_t turned;  // a bit for each pair that is
-  __device__ __forceinline__ int64_t row_of(const QkNormRotary &how, int64_t token) const { return how.half == 0 ? -1 : how.positions != nullptr ? how.positions[token] : token; }
-  __device__ __forceinline__ void load(const QkNormRotary &how, int64_t row, int part) {
-    turned = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = s[i] = NAN;
-      turned |= (row >= 0 && qk_pair_of<L, FORM, STRIPE>(part, i) < how.half ? 1u : 0u) << i;
-    }
-    if (row >= how.rows) return;
+  bool broken;
+  // Of a token: requested first, since loads come back in order and the tables' wait for it.
+  static __device__ __forceinline__ int request(const QkNormRotary &how, int64_t token) {
+    int position = 0;
+    if (how.positions != nullptr) position = how.positions[token];
+    __builtin_amdgcn_sched_barrier(0);
+    return position;
+  }
+  __device__ __forceinline__ void load(const QkNormRotary &how, int64_t token, int position, int part) {
     constexpr int IN_ROW = FORM == QK_STRIPES ? STRIPE / 2 : 8;  // pairs
-    const int64_t at = row * how.half;
+    turned = 0;
+    broken = false;
+    if (how.half == 0) return;
+    const int64_t row = how.positions != nullptr ? position : token;
+#pragma unroll
+    for (int i = 0; i < 8; i += IN_ROW) turned |= ((1u << min(max(how.half - qk_pair_of<L, FORM, STRIPE>(part, i), 0), IN_ROW)) - 1u) << i;
+    turned = row >= 0 ? turned : 0;
+    broken = row >= how.rows;
+    if (how.rows == 0) return;
+    const int64_t at = min(max(row, static_cast<int64_t>(0)), how.rows - 1) * how.half;
 #pragma unroll
     for (int i = 0; i < 8; i += IN_ROW) {
       if (how.table_wide) {
-        if ((turned >> i & 1) == 0) continue;
-        const int64_t from = at + qk_pair_of<L, FORM, STRIPE>(part, i);
+        const int64_t from = at + min(qk_pair_of<L, FORM, STRIPE>(part, i), how.half - IN_ROW);
 #pragma unroll
         for (int e = 0; e < IN_ROW; e += IN_ROW < 4 ? 2 : 4) {
           if constexpr (IN_ROW < 4) {
@@ -243,9 +262,9 @@ struct QkTurn {
       } else {
 #pragma unroll
         for (int e = 0; e < IN_ROW; ++e) {
-          if ((turned >> (i + e) & 1) == 0) continue;
-          c[i + e] = how.cos[at + qk_pair_of<L, FORM, STRIPE>(part, i + e)];
-          s[i + e] = how.sin[at + qk_pair_of<L, FORM, STRIPE>(part, i + e)];
+          const int64_t from = at + min(qk_pair_of<L, FORM, STRIPE>(part, i + e), how.half - 1);
+          c[i + e] = how.cos[from];
+          s[i + e] = how.sin[from];
         }
       }
     }
@@ -262,7 +281,24 @@ __device__ __forceinline__ void qk_apply(const QkNormRotary &how, const float (&
       b[i] = b[i] * r * wb[i];
     }
   }
-  if (turn.turned == 0) return;
+  if (how.half == 0) return;
+  if (turn.turned == 0xffu && !turn.broken) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float u = a[i] * turn.c[i] - b[i] * turn.s[i];
+      b[i] = b[i] * turn.c[i] + a[i] * turn.s[i];
+      a[i] = u;
+    }
+    return;
+  }
+  if (turn.broken) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = turn.turned >> i & 1 ? NAN : a[i];
+      b[i] = turn.turned >> i & 1 ? NAN : b[i];
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float u = a[i] * turn.c[i] - b[i] * turn.s[i], v = b[i] * turn.c[i] + a[i] * turn.s[i];
@@ -289,14 +325,14 @@ __device__ __forceinline__ void qk_put(void *p, int64_t at, const float *y) {
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) = make_uint2(w[0], w[1]);
   }
 }
-template <int DT, int L, int FORM, int PIECE, int STRIPE>
+template <int DT, int L, int FORM, int PIECE, int STRIPE, bool FULL>
 __device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, int dim, const QkNormRotary &how, const float (&a)[8], const float (&b)[8]) {
   if constexpr (FORM == QK_HALVES) {
 #pragma unroll
     for (int i = 0; i < 8; i += PIECE) {
       const int pair = 8 * part + i;
       const int2 d = qk_pair(pair, dim, how);
-      if (2 * pair < dim) {
+      if (FULL || 2 * pair < dim) {
         qk_put<DT, PIECE>(out, at + d.x, a + i);
         qk_put<DT, PIECE>(out, at + d.y, b + i);
       }
@@ -312,13 +348,13 @@ __device__ __forceinline__ void qk_store_pairs(void *out, int64_t at, int part, 
 #pragma unroll
     for (int i = 0; i < 16; i += AT_ONCE) {
       const int d = FORM == QK_STRIPES ? STRIPE * (L * (i / STRIPE) + part) : 16 * part + i;
-      if (d < dim) qk_put<DT, AT_ONCE>(out, at + d, v + i);
+      if (FULL || d < dim) qk_put<DT, AT_ONCE>(out, at + d, v + i);
     }
   }
 }
 
 // Workgroup `block` of a side: HEADS heads of a token for every L lanes.
-template <int DT, int L, int FORM, int PIECE, int THREADS, int HEADS>
+template <int DT, int L, int FORM, int PIECE, bool FULL, int THREADS, int HEADS>
 __device__ __forceinline__ void qk_heads_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
   constexpr int UNITS = THREADS / L, STRIPE = qk_stripe(DT);
   const int lane = threadIdx.x & 63, part = qk_part_of<L>(lane);
@@ -328,27 +364,30 @@ __device__ __forceinline__ void qk_heads_block(const QkNormRotary &how, const Qk
   const int64_t token = static_cast<int64_t>(row) + down;
   const int head = static_cast<int>(n - down * groups) * HEADS;
   if (token >= tokens) return;  // (all of a unit's lanes)
-  QkRaw<DT, L, FORM, PIECE, STRIPE> raw[HEADS];
+  QkRaw<DT, L, FORM, PIECE, STRIPE, FULL> raw[HEADS];
   float wa[8], wb[8];
   QkTurn<L, FORM, STRIPE> turn;
-  const int64_t position = turn.row_of(how, token), at = token * side.token_stride;
+  QkWeight<L, FORM, PIECE, STRIPE, FULL> weight;
+  const int position = turn.request(how, token);
+  const int64_t at = token * side.token_stride;
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) raw[h].request(side.x, at + min(head + h, side.heads - 1) * side.head_stride, part, dim, how);
-  turn.load(how, position, part);
-  qk_load_weight<L, FORM, PIECE, STRIPE>(how, which, part, dim, wa, wb);
+  weight.request(how, which, part, dim);
+  turn.load(how, token, position, part);
+  weight.pairs(how, which, wa, wb);
 #pragma unroll
   for (int h = 0; h < HEADS; ++h) {
     if (h > 0 && head + h >= side.heads) break;
     float a[8], b[8];
     raw[h].pairs(a, b);
     qk_apply(how, wa, wb, turn, a, b);
-    qk_store_pairs<DT, L, FORM, PIECE, STRIPE>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
+    qk_store_pairs<DT, L, FORM, PIECE, STRIPE, FULL>(side.out, (token * side.heads + head + h) * dim, part, dim, how, a, b);
   }
 }
-template <int DT, int L, int FORM, int PIECE, int THREADS>
+template <int DT, int L, int FORM, int PIECE, bool FULL, int THREADS>
 __device__ __forceinline__ void qk_block(const QkNormRotary &how, const QkSide &side, int which, int64_t tokens, int dim, uint32_t block) {
-  if (side.each == 1) qk_heads_block<DT, L, FORM, PIECE, THREADS, 1>(how, side, which, tokens, dim, block);
-  else qk_heads_block<DT, L, FORM, PIECE, THREADS, kQkHeads>(how, side, which, tokens, dim, block);
+  if (side.each == 1) qk_heads_block<DT, L, FORM, PIECE, FULL, THREADS, 1>(how, side, which, tokens, dim, block);
+  else qk_heads_block<DT, L, FORM, PIECE, FULL, THREADS, kQkHeads>(how, side, which, tokens, dim, block);
 }
 
 }  // namespace oq

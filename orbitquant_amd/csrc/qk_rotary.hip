@@ -7,23 +7,24 @@ namespace oq {
 namespace {
 
 // The first workgroups have the queries, the others the keys.
-template <int DT, int L, int PIECE, bool INTERLEAVED>
+template <int DT, int L, int PIECE, bool INTERLEAVED, bool FULL>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rotary_kernel(QkArgs a) {
   const bool keys = blockIdx.x >= a.q_blocks;
-  qk_block<DT, L, qk_form(INTERLEAVED, L, PIECE), PIECE, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
+  qk_block<DT, L, qk_form(INTERLEAVED, L, PIECE), PIECE, FULL, kQkThreads>(a.how, a.side[keys], keys, a.tokens, a.dim, blockIdx.x - (keys ? a.q_blocks : 0));
 }
 
-template <int DT, int L, int PIECE>
+template <int DT, int L, int PIECE, bool FULL>
 void launch(const QkArgs &a, hipStream_t stream) {
   const dim3 grid(a.q_blocks + a.k_blocks);
-  if (a.how.interleaved) launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, true>, grid, dim3(kQkThreads), 0, stream, a);
-  else launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, false>, grid, dim3(kQkThreads), 0, stream, a);
+  if (a.how.interleaved) launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, true, FULL>, grid, dim3(kQkThreads), 0, stream, a);
+  else launch_kernel(qk_norm_rotary_kernel<DT, L, PIECE, false, FULL>, grid, dim3(kQkThreads), 0, stream, a);
 }
 template <int DT, int L>
 void launch(const QkArgs &a, hipStream_t stream) {
-  if (a.how.piece == 8) launch<DT, L, 8>(a, stream);
-  else if (a.how.piece == 4) launch<DT, L, 4>(a, stream);
-  else launch<DT, L, 1>(a, stream);
+  if (a.how.piece == 8 && a.dim == 16 * L) launch<DT, L, 8, true>(a, stream);
+  else if (a.how.piece == 8) launch<DT, L, 8, false>(a, stream);
+  else if (a.how.piece == 4) launch<DT, L, 4, false>(a, stream);
+  else launch<DT, L, 1, false>(a, stream);
 }
 template <int L>
 void launch(const QkArgs &a, int dtype, hipStream_t stream) {

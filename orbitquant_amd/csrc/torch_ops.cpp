@@ -466,7 +466,7 @@ pybind11::object qk_norm_rotary(const Tensor &q, const Tensor &k, const OptTenso
       !plan_of(q, cos, sin, q_weight, k_weight, eps, interleaved, positions, p))
     return pybind11::none();
   const c10::OptionalDeviceGuard guard(q.device());
-  // Small results share one allocation, a microsecond less; large ones can be freed by themselves.
+  // Small results share one allocation, half a microsecond less; large ones can be freed by themselves.
   constexpr int64_t kShared = 1 << 18;
   const int64_t q_bytes = (static_cast<int64_t>(q.numel() * q.element_size()) + 15) & ~int64_t{15}, bytes = q_bytes + static_cast<int64_t>(k.numel() * k.element_size());
   Tensor q_out, k_out;
