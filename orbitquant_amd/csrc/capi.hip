@@ -893,6 +893,12 @@ int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const 
   if (requests == 0 && !pages) return OQ_OK;
   if ((requests > 0 && (lengths == nullptr || starts == nullptr || lengths_after == nullptr || (most > 0 && kept == nullptr))) || (tokens > 0 && slots == nullptr))
     return fail(OQ_ERR_INVALID, "kv_keep: null pointer");
+  // (a path that is moved twice: the second reads what the first has moved already)
+  for (int64_t i = 1; requests > 0 && i < cache_count; ++i) {
+    for (int64_t j = 0; j < i; ++j) {
+      if (caches[i].k_codes == caches[j].k_codes) return fail(OQ_ERR_INVALID, "kv_keep: cache %lld is cache %lld again", (long long)i, (long long)j);
+    }
+  }
   oq::KvKeepArgs a{};
   a.kept = kept; a.lengths = lengths; a.starts = starts; a.slots = slots; a.tokens = tokens; a.pages = first.pages; a.table_stride = table_stride;
   a.requests = static_cast<int>(requests); a.most = static_cast<int>(most); a.heads = first.heads; a.page_shift = first.page_shift;

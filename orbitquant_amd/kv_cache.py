@@ -472,7 +472,7 @@ def kv_keep(kept: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, slo
     kept     int32 [requests, most], most at most 256: which of the request's new tokens, in rising order, -1 behind the last.  A list ends at the first
              entry that does not rise, is none of the request's new tokens or has no slot.  The i-th one's entries move to where its i-th new token's are
     lengths, starts, slots   as `kv_assign` gave them for the step
-    caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them)
+    caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once
     block_table, free_pages, taken   as they are after that `kv_assign` (`taken`: its result), all or none of them.  Pages behind the kept tokens go back
              onto the list, in place, in front of those that it gives out next.  The table's columns behind the kept pages stand for nothing from then on"""
     if (block_table is None) != (free_pages is None) or (free_pages is None) != (taken is None):

@@ -112,6 +112,14 @@ def test_caches_of_different_shapes(other):
     assert _keep(_cache_struct(), _cache_struct(**other)) == INVALID
 
 
+@pytest.mark.parametrize("first,again", [(0, 1), (0, 3), (1, 2), (2, 3)])
+def test_a_cache_twice(first, again):
+    """Two wavefronts would move the same entries, one of them what the other has moved already."""
+    layers = [_cache_struct(k_codes=NOWHERE + 4096 * i) for i in range(4)]
+    layers[again] = layers[first]
+    assert _keep(*layers) == INVALID and b"cache %d is cache %d again" % (again, first) in _lib.load().oq_last_error()
+
+
 def test_python_refuses_the_host():
     """Tensors on the host, and what is wrong whatever they are on."""
     q, k = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
