@@ -617,7 +617,9 @@ uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t 
  *            a cache that layers share stands there once
  * table, free_pages, taken NULL, or as oq_kv_assign left them (taken: taken_after): pages behind the kept tokens go back onto the free
  *            list, in front of those that it gives out next; the table is not changed, its columns behind the kept pages
- *            stand for nothing.  Requests <= 8192
+ *            stand for nothing.  Requests <= 8192.  The pages that oq_kv_assign drew for columns behind the table's end go back too, in a call
+ *            for all of its requests; but for a step in which the list ran out and no column of the table got a page: which pages
+ *            were drawn is not known then.  (A table with room for every new token never has such pages.)
  * lengths_after int32 [requests]: without the forgotten tokens; taken_after int32 [1]
  * No slot twice in slots.  No output may overlap an input other than the caches and free_pages.
  */

@@ -105,9 +105,134 @@ __device__ __forceinline__ int kept_of(const KvKeepArgs &a, int r, const Path &p
   return a.most;
 }
 
-// Lengths, and the pages behind them onto the free list again, in front of those that it gives out next, in request order.
+// The pages that kv_assign has drawn for request r's new tokens: for columns [have, need), also where these lie behind the table.
+struct Fresh {
+  int have, need;
+};
+__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int length, int fresh) {
+  const auto pages_of = [&](int tokens) { return static_cast<int>((static_cast<uint32_t>(tokens) + (1u << a.page_shift) - 1) >> a.page_shift); };
+  return {pages_of(max(length - fresh, 0)), pages_of(length)};
+}
+__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int r) { return fresh_of(a, max(a.lengths[r], 0), path_of(a, r).fresh); }
+__device__ __forceinline__ int dropped_from(const KvKeepArgs &a, const Fresh &f) { return max(f.have, a.table_width); }  // the first of them behind the table
+
+// Before every thread of the workgroup's `own`, the sum of the threads before; upto[kKeepThreads]: of all.  Behind a barrier, and one behind it.
+__device__ void upto_of(int own, int (&upto)[kKeepThreads + 1]) {
+  __shared__ int wave_sums[kKeepThreads / 64];
+  const int tid = threadIdx.x, wave = tid >> 6, sum = kv_sums(own);
+  if ((tid & 63) == 63) wave_sums[wave] = sum;
+  __syncthreads();
+  int ahead = sum - own;
+#pragma unroll
+  for (int w = 0; w < kKeepThreads / 64; ++w) ahead += w < wave ? wave_sums[w] : 0;
+  upto[tid] = ahead;
+  if (tid == kKeepThreads - 1) upto[kKeepThreads] = ahead + own;
+  __syncthreads();
+}
+
+// Pages for columns that the table does not have: kv_assign has drawn them too, and no row names them.  But the step's pages are the last of the list before `taken`, in
+// request order, so that they are found there: moved up to the end of what is taken, their number is the result.  Where the step's first page is:
+//   - a column that got one (the first such) names it, and its place in the list tells;
+//   - where no column has got one, `taken` less the step's pages, unless the list may have run out (then some were not drawn, and which is not known).
+// Neither is believed where the call has but a part of kv_assign's requests, whose pages are not the list's last: the pages are lost then, never listed twice.
+// A rare path, at the end of a request's row: latency of a few loads and barriers, 64 requests that are all there 3.6 us, and 2.5 without it; elsewhere one comparison a request.
+__device__ int keep_dropped(const KvKeepArgs &a, int taken) {
+  __shared__ int fresh_upto[kKeepThreads + 1], dropped_upto[kKeepThreads + 1];
+  __shared__ int anchor, anchor_page, found, others;
+  constexpr int kNone = 0x7fffffff;
+  const int tid = threadIdx.x, run = (a.requests + kKeepThreads - 1) / kKeepThreads;
+  const auto first_of = [&](int thread) { return min(thread * run, a.requests); };
+  const int from = first_of(tid), to = first_of(tid + 1);
+  if (tid == 0) {
+    anchor = kNone;
+    found = -1;
+    others = 0;
+  }
+  int own = 0;
+  for (int r = from; r < to; ++r) {
+    const Fresh f = fresh_of(a, r);
+    own += f.need - f.have;
+  }
+  upto_of(own, fresh_upto);
+  const int total = fresh_upto[kKeepThreads];
+  int named = kNone, page = -1, index = fresh_upto[tid];
+  for (int r = from; r < to && named == kNone; ++r) {
+    const Fresh f = fresh_of(a, r);
+    for (int column = f.have; column < min(f.need, a.table_width) && named == kNone; ++column) {
+      page = a.table[r * a.table_stride + column];
+      if (page >= 0) named = index + column - f.have;
+    }
+    index += f.need - f.have;
+  }
+  if (named != kNone) atomicMin(&anchor, named);
+  __syncthreads();
+  if (named != kNone && named == anchor) anchor_page = page;
+  __syncthreads();
+  const int last = start_of(a.starts, a.tokens, a.requests);
+  if (anchor != kNone) {
+    for (int i = max(taken - total, 0) + tid; i < taken; i += kKeepThreads) {
+      if (a.free_pages[i] == anchor_page) atomicMax(&found, i);
+    }
+  } else {
+    for (int64_t t = static_cast<int64_t>(last) + tid; t < a.tokens; t += kKeepThreads) {
+      if (slot_at(a, t) >= 0) others = 1;
+    }
+  }
+  __syncthreads();
+  const int first = anchor != kNone ? found - anchor : taken - total;  // of the step's pages
+  const int64_t behind = static_cast<int64_t>(first) + total;
+  const bool known = anchor != kNone ? found >= 0 && (behind == taken || (behind > taken && taken == a.free_count))
+                                     : taken < a.free_count && others == 0 && a.starts[0] <= 0 && a.starts[a.requests] <= a.tokens;
+  if (first < 0 || !known) return 0;  // (the same for all)
+  const auto dropped_of = [&](const Fresh &f, int index) {  // of a request whose first page is the step's `index`-th; a list that has run out has not given all
+    return max(min(taken - first - (index + dropped_from(a, f) - f.have), f.need - dropped_from(a, f)), 0);
+  };
+  own = 0;
+  index = fresh_upto[tid];
+  for (int r = from; r < to; ++r) {
+    const Fresh f = fresh_of(a, r);
+    own += dropped_of(f, index);
+    index += f.need - f.have;
+  }
+  upto_of(own, dropped_upto);
+  const int dropped = dropped_upto[kKeepThreads];
+  if (dropped < 0 || dropped > taken - first) return 0;  // (starts that are nobody's, whose sums pass 32 bits)
+  // From the last one on: none moves down, so that what is read has not been written.
+  for (int top = dropped; top > 0; top -= kKeepThreads) {
+    int rest = top - 1 - tid;
+    const int to_place = taken - dropped + rest;
+    page = -1;
+    if (rest >= 0) {
+      int low = 0;
+      for (int high = kKeepThreads; high - low > 1;) {
+        const int mid = (low + high) >> 1;
+        if (dropped_upto[mid] <= rest) low = mid; else high = mid;
+      }
+      rest -= dropped_upto[low];
+      index = fresh_upto[low];
+      for (int r = first_of(low); r < first_of(low + 1); ++r) {
+        const Fresh f = fresh_of(a, r);
+        const int count = dropped_of(f, index);
+        if (rest < count) {
+          const int at = first + index + dropped_from(a, f) - f.have + rest;
+          if (at >= first && at < taken) page = a.free_pages[at];  // (the same)
+          break;
+        }
+        rest -= count;
+        index += f.need - f.have;
+      }
+    }
+    __syncthreads();
+    if (top - 1 - tid >= 0) a.free_pages[to_place] = page;
+    __syncthreads();
+  }
+  return dropped;
+}
+
+// Lengths, and the pages behind them onto the free list again, in front of those that it gives out next, in request order (those that no row names behind the others).
 __device__ void keep_counts(const KvKeepArgs &a) {
   __shared__ int wave_sums[kKeepThreads / 64];
+  __shared__ bool wave_dropped[kKeepThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.requests + kKeepThreads - 1) / kKeepThreads, from = min(tid * run, a.requests), to = min(from + run, a.requests);
   const int taken = a.taken != nullptr ? min(max(*a.taken, 0), a.free_count) : 0;
@@ -126,24 +251,34 @@ __device__ void keep_counts(const KvKeepArgs &a) {
     }
   };
   int own = 0;
+  bool dropped = false;
   for (int r = from; r < to; ++r) {
     const int length = max(a.lengths[r], 0);
     const Path path = path_of(a, r);
     const int kept = max(length - path.fresh, 0) + kept_of(a, r, path);
     a.lengths_after[r] = kept;
-    if (a.taken != nullptr) over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
+    if (a.taken == nullptr) continue;
+    over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
+    const Fresh f = fresh_of(a, length, path.fresh);
+    dropped |= dropped_from(a, f) < f.need;
   }
   if (a.taken == nullptr) return;
   const int sum = kv_sums(own);
-  if (lane == 63) wave_sums[wave] = sum;
+  const bool some_dropped = __builtin_amdgcn_ballot_w64(dropped) != 0;
+  if (lane == 63) {
+    wave_sums[wave] = sum;
+    wave_dropped[wave] = some_dropped;
+  }
   __syncthreads();
   int ahead = sum - own, all = 0;
+  bool any_dropped = false;
 #pragma unroll
   for (int w = 0; w < kKeepThreads / 64; ++w) {
     ahead += w < wave ? wave_sums[w] : 0;
     all += wave_sums[w];
+    any_dropped |= wave_dropped[w];
   }
-  const int begin = taken - all;
+  const int begin = taken - all - (any_dropped ? keep_dropped(a, taken) : 0);
   if (tid == 0) *a.taken_after = max(begin, 0);
   if (own == 0) return;
   int at = begin + ahead;

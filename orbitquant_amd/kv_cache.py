@@ -474,7 +474,9 @@ def kv_keep(kept: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, slo
     lengths, starts, slots   as `kv_assign` gave them for the step
     caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once
     block_table, free_pages, taken   as they are after that `kv_assign` (`taken`: its result), all or none of them.  Pages behind the kept tokens go back
-             onto the list, in place, in front of those that it gives out next.  The table's columns behind the kept pages stand for nothing from then on"""
+             onto the list, in place, in front of those that it gives out next.  The table's columns behind the kept pages stand for nothing from then on.
+             Pages that `kv_assign` drew for columns that the table does not have go back too, if the call is for all of its requests; only of a step in which the list ran out
+             and no column got a page is it not known which these were (a table with room for every new token never has any)"""
     if (block_table is None) != (free_pages is None) or (free_pages is None) != (taken is None):
         raise ValueError("block_table, free_pages and taken go together")
     caches = list(caches)
