@@ -611,7 +611,7 @@ uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t 
  * After the step: of each request's new tokens those of an accepted path stay, as if they had been its only ones.
  *
  * kept       int32 [requests, most], most <= 256: of the request's new tokens, rising; the list ends at the first entry that does not rise, is
- *            not one of them (-1, say) or has no slot.  The i-th kept token's entries go to the i-th new token's slot
+ *            not one of them (-1, say), has no slot or would go where there is none.  The i-th kept token's entries go to the i-th new token's slot
  * lengths, starts, slots   as oq_kv_assign gave them for the step (lengths_after, starts, slots [tokens])
  * caches     host memory: the caches of cache_count layers, of one shape, all moved in one launch (for every 64 of them);
  *            a cache that layers share stands there once

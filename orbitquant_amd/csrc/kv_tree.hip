@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
 
 // ---- the accepted path -----------------------------------------------------------------------------------------------
 // kept[r] names tokens of request r's new ones in rising order; the i-th becomes its i-th new token, and the others are forgotten.
-// The list ends at its first entry that does not rise, is none of the request's tokens or has no slot.
+// The list ends at its first entry that does not rise, is none of the request's tokens, has no slot, or would go where there is none.
 //
 // One launch for all layers.  A wavefront takes one head of one request in one cache.  A lane has the same bytes of all
 // entries: a dword of the keys, a row of the values (two of heads of 256), a scale.  So whatever an entry moves onto, its lane has read before:
@@ -91,14 +91,16 @@ __device__ __forceinline__ int kept_of(const KvKeepArgs &a, int r, const Path &p
   int last = -1;
   for (int base = 0; base < a.most; base += kKeepBatch) {
     int k[kKeepBatch];
-    int64_t slot[kKeepBatch];
+    int64_t slot[kKeepBatch], place[kKeepBatch];
 #pragma unroll
     for (int b = 0; b < kKeepBatch; ++b) k[b] = base + b < a.most ? a.kept[static_cast<int64_t>(r) * a.most + base + b] : -1;
 #pragma unroll
     for (int b = 0; b < kKeepBatch; ++b) slot[b] = k[b] >= 0 && k[b] < path.fresh ? slot_at(a, static_cast<int64_t>(path.first) + k[b]) : -1;
 #pragma unroll
+    for (int b = 0; b < kKeepBatch; ++b) place[b] = k[b] > base + b && k[b] < path.fresh ? slot_at(a, static_cast<int64_t>(path.first) + base + b) : 0;  // (of what moves)
+#pragma unroll
     for (int b = 0; b < kKeepBatch; ++b) {
-      if (k[b] <= last || slot[b] < 0) return base + b;
+      if (k[b] <= last || slot[b] < 0 || place[b] < 0) return base + b;
       last = k[b];
     }
   }
@@ -315,6 +317,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepArgs a) {
     if (k > last && k < path.fresh) {
       source = slot_at(a, static_cast<int64_t>(path.first) + k);
       target = slot_at(a, static_cast<int64_t>(path.first) + i);  // (i <= k: a token of the request)
+      if (target < 0) source = -1;
     }
     const uint64_t bad = __builtin_amdgcn_ballot_w64(source < 0);
     const int good = bad == 0 ? 64 : __builtin_ctzll(bad);
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv_keep_kernel(KvKeepArgs a) {
       return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), from))) |
                                   static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), from))) << 32);
     };
-    uint64_t moves = __builtin_amdgcn_ballot_w64(lane < good && source != target && target >= 0);
+    uint64_t moves = __builtin_amdgcn_ballot_w64(lane < good && source != target);
     while (moves != 0) {
       constexpr int ROWS = (D / 2 + 63) / 64;
       int64_t to[kKeepBatch];

@@ -470,7 +470,7 @@ def kv_keep(kept: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, slo
     """After a step of drafted tokens: of each request's new tokens the `kept` ones stay, as if they had been its only ones (`oq_kv_keep`).
 
     kept     int32 [requests, most], most at most 256: which of the request's new tokens, in rising order, -1 behind the last.  A list ends at the first
-             entry that does not rise, is none of the request's new tokens or has no slot.  The i-th one's entries move to where its i-th new token's are
+             entry that does not rise, is none of the request's new tokens, has no slot or would go where there is none.  The i-th one's entries move to where its i-th new token's are
     lengths, starts, slots   as `kv_assign` gave them for the step
     caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once
     block_table, free_pages, taken   as they are after that `kv_assign` (`taken`: its result), all or none of them.  Pages behind the kept tokens go back
