@@ -614,7 +614,7 @@ uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t 
  *            not one of them (-1, say), has no slot or would go where there is none.  The i-th kept token's entries go to the i-th new token's slot
  * lengths, starts, slots   as oq_kv_assign gave them for the step (lengths_after, starts, slots [tokens])
  * caches     host memory: the caches of cache_count layers, of one shape, all moved in one launch (for every 64 of them);
- *            a cache that layers share stands there once
+ *            a cache that layers share stands there once, and no two parts of caches share memory (OQ_ERR_INVALID)
  * table, free_pages, taken NULL, or as oq_kv_assign left them (taken: taken_after): pages behind the kept tokens go back onto the free
  *            list, in front of those that it gives out next; the table is not changed, its columns behind the kept pages
  *            stand for nothing.  Requests <= 8192.  The pages that oq_kv_assign drew for columns behind the table's end go back too, in a call

@@ -4,8 +4,11 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <map>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <utility>
 
 #include "dense_gemm.h"
@@ -870,6 +873,40 @@ int oq_kv_tree(const int32_t *parents, const int32_t *starts, const int32_t *len
   return oq::kv_tree_dispatch({parents, starts, lengths, static_cast<int>(requests), static_cast<int>(mask_words), tokens, positions, masks}, as_stream(stream));
 }
 
+namespace {
+// No two parts of the caches may share memory: two wavefronts would move the same entries, one of them what the other has moved already.  Parts sorted by where they
+// begin, four a cache (eight caches 1 us of the host, 64, which one launch takes, 6).
+int keep_caches_apart(const oq_kv_cache *caches, int64_t count) {
+  struct Part {
+    uintptr_t begin, end;
+    int64_t cache;
+  };
+  Part few[4 * 16];
+  const std::unique_ptr<Part[]> many(count > 16 ? new (std::nothrow) Part[4 * count] : nullptr);
+  Part *const parts = count > 16 ? many.get() : few;
+  if (parts == nullptr) return fail(OQ_ERR_UNSUPPORTED, "kv_keep: no memory to look %lld caches over", (long long)count);
+  const uint64_t vectors = static_cast<uint64_t>(caches->pages) * caches->kv_heads * caches->page_size, codes = vectors * (caches->head_dim / 2), scales = vectors * 2;
+  for (int64_t i = 0; i < count; ++i) {
+    const auto put = [&](int part, const void *p, uint64_t bytes) { parts[4 * i + part] = {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, i}; };
+    put(0, caches[i].k_codes, codes);
+    put(1, caches[i].v_codes, codes);
+    put(2, caches[i].k_scales, scales);
+    put(3, caches[i].v_scales, scales);
+  }
+  std::sort(parts, parts + 4 * count, [](const Part &a, const Part &b) { return a.begin < b.begin; });
+  for (int64_t i = 1; i < 4 * count; ++i) {  // (in front of the first that overlaps, each begins behind the one before)
+    if (parts[i].begin >= parts[i - 1].end) continue;
+    for (int64_t a = 1; a < count; ++a) {
+      for (int64_t b = 0; b < a; ++b) {
+        if (caches[a].k_codes == caches[b].k_codes) return fail(OQ_ERR_INVALID, "kv_keep: cache %lld is cache %lld again", (long long)a, (long long)b);
+      }
+    }
+    return fail(OQ_ERR_INVALID, "kv_keep: parts of cache %lld and cache %lld share memory", (long long)parts[i - 1].cache, (long long)parts[i].cache);
+  }
+  return OQ_OK;
+}
+}  // namespace
+
 int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const int32_t *starts, const int64_t *slots, int64_t requests, int64_t tokens,
                const oq_kv_cache *caches, int64_t cache_count, const int32_t *table, int64_t table_stride, int64_t table_width, int32_t *free_pages,
                int64_t free_count, const int32_t *taken, int32_t *lengths_after, int32_t *taken_after, void *stream) {
@@ -893,11 +930,8 @@ int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const 
   if (requests == 0 && !pages) return OQ_OK;
   if ((requests > 0 && (lengths == nullptr || starts == nullptr || lengths_after == nullptr || (most > 0 && kept == nullptr))) || (tokens > 0 && slots == nullptr))
     return fail(OQ_ERR_INVALID, "kv_keep: null pointer");
-  // (a path that is moved twice: the second reads what the first has moved already)
-  for (int64_t i = 1; requests > 0 && i < cache_count; ++i) {
-    for (int64_t j = 0; j < i; ++j) {
-      if (caches[i].k_codes == caches[j].k_codes) return fail(OQ_ERR_INVALID, "kv_keep: cache %lld is cache %lld again", (long long)i, (long long)j);
-    }
+  if (requests > 0) {
+    if (const int status = keep_caches_apart(caches, cache_count)) return status;
   }
   oq::KvKeepArgs a{};
   a.kept = kept; a.lengths = lengths; a.starts = starts; a.slots = slots; a.tokens = tokens; a.pages = first.pages; a.table_stride = table_stride;

@@ -472,7 +472,8 @@ def kv_keep(kept: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, slo
     kept     int32 [requests, most], most at most 256: which of the request's new tokens, in rising order, -1 behind the last.  A list ends at the first
              entry that does not rise, is none of the request's new tokens, has no slot or would go where there is none.  The i-th one's entries move to where its i-th new token's are
     lengths, starts, slots   as `kv_assign` gave them for the step
-    caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once
+    caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once; caches that
+             share memory otherwise are refused
     block_table, free_pages, taken   as they are after that `kv_assign` (`taken`: its result), all or none of them.  Pages behind the kept tokens go back
              onto the list, in place, in front of those that it gives out next.  The table's columns behind the kept pages stand for nothing from then on.
              Pages that `kv_assign` drew for columns that the table does not have go back too, if the call is for all of its requests; only of a step in which the list ran out

@@ -1,4 +1,4 @@
-"""`kv_keep`: lists that name what has no place to go."""
+"""`kv_keep`: lists that name what has no place to go, and caches whose parts touch."""
 
 import numpy as np
 import pytest
@@ -62,3 +62,27 @@ def test_a_long_list_that_ends_behind_its_first_batch():
         got = kv_keep(_i32([kept]), _i32([230]), _i32([0, 200]), torch.from_numpy(slots).cuda(), [cache], block_table=table, free_pages=free, taken=_i32([20]))
         assert got.lengths.tolist() == [30 + hole] and got.taken.tolist() == [20 - (-(-230 // 16) - -(-(30 + hole) // 16))]
         _check_moves([cache], was, [(int(slots[k]), int(slots[i])) for i, k in enumerate(kept[:hole])], 16)
+
+
+def test_caches_side_by_side():
+    """Layers that are parts of one tensor touch, and do not overlap."""
+    from orbitquant_amd import OrbitKVCache, kv_keep
+
+    whole = _random(_cache(12, 2, 64, 16))
+    layers = [OrbitKVCache(*(t[4 * i:4 * i + 4] for t in whole[:4]), whole.signs) for i in range(3)]
+    was = [kv_oracle.cache_codes(c) for c in layers]
+    got = kv_keep(_i32([[0, 2]]), _i32([9]), _i32([0, 3]), torch.tensor([20, 21, 40], device="cuda"), layers)
+    assert got.lengths.tolist() == [8]
+    _check_moves(layers, was, [(40, 21)], 16)
+
+
+def test_caches_that_share_a_part_are_refused():
+    from orbitquant_amd import kv_keep
+
+    one, other = _cache(4, 2, 64, 16), _cache(4, 2, 64, 16)
+    slots = torch.tensor([20, 21, 40], device="cuda")
+    for at in range(4):
+        shared = other._replace(**{one._fields[at]: one[at]})
+        for caches in ([one, shared], [_cache(4, 2, 64, 16), one, _cache(4, 2, 64, 16), shared]):
+            with pytest.raises(ValueError, match="cache"):
+                kv_keep(_i32([[0, 2]]), _i32([9]), _i32([0, 3]), slots, caches)
