@@ -612,6 +612,7 @@ uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t 
  *
  * kept       int32 [requests, most], most <= 256: of the request's new tokens, rising; the list ends at the first entry that does not rise, is
  *            not one of them (-1, say), has no slot or would go where there is none.  The i-th kept token's entries go to the i-th new token's slot
+ *            OQ_KV_KEEP_ALL as a list's first entry: all of the request's new tokens stay, however many they are (a prompt in a step with trees)
  * lengths, starts, slots   as oq_kv_assign gave them for the step (lengths_after, starts, slots [tokens])
  * caches     host memory: the caches of cache_count layers, of one shape, all moved in one launch (for every 64 of them);
  *            a cache that layers share stands there once, and no two parts of caches share memory (OQ_ERR_INVALID)
@@ -623,6 +624,7 @@ uint64_t oq_kv_attend_tree_workspace_bytes(int q_dtype, int64_t tokens, int64_t 
  * lengths_after int32 [requests]: without the forgotten tokens; taken_after int32 [1]
  * No slot twice in slots.  No output may overlap an input other than the caches and free_pages.
  */
+enum { OQ_KV_KEEP_ALL = -2 };
 int oq_kv_keep(const int32_t *kept, int64_t most, const int32_t *lengths, const int32_t *starts, const int64_t *slots,
                int64_t requests, int64_t tokens, const oq_kv_cache *caches, int64_t cache_count, const int32_t *table,
                int64_t table_stride, int64_t table_width, int32_t *free_pages, int64_t free_count,

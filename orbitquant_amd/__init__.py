@@ -15,14 +15,14 @@ from .rotations import RPBHRotation, get_rpbh_rotation
 from .weights import quantize_weight
 from . import ops  # noqa: E402
 from .qk_rotary import QKNormRotary, qk_norm_rotary  # noqa: E402
-from .kv_cache import KVAssignment, KVKept, KVTree, OrbitKVCache, kv_append, kv_assign, kv_attend, kv_keep, kv_read, kv_tree, kv_write  # noqa: E402
+from .kv_cache import KEEP_ALL, KVAssignment, KVKept, KVTree, OrbitKVCache, kv_append, kv_assign, kv_attend, kv_keep, kv_read, kv_tree, kv_write  # noqa: E402
 from .layers import OrbitLinear, OrbitLinearGroup  # noqa: E402
 from .adaln import RTNInt4Linear, quantize_adaln_weight  # noqa: E402
 from .attention import OrbitCachedAttention  # noqa: E402
 from .artifacts import load_artifact, save_artifact  # noqa: E402
 
 __all__ = [
-    "KVAssignment", "KVKept", "KVTree", "LloydMaxCodebook", "OrbitCachedAttention", "OrbitKVCache", "OrbitLinear", "OrbitLinearGroup", "OrbitQuantConfig",
+    "KEEP_ALL", "KVAssignment", "KVKept", "KVTree", "LloydMaxCodebook", "OrbitCachedAttention", "OrbitKVCache", "OrbitLinear", "OrbitLinearGroup", "OrbitQuantConfig",
     "QKNormRotary", "RPBHRotation", "RTNInt4Linear", "get_codebook", "get_rpbh_rotation", "kv_append", "kv_assign", "kv_attend", "kv_keep", "kv_read", "kv_tree",
     "kv_write", "load_artifact", "ops", "pack_lowbit", "packed_length", "qk_norm_rotary", "quantize_adaln_weight",
     "quantize_weight", "recipe", "save_artifact", "unpack_lowbit",

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
 
 // ---- the accepted path -----------------------------------------------------------------------------------------------
 // kept[r] names tokens of request r's new ones in rising order; the i-th becomes its i-th new token, and the others are forgotten.
-// The list ends at its first entry that does not rise, is none of the request's tokens, has no slot, or would go where there is none.
+// A list that begins with OQ_KV_KEEP_ALL is a request that stays as the step left it.  Another ends at its first entry that does not rise, is none of the request's tokens, has no slot, or would go where there is none.
 //
 // One launch for all layers.  A wavefront takes one head of one request in one cache.  A lane has the same bytes of all
 // entries: a dword of the keys, a row of the values (two of heads of 256), a scale.  So whatever an entry moves onto, its lane has read before:
@@ -85,6 +85,9 @@ __device__ __forceinline__ int64_t slot_at(const KvKeepArgs &a, int64_t token) {
   const int64_t slot = a.slots[token];
   return slot < a.pages << a.page_shift ? slot : -1;
 }
+
+// A request of which everything stays (a prompt beside trees, say, longer than any list).
+__device__ __forceinline__ bool all_stay(const KvKeepArgs &a, int r) { return a.most > 0 && a.kept[static_cast<int64_t>(r) * a.most] == OQ_KV_KEEP_ALL; }
 
 // How many entries of a request's list count.  Eight at a time, whose loads do not wait for each other.
 __device__ __forceinline__ int kept_of(const KvKeepArgs &a, int r, const Path &path) {
@@ -107,16 +110,16 @@ __device__ __forceinline__ int kept_of(const KvKeepArgs &a, int r, const Path &p
   return a.most;
 }
 
-// The pages that kv_assign has drawn for request r's new tokens: for columns [have, need), also where these lie behind the table.
+// The pages that kv_assign has drawn for a request's new tokens: for columns [have, need), also where these lie behind the table, which go back from `dropped` on.
 struct Fresh {
-  int have, need;
+  int have, need, dropped;
 };
-__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int length, int fresh) {
+__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int length, int fresh, bool all) {
   const auto pages_of = [&](int tokens) { return static_cast<int>((static_cast<uint32_t>(tokens) + (1u << a.page_shift) - 1) >> a.page_shift); };
-  return {pages_of(max(length - fresh, 0)), pages_of(length)};
+  const int have = pages_of(max(length - fresh, 0)), need = pages_of(length);
+  return {have, need, all ? need : max(have, a.table_width)};
 }
-__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int r) { return fresh_of(a, max(a.lengths[r], 0), path_of(a, r).fresh); }
-__device__ __forceinline__ int dropped_from(const KvKeepArgs &a, const Fresh &f) { return max(f.have, a.table_width); }  // the first of them behind the table
+__device__ __forceinline__ Fresh fresh_of(const KvKeepArgs &a, int r) { return fresh_of(a, max(a.lengths[r], 0), path_of(a, r).fresh, all_stay(a, r)); }
 
 // Before every thread of the workgroup's `own`, the sum of the threads before; upto[kKeepThreads]: of all.  Behind a barrier, and one behind it.
 __device__ void upto_of(int own, int (&upto)[kKeepThreads + 1]) {
@@ -187,7 +190,7 @@ __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
                                      : taken < a.free_count && others == 0 && a.starts[0] <= 0 && a.starts[a.requests] <= a.tokens;
   if (first < 0 || !known) return 0;  // (the same for all)
   const auto dropped_of = [&](const Fresh &f, int index) {  // of a request whose first page is the step's `index`-th; a list that has run out has not given all
-    return max(min(taken - first - (index + dropped_from(a, f) - f.have), f.need - dropped_from(a, f)), 0);
+    return max(min(taken - first - (index + f.dropped - f.have), f.need - f.dropped), 0);
   };
   own = 0;
   index = fresh_upto[tid];
@@ -216,7 +219,7 @@ __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
         const Fresh f = fresh_of(a, r);
         const int count = dropped_of(f, index);
         if (rest < count) {
-          const int at = first + index + dropped_from(a, f) - f.have + rest;
+          const int at = first + index + f.dropped - f.have + rest;
           if (at >= first && at < taken) page = a.free_pages[at];  // (the same)
           break;
         }
@@ -257,12 +260,13 @@ __device__ void keep_counts(const KvKeepArgs &a) {
   for (int r = from; r < to; ++r) {
     const int length = max(a.lengths[r], 0);
     const Path path = path_of(a, r);
-    const int kept = max(length - path.fresh, 0) + kept_of(a, r, path);
+    const bool all = all_stay(a, r);
+    const int kept = all ? length : max(length - path.fresh, 0) + kept_of(a, r, path);
     a.lengths_after[r] = kept;
     if (a.taken == nullptr) continue;
     over_pages(r, pages_of(kept), pages_of(length), [&](int) { ++own; });
-    const Fresh f = fresh_of(a, length, path.fresh);
-    dropped |= dropped_from(a, f) < f.need;
+    const Fresh f = fresh_of(a, length, path.fresh, all);
+    dropped |= f.dropped < f.need;
   }
   if (a.taken == nullptr) return;
   const int sum = kv_sums(own);

@@ -25,6 +25,9 @@ from .qk_rotary import _HOW, QKNormRotary, _plan, _vectors
 from .rotations import get_rpbh_rotation
 
 
+KEEP_ALL = -2   # of `kv_keep`'s lists, as the first entry (OQ_KV_KEEP_ALL)
+
+
 class OrbitKVCache(NamedTuple):
     """The tensors of a cache, contiguous, on one GPU:
 
@@ -471,6 +474,7 @@ def kv_keep(kept: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, slo
 
     kept     int32 [requests, most], most at most 256: which of the request's new tokens, in rising order, -1 behind the last.  A list ends at the first
              entry that does not rise, is none of the request's new tokens, has no slot or would go where there is none.  The i-th one's entries move to where its i-th new token's are
+             A list that begins with `KEEP_ALL` keeps all of the request's new tokens, however many: a prompt beside trees
     lengths, starts, slots   as `kv_assign` gave them for the step
     caches   the OrbitKVCaches of all layers, of one shape, changed in place (one launch for every 64 of them); one that layers share, once; caches that
              share memory otherwise are refused
