@@ -434,7 +434,7 @@ def kv_tree(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, 
              hangs on what the request has cached
     starts, lengths   int32 [requests + 1] and [requests], as `kv_assign` gives them for these tokens
     max_new  the largest number of new tokens of a request that is a tree, at most 256: it decides on the masks' words.  A request with more than
-             these have bits is a prompt, whose tokens follow each other
+             these have bits is a prompt, whose tokens follow each other whatever its parents say: a tree of 70 nodes needs max_new=70, and is a chain without it
 
     A token's position is its depth behind the cached ones: what `kv_append` wants for it, where `kv_assign`'s are its place's.  Tokens of no request have
     position -1 and empty masks."""
