@@ -24,7 +24,12 @@ class OrbitCachedAttention(nn.Module):
 
     q, k, v, out: OrbitLinear modules; k and v have the cache's heads, q a multiple of them.  `cache`: the layer's own.  `rotary`: a `QKNormRotary`,
     which `kv_append` applies in one launch with the write; or `rotary(q, k, positions)` -> (q, k), applied to [tokens, heads, D] with the positions
-    int32 [tokens], -1 for tokens of no request.  `window`: of the keys that a token sees, the last ones only."""
+    int32 [tokens], -1 for tokens of no request.  `window`: of the keys that a token sees, the last ones only.
+
+    A `QKNormRotary`'s weights are the module's parameters `q_norm_weight` and `k_norm_weight`, saved, loaded, moved and converted with its linears; its tables move with
+    it, are not saved and stay fp32.  (A state without the weights, as it was saved before they were part of one, leaves them as they are.)  The cache stays where it is."""
+
+    _version = 2   # of the state: 1 has no norms' weights
 
     def __init__(self, q: OrbitLinear, k: OrbitLinear, v: OrbitLinear, out: OrbitLinear, cache: OrbitKVCache, *,
                  rotary: QKNormRotary | Callable | None = None, window: int | None = None) -> None:
@@ -38,8 +43,52 @@ class OrbitCachedAttention(nn.Module):
             raise ValueError(f"out takes {out.in_features} values, q gives {q.out_features}")
         self.q, self.k, self.v, self.out = q, k, v, out
         self.cache = cache
-        self.rotary = rotary
+        self._hold(rotary)
         self.window = window
+
+    def _hold(self, rotary) -> None:
+        self._rotary = None
+        for name in ("_rotary_cos", "_rotary_sin"):
+            self.register_buffer(name, None, persistent=False)
+        for name in ("q_norm_weight", "k_norm_weight"):
+            self.register_parameter(name, None)
+        self.rotary = rotary
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        if "_rotary" not in self.__dict__:  # a module pickled whole when its rotary was an attribute like any other
+            self._hold(self.__dict__.pop("rotary", None) or self._modules.get("rotary"))
+
+    @property
+    def rotary(self) -> QKNormRotary | Callable | None:
+        module = self._modules.get("rotary")    # (a callable that is a module is one of this module's)
+        if module is not None:
+            return module
+        if not isinstance(self._rotary, QKNormRotary):
+            return self._rotary
+        return QKNormRotary(self._rotary_cos, self._rotary_sin, self.q_norm_weight, self.k_norm_weight, self._rotary.eps, self._rotary.interleaved)
+
+    @rotary.setter
+    def rotary(self, rotary: QKNormRotary | Callable | None) -> None:
+        plan = rotary if isinstance(rotary, QKNormRotary) else QKNormRotary()
+        self._rotary = QKNormRotary(eps=plan.eps, interleaved=plan.interleaved) if rotary is plan else rotary
+        self._rotary_cos, self._rotary_sin = (None if t is None else t.detach() for t in (plan.cos, plan.sin))
+        for name, weight in (("q_norm_weight", plan.q_weight), ("k_norm_weight", plan.k_weight)):
+            setattr(self, name, weight if weight is None or isinstance(weight, nn.Parameter) else nn.Parameter(weight.detach(), requires_grad=False))
+
+    def _apply(self, fn, recurse: bool = True):
+        tables = self._rotary_cos, self._rotary_sin
+        super()._apply(fn, recurse)
+        if tables[0] is not None and self._rotary_cos.dtype != torch.float32:    # a conversion: tables are fp32 whatever the model is
+            self._rotary_cos, self._rotary_sin = (t.to(moved.device) for t, moved in zip(tables, (self._rotary_cos, self._rotary_sin)))
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        if (local_metadata.get("version") or 1) < 2:
+            for name in ("q_norm_weight", "k_norm_weight"):
+                if getattr(self, name) is not None and prefix + name not in state_dict:
+                    state_dict[prefix + name] = getattr(self, name).detach()
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def forward(self, x: torch.Tensor, assignment: KVAssignment, block_table: torch.Tensor, *, tree: KVTree | None = None, one_each: bool = False,
                 max_new: int | None = None, max_length: int | None = None) -> torch.Tensor:
@@ -53,11 +102,12 @@ class OrbitCachedAttention(nn.Module):
         q, k, v = OrbitLinearGroup(self.q, self.k, self.v)(x)
         q, k, v = (t.view(tokens, t.shape[1] // dim, dim) for t in (q, k, v))
         positions, masks = (assignment.positions, None) if tree is None else tree
-        if isinstance(self.rotary, QKNormRotary):
-            q = kv_append(q, k, v, assignment.slots, self.cache, self.rotary, positions)
+        rotary = self.rotary
+        if isinstance(rotary, QKNormRotary):
+            q = kv_append(q, k, v, assignment.slots, self.cache, rotary, positions)
         else:
-            if self.rotary is not None:
-                q, k = self.rotary(q, k, positions)
+            if rotary is not None:
+                q, k = rotary(q, k, positions)
             kv_write(k, v, assignment.slots, self.cache)
         attended = kv_attend(q, self.cache, block_table, assignment.lengths, starts=None if one_each else assignment.starts, masks=masks, max_new=max_new,
                              max_length=max_length, window=self.window)
