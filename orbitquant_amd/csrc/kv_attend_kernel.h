@@ -1359,11 +1359,12 @@ __global__ __launch_bounds__(64 * kv_many_waves<D>(), 2) void kv_attend_many_ker
         broken.look(vs, step);
       }
       const float top_exponent = kv_exponent_of(kv_largest_scale(vs));
-      const auto mixed = [&] {  // (a lane for each key, against the first, which is the smaller one if one is)
+      const auto mixed = [&] {  // (a lane for each key that is there, the others' scales may be anything; against the first, which is the smaller one if one is, and 0 if it is not there)
         int key = lane;
         asm volatile("" : "+v"(key));
-        const int scale = __float_as_int(from.vs[key]);
-        return static_cast<uint32_t>(scale - kv_uniform(scale) + (2 << 23)) >= static_cast<uint32_t>(kKvMixed) << 23;
+        const bool there = here && first + key <= r.last_key;
+        const int scale = there ? __float_as_int(from.vs[key]) : 0;
+        return there && static_cast<uint32_t>(scale - kv_uniform(scale) + (2 << 23)) >= static_cast<uint32_t>(kKvMixed) << 23;
       };
       kv_f16x8 p[RT][2], p_rest[RT][SPLIT > 1 ? 2 : 1];
 #pragma unroll
