@@ -546,7 +546,8 @@ uint64_t oq_kv_attend_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_
  *   s  = sum of squares: the two of a pair, then pairs 4, 2, 1 apart of each eight, then eights 1, 2, 4, ... apart
  *   y  = (x * (1 / sqrt(s * fp32(1/D) + eps))) * w              where norm is set; w = 1 where there is no weight
  *   (y0, y1) -> (y0 c - y1 s, y1 c + y0 s)                      of the first R/2 pairs; c, s: the position's row of the tables
- * and rounded once to the output's type.  Squares are fp32: norms are right for values below 2^59.
+ * and rounded once to the output's type.  Squares are fp32: norms are right for values below 2^59 where mean square + eps is a normal fp32
+ * number (2^-126 and more; with eps = 0 smaller heads lose digits and then become infinite, and one of zeros NaN, as 0 / 0 is).
  * The struct is host memory, read during the call.
  */
 typedef struct {

@@ -26,6 +26,9 @@ class QKNormRotary(NamedTuple):
     eps          of the norms x / sqrt(mean(x^2) + eps) of each head; None: there is no norm
     interleaved  pairs are dimensions 2p and 2p + 1; otherwise p and p + R/2 of the first R
 
+    The norm is each head's own (a model that norms all heads of a projection together needs its own).  Squares are fp32: it is right for values below 2^59
+    where mean square + eps is at least 2^-126, which any usual eps sees to.
+
     Dimensions behind the first R are not turned.  The arithmetic is fp32, rounded once in the end, and stated in include/orbitquant_hip.h."""
 
     cos: torch.Tensor | None = None
