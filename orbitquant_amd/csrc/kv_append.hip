@@ -22,6 +22,9 @@ __device__ __forceinline__ void load_vector(const void *p, int64_t at, int part,
 // The workgroups of kv_write (one head of sixteen tokens each), whose keys go through the norm and the rotation first, and behind them
 // those of the queries.  A wavefront has keys or values, never both.  MI355X, 8192 tokens, 32 query heads on 8 of 128, bf16, 181 MB: 38.3 us, 4.7 TB/s (a copy
 // of as many bytes 35); vector instructions issue in 89 % of the cycles, twenty a value.  One token 4.4 us, of them some 2 the launch.
+// In fp16 38.5, in fp32 70 (331 MB); half of the head turned, through LDS, 41, 40 and 73.
+// Pieces are of eight values or of one.  Where four at a time would do (parts of four pairs and not of eight, vectors that begin on eight bytes) they go one by one, four times as long:
+// 72 of 128 dimensions turned as halves 157 us, all of them from bf16 vectors that begin on eight bytes 130.  (qk_norm_rotary, which has pieces of four, 37 and 34 us.)
 template <int D, int DT, int LAYOUT, int PIECE>
 __global__ __launch_bounds__(kv_write_threads(D)) void kv_append_kernel(KvAppendArgs a) {
   constexpr int E = 16, L = D / E, THREADS = kv_write_threads(D);

@@ -741,7 +741,7 @@ __device__ __forceinline__ float kv_exponent_alone(float scale) {
 // x: scores minus R.  Raises R where a weight could pass 2^15, O along with it.  The exponent of the largest of the sixteen scales belongs to a key
 // that the row may not see or hardly weigh: it tells cheaply that no weight is near 2^15, and where the scales are of about one size, where R goes.
 // Where they are not (mixed()), each key is taken with its own exponent, so that a large value raises R for the rows that it has weight in, and the
-// others keep their weights' digits.  (Always with its own: a prompt of 2048, D = 64, 46.0 -> 50 us; so 46.6.)
+// others keep their weights' digits.  (Always with its own: a prompt of 2048, D = 64, 46.0 -> 50 us; so 46.7.)
 template <int D, typename Mixed>
 __device__ __forceinline__ void kv_keep_in_range(float (&x)[16], const float (&vs)[16], float top_exponent, const Mixed &mixed, KvState &st, kv_f32x4 (&o)[D / 16]) {
   float best = kv_max3(x[0], x[1], x[2]), other = kv_max3(x[3], x[4], x[5]);

@@ -69,9 +69,11 @@ __global__ __launch_bounds__(64 * WORDS) void kv_tree_kernel(KvTreeArgs a) {
 // One launch for all layers.  A wavefront takes one head of one request in one cache.  A lane has the same bytes of all
 // entries: a dword of the keys, a row of the values (two of heads of 256), a scale.  So whatever an entry moves onto, its lane has read before:
 // the places rise with the list and are never behind their sources, and of a batch all are read before the first is written.
-// The bytes are few (132 an entry at D = 128): bound by the latency of four loads one behind the other (starts, list, slots, entries), 5.3 us for one request and two
-// layers, and by the lines that values lie on, one of 128 bytes for every one or two rows: 64 requests, eight layers of eight heads, three or four entries each, 16.4 us (pages of 16
-// tokens 11, of 128 21).
+// The bytes are few (132 an entry at D = 128): bound by the latency of four loads one behind the other (starts, list, slots, entries), 5.2 us for one request and two
+// layers, and by the lines that values lie on.  A page's rows of one byte a token are 16, 64 or 128 bytes apart, so an entry's 64 bytes of values are on 8, 32 or 64 lines of 128, read and
+// written: 64 requests, eight layers of eight heads, three entries that move, 7.5, 12.2 and 18.8 us, and with the same lists of entries that stay where they are 4.1, 3.7 and 3.7 (empty
+// lists 3.6, 3.2, 3.2): the chain that every wavefront walks for itself is four of these microseconds, the rest the lines, 0.2 for each.
+// The counts are one workgroup's, a thread for a run of requests, four or more lists one behind the other from a thousand on: 256 requests 5.2 us, 1024 14.7, 8192 137.
 constexpr int kKeepThreads = 256, kKeepBatch = 8;
 
 struct Path {
@@ -140,7 +142,7 @@ __device__ void upto_of(int own, int (&upto)[kKeepThreads + 1]) {
 //   - a column that got one (the first such) names it, and its place in the list tells;
 //   - where no column has got one, `taken` less the step's pages, unless the list may have run out (then some were not drawn, and which is not known).
 // Neither is believed where the call has but a part of kv_assign's requests, whose pages are not the list's last: the pages are lost then, never listed twice.
-// A rare path, at the end of a request's row: latency of a few loads and barriers, 64 requests that are all there 3.6 us, and 2.5 without it; elsewhere one comparison a request.
+// A rare path, at the end of a request's row: latency of a few loads and barriers, 64 requests that are all there 3.8 us, where none is 3.4; elsewhere one comparison a request.
 __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
   __shared__ int fresh_upto[kKeepThreads + 1], dropped_upto[kKeepThreads + 1];
   __shared__ int anchor, anchor_page, found, others;

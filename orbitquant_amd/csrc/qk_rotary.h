@@ -11,7 +11,7 @@
 // A lane holds eight pairs, `L` = 1, 2, 4, ... 32 lanes a head: both values of every pair are in one lane, the rotation needs no other, and
 // the sums need log2(L) exchanges.  Bound by memory: 32760 tokens, 40 heads of 128 for queries and keys each, bf16, 1.36 GB, 249 us (neighbours 252, as many
 // bytes in fp32 245), 5.4 TB/s, where a copy of the library reaches 5.2; vector instructions issue in 72 % of the cycles.  Few tokens by latency, 3.1 us for one.
-// (Converted as they were fetched, head by head, 344 us; four heads a lane 260.)
+// (Converted as they were fetched, head by head, 352 us; four heads a lane 260.)
 #pragma once
 
 #include "kv_rows.h"
