@@ -79,8 +79,9 @@ class OrbitCachedAttention(nn.Module):
     def _apply(self, fn, recurse: bool = True):
         tables = self._rotary_cos, self._rotary_sin
         super()._apply(fn, recurse)
-        if tables[0] is not None and self._rotary_cos.dtype != torch.float32:    # a conversion: tables are fp32 whatever the model is
-            self._rotary_cos, self._rotary_sin = (t.to(moved.device) for t, moved in zip(tables, (self._rotary_cos, self._rotary_sin)))
+        # Nothing saves or rebuilds the tables: what they hold goes along whatever becomes of the weights (another type, memory that is not filled).
+        self._rotary_cos, self._rotary_sin = (moved if t is None or t.is_meta or moved.is_meta else t.to(moved.device)
+                                              for t, moved in zip(tables, (self._rotary_cos, self._rotary_sin)))
         return self
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):

@@ -79,6 +79,15 @@ def test_tables_stay_fp32(convert):
     torch.testing.assert_close(layer.rotary.q_weight.float(), how.q_weight.float(), rtol=0, atol=0)
 
 
+def test_memory_that_is_not_filled():
+    """A skeleton that a state is loaded into: the tables, which no state has, are what they were."""
+    how = _how()
+    layer, saved = _layer(how), _layer(how).state_dict()
+    layer.to_empty(device="cpu")
+    layer.load_state_dict(saved)
+    _equal(layer.rotary, how)
+
+
 def test_copies_are_their_own():
     layer = _layer(_how())
     other = copy.deepcopy(layer)
