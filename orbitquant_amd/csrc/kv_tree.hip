@@ -145,7 +145,7 @@ __device__ void upto_of(int own, int (&upto)[kKeepThreads + 1]) {
 // A rare path, at the end of a request's row: latency of a few loads and barriers, 64 requests that are all there 3.8 us, where none is 3.4; elsewhere one comparison a request.
 __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
   __shared__ int fresh_upto[kKeepThreads + 1], dropped_upto[kKeepThreads + 1];
-  __shared__ int anchor, anchor_page, found, others;
+  __shared__ int anchor, anchor_page, found, others, elsewhere;  // (each written between two barriers alone)
   constexpr int kNone = 0x7fffffff;
   const int tid = threadIdx.x, run = (a.requests + kKeepThreads - 1) / kKeepThreads;
   const auto first_of = [&](int thread) { return min(thread * run, a.requests); };
@@ -154,6 +154,7 @@ __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
     anchor = kNone;
     found = -1;
     others = 0;
+    elsewhere = 0;
   }
   int own = 0;
   for (int r = from; r < to; ++r) {
@@ -191,6 +192,18 @@ __device__ int keep_dropped(const KvKeepArgs &a, int taken) {
   const bool known = anchor != kNone ? found >= 0 && (behind == taken || (behind > taken && taken == a.free_count))
                                      : taken < a.free_count && others == 0 && a.starts[0] <= 0 && a.starts[a.requests] <= a.tokens;
   if (first < 0 || !known) return 0;  // (the same for all)
+  // Every page that a column got has to stand where it would: a list that was given its pages back already, or in parts, is another one.
+  index = fresh_upto[tid];
+  for (int r = from; r < to; ++r) {
+    const Fresh f = fresh_of(a, r);
+    for (int column = f.have; column < min(f.need, a.table_width); ++column) {
+      const int at = first + index + column - f.have, got = a.table[r * a.table_stride + column];
+      if (at >= 0 && at < taken ? a.free_pages[at] != got : got >= 0) elsewhere = 1;
+    }
+    index += f.need - f.have;
+  }
+  __syncthreads();
+  if (elsewhere != 0) return 0;
   const auto dropped_of = [&](const Fresh &f, int index) {  // of a request whose first page is the step's `index`-th; a list that has run out has not given all
     return max(min(taken - first - (index + f.dropped - f.have), f.need - f.dropped), 0);
   };

@@ -156,6 +156,57 @@ def test_a_part_of_the_requests(before, order):
         assert len(set(listed)) == len(listed) and not others & set(listed)
 
 
+@pytest.mark.parametrize("before", [[60, 3, 64, 40, 62], [20, 60, 3, 64], [3, 64, 20], [64, 62]])
+@pytest.mark.parametrize("kept", [[], [0], [0, 1, 2, 3, 4]])
+def test_a_call_repeated(before, kept):
+    """With the count that it was first given, over the list that it has changed: no page is listed that a request holds, and none twice."""
+    from orbitquant_amd import kv_assign, kv_keep
+
+    pool = Pool(np.random.RandomState(4), before, 4, 60)
+    new = [26, 40, 20, 30, 9][:len(before)]
+    got = kv_assign(pool.lengths, _i32(new), pool.table, pool.free, pool.taken, page_size=PAGE, tokens=sum(new))
+    rows = _i32([kept + [-1] * (5 - len(kept))] * len(before))
+    for again in range(3):
+        after = kv_keep(rows, got.lengths, got.starts, got.slots, pool.caches, block_table=pool.table, free_pages=pool.free, taken=got.taken)
+        pool.lengths, pool.taken = after.lengths, after.taken
+        pages = pool.held() + pool.listed()
+        assert len(set(pages)) == len(pages) and (again > 0 or pool.whole())
+
+
+def test_captured_at_the_tables_end():
+    """A step at a row's end captured once and replayed, the state moving on, against the eager steps."""
+    from orbitquant_amd import kv_assign, kv_keep
+
+    eager, graphed = (Pool(np.random.RandomState(5), [60, 3, 64, 20], 4, 40) for _ in range(2))
+    new, rows = _i32([26, 9, 20, 30]), _i32([[0, -1]] * 4)
+
+    def step(pool):
+        got = kv_assign(pool.lengths, new, pool.table, pool.free, pool.taken, page_size=PAGE, tokens=85)
+        after = kv_keep(rows, got.lengths, got.starts, got.slots, pool.caches, block_table=pool.table, free_pages=pool.free, taken=got.taken)
+        pool.lengths.copy_(after.lengths)
+        pool.taken.copy_(after.taken)
+
+    state = (graphed.lengths, graphed.taken, graphed.table, graphed.free)
+    was = [t.clone() for t in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(graphed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(graphed)
+    for t, old in zip(state, was):
+        t.copy_(old)
+    for _ in range(8):
+        step(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert eager.whole() and graphed.whole()
+        for a, b in zip((eager.lengths, eager.taken, eager.table, eager.free), state):
+            assert torch.equal(a, b)
+
+
 def test_the_example_at_its_tables_end():
     """The drafting example's steps where a request has as many tokens as its row has places."""
     from orbitquant_amd import OrbitKVCache
